@@ -251,6 +251,84 @@ MAG_CUDA_EXPORT int mag_cuda_img_draw_box(mag_compute_device_t* dvc, mag_tensor_
 MAG_CUDA_EXPORT int mag_cuda_img_draw_text(mag_compute_device_t* dvc, mag_tensor_t* t, int32_t x, int32_t y,
                                            int32_t size, uint32_t rgb, const char* txt);
 
+/* ---- language-model rows: norm, 8-bit operands and their product, token log probabilities ----
+ * (no counterpart in the reference, whose storage has one type, f32)
+ *
+ * An e4m3 operand of rows x cols values is
+ *   q  uint8_t [rows][ld], ld = mag_cuda_e4m3_ld(cols) (cols rounded up to 128), each byte one
+ *      e4m3 value (1 sign, 4 exponent, 3 mantissa bits, largest 448, no infinity), zero past cols;
+ *   s  float, one scale per group of 128 columns, G = ld / 128:
+ *      MAG_CUDA_E4M3_ROW    [rows][G]             the group is 1 x 128 (activations, gradients)
+ *      MAG_CUDA_E4M3_BLOCK  [ceil(rows / 128)][G] the group is 128 x 128 (weights)
+ * and stands for s * q.  q must be 16-byte aligned.  A group's scale is max(amax, 2^-100) / 448 with
+ * amax its largest magnitude, and q = v / s rounded to nearest even, so a group of zeros has zero
+ * bytes and a small scale; a NaN in a group makes the whole group NaN, an infinity makes its scale
+ * infinite and itself NaN, and both reach every product that reads the group.
+ *
+ * Calls check their arguments before any work (MAG_CUDA_E_INVALID), take rows = 0 as nothing to do,
+ * and may be captured into a CUDA graph of mag_cuda_stream: a captured call allocates nothing that
+ * outlives the graph, and returns MAG_CUDA_E_INVALID for tensor storage that was never written or
+ * has an asynchronous copy in flight (neither a pending clear nor a wait belongs in the graph).
+ * Results depend on the inputs alone: sums are formed in a fixed order, without atomics. */
+#define MAG_CUDA_E4M3_ROW 0
+#define MAG_CUDA_E4M3_BLOCK 1
+/* Bytes per row of an e4m3 operand, and the number of its scales (0 for sizes below zero or a group
+ * that is neither of the two). */
+MAG_CUDA_EXPORT int64_t mag_cuda_e4m3_ld(int64_t cols);
+MAG_CUDA_EXPORT int64_t mag_cuda_e4m3_scales(int64_t rows, int64_t cols, int group);
+/* The rows x cols row-major matrix x, or with transpose != 0 its cols x rows transpose, as an e4m3
+ * operand with the given groups.  A weight in the framework's product order, Y [K][N], becomes the
+ * y operand of mag_cuda_matmul_e4m3 with transpose = 1. */
+MAG_CUDA_EXPORT int mag_cuda_quantize_e4m3(mag_compute_device_t* dvc, uint8_t* q, float* s, const float* x,
+                                           int64_t rows, int64_t cols, int group, int transpose);
+/* r [M][N] = x y^T for e4m3 operands x (M x K, ROW groups) and y (N x K, y_group groups), both with
+ * K along their rows: r[m][n] = sum over groups g of xs[m][g] ys[n or n/128][g] (sum over k in g of
+ * xq[m][k] yq[n][k]), groups added in f32 with rounding to nearest.  With the operands swapped and
+ * transposed by mag_cuda_quantize_e4m3 the same call gives both gradients of a layer: dX = dY W^T
+ * (W [K][N] quantised without transpose, BLOCK) and dW = X^T dY (both transposed, ROW).
+ * M, N < 2^31 - 256; K < 2^31 - 256. */
+MAG_CUDA_EXPORT int mag_cuda_matmul_e4m3(mag_compute_device_t* dvc, float* r, const uint8_t* xq, const float* xs,
+                                         const uint8_t* yq, const float* ys, int64_t M, int64_t K, int64_t N,
+                                         int y_group);
+/* Root-mean-square norm of each row of rows x cols, with the residual's addition:
+ *   t = x + residual (residual may be null: t = x),  rstd = 1 / sqrt(mean(t^2) + eps),  v = t rstd w.
+ * Outputs, each optional (null) except that y or q must be there: y = v in f32; q and s = v as an
+ * e4m3 operand with ROW groups (both or neither); h = t (the next layer's residual, and what the
+ * backward pass reads); rstd [rows].  h and y may each be x or residual (not the same one).
+ * The sum of squares is formed in f32 per thread over at most cols / 128 values and joined in f32. */
+MAG_CUDA_EXPORT int mag_cuda_rmsnorm_rows_f32(mag_compute_device_t* dvc, float* y, uint8_t* q, float* s, float* h,
+                                              float* rstd, const float* x, const float* residual, const float* w,
+                                              float eps, int64_t rows, int64_t cols);
+/* Its gradient: given dy (of v), h, w and rstd of the forward call, and dh (the gradient that reaches
+ * h from elsewhere, or null),
+ *   dx = dh + rstd (dy w - h rstd^2 mean(dy w h))     (also the residual's gradient),
+ *   dw [cols] = sum over rows of dy h rstd            (null: not wanted; zero for rows = 0).
+ * dx may be dy, h or dh. */
+MAG_CUDA_EXPORT int mag_cuda_rmsnorm_rows_backward_f32(mag_compute_device_t* dvc, float* dx, float* dw,
+                                                       const float* dy, const float* h, const float* w,
+                                                       const float* rstd, const float* dh, int64_t rows,
+                                                       int64_t cols);
+/* Log probabilities over rows of cols logits (row starts at ri * x_s1, x_s1 >= cols): with
+ * lse = log(sum exp(x)), logp = x[id] - lse, entropy = -sum p log p (p = exp(x - lse)), and the top
+ * (0..32, at most cols) largest log probabilities with their columns, largest first, equal logits by
+ * lower column (NaN above everything, +0 equal to -0).  Outputs, each optional (null): logp (needs id),
+ * lse, entropy [rows]; top_logp, top_id [rows][top].
+ * An id below 0 asks for nothing (logp 0, no gradient through logp); an id of cols or more gives NaN.
+ * A logit of -inf has probability 0; a row of nothing else has lse = logp = -inf, entropy 0 and zero
+ * gradient.  A NaN or +inf logit makes the row's lse, entropy and log probabilities NaN. */
+#define MAG_CUDA_TOP_MAX 32
+MAG_CUDA_EXPORT int mag_cuda_token_logprobs_f32(mag_compute_device_t* dvc, float* logp, float* lse, float* entropy,
+                                                float* top_logp, int32_t* top_id, const float* x, const int32_t* id,
+                                                int64_t rows, int64_t cols, int64_t x_s1, int top);
+/* Gradient with respect to the logits, from lse and entropy of the forward call:
+ *   dx[v] = g_logp (1[v = id] - p[v]) - g_entropy p[v] (log p[v] + entropy);
+ * g_logp (with id) or g_entropy (with entropy) may be null, not both.  Rows of dx start at
+ * ri * dx_s1; columns past cols are left as they were.  dx may be x when the strides are equal. */
+MAG_CUDA_EXPORT int mag_cuda_token_logprobs_backward_f32(mag_compute_device_t* dvc, float* dx, const float* x,
+                                                         const int32_t* id, const float* lse, const float* entropy,
+                                                         const float* g_logp, const float* g_entropy, int64_t rows,
+                                                         int64_t cols, int64_t x_s1, int64_t dx_s1);
+
 /* ---- allocation-free entry point (no counterpart in the reference) ----
  * R[M,N] = X[M,K] Y[K,N] for 1 <= M <= 16, the same split-K kernels as
  * mag_cuda_matmul_f32 uses for such shapes, but it never allocates: for callers

@@ -700,6 +700,70 @@ int mcu_dev_sync(mag_compute_device_t* dvc) { return mag_cuda_synchronize(dvc); 
 void mcu_dev_in(mag_compute_device_t* dvc, const void* p) { ext_in(dev_of(dvc), p); }
 void mcu_dev_out(mag_compute_device_t* dvc, void* p, size_t bytes) { ext_out(dev_of(dvc), p, bytes); }
 
+int mcu_call_begin(mcu_call* c, mag_compute_device_t* dvc, const mcu_buf* bufs, int n, size_t scratch_bytes) {
+    mcu_device* d = dev_of(dvc);
+    memset(c, 0, sizeof(*c));
+    c->dvc = dvc;
+    c->stream = d->stream;
+    c->status = d->d_status;
+    c->prev_device = d->ordinal;
+    cudaError_t e = cudaGetDevice(&c->prev_device);
+    if (e != cudaSuccess) return (int)e;
+    if (c->prev_device != d->ordinal && (e = cudaSetDevice(d->ordinal)) != cudaSuccess) return (int)e;
+    enum cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    int rc = (int)cudaStreamIsCapturing(d->stream, &cap);
+    const int captured = cap != cudaStreamCaptureStatusNone;
+    if (!rc && captured) {
+        for (int i = 0; i < n; ++i) {
+            mcu_block* b = bufs[i].p ? tab_find_containing(d, (uintptr_t)bufs[i].p) : NULL;
+            if (b && (b->zero_pending || b->io_pending)) rc = MAG_CUDA_E_INVALID;
+        }
+    }
+    if (!rc && scratch_bytes) {
+        if (captured) {
+            rc = (int)cudaMallocAsync(&c->scratch, scratch_bytes, d->stream);
+            c->own_scratch = !rc;
+        } else {
+            /* grown by its own allocation, so that a failure returns instead of ending the process */
+            if (!d->scratch || scratch_bytes > d->scratch_bytes) {
+                const size_t sz = scratch_bytes < ((size_t)1 << 20) ? ((size_t)1 << 20) : scratch_bytes;
+                void* p = NULL;
+                rc = (int)cudaMallocAsync(&p, sz, d->stream);
+                if (!rc) {
+                    if (d->scratch) rc = (int)cudaFreeAsync(d->scratch, d->stream);
+                    d->scratch = p;
+                    d->scratch_bytes = sz;
+                }
+            }
+            c->scratch = d->scratch;
+        }
+    }
+    if (rc) {
+        if (rc == (int)cudaErrorMemoryAllocation) cudaGetLastError();
+        if (c->prev_device != d->ordinal) cudaSetDevice(c->prev_device);
+        return rc;
+    }
+    for (int i = 0; i < n; ++i)
+        if (bufs[i].p && !bufs[i].out) ext_in(d, bufs[i].p);
+    for (int i = 0; i < n; ++i)
+        if (bufs[i].p && bufs[i].out) ext_out(d, (void*)bufs[i].p, bufs[i].bytes);
+    return 0;
+}
+
+int mcu_call_end(mcu_call* c, int rc, int kernels) {
+    mcu_device* d = dev_of(c->dvc);
+    if (c->own_scratch) {
+        const int e = (int)cudaFreeAsync(c->scratch, d->stream);
+        if (!rc) rc = e;
+    }
+    if (c->prev_device != d->ordinal) {
+        const int e = (int)cudaSetDevice(c->prev_device);
+        if (!rc) rc = e;
+    }
+    if (!rc && kernels) mcu_count_launches(kernels);
+    return rc;
+}
+
 int mag_cuda_set_matmul_mode(mag_compute_device_t* dvc, int mode) {
     if (mode < 0 || mode > 2) return MAG_CUDA_E_INVALID;
     if (mode == 2 && !mcu_matmul_tc_supported()) return MAG_CUDA_E_UNSUPPORTED;

@@ -130,6 +130,30 @@ int mcu_launch_matmul_tc_batched(float* r, const float* x, const float* y, int64
 int mcu_launch_matmul_tc_ex(float* r, const float* x, const float* y, int64_t M, int64_t K, int64_t N,
                             void* scratch, int* status, cudaStream_t st, const mcu_tc_epilogue* ep, int f16);
 
+/* The language-model row operators: arguments as in magnetron_cuda.h, already checked, rows (M, N) > 0.
+ * *launches = kernels launched. */
+/* k_rmsnorm.cu: the backward pass needs mcu_rmsnorm_backward_scratch_bytes of scratch when dw is set. */
+int mcu_launch_rmsnorm(float* y, uint8_t* q, float* s, float* h, float* rstd, const float* x, const float* res,
+                       const float* w, float eps, int64_t rows, int64_t cols, cudaStream_t st, int* launches);
+size_t mcu_rmsnorm_backward_scratch_bytes(int64_t rows, int64_t cols);
+int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy, const float* h, const float* w,
+                                const float* rstd, const float* dh, int64_t rows, int64_t cols, void* scratch,
+                                cudaStream_t st, int* launches);
+/* k_matmul_e4m3.cu */
+int mcu_launch_quantize_e4m3(uint8_t* q, float* s, const float* x, int64_t rows, int64_t cols, int block,
+                             int transpose, cudaStream_t st, int* launches);
+size_t mcu_matmul_e4m3_scratch_bytes(int64_t M, int64_t K, int64_t N);
+int mcu_launch_matmul_e4m3(float* r, const uint8_t* xq, const float* xs, const uint8_t* yq, const float* ys, int64_t M,
+                           int64_t K, int64_t N, int y_block, void* scratch, int* status, cudaStream_t st,
+                           int* launches);
+/* k_logprobs.cu */
+int mcu_launch_logprobs(float* logp, float* lse, float* entropy, float* top_logp, int32_t* top_id, const float* x,
+                        const int32_t* id, int64_t rows, int64_t cols, int64_t x_s1, int top, cudaStream_t st,
+                        int* launches);
+int mcu_launch_logprobs_backward(float* dx, const float* x, const int32_t* id, const float* lse, const float* entropy,
+                                 const float* g_logp, const float* g_entropy, int64_t rows, int64_t cols, int64_t x_s1,
+                                 int64_t dx_s1, cudaStream_t st, int* launches);
+
 #ifdef __cplusplus
 }
 #endif

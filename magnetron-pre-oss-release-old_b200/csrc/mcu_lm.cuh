@@ -1,0 +1,37 @@
+// Device helpers of the language-model row kernels (norm, e4m3 quantiser and product, log probabilities).
+#ifndef MCU_LM_CUH
+#define MCU_LM_CUH
+#include <cstdint>
+
+namespace mcu {
+
+constexpr float kE4m3Max = 448.0f;
+// The smallest largest magnitude a scale is formed from, 2^-100: the scale and its reciprocal stay
+// normal f32 values, so a group of zeros (or of subnormals) divides cleanly.
+constexpr float kE4m3Tiny = 7.8886090522101181e-31f;
+
+// Four values as e4m3 bytes, a in the lowest; rounded to nearest even, saturating, NaN kept.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+// |v| as an integer whose order is the magnitude's, NaN above infinity: a maximum over these keeps NaN.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// A group's scale from the bits of its largest magnitude.
+__device__ __forceinline__ float e4m3_scale(uint32_t amax_bits) {
+    const float a = __uint_as_float(amax_bits);
+    return __fdiv_rn(a < kE4m3Tiny ? kE4m3Tiny : a, kE4m3Max);
+}
+
+__device__ __forceinline__ float warp_sum_f(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+}  // namespace mcu
+#endif

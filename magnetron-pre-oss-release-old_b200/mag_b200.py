@@ -47,6 +47,8 @@ TFLAG_OWNER, TFLAG_VIEW = 1, 2
 
 E_INVALID, E_DEVICE_WAIT, E_UNSUPPORTED, E_SCRATCH_LIMIT, E_IO = 10001, 10002, 10003, 10004, 10005
 TC_SPLIT_TF32, TC_SPLIT_F16 = 0, 1  # mag_cuda_set_tc_split
+E4M3_ROW, E4M3_BLOCK = 0, 1  # groups of an e4m3 operand's scales: 1 x 128 or 128 x 128
+TOP_MAX = 32  # alternatives of token_logprobs
 
 
 # ---------------------------------------------------------------- ABI structs
@@ -132,6 +134,14 @@ def load_library(path: str = LIB_PATH):
         "mag_cuda_kernel_launches": ([], C.c_uint64),
         "mag_cuda_matmul_skinny_f32_noalloc": ([vp, vp, vp, vp, i64, i64, i64], C.c_int),
         "mag_cuda_matmul_skinny_noalloc_limit": ([], C.c_size_t),
+        "mag_cuda_e4m3_ld": ([i64], i64),
+        "mag_cuda_e4m3_scales": ([i64, i64, C.c_int], i64),
+        "mag_cuda_quantize_e4m3": ([vp, vp, vp, vp, i64, i64, C.c_int, C.c_int], C.c_int),
+        "mag_cuda_matmul_e4m3": ([vp] * 6 + [i64, i64, i64, C.c_int], C.c_int),
+        "mag_cuda_rmsnorm_rows_f32": ([vp] * 9 + [C.c_float, i64, i64], C.c_int),
+        "mag_cuda_rmsnorm_rows_backward_f32": ([vp] * 8 + [i64, i64], C.c_int),
+        "mag_cuda_token_logprobs_f32": ([vp] * 8 + [i64, i64, i64, C.c_int], C.c_int),
+        "mag_cuda_token_logprobs_backward_f32": ([vp] * 8 + [i64, i64, i64, i64], C.c_int),
         "mag_cuda_fill_uniform_pcg_f32": ([vp, vp, i64, C.c_float, C.c_float, C.POINTER(C.c_uint64), C.c_uint64],
                                           C.c_int),
         "mag_cuda_fill_normal_pcg_f32": ([vp, vp, i64, C.c_float, C.c_float, C.POINTER(C.c_uint64), C.c_uint64],
@@ -268,6 +278,26 @@ class CudaError(RuntimeError):
 def check(rc: int, what: str):
     if rc:
         raise CudaError(f"{what} failed with code {rc}")
+
+
+def address(t) -> int | None:
+    """The device address of a Tensor, or an address itself (memory that this library did not
+    allocate, ordered against Device.stream by the caller); None stays None."""
+    return t.data_ptr if isinstance(t, Tensor) else t
+
+
+def e4m3_ld(cols: int) -> int:
+    """Bytes per row of an e4m3 operand: cols rounded up to 128."""
+    return -(-cols // 128) * 128
+
+
+def e4m3_values() -> np.ndarray:
+    """The 256 values of the e4m3 bytes, in order (0x7F and 0xFF are NaN)."""
+    b = np.arange(256)
+    e, m = (b >> 3) & 15, b & 7
+    v = np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e - 10.0))
+    v[(b & 0x7F) == 0x7F] = np.nan
+    return np.where(b & 0x80, -v, v).astype(np.float32)
 
 
 # ------------------------------------------------------------------- tensors
@@ -439,6 +469,60 @@ class Device:
     def reduce_combine(self, name: str, r_ptr: int, parts_ptr: int, nparts: int):
         """r[0] = SUM/MEAN/MIN/MAX over nparts records at parts_ptr, in record order."""
         check(self.L.mag_cuda_reduce_combine_f32(self.p, OP[name], r_ptr, parts_ptr, nparts), "reduce_combine")
+
+    # ---- language-model rows.  Arrays are Tensors or device addresses; sizes are of the row-major
+    # matrices (a Tensor of shape (cols, rows)); e4m3 operands and int32 ids are raw bytes in Tensors.
+    def e4m3(self, rows: int, cols: int, block: bool = False):
+        """Storage of an e4m3 operand: its bytes [rows][e4m3_ld(cols)] and its scales."""
+        g = e4m3_ld(cols) // 128
+        return self.tensor((32 * g, rows)), self.tensor((g, -(-rows // 128) if block else rows))
+
+    def ids(self, a) -> Tensor:
+        """int32 values (token ids) in a Tensor, as their bits."""
+        a = np.ascontiguousarray(a, np.int32)
+        t = self.tensor((max(1, a.size),))
+        if a.size:
+            t.write(a.reshape(-1).view(np.float32))
+        return t
+
+    def quantize_e4m3(self, rows: int, cols: int, x, q, q_scale, *, block: bool = False, transpose: bool = False):
+        """q, q_scale = x (rows x cols), or its transpose, with scales per 1 x 128 or 128 x 128."""
+        check(self.L.mag_cuda_quantize_e4m3(self.p, address(q), address(q_scale), address(x), rows, cols,
+                                            E4M3_BLOCK if block else E4M3_ROW, int(transpose)), "quantize_e4m3")
+
+    def matmul_e4m3(self, m: int, k: int, n: int, r, xq, x_scale, yq, y_scale, *, y_block: bool = True):
+        """r [m][n] = x y^T of e4m3 operands x (m x k, 1 x 128 groups) and y (n x k)."""
+        check(self.L.mag_cuda_matmul_e4m3(self.p, address(r), address(xq), address(x_scale), address(yq),
+                                          address(y_scale), m, k, n, E4M3_BLOCK if y_block else E4M3_ROW),
+              "matmul_e4m3")
+
+    def rmsnorm_rows(self, rows: int, cols: int, x, w, eps: float, *, residual=None, y=None, q=None, q_scale=None,
+                     h=None, rstd=None):
+        """Norm of the rows of x + residual into y (f32) and/or q, q_scale (e4m3); h = the sum."""
+        check(self.L.mag_cuda_rmsnorm_rows_f32(self.p, address(y), address(q), address(q_scale), address(h),
+                                               address(rstd), address(x), address(residual), address(w), eps, rows,
+                                               cols), "rmsnorm_rows")
+
+    def rmsnorm_rows_backward(self, rows: int, cols: int, dx, dw, dy, h, w, rstd, *, dh=None):
+        """dx and dw of rmsnorm_rows, from the gradient dy of its output and dh of h."""
+        check(self.L.mag_cuda_rmsnorm_rows_backward_f32(self.p, address(dx), address(dw), address(dy), address(h),
+                                                        address(w), address(rstd), address(dh), rows, cols),
+              "rmsnorm_rows_backward")
+
+    def token_logprobs(self, rows: int, cols: int, x, ids=None, *, logp=None, lse=None, entropy=None, top: int = 0,
+                       top_logp=None, top_id=None, x_stride: int | None = None):
+        """Log probabilities of ids under the rows' logits, their entropy and the top alternatives."""
+        check(self.L.mag_cuda_token_logprobs_f32(self.p, address(logp), address(lse), address(entropy),
+                                                 address(top_logp), address(top_id), address(x), address(ids), rows,
+                                                 cols, cols if x_stride is None else x_stride, top), "token_logprobs")
+
+    def token_logprobs_backward(self, rows: int, cols: int, dx, x, ids, lse, entropy=None, g_logp=None,
+                                g_entropy=None, *, x_stride: int | None = None, dx_stride: int | None = None):
+        """dx of token_logprobs, from the gradients of logp and entropy."""
+        check(self.L.mag_cuda_token_logprobs_backward_f32(
+            self.p, address(dx), address(x), address(ids), address(lse), address(entropy), address(g_logp),
+            address(g_entropy), rows, cols, cols if x_stride is None else x_stride,
+            cols if dx_stride is None else dx_stride), "token_logprobs_backward")
 
     # ---- .magnetron storage (mag_tensor_save / mag_tensor_load, magnetron/magnetron.c:2931-2977)
     def save(self, path: str, tensors):
