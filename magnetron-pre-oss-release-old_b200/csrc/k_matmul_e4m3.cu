@@ -1,10 +1,10 @@
 // k_matmul_e4m3.cu - the e4m3 quantiser and the product of e4m3 operands with one scale per 128 of K
 // (mag_cuda_quantize_e4m3, mag_cuda_matmul_e4m3).
 #include <cuda_runtime.h>
-#include <cuda_fp8.h>
 #include <cstdint>
 #include "mcu_kernels.h"
 #include "mcu_lm.cuh"
+#include "mcu_tc.cuh"
 
 using namespace mcu;
 
@@ -46,43 +46,550 @@ __global__ void __launch_bounds__(256) quantize_tile(uint8_t* q, float* s, const
     }
 }
 
-__device__ __forceinline__ float from_e4m3(uint8_t v) {
-    __nv_fp8_e4m3 t;
-    t.__x = v;
-    return (float)t;
+// ------------------------------------------------------------ the product
+//
+// r = x y^T over groups of 128 of K: S = sum_g xs_g ys_g (xq_g . yq_g).  A group is one 128-byte row of a
+// 128-byte-swizzled tile, four tcgen05.mma kind::f8f6f4 of 32 bytes of K each, accumulated from zero in
+// one of two TMEM accumulators; the epilogue warps multiply it by the two scales and add it to the sums
+// they hold in registers, in f32 with rounding to nearest, while the next group's MMAs run.  (Scales of
+// any f32 value cannot ride on the tensor core's own block scaling, which takes powers of two.)
+
+__device__ __forceinline__ void umma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void umma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// D f32, A and B e4m3 (format 0), both K-major.
+__host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// 32 x 32 outputs per block of 256, K in steps of 32 through shared memory.
-__global__ void __launch_bounds__(256) matmul_e4m3_simple(float* r, const uint8_t* xq, const float* xs,
-                                                          const uint8_t* yq, const float* ys, int64_t M, int64_t N,
-                                                          int64_t groups, int64_t col_tiles, int y_block) {
-    __shared__ float tx[32][33], ty[32][33];
-    const int64_t m0 = (int64_t)(blockIdx.x / col_tiles) * 32, n0 = (int64_t)(blockIdx.x % col_tiles) * 32;
-    const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int64_t n = n0 + c;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t g = 0; g < groups; ++g) {
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k0 = 0; k0 < 128; k0 += 32) {
-            for (int i = 0; i < 4; ++i) {
-                const int u = w + 8 * i;
-                tx[u][c] = m0 + u < M ? from_e4m3(xq[((m0 + u) * groups + g) * 128 + k0 + c]) : 0.0f;
-                ty[u][c] = n0 + u < N ? from_e4m3(yq[((n0 + u) * groups + g) * 128 + k0 + c]) : 0.0f;
+// 32 lanes x 32 columns of TMEM; the values are there after tmem_wait.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+// 16 columns, waited for.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Waits for this thread's TMEM loads; v is tied to the wait so that no use moves ahead of it.
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                   "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void bar_named(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// On a give-up: the loads that this thread issued (up to load `it`) have to land before the block ends.
+template <int STAGES>
+__device__ __forceinline__ void drain_loads(uint64_t* full, uint32_t it) {
+    for (uint32_t k = it > STAGES ? it - STAGES : 0; k < it; ++k)
+        for (uint32_t i = 0; i < kWaitLimit && !mbar_test(&full[k % STAGES], (k / STAGES) & 1); ++i) __nanosleep(64);
+}
+
+// ---- large products: CTA pairs, 256 x 256 tiles, persistent
+constexpr int kPairThreads = 384;  // warpgroup 0: producer, MMA issuer, two idle warps; 1 and 2: epilogue
+// 128 * kPairCtrl + 256 * kPairEpi = 384 * kPairLaunch: the epilogue holds 128 sums a thread
+constexpr int kPairLaunch = 168, kPairCtrl = 40, kPairEpi = 232;
+static_assert(128 * kPairCtrl + 256 * kPairEpi == kPairThreads * kPairLaunch, "register split must match the launch");
+constexpr int kPanel = 8;  // groups of per-column scales staged at a time
+constexpr int kGroupRows = 8;  // 256-row blocks that sweep the columns together, so that operands stay in L2
+
+template <bool YROW>
+struct PairCfg {
+    static constexpr int STAGES = YROW ? 5 : 6;
+    static constexpr int HALF = 128 * 128;  // this CTA's rows of x, or its half of y's, one group
+    static constexpr int STAGE = 2 * HALF;
+    static constexpr int BARS = STAGES * STAGE;
+    static constexpr int SLOTS = BARS + 1024;              // 8 epilogue warps x 32 x 32 f32
+    static constexpr int PANEL = SLOTS + 8 * 4096;         // 2 halves x kPanel x 128 scales
+    static constexpr int SMEM = PANEL + (YROW ? 2 * kPanel * 128 * 4 : 0) + 1024;
+    static_assert(SMEM <= 227 * 1024, "must fit shared memory");
+};
+
+__device__ __forceinline__ void pair_tile(int t, int num_m, int num_n, int& mb, int& nb) {
+    const int per = kGroupRows * num_n, g = t / per, first = g * kGroupRows, rows = min(num_m - first, kGroupRows);
+    mb = first + (t - g * per) % rows;
+    nb = (t - g * per) / rows;
+}
+
+template <bool YROW>
+__global__ void __maxnreg__(kPairLaunch)
+    gemm_e4m3_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
+                   const float* __restrict__ xs, const float* __restrict__ ys, float* __restrict__ r, int M, int N, int G,
+                   int* status) {
+    using C = PairCfg<YROW>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = (uint64_t*)(smem + C::BARS);
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* acc_full = empty + C::STAGES;
+    uint64_t* acc_empty = acc_full + 2;
+    uint64_t* drain = acc_empty + 2;
+    uint32_t* tmem_slot = (uint32_t*)(drain + 1);
+    volatile int* gave_up = (volatile int*)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int num_m = (M + 255) >> 8, num_n = (N + 255) >> 8, tiles = num_m * num_n;
+    const Abort ab{gave_up, status};
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&acc_full[a], 1);
+            mbar_init(&acc_empty[a], 16);  // one arrival per epilogue warp of both CTAs
+        }
+        mbar_init(drain, 1);
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    pdl_begin();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairCtrl));
+        if (warp == 0 && lane == 0) {  // ---- TMA producer
+            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_x) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_y) : "memory");
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                int mb, nb;
+                pair_tile(t, num_m, num_n, mb, nb);
+                for (int g = 0; g < G; ++g, ++it) {
+                    const uint32_t s = it % C::STAGES;
+                    if (!(ok = mbar_wait(&empty[s], (it / C::STAGES & 1) ^ 1, ab, 11))) break;
+                    // both CTAs' loads complete on the leader's barrier, which expects both
+                    const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
+                    uint8_t* st = smem + s * C::STAGE;
+                    if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
+                    tma_load_2d_pair(&map_x, fb, st, g * 128, mb * 256 + (int)rank * 128);
+                    tma_load_2d_pair(&map_y, fb, st + C::HALF, g * 128, nb * 256 + (int)rank * 128);
+                }
             }
-            __syncthreads();
-            for (int k = 0; k < 32; ++k)
-                for (int i = 0; i < 4; ++i) part[i] += tx[w + 8 * i][k] * ty[c][k];
-            __syncthreads();
+            if (!ok && rank == 0) drain_loads<C::STAGES>(full, it);
+        } else if (warp == 1 && lane == 0 && rank == 0) {  // ---- MMA issuer, for both CTAs
+            constexpr uint32_t idesc = idesc_f8(256, 256);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                for (int g = 0; g < G; ++g, ++it) {
+                    const uint32_t s = it % C::STAGES, b = it & 1;
+                    if (!(ok = mbar_wait(&acc_empty[b], (it >> 1 & 1) ^ 1, ab, 12))) break;
+                    if (!(ok = mbar_wait(&full[s], it / C::STAGES & 1, ab, 13))) break;
+                    tc_fence_after();
+                    const uint32_t base = smem_u32(smem + s * C::STAGE);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_f8_pair(tmem + b * 256, sw_desc<128>(base + k * 32), sw_desc<128>(base + C::HALF + k * 32), idesc, k);
+                    umma_commit_pair(&empty[s]);
+                    umma_commit_pair(&acc_full[b]);
+                }
+            }
         }
-        for (int i = 0; i < 4; ++i) {
-            const int64_t m = m0 + w + 8 * i;
-            if (m < M && n < N) sum[i] += xs[m * groups + g] * ys[(y_block ? n / 128 : n) * groups + g] * part[i];
+    } else {  // ---- epilogue: lane = row, warpgroup = half of the columns
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairEpi));
+        const int q = warp & 3, half = (warp >> 2) - 1;
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const uint32_t slot = smem_u32(smem + C::SLOTS + (warp - 4) * 4096);
+        float* panel = (float*)(smem + C::PANEL) + half * kPanel * 128;
+        const uint32_t free0 = mapa_rank(smem_u32(&acc_empty[0]), 0), free1 = mapa_rank(smem_u32(&acc_empty[1]), 0);
+        const bool vec = (N & 3) == 0 && ((uintptr_t)r & 15) == 0;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = pair; t < tiles; t += pairs) {
+            int mb, nb;
+            pair_tile(t, num_m, num_n, mb, nb);
+            const int row0 = mb * 256 + (int)rank * 128 + q * 32, col0 = nb * 256 + half * 128;
+            const float* px = xs + (int64_t)min(row0 + lane, M - 1) * G;
+            // per-block scales: one per group; per-row scales: thread i of the warpgroup fetches column i's
+            const float* py = ys + (int64_t)(YROW ? min(col0 + q * 32 + lane, N - 1) : min(col0, N - 1) >> 7) * G;
+            float sum[128];
+#pragma unroll
+            for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
+            float ax = __ldg(px), ay = YROW ? 0.0f : __ldg(py);
+            for (int g = 0; g < G; ++g, ++it) {
+                const uint32_t b = it & 1;
+                float nx = 0.0f, ny = 0.0f;
+                if (g + 1 < G) {  // the next group's scales
+                    nx = __ldg(px + g + 1);
+                    if (!YROW) ny = __ldg(py + g + 1);
+                }
+                if (YROW && (g & (kPanel - 1)) == 0) {
+                    float p[kPanel];
+#pragma unroll
+                    for (int i = 0; i < kPanel; ++i) p[i] = g + i < G ? __ldg(py + g + i) : 0.0f;
+                    bar_named(1 + half, 128);  // the warpgroup is done with the old panel
+#pragma unroll
+                    for (int i = 0; i < kPanel; ++i) panel[i * 128 + q * 32 + lane] = p[i];
+                    bar_named(1 + half, 128);
+                }
+                // (a warp that gives up goes on without waiting, so that the named barriers stay matched)
+                ok &= mbar_wait(&acc_full[b], it >> 1 & 1, ab, 14);
+                tc_fence_after();
+                const float sc = YROW ? ax : __fmul_rn(ax, ay);
+                const uint32_t src = tmem + lanes + b * 256 + half * 128;
+                const uint32_t pan = smem_u32(panel + (g & (kPanel - 1)) * 128);
+                uint32_t v[2][32];
+                tmem_ld32_start(src, v[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tmem_wait(v[c & 1]);
+                    if (c < 3) {
+                        tmem_ld32_start(src + (c + 1) * 32, v[(c + 1) & 1]);
+                    } else {  // everything read: the accumulator goes back to the leader's MMA issuer
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(b ? free1 : free0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        float4 s4 = make_float4(sc, sc, sc, sc);
+                        if (YROW) {
+                            const float4 y4 = lds4(pan + (c * 32 + j) * 4);
+                            s4 = make_float4(__fmul_rn(sc, y4.x), __fmul_rn(sc, y4.y), __fmul_rn(sc, y4.z), __fmul_rn(sc, y4.w));
+                        }
+                        sum[c * 32 + j] = __fmaf_rn(__uint_as_float(v[c & 1][j]), s4.x, sum[c * 32 + j]);
+                        sum[c * 32 + j + 1] = __fmaf_rn(__uint_as_float(v[c & 1][j + 1]), s4.y, sum[c * 32 + j + 1]);
+                        sum[c * 32 + j + 2] = __fmaf_rn(__uint_as_float(v[c & 1][j + 2]), s4.z, sum[c * 32 + j + 2]);
+                        sum[c * 32 + j + 3] = __fmaf_rn(__uint_as_float(v[c & 1][j + 3]), s4.w, sum[c * 32 + j + 3]);
+                    }
+                }
+                ax = nx;
+                ay = ny;
+            }
+            // 32 x 32 chunks through this warp's slot, so that rows leave as 128-byte stores
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int col = col0 + c * 32;
+                if (!ok || row0 >= M || col >= N) break;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    sts4(slot + lane * 128 + (((j >> 2) ^ (lane & 7)) << 4), sum[c * 32 + j], sum[c * 32 + j + 1],
+                         sum[c * 32 + j + 2], sum[c * 32 + j + 3]);
+                __syncwarp();
+                if (vec) {
+                    const int cc = (lane & 7) * 4;
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) {
+                        const int rr = 4 * i + (lane >> 3);
+                        const float4 o = lds4(slot + rr * 128 + (((cc >> 2) ^ (rr & 7)) << 4));
+                        if (row0 + rr < M && col + cc < N) __stcs((float4*)(r + (int64_t)(row0 + rr) * N + col + cc), o);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int rr = 0; rr < 32 && row0 + rr < M; ++rr) {
+                        float o;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(o) : "r"(slot + rr * 128 + (((lane >> 2) ^ (rr & 7)) << 4) + (lane & 3) * 4) : "memory");
+                        if (col + lane < N) r[(int64_t)(row0 + rr) * N + col + lane] = o;
+                    }
+                }
+                __syncwarp();
+            }
         }
     }
-    for (int i = 0; i < 4; ++i) {
-        const int64_t m = m0 + w + 8 * i;
-        if (m < M && n < N) r[m * N + n] = sum[i];
+    __syncthreads();
+    if (warp == 1 && lane == 0 && rank == 0 && *gave_up) {  // MMAs in flight end before the accumulators go
+        umma_commit_pair_local(drain);
+        for (uint32_t i = 0; i < kWaitLimit && !mbar_test(drain, 0); ++i) __nanosleep(64);
     }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // neither CTA leaves while its peer may still signal it or write its TMEM
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+}
+
+// ---- few rows of x: one CTA per 128 rows of y (the MMA's rows) and BN rows of x, K split over a cluster
+template <int BN>
+struct NarrowCfg {
+    static constexpr int A = 128 * 128, B = BN * 128, STAGE = A + B;
+    static constexpr int STAGES = BN <= 16 ? 6 : BN <= 32 ? 5 : BN <= 64 ? 4 : 6;  // two CTAs per SM up to BN = 64
+    static constexpr int PER_SM = BN <= 64 ? 2 : 1;
+    static constexpr int PANEL = STAGES * STAGE;  // kNarrowPanel x BN scales of x
+    static constexpr int BARS = PANEL + 16 * BN * 4;
+    static constexpr int SMEM = BARS + 512 + 1024;
+    static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;
+    static_assert(PER_SM * SMEM <= 227 * 1024 && 128 * BN * 4 <= STAGES * STAGE, "must fit shared memory");
+};
+constexpr int kNarrowPanel = 16;  // groups of x's scales staged at a time
+
+template <int BN, bool YROW>
+__global__ void __launch_bounds__(192, NarrowCfg<BN>::PER_SM)
+    gemm_e4m3_narrow(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
+                     const float* __restrict__ xs, const float* __restrict__ ys, float* __restrict__ r, int M, int N, int G,
+                     int parts, int per, int* status) {
+    using C = NarrowCfg<BN>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = (uint64_t*)(smem + C::BARS);
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* acc_full = empty + C::STAGES;
+    uint64_t* acc_empty = acc_full + 2;
+    uint64_t* drain = acc_empty + 2;
+    uint32_t* tmem_slot = (uint32_t*)(drain + 1);
+    volatile int* gave_up = (volatile int*)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int mt = (M + BN - 1) / BN;
+    const int part = blockIdx.x % parts, tile = blockIdx.x / parts;
+    const int m0 = tile % mt * BN, n0 = tile / mt * 128;
+    const int g0 = min(part * per, G), g1 = min(g0 + per, G), ng = g1 - g0;
+    const Abort ab{gave_up, status};
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&acc_full[a], 1);
+            mbar_init(&acc_empty[a], 4);
+        }
+        mbar_init(drain, 1);
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)C::COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_begin();
+    const uint32_t tmem = *tmem_slot;
+    float sum[BN];  // this lane's row of y against BN rows of x
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {  // ---- TMA producer
+            uint32_t it = 0;
+            for (int g = g0; g < g1; ++g, ++it) {
+                const uint32_t s = it % C::STAGES;
+                if (!(ok = mbar_wait(&empty[s], (it / C::STAGES & 1) ^ 1, ab, 15))) break;
+                mbar_expect_tx(&full[s], C::STAGE);
+                tma_load_2d(&map_y, &full[s], smem + s * C::STAGE, g * 128, n0);
+                tma_load_2d(&map_x, &full[s], smem + s * C::STAGE + C::A, g * 128, m0);
+            }
+            if (!ok) drain_loads<C::STAGES>(full, it);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {  // ---- MMA issuer
+            constexpr uint32_t idesc = idesc_f8(128, BN);
+            for (uint32_t it = 0; it < (uint32_t)ng; ++it) {
+                const uint32_t s = it % C::STAGES, b = it & 1;
+                if (!(ok = mbar_wait(&acc_empty[b], (it >> 1 & 1) ^ 1, ab, 16))) break;
+                if (!(ok = mbar_wait(&full[s], it / C::STAGES & 1, ab, 17))) break;
+                tc_fence_after();
+                const uint32_t base = smem_u32(smem + s * C::STAGE);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_f8(tmem + b * BN, sw_desc<128>(base + k * 32), sw_desc<128>(base + C::A + k * 32), idesc, k);
+                umma_commit(&empty[s]);
+                umma_commit(&acc_full[b]);
+            }
+        }
+    } else {  // ---- epilogue: lane = row of y
+        const int q = warp & 3, tid = threadIdx.x - 64;
+        const int n = n0 + q * 32 + lane;
+        const float* py = ys + (int64_t)(YROW ? min(n, N - 1) : n0 >> 7) * G + g0;
+        float* panel = (float*)(smem + C::PANEL);
+#pragma unroll
+        for (int j = 0; j < BN; ++j) sum[j] = 0.0f;
+        float ay = ng > 0 ? __ldg(py) : 0.0f;
+        for (uint32_t it = 0; it < (uint32_t)ng; ++it) {
+            const uint32_t b = it & 1;
+            if ((it & (kNarrowPanel - 1)) == 0) {  // x's scales: BN rows x 16 groups
+                if (it) bar_named(1, 128);
+                for (int i = tid; i < BN * kNarrowPanel; i += 128) {
+                    const int m = m0 + i / kNarrowPanel, g = g0 + (int)it + i % kNarrowPanel;
+                    panel[i % kNarrowPanel * BN + i / kNarrowPanel] = m < M && g < g1 ? __ldg(xs + (int64_t)m * G + g) : 0.0f;
+                }
+                bar_named(1, 128);
+            }
+            const float ny = it + 1 < (uint32_t)ng ? __ldg(py + it + 1) : 0.0f;
+            ok &= mbar_wait(&acc_full[b], it >> 1 & 1, ab, 18);
+            tc_fence_after();
+            const uint32_t pan = smem_u32(panel + (it & (kNarrowPanel - 1)) * BN);
+            constexpr int W = BN < 32 ? BN : 32;
+            const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + b * BN;
+#pragma unroll
+            for (int c = 0; c < BN / W; ++c) {
+                uint32_t v[32];
+                if constexpr (W == 16) {
+                    tmem_ld16(src, v);
+                } else {
+                    tmem_ld32_start(src + c * W, v);
+                    tmem_wait(v);
+                }
+                if (c == BN / W - 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[b]);
+                }
+#pragma unroll
+                for (int j = 0; j < W; j += 4) {
+                    const float4 x4 = lds4(pan + (c * W + j) * 4);
+                    float* s = sum + c * W + j;
+                    s[0] = __fmaf_rn(__uint_as_float(v[j]), __fmul_rn(ay, x4.x), s[0]);
+                    s[1] = __fmaf_rn(__uint_as_float(v[j + 1]), __fmul_rn(ay, x4.y), s[1]);
+                    s[2] = __fmaf_rn(__uint_as_float(v[j + 2]), __fmul_rn(ay, x4.z), s[2]);
+                    s[3] = __fmaf_rn(__uint_as_float(v[j + 3]), __fmul_rn(ay, x4.w), s[3]);
+                }
+            }
+            ay = ny;
+        }
+        if (ok && parts == 1 && n < N) {
+#pragma unroll
+            for (int j = 0; j < BN; ++j)
+                if (m0 + j < M) r[(int64_t)(m0 + j) * N + n] = sum[j];
+        }
+        if (ok && parts > 1) {  // every group has been read from the ring: it holds this part's sums now
+            float* own = (float*)smem;
+#pragma unroll
+            for (int j = 0; j < BN; ++j) own[j * 128 + q * 32 + lane] = sum[j];
+        }
+    }
+    __syncthreads();
+    if (parts > 1) {
+        __syncwarp();
+        cluster_sync();
+        const bool good = !*gave_up;
+        // columns are shared out over the cluster; the parts are added in their order
+        for (int i = part * 192 + threadIdx.x; good && i < 128 * BN; i += 192 * parts) {
+            const int m = m0 + (i >> 7), n = n0 + (i & 127);
+            if (m >= M || n >= N) continue;
+            const uint32_t at = smem_u32(smem) + i * 4;
+            float a = 0.0f;
+            for (int p = 0; p < parts; ++p) {
+                float v;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_rank(at, p)) : "memory");
+                a = __fadd_rn(a, v);
+            }
+            r[(int64_t)m * N + n] = a;
+        }
+        __syncwarp();
+        cluster_sync();  // a CTA's sums stay until every peer has read them
+    }
+    if (warp == 1) {
+        if (lane == 0 && *gave_up) {
+            umma_commit(drain);
+            for (uint32_t i = 0; i < kWaitLimit && !mbar_test(drain, 0); ++i) __nanosleep(64);
+        }
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::COLS));
+    }
+}
+
+// ------------------------------------------------------------ host side
+// 2-D map over an operand's bytes [rows][ld], box 128 bytes x box_rows, 128-byte swizzle; rows past the
+// end read as zero.
+bool e4m3_map(CUtensorMap* m, const uint8_t* q, int64_t rows, int64_t ld, int box_rows) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)ld, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)q, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sms() {
+    static int n = 0;
+    if (!n) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    }
+    return n > 0 ? n : 148;
+}
+
+// A launch with a cluster of `cluster` CTAs, as a programmatic dependent of the stream's previous kernel.
+template <typename K, typename... A>
+int launch(K kern, int64_t grid, int threads, int smem, int cluster, cudaStream_t st, A... args) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+template <bool YROW>
+int run_pair(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, const float* ys, float* r, int64_t M, int64_t N,
+             int64_t G, int* status, cudaStream_t st) {
+    const int64_t tiles = (M + 255) / 256 * ((N + 255) / 256);
+    if (tiles > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    const int64_t pairs = tiles < sms() / 2 ? tiles : sms() / 2;
+    return launch(gemm_e4m3_pair<YROW>, 2 * pairs, kPairThreads, PairCfg<YROW>::SMEM, 2, st, mx, my, xs, ys, r, (int)M, (int)N,
+                  (int)G, status);
+}
+
+template <int BN>
+int run_narrow(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, const float* ys, float* r, int64_t M, int64_t N,
+               int64_t G, int y_block, int* status, cudaStream_t st) {
+    const int64_t tiles = (M + BN - 1) / BN * ((N + 127) / 128);
+    int parts = 1;  // CTAs per tile: up to 8, while they all run at once and have at least two groups each
+    while (parts < 8 && tiles * parts * 2 <= sms() * NarrowCfg<BN>::PER_SM && G >= 4 * parts) parts *= 2;
+    if (tiles * parts > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    const int per = (int)((G + parts - 1) / parts);
+    if (y_block)
+        return launch(gemm_e4m3_narrow<BN, false>, tiles * parts, 192, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
+                      (int)N, (int)G, parts, per, status);
+    return launch(gemm_e4m3_narrow<BN, true>, tiles * parts, 192, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
+                  (int)N, (int)G, parts, per, status);
 }
 
 }  // namespace
@@ -103,11 +610,20 @@ extern "C" int mcu_launch_quantize_e4m3(uint8_t* q, float* s, const float* x, in
 extern "C" size_t mcu_matmul_e4m3_scratch_bytes(int64_t, int64_t, int64_t) { return 0; }
 
 extern "C" int mcu_launch_matmul_e4m3(float* r, const uint8_t* xq, const float* xs, const uint8_t* yq,
-                                      const float* ys, int64_t M, int64_t K, int64_t N, int y_block, void*, int*,
+                                      const float* ys, int64_t M, int64_t K, int64_t N, int y_block, void*, int* status,
                                       cudaStream_t st, int* launches) {
-    const int64_t ct = (N + 31) / 32, tiles = (M + 31) / 32 * ct;
-    if (tiles > 0x7fffffff) return (int)cudaErrorInvalidValue;
-    matmul_e4m3_simple<<<(unsigned)tiles, 256, 0, st>>>(r, xq, xs, yq, ys, M, N, (K + 127) / 128, ct, y_block);
+    const int64_t G = (K + 127) / 128, ld = G * 128;
+    const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 1024 ? 128 : 0;
+    CUtensorMap mx, my;
+    if (!e4m3_map(&mx, xq, M, ld, bn ? bn : 128) || !e4m3_map(&my, yq, N, ld, 128)) return (int)cudaErrorInvalidValue;
     *launches = 1;
-    return (int)cudaGetLastError();
+    switch (bn) {
+        case 16: return run_narrow<16>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
+        case 32: return run_narrow<32>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
+        case 64: return run_narrow<64>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
+        case 128: return run_narrow<128>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
+        default:
+            return y_block ? run_pair<false>(mx, my, xs, ys, r, M, N, G, status, st)
+                           : run_pair<true>(mx, my, xs, ys, r, M, N, G, status, st);
+    }
 }

@@ -42,6 +42,7 @@
 #include <cstring>
 #include "mcu_kernels.h"
 #include "mcu_math.cuh"
+#include "mcu_tc.cuh"
 
 #include <utility>
 
@@ -60,7 +61,6 @@ constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
 // 128-column segment sums without spilling.  128*kCtrlRegs + 256*kEpiRegs == kThreads*kLaunchRegs.
 constexpr int kLaunchRegs = 168, kCtrlRegs = 40, kEpiRegs = 232;
 static_assert(128 * kCtrlRegs + 256 * kEpiRegs == kThreads * kLaunchRegs, "register split must match the launch");
-constexpr uint32_t kWaitLimit = 1u << 22;
 
 int sm_count() {
     static int n = 0;
@@ -73,108 +73,7 @@ int sm_count() {
     return n;
 }
 
-// ------------------------------------------------------------ PTX wrappers
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ float4 lds4(uint32_t a) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ void sts4(uint32_t a, float x, float y, float z, float w) {
-    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-struct Abort {
-    volatile int* flag;  // shared: set once any role gives up
-    int* status;         // global status word
-};
-
-// Bounded wait on the phase of `parity`.  False when this or another role gave up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
-    for (uint32_t i = 0;; ++i) {
-        if (mbar_test(bar, parity)) return true;
-        if (*ab.flag) return false;
-        if (i >= kWaitLimit) {
-            *ab.flag = 1;
-            atomicCAS(ab.status, 0, code);
-            return false;
-        }
-        if (i > 32) __nanosleep(64);
-    }
-}
-
-__device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* bar, void* dst, int c0, int c1) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::
-            "r"(smem_u32(dst)),
-        "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
-        : "memory");
-}
-
-// Programmatic dependent launch: every kernel of a product's chain after the first is launched so
-// that it may be scheduled while its predecessor finishes; each kernel waits for the previous
-// grid's completion (and memory) before it touches memory, and lets its own dependents be
-// scheduled at once.  Both are no-ops for a kernel launched without the attribute.
-__device__ __forceinline__ void pdl_begin() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;");
-}
-
-// ---- CTA pairs (2-CTA clusters): the leader (rank 0) issues the MMAs for both CTAs
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// The shared::cluster address of `saddr` (a shared::cta address) in the CTA of rank `rank`.
-__device__ __forceinline__ uint32_t mapa_rank(uint32_t saddr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Arrive on an mbarrier given by its shared::cluster address (this CTA's or the peer's).
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t caddr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
-}
-// TMA load into this CTA's shared memory whose completion is counted on an mbarrier of
-// either CTA of the pair (no multicast).
-__device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap* map, uint32_t bar_caddr, void* dst, int c0, int c1) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::
-            "r"(smem_u32(dst)),
-        "l"((uint64_t)map), "r"(bar_caddr), "r"(c0), "r"(c1)
-        : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
+// ------------------------------------------------------------ the split's MMAs
 // D(tmem) (+)= A(smem) * B(smem)^T, kind::tf32 or kind::f16 (both operands the same
 // type), issued by one thread.
 template <bool F16, bool PAIR = false>
@@ -209,39 +108,6 @@ __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t adesc, uint64_t b
     }
 }
 
-// Arrives on `bar` once every tcgen05.mma issued so far by this thread has completed.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-// Pair form: arrives on the barrier at the same offset in both CTAs of the pair.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-            smem_u32(bar)),
-        "h"((uint16_t)0x3)
-        : "memory");
-}
-// Pair form, this CTA's barrier only.
-__device__ __forceinline__ void umma_commit_pair_local(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-
-// Shared-memory matrix descriptor: K-major rows of ROW_BYTES bytes, swizzled (64B
-// or 128B), 8-row atoms 8*ROW_BYTES bytes apart.
-template <int RB = ROW_BYTES>
-__device__ __forceinline__ uint64_t sw_desc(uint32_t saddr) {
-    constexpr uint32_t row_bytes = RB;
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)1 << 16;                         // leading byte offset (unused for swizzled K-major)
-    d |= (uint64_t)((8 * row_bytes) >> 4) << 32;    // stride byte offset between 8-row atoms
-    d |= (uint64_t)1 << 46;                         // descriptor version for tcgen05
-    d |= (uint64_t)(row_bytes == 128 ? 2 : 4) << 61; // SWIZZLE_128B or SWIZZLE_64B
-    return d;
-}
-
 // Instruction descriptor: D f32, A/B tf32 (format 2, kind::tf32) or f16 (format 0,
 // kind::f16), both K-major, M = 128 (one CTA) or 256 (a CTA pair), N=BN.
 __host__ __device__ constexpr uint32_t idesc_3x(int n, bool f16, int m = BM) {
@@ -255,19 +121,6 @@ __host__ __device__ constexpr uint32_t idesc_3x(int n, bool f16, int m = BM) {
 __device__ __forceinline__ float unscale(float v, int s) {
     const int s1 = s >> 1, s2 = s - s1;
     return __fmul_rn(__fmul_rn(v, __int_as_float((127 - s1) << 23)), __int_as_float((127 - s2) << 23));
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // ------------------------------------------------------------ tile order
@@ -1361,18 +1214,6 @@ __global__ void __launch_bounds__(256) fix_outputs(const float* __restrict__ x, 
 }
 
 // ------------------------------------------------------------ host side
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    if (!fn) {
-        cudaDriverEntryPointQueryResult q;
-        void* p = nullptr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
-    }
-    return fn;
-}
-
 // 2-D map over a [rows][Kp] array of f32 or f16, box = box_rows x rb bytes (64 or 128), swizzled
 // by rb bytes.
 bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t kp, int box_rows, bool f16,
@@ -1583,24 +1424,6 @@ bool make_bias_map(CUtensorMap* m, const float* bias, int64_t M, int64_t N) {
 int test_stall() {
     const char* e = getenv("MAG_CUDA_TC_TEST_STALL");
     return e && e[0] == '1';
-}
-
-// A kernel of a product's chain launched as a programmatic dependent of the previous kernel on the
-// stream (it waits in the kernel, pdl_begin, before touching memory).
-template <typename... KArgs, typename... Args>
-cudaError_t launch_dep(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                       Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
 template <bool FUSED, bool F16, bool PAIR, int RB = ROW_BYTES>
