@@ -1,50 +1,10 @@
-// k_matmul_e4m3.cu - the e4m3 quantiser and the product of e4m3 operands with one scale per 128 of K
-// (mag_cuda_quantize_e4m3, mag_cuda_matmul_e4m3).
+// k_matmul_e4m3.cu - the product of e4m3 operands with one scale per 128 of K (mag_cuda_matmul_e4m3).
 #include <cuda_runtime.h>
 #include <cstdint>
 #include "mcu_kernels.h"
-#include "mcu_lm.cuh"
 #include "mcu_tc.cuh"
 
-using namespace mcu;
-
 namespace {
-
-// One block per 128 x 128 tile of the operand (its rows a, its columns b), held in shared memory.
-__global__ void __launch_bounds__(256) quantize_tile(uint8_t* q, float* s, const float* x, int64_t a, int64_t b,
-                                                     int64_t groups, int block, int transpose) {
-    extern __shared__ float tile[];  // [128][129]
-    __shared__ uint32_t top;
-    const int64_t a0 = (int64_t)(blockIdx.x / groups) * 128, b0 = (int64_t)(blockIdx.x % groups) * 128;
-    if (threadIdx.x == 0) top = 0;
-    for (int i = threadIdx.x; i < 128 * 128; i += 256) {
-        const int u = i >> 7, v = i & 127;  // v runs along x's rows
-        const int64_t ia = a0 + (transpose ? v : u), ib = b0 + (transpose ? u : v);
-        const float t = ia < a && ib < b ? x[transpose ? ib * a + ia : ia * b + ib] : 0.0f;
-        tile[(transpose ? v : u) * 129 + (transpose ? u : v)] = t;
-    }
-    __syncthreads();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (block) {
-        uint32_t m = 0;
-        for (int i = threadIdx.x; i < 128 * 128; i += 256) m = max(m, abs_bits(tile[(i >> 7) * 129 + (i & 127)]));
-        m = __reduce_max_sync(0xffffffffu, m);
-        if (lane == 0) atomicMax(&top, m);
-        __syncthreads();
-    }
-    for (int u = warp; u < 128 && a0 + u < a; u += 8) {
-        float v[4];
-        uint32_t m = 0;
-        for (int i = 0; i < 4; ++i) {
-            v[i] = tile[u * 129 + lane * 4 + i];
-            m = max(m, abs_bits(v[i]));
-        }
-        const float sc = e4m3_scale(block ? top : __reduce_max_sync(0xffffffffu, m)), inv = __frcp_rn(sc);
-        *(uint32_t*)(q + ((a0 + u) * groups + b0 / 128) * 128 + lane * 4) =
-            e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-        if (lane == 0 && !(block && u)) s[(block ? a0 / 128 : a0 + u) * groups + b0 / 128] = sc;
-    }
-}
 
 // ------------------------------------------------------------ the product
 //
@@ -593,19 +553,6 @@ int run_narrow(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, co
 }
 
 }  // namespace
-
-extern "C" int mcu_launch_quantize_e4m3(uint8_t* q, float* s, const float* x, int64_t rows, int64_t cols, int block,
-                                        int transpose, cudaStream_t st, int* launches) {
-    const int64_t a = transpose ? cols : rows, b = transpose ? rows : cols, groups = (b + 127) / 128;
-    const int64_t tiles = (a + 127) / 128 * groups;
-    if (tiles > 0x7fffffff) return (int)cudaErrorInvalidValue;
-    constexpr int smem = 128 * 129 * 4;
-    cudaError_t e = cudaFuncSetAttribute(quantize_tile, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
-    quantize_tile<<<(unsigned)tiles, 256, smem, st>>>(q, s, x, a, b, groups, block, transpose);
-    *launches = 1;
-    return (int)cudaGetLastError();
-}
 
 extern "C" size_t mcu_matmul_e4m3_scratch_bytes(int64_t, int64_t, int64_t) { return 0; }
 

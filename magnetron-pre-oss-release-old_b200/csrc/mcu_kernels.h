@@ -139,9 +139,10 @@ size_t mcu_rmsnorm_backward_scratch_bytes(int64_t rows, int64_t cols);
 int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy, const float* h, const float* w,
                                 const float* rstd, const float* dh, int64_t rows, int64_t cols, void* scratch,
                                 cudaStream_t st, int* launches);
-/* k_matmul_e4m3.cu */
+/* k_quantize_e4m3.cu */
 int mcu_launch_quantize_e4m3(uint8_t* q, float* s, const float* x, int64_t rows, int64_t cols, int block,
                              int transpose, cudaStream_t st, int* launches);
+/* k_matmul_e4m3.cu */
 size_t mcu_matmul_e4m3_scratch_bytes(int64_t M, int64_t K, int64_t N);
 int mcu_launch_matmul_e4m3(float* r, const uint8_t* xq, const float* xs, const uint8_t* yq, const float* ys, int64_t M,
                            int64_t K, int64_t N, int y_block, void* scratch, int* status, cudaStream_t st,

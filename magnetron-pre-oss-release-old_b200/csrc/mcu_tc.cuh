@@ -6,7 +6,7 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 #include <cstdint>
-#include <utility>
+#include "mcu_launch.cuh"
 
 namespace {
 
@@ -70,15 +70,6 @@ __device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* ba
             "r"(smem_u32(dst)),
         "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
         : "memory");
-}
-
-// Programmatic dependent launch: every kernel of a product's chain after the first is launched so
-// that it may be scheduled while its predecessor finishes; each kernel waits for the previous
-// grid's completion (and memory) before it touches memory, and lets its own dependents be
-// scheduled at once.  Both are no-ops for a kernel launched without the attribute.
-__device__ __forceinline__ void pdl_begin() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;");
 }
 
 // ---- CTA pairs (2-CTA clusters): the leader (rank 0) issues the MMAs for both CTAs
@@ -169,24 +160,6 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
             fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
     }
     return fn;
-}
-
-// A kernel of a product's chain launched as a programmatic dependent of the previous kernel on the
-// stream (it waits in the kernel, pdl_begin, before touching memory).
-template <typename... KArgs, typename... Args>
-cudaError_t launch_dep(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                       Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
 }  // namespace
