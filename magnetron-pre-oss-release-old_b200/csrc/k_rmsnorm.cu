@@ -3,82 +3,375 @@
 #include <cuda_runtime.h>
 #include <cstdint>
 #include "mcu_kernels.h"
+#include "mcu_launch.cuh"
 #include "mcu_lm.cuh"
 
 using namespace mcu;
 
 namespace {
 
-constexpr int kThreads = 256;
+// Every kernel here gives a warp whole groups of 128 columns (warp w of W: groups w, w + W, ...), so a
+// group's largest magnitude is one warp reduction.  A lane holds four of a group's columns: neighbours
+// with one 16-byte access (VEC), or columns 32 apart with four 4-byte ones where a row does not start on
+// a 16-byte boundary.
+template <bool VEC>
+__device__ __forceinline__ int lane_col(int lane, int j) { return VEC ? lane * 4 + j : lane + 32 * j; }
 
-// Sum over the block of 256, the same on every thread.
-__device__ float block_sum(float v) {
-    __shared__ float sh[kThreads / 32];
+// Columns past the row's end read as zero.  (Plain loads: a result may lie over an input.)
+template <bool VEC>
+__device__ __forceinline__ void load_group(float (&v)[4], const float* p, int c0, int cols, int lane) {
+    if (VEC) {
+        const float4 t = c0 + lane * 4 < cols ? __ldcs((const float4*)(p + c0 + lane * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[0] = t.x;
+        v[1] = t.y;
+        v[2] = t.z;
+        v[3] = t.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = c0 + lane + 32 * j < cols ? __ldcs(p + c0 + lane + 32 * j) : 0.0f;
+    }
+}
+// The same for values that every row reads again (weights): kept in the caches.
+template <bool VEC>
+__device__ __forceinline__ void load_weight(float (&v)[4], const float* __restrict__ p, int c0, int cols, int lane) {
+    if (VEC) {
+        const float4 t = c0 + lane * 4 < cols ? __ldg((const float4*)(p + c0 + lane * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[0] = t.x;
+        v[1] = t.y;
+        v[2] = t.z;
+        v[3] = t.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = c0 + lane + 32 * j < cols ? __ldg(p + c0 + lane + 32 * j) : 0.0f;
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void store_group(float* p, const float (&v)[4], int c0, int cols, int lane) {
+    if (VEC) {
+        if (c0 + lane * 4 < cols) *(float4*)(p + c0 + lane * 4) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c0 + lane + 32 * j < cols) p[c0 + lane + 32 * j] = v[j];
+    }
+}
+
+// Sum over the block's W warps, the same on every thread.
+template <int W>
+__device__ __forceinline__ float block_sum(float v, float* sh, int warp, int lane) {
     v = warp_sum_f(v);
+    if (lane == 0) sh[warp] = v;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = 0.0f;
-    for (int i = 0; i < kThreads / 32; ++i) t += sh[i];
-    return t;
+    return warp_sum_f(lane < W ? sh[lane] : 0.0f);
 }
 
-// One block per row, two passes over it.
-__global__ void __launch_bounds__(kThreads) rmsnorm_row(float* y, uint8_t* q, float* s, float* h, float* rstd,
-                                                        const float* x, const float* res, const float* w, float eps,
-                                                        int64_t cols) {
-    const int64_t row = blockIdx.x, o = row * cols;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float a = 0.0f;
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-        const float v = res ? x[o + c] + res[o + c] : x[o + c];
-        a += v * v;
+struct NormArgs {
+    float* y;
+    uint8_t* q;
+    float* s;
+    float* h;
+    float* rstd;
+    const float* x;
+    const float* res;
+    const float* w;
+    float eps;
+    int cols;
+};
+
+// One group's outputs from its sums t.
+template <bool VEC>
+__device__ __forceinline__ void norm_group(const NormArgs& a, const float (&t)[4], const float (&w)[4], float root,
+                                           int64_t row, int g, int groups, int lane) {
+    const int64_t o = row * a.cols;
+    if (a.h) store_group<VEC>(a.h + o, t, g * 128, a.cols, lane);
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(__fmul_rn(t[j], root), w[j]);
+    if (a.y) store_group<VEC>(a.y + o, v, g * 128, a.cols, lane);
+    if (a.q) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3]))));
+        const float sc = e4m3_scale(top), inv = __frcp_rn(sc);
+        if (lane == 0) a.s[row * groups + g] = sc;
+        const uint32_t b = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+        uint8_t* q = a.q + (row * groups + g) * 128;
+        if (VEC) {
+            *(uint32_t*)(q + lane * 4) = b;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[lane + 32 * j] = (uint8_t)(b >> (8 * j));
+        }
     }
-    const float root = rsqrtf(block_sum(a) / (float)cols + eps);
-    if (rstd && threadIdx.x == 0) rstd[row] = root;
-    const int64_t groups = (cols + 127) / 128;
-    for (int64_t g = warp; g < groups; g += kThreads / 32) {
-        float v[4];
-        uint32_t top = 0;
-        for (int i = 0; i < 4; ++i) {
-            const int64_t c = g * 128 + lane * 4 + i;
-            v[i] = 0.0f;
-            if (c < cols) {
-                const float t = res ? x[o + c] + res[o + c] : x[o + c];
-                if (h) h[o + c] = t;
-                v[i] = t * root * w[c];
-                if (y) y[o + c] = v[i];
+}
+
+// One block of W warps per row, the row held in registers (V groups a warp): one read and one write of
+// every value, bound by HBM where rows abound and by latency (loads, one barrier) where they are few.
+template <int W, int V, bool VEC>
+__global__ void __launch_bounds__(W * 32) rmsnorm_row(const NormArgs a) {
+    __shared__ float sh[W];
+    pdl_begin();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = blockIdx.x, o = row * a.cols;
+    const int groups = (a.cols + 127) >> 7;
+    float t[V][4], w[V][4];
+#pragma unroll
+    for (int i = 0; i < V; ++i) load_group<VEC>(t[i], a.x + o, (warp + i * W) * 128, a.cols, lane);
+    if (a.res) {
+        float u[V][4];
+#pragma unroll
+        for (int i = 0; i < V; ++i) load_group<VEC>(u[i], a.res + o, (warp + i * W) * 128, a.cols, lane);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[i][j] = __fadd_rn(t[i][j], u[i][j]);
+    }
+    if (V <= 2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) load_weight<VEC>(w[i], a.w, (warp + i * W) * 128, a.cols, lane);
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss = fmaf(t[i][j], t[i][j], ss);
+    const float root = rsqrtf(__fdiv_rn(block_sum<W>(ss, sh, warp, lane), (float)a.cols) + a.eps);
+    if (a.rstd && threadIdx.x == 0) a.rstd[row] = root;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int g = warp + i * W;
+        if (g >= groups) break;
+        if (V > 2) load_weight<VEC>(w[i], a.w, g * 128, a.cols, lane);
+        norm_group<VEC>(a, t[i], w[i], root, row, g, groups, lane);
+    }
+}
+
+// Rows that do not fit the registers: the second pass reads the row again (from L2).
+template <bool VEC>
+__global__ void __launch_bounds__(1024) rmsnorm_wide(const NormArgs a) {
+    __shared__ float sh[32];
+    pdl_begin();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = blockIdx.x, o = row * a.cols;
+    const int groups = (a.cols + 127) >> 7;
+    const auto sum = [&](float (&t)[4], int g) {
+        load_group<VEC>(t, a.x + o, g * 128, a.cols, lane);
+        if (a.res) {
+            float u[4];
+            load_group<VEC>(u, a.res + o, g * 128, a.cols, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = __fadd_rn(t[j], u[j]);
+        }
+    };
+    float ss = 0.0f;
+#pragma unroll 4
+    for (int g = warp; g < groups; g += 32) {
+        float t[4];
+        sum(t, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss = fmaf(t[j], t[j], ss);
+    }
+    const float root = rsqrtf(__fdiv_rn(block_sum<32>(ss, sh, warp, lane), (float)a.cols) + a.eps);
+    if (a.rstd && threadIdx.x == 0) a.rstd[row] = root;
+    for (int g = warp; g < groups; g += 32) {
+        float t[4], w[4];
+        sum(t, g);
+        load_weight<VEC>(w, a.w, g * 128, a.cols, lane);
+        norm_group<VEC>(a, t, w, root, row, g, groups, lane);
+    }
+}
+
+// ---- the gradient
+struct BackArgs {
+    float* dx;
+    float* part;  // [grid][cols] sums of dy h rstd over a block's rows, or null
+    const float* dy;
+    const float* h;
+    const float* w;
+    const float* rstd;
+    const float* dh;
+    int64_t rows;
+    int cols;
+};
+
+// W warps go through rows blockIdx.x, + grid, ...; a thread keeps the same columns in every row and so its
+// sums for the weight's gradient in registers.  The next row's dy and h are loaded before the present
+// row's reduction.  Bound by HBM: 12 bytes read and 4 written a value.
+template <int W, int V, bool VEC>
+__global__ void __launch_bounds__(W * 32) rmsnorm_backward_row(const BackArgs a) {
+    __shared__ float sh[2][W];
+    pdl_begin();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const auto base = [&](int i) { return (warp + i * W) * 128; };
+    float sum[V][4], dy[V][4], h[V][4];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[i][j] = 0.0f;
+    int turn = 0;
+    int64_t row = blockIdx.x;
+    float root = __ldg(a.rstd + row);
+#pragma unroll
+    for (int i = 0; i < V; ++i) load_group<VEC>(dy[i], a.dy + row * a.cols, base(i), a.cols, lane);
+#pragma unroll
+    for (int i = 0; i < V; ++i) load_group<VEC>(h[i], a.h + row * a.cols, base(i), a.cols, lane);
+    for (; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const int64_t o = row * a.cols, next = row + gridDim.x;
+        float u[V][4];
+        float along = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float w[4];
+            load_weight<VEC>(w, a.w, base(i), a.cols, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[i][j] = dy[i][j] * w[j];
+                along = fmaf(u[i][j], h[i][j], along);
+                sum[i][j] = fmaf(dy[i][j], h[i][j] * root, sum[i][j]);
             }
-            top = max(top, abs_bits(v[i]));
         }
-        if (q) {
-            const float sc = e4m3_scale(__reduce_max_sync(0xffffffffu, top)), inv = __frcp_rn(sc);
-            if (lane == 0) s[row * groups + g] = sc;
-            *(uint32_t*)(q + (row * groups + g) * 128 + lane * 4) = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+        float g[V][4];  // the residual path's gradient, then the result
+        if (a.dh) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) load_group<VEC>(g[i], a.dh + o, base(i), a.cols, lane);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) g[i][j] = 0.0f;
         }
+        const float next_root = next < a.rows ? __ldg(a.rstd + next) : 0.0f;
+        if (next < a.rows) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) load_group<VEC>(dy[i], a.dy + next * a.cols, base(i), a.cols, lane);
+        }
+        const float f = root * root * __fdiv_rn(block_sum<W>(along, sh[turn], warp, lane), (float)a.cols);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float d = root * fmaf(-h[i][j], f, u[i][j]);
+                g[i][j] = a.dh ? __fadd_rn(g[i][j], d) : d;
+            }
+            store_group<VEC>(a.dx + o, g[i], base(i), a.cols, lane);
+        }
+        if (next < a.rows) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) load_group<VEC>(h[i], a.h + next * a.cols, base(i), a.cols, lane);
+        }
+        root = next_root;
+    }
+    if (a.part) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) store_group<VEC>(a.part + (int64_t)blockIdx.x * a.cols, sum[i], base(i), a.cols, lane);
     }
 }
 
-__global__ void __launch_bounds__(kThreads) rmsnorm_backward_row(float* dx, const float* dy, const float* h,
-                                                                 const float* w, const float* rstd, const float* dh,
-                                                                 int64_t cols) {
-    const int64_t row = blockIdx.x, o = row * cols;
-    float a = 0.0f;
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) a += dy[o + c] * w[c] * h[o + c];
-    const float root = rstd[row], f = root * root * (block_sum(a) / (float)cols);
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-        const float u = root * (dy[o + c] * w[c] - h[o + c] * f);
-        dx[o + c] = dh ? dh[o + c] + u : u;
+// Rows that do not fit: dx in two passes over the row, dw's partial sums by columns over a share of rows.
+template <bool VEC>
+__global__ void __launch_bounds__(1024) rmsnorm_backward_wide(const BackArgs a) {
+    __shared__ float sh[32];
+    pdl_begin();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = blockIdx.x, o = row * a.cols;
+    const int groups = (a.cols + 127) >> 7;
+    const float root = __ldg(a.rstd + row);
+    float along = 0.0f;
+#pragma unroll 2
+    for (int g = warp; g < groups; g += 32) {
+        float dy[4], h[4], w[4];
+        load_group<VEC>(dy, a.dy + o, g * 128, a.cols, lane);
+        load_group<VEC>(h, a.h + o, g * 128, a.cols, lane);
+        load_weight<VEC>(w, a.w, g * 128, a.cols, lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) along = fmaf(dy[j] * w[j], h[j], along);
+    }
+    const float f = root * root * __fdiv_rn(block_sum<32>(along, sh, warp, lane), (float)a.cols);
+#pragma unroll 2
+    for (int g = warp; g < groups; g += 32) {
+        float dy[4], h[4], w[4], t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        load_group<VEC>(dy, a.dy + o, g * 128, a.cols, lane);
+        load_group<VEC>(h, a.h + o, g * 128, a.cols, lane);
+        load_weight<VEC>(w, a.w, g * 128, a.cols, lane);
+        if (a.dh) load_group<VEC>(t, a.dh + o, g * 128, a.cols, lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float d = root * fmaf(-h[j], f, dy[j] * w[j]);
+            t[j] = a.dh ? __fadd_rn(t[j], d) : d;
+        }
+        store_group<VEC>(a.dx + o, t, g * 128, a.cols, lane);
     }
 }
 
-__global__ void __launch_bounds__(kThreads) rmsnorm_backward_weight(float* dw, const float* dy, const float* h,
-                                                                    const float* rstd, int64_t rows, int64_t cols) {
-    const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (c >= cols) return;
-    float a = 0.0f;
-    for (int64_t r = 0; r < rows; ++r) a += dy[r * cols + c] * (h[r * cols + c] * rstd[r]);
-    dw[c] = a;
+__global__ void __launch_bounds__(256) rmsnorm_weight_part(const BackArgs a, int64_t col_blocks, int64_t per) {
+    pdl_begin();
+    const int64_t c = (int64_t)(blockIdx.x % col_blocks) * 256 + threadIdx.x, slice = blockIdx.x / col_blocks;
+    if (c >= a.cols) return;
+    float t = 0.0f;
+    for (int64_t r = slice * per; r < min(slice * per + per, a.rows); ++r)
+        t = fmaf(a.dy[r * a.cols + c], a.h[r * a.cols + c] * __ldg(a.rstd + r), t);
+    a.part[slice * a.cols + c] = t;
+}
+
+// dw = the sum of the partial sums, in their order: 32 columns a block, 8 warps of consecutive parts.
+__global__ void __launch_bounds__(256) rmsnorm_weight_sum(float* __restrict__ dw, const float* __restrict__ part, int parts, int cols) {
+    __shared__ float sh[8][32];
+    pdl_begin();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, per = (parts + 7) / 8;
+    float t = 0.0f;
+    if (c < cols) {
+#pragma unroll 8
+        for (int p = warp * per; p < min(warp * per + per, parts); ++p) t += part[(int64_t)p * cols + c];
+    }
+    sh[warp][lane] = t;
+    __syncthreads();
+    if (warp == 0 && c < cols) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) t += sh[i][lane];
+        dw[c] = t;
+    }
+}
+
+constexpr int kSms = 148;
+constexpr int kWideParts = 64;
+
+// Blocks of the backward pass: as many as run at once.
+int back_warps(int64_t cols) { return cols <= 2048 ? 4 : cols <= 4096 ? 8 : cols <= 8192 ? 16 : 0; }
+int64_t back_blocks(int64_t rows, int64_t cols) {
+    const int w = back_warps(cols);
+    const int64_t n = kSms * (w == 4 ? 4 : w == 8 ? 2 : 1);
+    return rows < n ? rows : n;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <typename K>
+int go(K kern, int64_t grid, int threads, cudaStream_t st, const NormArgs& a) {
+    return (int)launch_dep(kern, dim3((unsigned)grid), dim3((unsigned)threads), 0, st, a);
+}
+template <bool VEC>
+int run_norm(const NormArgs& a, int64_t rows, cudaStream_t st) {
+    const int groups = (a.cols + 127) / 128;
+    // few rows: 32 warps share a row and each holds less of it
+    if (groups > 64 || (rows <= 2 * kSms && groups > 8)) {
+        if (groups <= 32) return go(rmsnorm_row<32, 1, VEC>, rows, 1024, st, a);
+        if (groups <= 64) return go(rmsnorm_row<32, 2, VEC>, rows, 1024, st, a);
+        if (groups <= 128) return go(rmsnorm_row<32, 4, VEC>, rows, 1024, st, a);
+        return go(rmsnorm_wide<VEC>, rows, 1024, st, a);
+    }
+    if (groups <= 8) return go(rmsnorm_row<8, 1, VEC>, rows, 256, st, a);
+    if (groups <= 16) return go(rmsnorm_row<8, 2, VEC>, rows, 256, st, a);
+    if (groups <= 32) return go(rmsnorm_row<8, 4, VEC>, rows, 256, st, a);
+    return go(rmsnorm_row<8, 8, VEC>, rows, 256, st, a);
+}
+
+template <bool VEC>
+int run_back(const BackArgs& a, int64_t blocks, cudaStream_t st) {
+    const dim3 grid((unsigned)blocks);
+    switch (back_warps(a.cols)) {
+        case 4: return (int)launch_dep(rmsnorm_backward_row<4, 4, VEC>, grid, dim3(128), 0, st, a);
+        case 8: return (int)launch_dep(rmsnorm_backward_row<8, 4, VEC>, grid, dim3(256), 0, st, a);
+        case 16: return (int)launch_dep(rmsnorm_backward_row<16, 4, VEC>, grid, dim3(512), 0, st, a);
+        default: return (int)launch_dep(rmsnorm_backward_wide<VEC>, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+    }
 }
 
 }  // namespace
@@ -86,22 +379,36 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_backward_weight(float* dw, c
 extern "C" int mcu_launch_rmsnorm(float* y, uint8_t* q, float* s, float* h, float* rstd, const float* x,
                                   const float* res, const float* w, float eps, int64_t rows, int64_t cols,
                                   cudaStream_t st, int* launches) {
-    rmsnorm_row<<<(unsigned)rows, kThreads, 0, st>>>(y, q, s, h, rstd, x, res, w, eps, cols);
+    const NormArgs a{y, q, s, h, rstd, x, res, w, eps, (int)cols};
     *launches = 1;
-    return (int)cudaGetLastError();
+    if (cols % 4 == 0 && aligned16(x) && aligned16(res) && aligned16(w) && aligned16(y) && aligned16(h)) return run_norm<true>(a, rows, st);
+    return run_norm<false>(a, rows, st);
 }
 
-extern "C" size_t mcu_rmsnorm_backward_scratch_bytes(int64_t, int64_t) { return 0; }
+extern "C" size_t mcu_rmsnorm_backward_scratch_bytes(int64_t rows, int64_t cols) {
+    return (size_t)((back_warps(cols) ? back_blocks(rows, cols) : kWideParts) * cols) * 4;
+}
 
 extern "C" int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy, const float* h, const float* w,
-                                           const float* rstd, const float* dh, int64_t rows, int64_t cols, void*,
+                                           const float* rstd, const float* dh, int64_t rows, int64_t cols, void* scratch,
                                            cudaStream_t st, int* launches) {
+    const BackArgs a{dx, dw ? (float*)scratch : nullptr, dy, h, w, rstd, dh, rows, (int)cols};
     *launches = 0;
-    if (dw) {  // first: dx may be dy or h
-        rmsnorm_backward_weight<<<(unsigned)((cols + kThreads - 1) / kThreads), kThreads, 0, st>>>(dw, dy, h, rstd, rows, cols);
+    int parts = (int)back_blocks(rows, cols), rc = 0;
+    if (dw && !back_warps(cols)) {  // before dx, which may lie over dy or h
+        const int64_t cb = (cols + 255) / 256, per = (rows + kWideParts - 1) / kWideParts;
+        parts = (int)((rows + per - 1) / per);
+        rc = (int)launch_dep(rmsnorm_weight_part, dim3((unsigned)(cb * parts)), dim3(256), 0, st, a, cb, per);
         ++*launches;
     }
-    rmsnorm_backward_row<<<(unsigned)rows, kThreads, 0, st>>>(dx, dy, h, w, rstd, dh, cols);
-    ++*launches;
-    return (int)cudaGetLastError();
+    if (!rc) {
+        rc = cols % 4 == 0 && aligned16(dx) && aligned16(dy) && aligned16(h) && aligned16(w) && aligned16(dh) ? run_back<true>(a, parts, st)
+                                                                                                               : run_back<false>(a, parts, st);
+        ++*launches;
+    }
+    if (!rc && dw) {
+        rc = (int)launch_dep(rmsnorm_weight_sum, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, st, dw, (const float*)a.part, parts, (int)cols);
+        ++*launches;
+    }
+    return rc;
 }
