@@ -11,6 +11,7 @@
 #include <cfloat>
 #include <cstdint>
 #include "mcu_kernels.h"
+#include "mcu_launch.cuh"
 #include "mcu_lm.cuh"
 
 namespace cg = cooperative_groups;
@@ -29,124 +30,146 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
-// The order of the alternatives as one integer: larger logit first, then lower column; NaN above
-// everything, -0 as +0.  0 stands for no element.
-__device__ __forceinline__ uint64_t rank_key(float v, uint32_t col) {
-    uint32_t b = __float_as_uint(v + 0.0f);
-    b = v != v ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-    return (uint64_t)b << 32 | (0xFFFFFFFFu - col);
+// The order of logits as an integer (NaN above everything, -0 as +0), and with the column below it, so
+// that of equal logits the lower column comes first.  0 stands for no element.
+__device__ __forceinline__ uint32_t order_of(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return v != v ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float key_value(uint64_t key) {
-    const uint32_t b = (uint32_t)(key >> 32);
-    return __uint_as_float((b & 0x80000000u) ? b & 0x7FFFFFFFu : ~b);
-}
+__device__ __forceinline__ uint64_t rank_key(uint32_t order, uint32_t col) { return (uint64_t)order << 32 | (0xFFFFFFFFu - col); }
+constexpr uint32_t kOrderInf = 0xFF800000u;  // of +inf
+__device__ __forceinline__ float order_value(uint32_t b) { return __uint_as_float((b & 0x80000000u) ? b & 0x7FFFFFFFu : ~b); }
+__device__ __forceinline__ float key_value(uint64_t key) { return order_value((uint32_t)(key >> 32)); }
 
-// Four logits of a row whose first one lies `off` floats past a 16-byte boundary: vector vi holds the
-// elements 4 vi - off .. + 3.  Only the first and the last one reach past the row; their elements there
-// are -inf, and nothing outside the row is read.
-__device__ __forceinline__ float4 load_logits(const float* p, int64_t vi, int64_t nvec, int off, int64_t cols) {
-    const int64_t c = vi * 4 - off;
-    if (c >= 0 && c + 4 <= cols) return __ldcs((const float4*)(p + c));
+// A row whose first logit lies `off` floats past a 16-byte boundary, as vectors of four: vector vi holds
+// the elements 4 vi - off .. + 3.  Only the first and the last one may reach past the row; their elements
+// there are -inf, and nothing outside the row is read.
+struct Row {
+    const float* p;
+    int64_t cols;
+    int off;
+    int full0, full1;  // vectors that lie inside the row
+};
+__device__ __forceinline__ Row row_of(const float* p, int64_t cols) {
+    const int off = (int)((uintptr_t)p >> 2) & 3;
+    return Row{p, cols, off, off ? 1 : 0, (int)((off + cols) >> 2)};
+}
+__device__ __forceinline__ int vectors_of(const Row& r) { return (int)((r.off + r.cols + 3) >> 2); }
+__device__ __noinline__ float4 load_edge(const float* p, int64_t cols, int64_t c) {
     float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    if (vi >= nvec) return v;
     if (c >= 0 && c < cols) v.x = p[c];
     if (c + 1 >= 0 && c + 1 < cols) v.y = p[c + 1];
     if (c + 2 >= 0 && c + 2 < cols) v.z = p[c + 2];
     if (c + 3 >= 0 && c + 3 < cols) v.w = p[c + 3];
     return v;
 }
+// The thread's kVecs vectors of the chunk of T * kVecs at `base`, those from v1 on as -inf.
+template <int T>
+__device__ __forceinline__ void load_chunk(float4 (&v)[kVecs], const Row& r, int base, int v1) {
+    const int first = base + (int)threadIdx.x;
+    const float4* q = (const float4*)(r.p - r.off) + first;
+    if (base >= r.full0 && base + T * kVecs <= min(r.full1, v1)) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) v[i] = __ldcs(q + i * T);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+        const int vi = first + i * T;
+        if (vi >= v1) v[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        else if (vi >= r.full0 && vi < r.full1) v[i] = __ldcs(q + i * T);
+        else v[i] = load_edge(r.p, r.cols, (int64_t)vi * 4 - r.off);
+    }
+}
 
 struct Part {
     float m;
     double s, t;
 };
-__device__ __forceinline__ Part join(const Part& a, const Part& b) {
-    const float m = fmaxf(a.m, b.m);
-    // (a part of nothing has s = t = 0 and the lowest maximum; the bounded distance keeps 0 * distance at 0)
-    const float ca = fmaxf(a.m - m, kFar), cb = fmaxf(b.m - m, kFar);
-    const double ea = (double)expf(ca), eb = (double)expf(cb);
-    // a maximum of infinity, or NaN terms, leave s NaN
-    return Part{m, a.s * ea + b.s * eb, (a.t + ca * a.s) * ea + (b.t + cb * b.s) * eb};
+// A warp's parts as one, on every lane: all are brought to the largest maximum, then added.  (A part of
+// nothing has s = t = 0 and the lowest maximum; the bounded distance keeps 0 * distance at 0.)
+__device__ __forceinline__ Part join_warp(Part a) {
+    float m = a.m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float c = fmaxf(a.m - m, kFar);
+    const double e = (double)expf(c);
+    a.t = (a.t + (double)c * a.s) * e;
+    a.s *= e;
+    a.m = m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+    }
+    return a;
 }
 
-// Best 32 of a warp's 32 keys in descending order over the lanes, and of two such lists.
-__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t min64(uint64_t a, uint64_t b) { return a < b ? a : b; }
-__device__ __forceinline__ uint64_t order_bitonic(uint64_t k, int lane) {
+// Bitonic networks over a warp's lanes, descending; K is a 32-bit order or a 64-bit key.
+template <typename K>
+__device__ __forceinline__ K order_bitonic(K k, int lane) {
 #pragma unroll
     for (int j = 16; j; j >>= 1) {
-        const uint64_t o = __shfl_xor_sync(0xffffffffu, k, j);
-        k = (lane & j) ? min64(k, o) : max64(k, o);
+        const K o = __shfl_xor_sync(0xffffffffu, k, j);
+        k = ((lane & j) != 0) == (k > o) ? o : k;
     }
     return k;
 }
-__device__ __forceinline__ uint64_t sort32(uint64_t k, int lane) {
+template <typename K>
+__device__ __forceinline__ K sort32(K k, int lane) {
 #pragma unroll
     for (int size = 2; size < 32; size <<= 1)
 #pragma unroll
         for (int j = size >> 1; j; j >>= 1) {
-            const uint64_t o = __shfl_xor_sync(0xffffffffu, k, j);
-            const bool up = (lane & size) != 0;  // every second run ascends
-            k = ((lane & j) != 0) != up ? min64(k, o) : max64(k, o);
+            const K o = __shfl_xor_sync(0xffffffffu, k, j);
+            // every second run ascends
+            k = (((lane & j) != 0) != ((lane & size) != 0)) == (k > o) ? o : k;
         }
     return order_bitonic(k, lane);
 }
 // b reversed against a: the larger of each pair are the best 32 of both, as a bitonic sequence.
-__device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
-    return order_bitonic(max64(a, __shfl_sync(0xffffffffu, b, 31 - lane)), lane);
+template <typename K>
+__device__ __forceinline__ K merge32(K a, K b, int lane) {
+    b = __shfl_sync(0xffffffffu, b, 31 - lane);
+    return order_bitonic(a > b ? a : b, lane);
 }
 
-// The block's candidates: everything pushed since the last selection and the best of before.
+// The candidates of a block: each warp fills a buffer of its own without asking the others, cut down to
+// its best 32 when a chunk leaves more than kKeep; at the end the warps' rests meet in the pool.
+constexpr int kKeep = 64;
 template <int T>
 struct Candidates {
-    static constexpr int kChunk = T * kVecs * 4;
-    static constexpr int kKeep = 512;  // selection starts when more are held after a chunk
-    uint64_t key[kKeep + kChunk];
-    uint64_t list[T / 32][32];
-    int count;
+    static constexpr int kWarps = T / 32;
+    uint64_t key[kWarps][kKeep + 32 * kVecs * 4];
+    uint64_t pool[kWarps * kKeep];
+    uint64_t list[kWarps][32];
+    uint32_t group[64];  // maxima of 64 groups of threads over the first chunk
+    uint32_t least;      // orders below it are no candidates: the first chunk's bound, raised by full buffers
+    int pooled;
 };
 
-// Joins the warps' sorted lists in shared memory; every thread gets lane's entry of the best 32.
-template <int T>
-__device__ uint64_t join_lists(uint64_t mine, uint64_t (*list)[32], int warp, int lane) {
-    __syncthreads();
-    list[warp][lane] = mine;
-#pragma unroll
-    for (int n = T / 64; n; n >>= 1) {
-        __syncthreads();
-        if (warp < n) {
-            mine = merge32(list[warp][lane], list[warp + n][lane], lane);
-            __syncwarp();
-            list[warp][lane] = mine;
-        }
-    }
-    __syncthreads();
-    return list[0][lane];
-}
-
-// The best 32 of the held candidates, sorted over the lanes of every warp.
-template <int T>
-__device__ uint64_t select_best(Candidates<T>& c, int warp, int lane) {
-    const int n = c.count;
+// The best 32 of n keys, sorted over the lanes of the calling warp.
+__device__ __forceinline__ uint64_t best_of(const uint64_t* key, int n, int lane) {
     uint64_t best = 0;
-    for (int i = warp * 32; i < n; i += T) {
-        const uint64_t k = i + lane < n ? c.key[i + lane] : 0;
+    for (int i = 0; i < n; i += 32) {
+        const uint64_t k = i + lane < n ? key[i + lane] : 0;
         // (a batch with nothing above the list's last entry changes nothing)
-        if (i < T || __any_sync(0xffffffffu, k > __shfl_sync(0xffffffffu, best, 31))) best = merge32(best, sort32(k, lane), lane);
+        if (!i) best = sort32(k, lane);
+        else if (__any_sync(0xffffffffu, k > __shfl_sync(0xffffffffu, best, 31))) best = merge32(best, sort32(k, lane), lane);
     }
-    return join_lists<T>(best, c.list, warp, lane);
+    return best;
 }
 
 // One cluster of `parts` CTAs of T threads per row; each streams its part of the row once, 16 logits a
 // thread and chunk, the next chunk's loads issued before the present one is worked on.
 //
-// Bound by HBM (4 bytes a logit) while rows abound: about 8 instructions a logit against 25 that the
-// SMs can issue in a logit's time.  Measured figures stand in the table of the design notes' section on
-// these operators.
-// Candidates: the k-th best of the first chunk's T per-thread maxima bounds the row's k-th best from
-// below, so the first chunk pushes about k keys and later chunks k ln(n / chunk) in all; a chunk's
-// elements are looked at one by one only where its maximum passes the bound.  The pushes' order does
-// not matter: keys are distinct and the selection sorts them.
+// Candidates: the top-th largest of 64 group maxima of the first chunk is a lower bound of the row's
+// top-th logit, so that about top (1.1 to 1.4 times) of the first chunk's logits pass it, and top / 8192
+// of all later ones (T = 512): a warp looks at single elements only where the maximum of a lane's 16
+// passes.  Later elements have higher columns than the at least `top` that reached the bound in the
+// first chunk, so they have to exceed it; a bound that a warp's full buffer gives has to be reached only,
+// since another warp may still be at lower columns.  The order in which candidates are found does not
+// matter: keys are distinct and sorted at the end.
 template <int T, bool TOP>
 __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__ logp, float* __restrict__ lse,
                                                              float* __restrict__ entropy, float* __restrict__ top_logp,
@@ -162,21 +185,18 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
     const int64_t row = blockIdx.x / parts;
     const int rank = blockIdx.x % parts;
     if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    const float* p = x + row * x_s1;
-    const int off = (int)((uintptr_t)p >> 2) & 3;
-    const int64_t nvec = (off + cols + 3) >> 2, per = (nvec + parts - 1) / parts;
-    const int64_t v0 = rank * per, v1 = min(v0 + per, nvec);
-    if (TOP && threadIdx.x == 0) cand.count = 0;
+    pdl_begin();
+    const Row r = row_of(x + row * x_s1, cols);
+    const int nvec = vectors_of(r), per = (nvec + parts - 1) / parts;
+    const int v0 = min(rank * per, nvec), v1 = min(v0 + per, nvec);
+    if (TOP && threadIdx.x == 0) cand.pooled = 0;
 
     float m = -FLT_MAX, s = 0.0f, t = 0.0f;
-    float bound = -INFINITY;  // later chunks push what is not at most this
+    int held = 0;         // keys in this warp's buffer
+    uint32_t exceed = 0;  // the least order of a candidate after the first chunk
     float4 next[kVecs];
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-        const int64_t vi = v0 + i * T + threadIdx.x;
-        next[i] = load_logits(p, vi < v1 ? vi : nvec, nvec, off, cols);
-    }
-    for (int64_t base = v0; base < v1; base += T * kVecs) {
+    load_chunk<T>(next, r, v0, v1);
+    for (int base = v0; base < v1; base += T * kVecs) {
         float v[kVecs * 4];
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
@@ -185,13 +205,7 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
             v[4 * i + 2] = next[i].z;
             v[4 * i + 3] = next[i].w;
         }
-        if (base + T * kVecs < v1) {
-#pragma unroll
-            for (int i = 0; i < kVecs; ++i) {
-                const int64_t vi = base + (kVecs + i) * T + threadIdx.x;
-                next[i] = load_logits(p, vi < v1 ? vi : nvec, nvec, off, cols);
-            }
-        }
+        if (base + T * kVecs < v1) load_chunk<T>(next, r, base + T * kVecs, v1);
         float cm = v[0];
 #pragma unroll
         for (int i = 1; i < kVecs * 4; ++i) cm = fmaxf(cm, v[i]);
@@ -209,77 +223,107 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
             t = fmaf(e, fmaxf(d, kFar), t);
         }
         s += cs;
-        if (TOP) {
-            // (columns of the chunk's elements; a NaN shows in cs)
-            const int64_t c0 = (base + threadIdx.x) * 4 - off;
-            bool over = false;
+        if constexpr (TOP) {
+            const uint32_t c0 = (uint32_t)(base + (int)threadIdx.x) * 4 - r.off;  // column of v[0]
+            const auto push = [&](bool yes, float value, int i) {
+                const uint32_t who = __ballot_sync(0xffffffffu, yes);
+                if (yes)
+                    cand.key[warp][held + __popc(who & ((1u << lane) - 1))] =
+                        rank_key(order_of(value), c0 + (i >> 2) * (T * 4) + (i & 3));
+                held += __popc(who);
+            };
             if (base == v0) {
-                uint64_t mine = 0;
-#pragma unroll
-                for (int i = 0; i < kVecs * 4; ++i) {
-                    const int64_t c = c0 + (i >> 2) * (T * 4) + (i & 3);
-                    if (c >= 0 && c < cols && base + (i >> 2) * T + threadIdx.x < v1) mine = max64(mine, rank_key(v[i], (uint32_t)c));
-                }
-                const uint64_t list = join_lists<T>(sort32(mine, lane), cand.list, warp, lane);
-                const uint64_t least = __shfl_sync(0xffffffffu, list, top - 1);
-                bound = key_value(least);
-                if (bound != bound) bound = INFINITY;
-                if (least == 0) bound = -INFINITY;
-                if (mine >= least && mine) {
+                // bit i: element i is one of the part's (not so past an edge of the row or the part)
+                uint32_t inside = 0xFFFF;
+                if (base < r.full0 || base + T * kVecs > min(r.full1, v1)) {
+                    inside = 0;
 #pragma unroll
                     for (int i = 0; i < kVecs * 4; ++i) {
-                        const int64_t c = c0 + (i >> 2) * (T * 4) + (i & 3);
-                        if (c >= 0 && c < cols && base + (i >> 2) * T + threadIdx.x < v1) {
-                            const uint64_t k = rank_key(v[i], (uint32_t)c);
-                            if (k >= least) cand.key[atomicAdd(&cand.count, 1)] = k;
-                        }
+                        const int vi = base + (i >> 2) * T + (int)threadIdx.x;
+                        const int64_t c = (int64_t)vi * 4 - r.off + (i & 3);
+                        inside |= (vi < v1 && c >= 0 && c < cols ? 1u : 0u) << i;
                     }
                 }
-            } else {
-                if (!(cm <= bound) || cs != cs) {
+                uint32_t big = inside == 0xFFFF && cs == cs ? order_of(cm) : 0;
+                if (inside != 0xFFFF || cs != cs) {
 #pragma unroll
                     for (int i = 0; i < kVecs * 4; ++i)
-                        if (!(v[i] <= bound)) {  // (elements past the row are -inf)
-                            const int at = atomicAdd(&cand.count, 1);
-                            cand.key[at] = rank_key(v[i], (uint32_t)(c0 + (i >> 2) * (T * 4) + (i & 3)));
-                            over |= at >= Candidates<T>::kKeep;
-                        }
+                        if (inside >> i & 1) big = max(big, order_of(v[i]));
                 }
-                if (__syncthreads_or(over)) {
-                    const uint64_t best = select_best<T>(cand, warp, lane);
-                    if (warp == 0) {
-                        cand.key[lane] = best;
-                        if (lane == 0) cand.count = 32;
+#pragma unroll
+                for (int o = 1; o < T / 64; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+                if (threadIdx.x % (T / 64) == 0) cand.group[threadIdx.x / (T / 64)] = big;
+                __syncthreads();
+                if (warp == 0) {
+                    const uint32_t list = merge32(sort32(cand.group[lane], lane), sort32(cand.group[lane + 32], lane), lane);
+                    const uint32_t least = __shfl_sync(0xffffffffu, list, top - 1);
+                    if (lane == 0) cand.least = least;
+                }
+                __syncthreads();
+                const uint32_t least = cand.least;
+                if (__any_sync(0xffffffffu, big >= least)) {
+#pragma unroll
+                    for (int i = 0; i < kVecs * 4; ++i) {
+                        const bool yes = (inside >> i & 1) && order_of(v[i]) >= least;
+                        if (__any_sync(0xffffffffu, yes)) push(yes, v[i], i);
                     }
-                    bound = key_value(__shfl_sync(0xffffffffu, best, top - 1));
-                    if (bound != bound) bound = INFINITY;
-                    __syncthreads();
                 }
+                exceed = least + (least < kOrderInf);
+            } else {
+                // as a logit, so that one comparison finds candidates and NaN; +inf where only NaN are above
+                const float least = order_value(min(max(exceed, *(volatile uint32_t*)&cand.least), kOrderInf));
+                if (__any_sync(0xffffffffu, !(cm < least) || cs != cs)) {
+#pragma unroll
+                    for (int i = 0; i < kVecs * 4; ++i) {  // (elements past the row are -inf, below any bound here)
+                        const bool yes = !(v[i] < least);
+                        if (__any_sync(0xffffffffu, yes)) push(yes, v[i], i);
+                    }
+                }
+            }
+            if (held > kKeep) {
+                __syncwarp();
+                const uint64_t best = best_of(cand.key[warp], held, lane);
+                __syncwarp();
+                cand.key[warp][lane] = best;
+                held = 32;
+                const uint32_t o = (uint32_t)(__shfl_sync(0xffffffffu, best, top - 1) >> 32);
+                if (lane == 0) atomicMax(&cand.least, o);
+                __syncwarp();
             }
         }
     }
 
-    Part mine{m, (double)s, (double)t};
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const Part b{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o),
-                     __shfl_xor_sync(0xffffffffu, mine.t, o)};
-        mine = join(mine, b);
-    }
+    Part mine = join_warp(Part{m, (double)s, (double)t});
     if (lane == 0) sh_part[warp] = mine;
-    __syncthreads();
     uint64_t list = 0;
-    if (TOP) list = select_best<T>(cand, warp, lane);
-    if (warp == 0) {
-        mine = lane < T / 32 ? sh_part[lane] : Part{-FLT_MAX, 0.0, 0.0};
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const Part b{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o),
-                         __shfl_xor_sync(0xffffffffu, mine.t, o)};
-            mine = join(mine, b);
+    if constexpr (TOP) {
+        __syncwarp();
+        int at = 0;
+        if (lane == 0 && held) at = atomicAdd(&cand.pooled, held);
+        at = __shfl_sync(0xffffffffu, at, 0);
+        for (int i = lane; i < held; i += 32) cand.pool[at + i] = cand.key[warp][i];
+        __syncthreads();
+        const int n = cand.pooled, lists = (n + 31) / 32;  // a list per 32 keys
+        if (warp < lists) {
+            for (int i = warp * 32; i < n; i += T) {
+                const uint64_t k = sort32(i + lane < n ? cand.pool[i + lane] : 0, lane);
+                list = i == warp * 32 ? k : merge32(list, k, lane);
+            }
+            cand.list[warp][lane] = list;
         }
+        for (int k = min(lists, T / 32); k > 1; k = (k + 1) / 2) {  // the upper half of the lists into the lower
+            __syncthreads();
+            const int h = (k + 1) / 2;
+            if (warp + h < k) {
+                list = merge32(list, cand.list[warp + h][lane], lane);
+                cand.list[warp][lane] = list;
+            }
+        }
+    } else {
+        __syncthreads();
     }
-    if (parts > 1) {  // the parts meet in the first CTA, joined in their order
+    if (warp == 0) mine = join_warp(lane < T / 32 ? sh_part[lane] : Part{-FLT_MAX, 0.0, 0.0});
+    if (parts > 1) {  // the parts meet in the first CTA
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA of the cluster runs
         cg::cluster_group cluster = cg::this_cluster();
         if (warp == 0) {
@@ -288,12 +332,18 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (rank) return;
-        if (warp == 0) {
-            mine = peer_part[0];
-            for (int i = 1; i < parts; ++i) mine = join(mine, peer_part[i]);
-            if (TOP)
-                for (int i = 1; i < parts; ++i) list = merge32(list, peer_list[i][lane], lane);
+        if constexpr (TOP) {
+            if (warp < parts) list = peer_list[warp][lane];
+            for (int k = parts; k > 1; k = (k + 1) / 2) {
+                const int h = (k + 1) / 2;
+                if (warp + h < k) {
+                    list = merge32(list, peer_list[warp + h][lane], lane);
+                    peer_list[warp][lane] = list;
+                }
+                __syncthreads();
+            }
         }
+        if (warp == 0) mine = join_warp(lane < parts ? peer_part[lane] : Part{-FLT_MAX, 0.0, 0.0});
     }
     if (warp) return;
     const bool empty = mine.s == 0.0;  // nothing but -inf
@@ -303,7 +353,7 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
         if (entropy) entropy[row] = empty ? 0.0f : (float)(ln - mine.t / mine.s);
         if (logp) {
             const int32_t i = id[row];
-            logp[row] = i < 0 ? 0.0f : i >= cols ? __int_as_float(0x7FC00000) : empty ? -INFINITY : (float)((double)p[i] - mine.m - ln);
+            logp[row] = i < 0 ? 0.0f : i >= cols ? __int_as_float(0x7FC00000) : empty ? -INFINITY : (float)((double)r.p[i] - mine.m - ln);
         }
     }
     if (TOP && lane < top) {
@@ -322,6 +372,7 @@ __global__ void __launch_bounds__(kBackThreads) logprobs_backward(float* dx, con
                                                                   const float* __restrict__ g_logp,
                                                                   const float* __restrict__ g_entropy, int64_t cols,
                                                                   int64_t x_s1, int64_t dx_s1, int64_t chunks) {
+    pdl_begin();
     const int64_t row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
     const float* p = x + row * x_s1;
     float* q = dx + row * dx_s1;
@@ -365,16 +416,18 @@ int run_rows(float* logp, float* lse, float* entropy, float* top_logp, int32_t* 
         if (e != cudaSuccess) return (int)e;
     }
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)parts;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)parts;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(rows * parts));
     cfg.blockDim = dim3(T);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = parts > 1 ? 1 : 0;
+    cfg.numAttrs = parts > 1 ? 2 : 1;
     return (int)cudaLaunchKernelEx(&cfg, kern, logp, lse, entropy, top_logp, top_id, x, id, cols, x_s1, top, parts);
 }
 
@@ -399,8 +452,7 @@ extern "C" int mcu_launch_logprobs_backward(float* dx, const float* x, const int
                                             int* launches) {
     const int64_t chunks = (cols + 3 + kBackThreads * kBackVecs * 4 - 1) / (kBackThreads * kBackVecs * 4);
     if (rows * chunks > 0x7fffffff) return (int)cudaErrorInvalidValue;
-    logprobs_backward<<<(unsigned)(rows * chunks), kBackThreads, 0, st>>>(dx, x, id, lse, entropy, g_logp, g_entropy, cols,
-                                                                          x_s1, dx_s1, chunks);
     *launches = 1;
-    return (int)cudaGetLastError();
+    return (int)launch_dep(logprobs_backward, dim3((unsigned)(rows * chunks)), dim3(kBackThreads), 0, st, dx, x, id, lse, entropy,
+                           g_logp, g_entropy, cols, x_s1, dx_s1, chunks);
 }
