@@ -66,6 +66,42 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
                  : "memory");
 }
 
+// One lane of a converged warp.  The narrow kernel's roles run as whole warps and elect the lane only around
+// the issue, so that waits, loop and descriptors stay warp-uniform: with a branch on the lane number around
+// the role each MMA took about 80 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// Whole-warp bounded waits on one or two phases, polled by one lane (a poll by 32 lanes takes twice as
+// long), which looks once without blocking first: by then the phase is usually complete.
+__device__ __forceinline__ bool mbar_ready(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
+    uint32_t ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = mbar_ready(bar, parity) || mbar_wait(bar, parity, ab, code);
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+__device__ __forceinline__ bool warp_wait2(uint64_t* bar0, uint32_t parity0, uint64_t* bar1, uint32_t parity1, const Abort& ab, int code) {
+    uint32_t ok = 1;
+    if ((threadIdx.x & 31) == 0) {
+        const bool r0 = mbar_ready(bar0, parity0), r1 = mbar_ready(bar1, parity1);
+        if (!r0) ok = mbar_wait(bar0, parity0, ab, code);
+        if (!r1 && ok) ok = mbar_wait(bar1, parity1, ab, code + 1);
+    }
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
 __device__ __forceinline__ void bar_named(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // On a give-up: the loads that this thread issued (up to load `it`) have to land before the block ends.
@@ -302,21 +338,25 @@ __global__ void __maxnreg__(kPairLaunch)
 }
 
 // ---- few rows of x: one CTA per 128 rows of y (the MMA's rows) and BN rows of x, K split over a cluster
+constexpr int kNarrowAcc = 4;     // accumulators, so that the MMAs run ahead of the epilogue
+constexpr int kNarrowPanel = 16;  // groups of x's scales staged at a time
+
 template <int BN>
 struct NarrowCfg {
     static constexpr int A = 128 * 128, B = BN * 128, STAGE = A + B;
-    static constexpr int STAGES = BN <= 16 ? 6 : BN <= 32 ? 5 : BN <= 64 ? 4 : 6;  // two CTAs per SM up to BN = 64
-    static constexpr int PER_SM = BN <= 64 ? 2 : 1;
+    static constexpr int STAGES = BN == 32 ? 5 : 6;
+    static constexpr int PER_SM = BN <= 32 ? 2 : 1;
+    static constexpr int EPI = BN >= 128 ? 16 : 4;  // epilogue warps: four quadrants of lanes, 16 or 32 columns each
+    static constexpr int WC = BN * 4 / EPI;       // columns of a warp
+    static constexpr int THREADS = 64 + 32 * EPI;
     static constexpr int PANEL = STAGES * STAGE;  // kNarrowPanel x BN scales of x
     static constexpr int BARS = PANEL + 16 * BN * 4;
     static constexpr int SMEM = BARS + 512 + 1024;
-    static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr int COLS = kNarrowAcc * BN;
     static_assert(PER_SM * SMEM <= 227 * 1024 && 128 * BN * 4 <= STAGES * STAGE, "must fit shared memory");
 };
-constexpr int kNarrowPanel = 16;  // groups of x's scales staged at a time
-
 template <int BN, bool YROW>
-__global__ void __launch_bounds__(192, NarrowCfg<BN>::PER_SM)
+__global__ void __launch_bounds__(NarrowCfg<BN>::THREADS, NarrowCfg<BN>::PER_SM)
     gemm_e4m3_narrow(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
                      const float* __restrict__ xs, const float* __restrict__ ys, float* __restrict__ r, int M, int N, int G,
                      int parts, int per, int* status) {
@@ -326,11 +366,11 @@ __global__ void __launch_bounds__(192, NarrowCfg<BN>::PER_SM)
     uint64_t* full = (uint64_t*)(smem + C::BARS);
     uint64_t* empty = full + C::STAGES;
     uint64_t* acc_full = empty + C::STAGES;
-    uint64_t* acc_empty = acc_full + 2;
-    uint64_t* drain = acc_empty + 2;
+    uint64_t* acc_empty = acc_full + kNarrowAcc;
+    uint64_t* drain = acc_empty + kNarrowAcc;
     uint32_t* tmem_slot = (uint32_t*)(drain + 1);
     volatile int* gave_up = (volatile int*)(tmem_slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int mt = (M + BN - 1) / BN;
     const int part = blockIdx.x % parts, tile = blockIdx.x / parts;
     const int m0 = tile % mt * BN, n0 = tile / mt * 128;
@@ -341,9 +381,9 @@ __global__ void __launch_bounds__(192, NarrowCfg<BN>::PER_SM)
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int a = 0; a < 2; ++a) {
+        for (int a = 0; a < kNarrowAcc; ++a) {
             mbar_init(&acc_full[a], 1);
-            mbar_init(&acc_empty[a], 4);
+            mbar_init(&acc_empty[a], C::EPI);
         }
         mbar_init(drain, 1);
         *gave_up = 0;
@@ -358,96 +398,112 @@ __global__ void __launch_bounds__(192, NarrowCfg<BN>::PER_SM)
     tc_fence_after();
     pdl_begin();
     const uint32_t tmem = *tmem_slot;
-    float sum[BN];  // this lane's row of y against BN rows of x
     bool ok = true;
 
-    if (warp == 0) {
-        if (lane == 0) {  // ---- TMA producer
-            uint32_t it = 0;
-            for (int g = g0; g < g1; ++g, ++it) {
-                const uint32_t s = it % C::STAGES;
-                if (!(ok = mbar_wait(&empty[s], (it / C::STAGES & 1) ^ 1, ab, 15))) break;
+    if (warp == 0) {  // ---- TMA producer
+        uint32_t s = 0, phase = 1;
+        for (int g = g0; g < g1; ++g) {
+            if (!(ok = warp_wait(&empty[s], phase, ab, 15))) break;
+            if (elect_one()) {
                 mbar_expect_tx(&full[s], C::STAGE);
                 tma_load_2d(&map_y, &full[s], smem + s * C::STAGE, g * 128, n0);
                 tma_load_2d(&map_x, &full[s], smem + s * C::STAGE + C::A, g * 128, m0);
             }
-            if (!ok) drain_loads<C::STAGES>(full, it);
+            __syncwarp();
+            if (++s == C::STAGES) s = 0, phase ^= 1;
         }
-    } else if (warp == 1) {
-        if (lane == 0) {  // ---- MMA issuer
-            constexpr uint32_t idesc = idesc_f8(128, BN);
-            for (uint32_t it = 0; it < (uint32_t)ng; ++it) {
-                const uint32_t s = it % C::STAGES, b = it & 1;
-                if (!(ok = mbar_wait(&acc_empty[b], (it >> 1 & 1) ^ 1, ab, 16))) break;
-                if (!(ok = mbar_wait(&full[s], it / C::STAGES & 1, ab, 17))) break;
-                tc_fence_after();
-                const uint32_t base = smem_u32(smem + s * C::STAGE);
+        // (a producer that gives up has at most the ring's loads in flight: they land before the block ends)
+        if (!ok && lane == 0)
+            for (int k = 0; k < C::STAGES; ++k)
+                for (uint32_t i = 0; i < kWaitLimit && !mbar_test(&full[k], k < (int)s ? phase ^ 1 : phase); ++i) __nanosleep(64);
+    } else if (warp == 1) {  // ---- MMA issuer
+        constexpr uint32_t idesc = idesc_f8(128, BN);
+        const uint64_t first = sw_desc<128>(smem_u32(smem));
+        uint32_t s = 0, phase = 0;
+        for (uint32_t it = 0; it < (uint32_t)ng; ++it) {
+            const uint32_t b = it % kNarrowAcc, ap = it / kNarrowAcc & 1;
+            if (!(ok = warp_wait2(&acc_empty[b], ap ^ 1, &full[s], phase, ab, 16))) break;
+            tc_fence_after();
+            const uint64_t dy = first + s * (C::STAGE >> 4), dx = dy + (C::A >> 4);
+            if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_f8(tmem + b * BN, sw_desc<128>(base + k * 32), sw_desc<128>(base + C::A + k * 32), idesc, k);
-                umma_commit(&empty[s]);
+                for (int k = 0; k < 4; ++k) umma_f8(tmem + b * BN, dy + k * 2, dx + k * 2, idesc, k);
                 umma_commit(&acc_full[b]);
+                umma_commit(&empty[s]);
             }
+            __syncwarp();
+            if (++s == C::STAGES) s = 0, phase ^= 1;
         }
-    } else {  // ---- epilogue: lane = row of y
-        const int q = warp & 3, tid = threadIdx.x - 64;
+    } else {  // ---- epilogue: lane = row of y, warps 6.. the second half of the columns
+        const int q = warp & 3, col = ((warp - 2) >> 2) * C::WC, tid = threadIdx.x - 64;
         const int n = n0 + q * 32 + lane;
         const float* py = ys + (int64_t)(YROW ? min(n, N - 1) : n0 >> 7) * G + g0;
         float* panel = (float*)(smem + C::PANEL);
+        float sum[C::WC];  // this lane's row of y against the warp's rows of x
 #pragma unroll
-        for (int j = 0; j < BN; ++j) sum[j] = 0.0f;
-        float ay = ng > 0 ? __ldg(py) : 0.0f;
-        for (uint32_t it = 0; it < (uint32_t)ng; ++it) {
-            const uint32_t b = it & 1;
-            if ((it & (kNarrowPanel - 1)) == 0) {  // x's scales: BN rows x 16 groups
-                if (it) bar_named(1, 128);
-                for (int i = tid; i < BN * kNarrowPanel; i += 128) {
-                    const int m = m0 + i / kNarrowPanel, g = g0 + (int)it + i % kNarrowPanel;
-                    panel[i % kNarrowPanel * BN + i / kNarrowPanel] = m < M && g < g1 ? __ldg(xs + (int64_t)m * G + g) : 0.0f;
-                }
-                bar_named(1, 128);
+        for (int j = 0; j < C::WC; ++j) sum[j] = 0.0f;
+        // x's scales, BN rows x 16 groups at a time (a block's scale of y already multiplied in), the next
+        // panel's values fetched one panel ahead
+        constexpr int PV = BN * kNarrowPanel / (32 * C::EPI);
+        float ahead[PV];
+        const auto fetch = [&](int it) {
+#pragma unroll
+            for (int i = 0; i < PV; ++i) {
+                const int e = tid + i * 32 * C::EPI, m = m0 + e / kNarrowPanel, g = it + e % kNarrowPanel;
+                const bool in = m < M && g < ng;
+                ahead[i] = in ? __ldg(xs + (int64_t)m * G + g0 + g) : 0.0f;
+                if (!YROW && in) ahead[i] = __fmul_rn(ahead[i], __ldg(py + g));
             }
-            const float ny = it + 1 < (uint32_t)ng ? __ldg(py + it + 1) : 0.0f;
-            ok &= mbar_wait(&acc_full[b], it >> 1 & 1, ab, 18);
+        };
+        fetch(0);
+        float ay = YROW && ng > 0 ? __ldg(py) : 0.0f;
+        bool ready = false;
+        for (uint32_t it = 0; it < (uint32_t)ng; ++it) {
+            const uint32_t b = it % kNarrowAcc, ap = it / kNarrowAcc & 1;
+            if ((it & (kNarrowPanel - 1)) == 0) {
+                if (it) bar_named(1, 32 * C::EPI);
+#pragma unroll
+                for (int i = 0; i < PV; ++i) {
+                    const int e = tid + i * 32 * C::EPI;
+                    panel[e % kNarrowPanel * BN + e / kNarrowPanel] = ahead[i];
+                }
+                bar_named(1, 32 * C::EPI);
+                if (it + kNarrowPanel < (uint32_t)ng) fetch(it + kNarrowPanel);
+            }
+            const float ny = YROW && it + 1 < (uint32_t)ng ? __ldg(py + it + 1) : 0.0f;
+            // (a warp that gives up goes on without waiting, so that the named barriers stay matched)
+            if (!ready) ok &= warp_wait(&acc_full[b], ap, ab, 18);
             tc_fence_after();
-            const uint32_t pan = smem_u32(panel + (it & (kNarrowPanel - 1)) * BN);
-            constexpr int W = BN < 32 ? BN : 32;
-            const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + b * BN;
+            const uint32_t pan = smem_u32(panel + (it & (kNarrowPanel - 1)) * BN + col);
+            const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + b * BN + col;
+            uint32_t v[32];
+            if constexpr (C::WC == 16) tmem_ld16(src, v);
+            else tmem_ld32(src, v);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+            // the next accumulator is usually complete: looked at here, ahead of the sums
+            ready = it + 1 < (uint32_t)ng && __all_sync(0xffffffffu, mbar_ready(&acc_full[(it + 1) % kNarrowAcc], (it + 1) / kNarrowAcc & 1));
 #pragma unroll
-            for (int c = 0; c < BN / W; ++c) {
-                uint32_t v[32];
-                if constexpr (W == 16) {
-                    tmem_ld16(src, v);
-                } else {
-                    tmem_ld32_start(src + c * W, v);
-                    tmem_wait(v);
-                }
-                if (c == BN / W - 1) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&acc_empty[b]);
-                }
-#pragma unroll
-                for (int j = 0; j < W; j += 4) {
-                    const float4 x4 = lds4(pan + (c * W + j) * 4);
-                    float* s = sum + c * W + j;
-                    s[0] = __fmaf_rn(__uint_as_float(v[j]), __fmul_rn(ay, x4.x), s[0]);
-                    s[1] = __fmaf_rn(__uint_as_float(v[j + 1]), __fmul_rn(ay, x4.y), s[1]);
-                    s[2] = __fmaf_rn(__uint_as_float(v[j + 2]), __fmul_rn(ay, x4.z), s[2]);
-                    s[3] = __fmaf_rn(__uint_as_float(v[j + 3]), __fmul_rn(ay, x4.w), s[3]);
-                }
+            for (int j = 0; j < C::WC; j += 4) {
+                const float4 x4 = lds4(pan + j * 4);
+                const uint32_t* w = v + j;
+                sum[j] = __fmaf_rn(__uint_as_float(w[0]), YROW ? __fmul_rn(ay, x4.x) : x4.x, sum[j]);
+                sum[j + 1] = __fmaf_rn(__uint_as_float(w[1]), YROW ? __fmul_rn(ay, x4.y) : x4.y, sum[j + 1]);
+                sum[j + 2] = __fmaf_rn(__uint_as_float(w[2]), YROW ? __fmul_rn(ay, x4.z) : x4.z, sum[j + 2]);
+                sum[j + 3] = __fmaf_rn(__uint_as_float(w[3]), YROW ? __fmul_rn(ay, x4.w) : x4.w, sum[j + 3]);
             }
             ay = ny;
         }
         if (ok && parts == 1 && n < N) {
 #pragma unroll
-            for (int j = 0; j < BN; ++j)
-                if (m0 + j < M) r[(int64_t)(m0 + j) * N + n] = sum[j];
+            for (int j = 0; j < C::WC; ++j)
+                if (m0 + col + j < M) r[(int64_t)(m0 + col + j) * N + n] = sum[j];
         }
-        if (ok && parts > 1) {  // every group has been read from the ring: it holds this part's sums now
+        if (ok && parts > 1) {  // the last accumulator was complete, so no MMA reads the ring: it holds the sums now
             float* own = (float*)smem;
 #pragma unroll
-            for (int j = 0; j < BN; ++j) own[j * 128 + q * 32 + lane] = sum[j];
+            for (int j = 0; j < C::WC; ++j) own[(col + j) * 128 + q * 32 + lane] = sum[j];
         }
     }
     __syncthreads();
@@ -456,7 +512,7 @@ __global__ void __launch_bounds__(192, NarrowCfg<BN>::PER_SM)
         cluster_sync();
         const bool good = !*gave_up;
         // columns are shared out over the cluster; the parts are added in their order
-        for (int i = part * 192 + threadIdx.x; good && i < 128 * BN; i += 192 * parts) {
+        for (int i = part * C::THREADS + threadIdx.x; good && i < 128 * BN; i += C::THREADS * parts) {
             const int m = m0 + (i >> 7), n = n0 + (i & 127);
             if (m >= M || n >= N) continue;
             const uint32_t at = smem_u32(smem) + i * 4;
@@ -546,28 +602,35 @@ int run_narrow(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, co
     if (tiles * parts > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const int per = (int)((G + parts - 1) / parts);
     if (y_block)
-        return launch(gemm_e4m3_narrow<BN, false>, tiles * parts, 192, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
+        return launch(gemm_e4m3_narrow<BN, false>, tiles * parts, NarrowCfg<BN>::THREADS, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
                       (int)N, (int)G, parts, per, status);
-    return launch(gemm_e4m3_narrow<BN, true>, tiles * parts, 192, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
+    return launch(gemm_e4m3_narrow<BN, true>, tiles * parts, NarrowCfg<BN>::THREADS, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
                   (int)N, (int)G, parts, per, status);
+}
+
+// Both kernels run in waves of the GPU: 148 tiles of 128 x 128 at a time, or 74 of 256 x 256.  A wave takes
+// 0.51 and 0.73 us a group of K with scales of y per block, 0.69 and 1.0 us with scales per row (N = 4096
+// and 14336, K = 4096 and 2500), so the pairs win where their larger tiles fill their last wave:
+// 512 x 4096 x 4096 16.8 us against 23.5, 1024 x 4096 x 4096 33.4 us against 23.5.
+bool pair_is_faster(int64_t M, int64_t N, int y_block) {
+    const int64_t narrow = (M + 127) / 128 * ((N + 127) / 128), pair = (M + 255) / 256 * ((N + 255) / 256);
+    const int64_t n = sms(), wn = (narrow + n - 1) / n, wp = (pair + n / 2 - 1) / (n / 2);
+    return wp * (y_block ? 73 : 100) < wn * (y_block ? 51 : 69);
 }
 
 }  // namespace
 
-extern "C" size_t mcu_matmul_e4m3_scratch_bytes(int64_t, int64_t, int64_t) { return 0; }
-
 extern "C" int mcu_launch_matmul_e4m3(float* r, const uint8_t* xq, const float* xs, const uint8_t* yq,
-                                      const float* ys, int64_t M, int64_t K, int64_t N, int y_block, void*, int* status,
+                                      const float* ys, int64_t M, int64_t K, int64_t N, int y_block, int* status,
                                       cudaStream_t st, int* launches) {
     const int64_t G = (K + 127) / 128, ld = G * 128;
-    const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 1024 ? 128 : 0;
+    const int bn = M <= 16 ? 16 : M <= 32 ? 32 : !pair_is_faster(M, N, y_block) ? 128 : 0;
     CUtensorMap mx, my;
     if (!e4m3_map(&mx, xq, M, ld, bn ? bn : 128) || !e4m3_map(&my, yq, N, ld, 128)) return (int)cudaErrorInvalidValue;
     *launches = 1;
     switch (bn) {
         case 16: return run_narrow<16>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
         case 32: return run_narrow<32>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
-        case 64: return run_narrow<64>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
         case 128: return run_narrow<128>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
         default:
             return y_block ? run_pair<false>(mx, my, xs, ys, r, M, N, G, status, st)

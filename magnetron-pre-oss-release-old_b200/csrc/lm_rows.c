@@ -51,10 +51,9 @@ int mag_cuda_matmul_e4m3(mag_compute_device_t* dvc, float* r, const uint8_t* xq,
     if (!M || !N) return 0;
     const mcu_buf bufs[] = {{xq, 0, 0}, {xs, 0, 0}, {yq, 0, 0}, {ys, 0, 0}, {r, (size_t)(M * N) * 4, 1}};
     mcu_call c;
-    int k = 0, rc = mcu_call_begin(&c, dvc, bufs, 5, mcu_matmul_e4m3_scratch_bytes(M, K, N));
+    int k = 0, rc = mcu_call_begin(&c, dvc, bufs, 5, 0);
     if (rc) return rc;
-    rc = mcu_launch_matmul_e4m3(r, xq, xs, yq, ys, M, K, N, y_group == MAG_CUDA_E4M3_BLOCK, c.scratch, c.status,
-                                c.stream, &k);
+    rc = mcu_launch_matmul_e4m3(r, xq, xs, yq, ys, M, K, N, y_group == MAG_CUDA_E4M3_BLOCK, c.status, c.stream, &k);
     return mcu_call_end(&c, rc, k);
 }
 

@@ -143,10 +143,8 @@ int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy, const flo
 int mcu_launch_quantize_e4m3(uint8_t* q, float* s, const float* x, int64_t rows, int64_t cols, int block,
                              int transpose, cudaStream_t st, int* launches);
 /* k_matmul_e4m3.cu */
-size_t mcu_matmul_e4m3_scratch_bytes(int64_t M, int64_t K, int64_t N);
 int mcu_launch_matmul_e4m3(float* r, const uint8_t* xq, const float* xs, const uint8_t* yq, const float* ys, int64_t M,
-                           int64_t K, int64_t N, int y_block, void* scratch, int* status, cudaStream_t st,
-                           int* launches);
+                           int64_t K, int64_t N, int y_block, int* status, cudaStream_t st, int* launches);
 /* k_logprobs.cu */
 int mcu_launch_logprobs(float* logp, float* lse, float* entropy, float* top_logp, int32_t* top_id, const float* x,
                         const int32_t* id, int64_t rows, int64_t cols, int64_t x_s1, int top, cudaStream_t st,
