@@ -412,7 +412,8 @@ int run_rows(float* logp, float* lse, float* entropy, float* top_logp, int32_t* 
     const int smem = TOP ? (int)sizeof(Candidates<T>) : 0;
     const auto kern = logprobs_rows<T, TOP>;
     if (smem) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        static bool done[64];
+        cudaError_t e = allow_smem(kern, smem, done);
         if (e != cudaSuccess) return (int)e;
     }
     cudaLaunchConfig_t cfg = {};

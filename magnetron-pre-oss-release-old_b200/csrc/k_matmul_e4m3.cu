@@ -563,9 +563,10 @@ int sms() {
 }
 
 // A launch with a cluster of `cluster` CTAs, as a programmatic dependent of the stream's previous kernel.
-template <typename K, typename... A>
-int launch(K kern, int64_t grid, int threads, int smem, int cluster, cudaStream_t st, A... args) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <auto kern, typename... A>
+int launch(int64_t grid, int threads, int smem, int cluster, cudaStream_t st, A... args) {
+    static bool done[64];
+    cudaError_t e = allow_smem(kern, smem, done);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -589,7 +590,7 @@ int run_pair(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, cons
     const int64_t tiles = (M + 255) / 256 * ((N + 255) / 256);
     if (tiles > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const int64_t pairs = tiles < sms() / 2 ? tiles : sms() / 2;
-    return launch(gemm_e4m3_pair<YROW>, 2 * pairs, kPairThreads, PairCfg<YROW>::SMEM, 2, st, mx, my, xs, ys, r, (int)M, (int)N,
+    return launch<gemm_e4m3_pair<YROW>>(2 * pairs, kPairThreads, PairCfg<YROW>::SMEM, 2, st, mx, my, xs, ys, r, (int)M, (int)N,
                   (int)G, status);
 }
 
@@ -602,9 +603,9 @@ int run_narrow(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, co
     if (tiles * parts > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const int per = (int)((G + parts - 1) / parts);
     if (y_block)
-        return launch(gemm_e4m3_narrow<BN, false>, tiles * parts, NarrowCfg<BN>::THREADS, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
+        return launch<gemm_e4m3_narrow<BN, false>>(tiles * parts, NarrowCfg<BN>::THREADS, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
                       (int)N, (int)G, parts, per, status);
-    return launch(gemm_e4m3_narrow<BN, true>, tiles * parts, NarrowCfg<BN>::THREADS, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
+    return launch<gemm_e4m3_narrow<BN, true>>(tiles * parts, NarrowCfg<BN>::THREADS, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
                   (int)N, (int)G, parts, per, status);
 }
 

@@ -56,13 +56,12 @@ __device__ __forceinline__ void store_group(float* p, const float (&v)[4], int c
     }
 }
 
-// Sum over the block's W warps, the same on every thread.
-template <int W>
-__device__ __forceinline__ float block_sum(float v, float* sh, int warp, int lane) {
+// Sum over the block's warps, the same on every thread.
+__device__ __forceinline__ float block_sum(float v, float* sh, int warp, int lane, int warps) {
     v = warp_sum_f(v);
     if (lane == 0) sh[warp] = v;
     __syncthreads();
-    return warp_sum_f(lane < W ? sh[lane] : 0.0f);
+    return warp_sum_f(lane < warps ? sh[lane] : 0.0f);
 }
 
 struct NormArgs {
@@ -133,7 +132,7 @@ __global__ void __launch_bounds__(W * 32) rmsnorm_row(const NormArgs a) {
     for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) ss = fmaf(t[i][j], t[i][j], ss);
-    const float root = rsqrtf(__fdiv_rn(block_sum<W>(ss, sh, warp, lane), (float)a.cols) + a.eps);
+    const float root = rsqrtf(__fdiv_rn(block_sum(ss, sh, warp, lane, W), (float)a.cols) + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = root;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -169,7 +168,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_wide(const NormArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) ss = fmaf(t[j], t[j], ss);
     }
-    const float root = rsqrtf(__fdiv_rn(block_sum<32>(ss, sh, warp, lane), (float)a.cols) + a.eps);
+    const float root = rsqrtf(__fdiv_rn(block_sum(ss, sh, warp, lane, 32), (float)a.cols) + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = root;
     for (int g = warp; g < groups; g += 32) {
         float t[4], w[4];
@@ -192,15 +191,19 @@ struct BackArgs {
     int cols;
 };
 
-// W warps go through rows blockIdx.x, + grid, ...; a thread keeps the same columns in every row and so its
-// sums for the weight's gradient in registers.  The next row's dy and h are loaded before the present
-// row's reduction.  Bound by HBM: 12 bytes read and 4 written a value.
-template <int W, int V, bool VEC>
-__global__ void __launch_bounds__(W * 32) rmsnorm_backward_row(const BackArgs a) {
-    __shared__ float sh[2][W];
+// A block goes through rows blockIdx.x, + grid, ...; a thread keeps the same columns in every row and so its
+// sums for the weight's gradient in registers.  The next row's dy and h and this row's dh are in flight
+// during the row's reduction, which has one barrier: with h loaded after the row's stores instead, every
+// row waited for it (4099 x 5000: 71 us).  Bound by HBM: 12 bytes read and 4 written a value.
+constexpr int kBackV = 4;  // groups a warp
+
+template <bool VEC>
+__global__ void __launch_bounds__(512, 1) rmsnorm_backward_row(const BackArgs a) {
+    constexpr int V = kBackV;
+    __shared__ float sh[2][16];
     pdl_begin();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const auto base = [&](int i) { return (warp + i * W) * 128; };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const auto base = [&](int i) { return (warp + i * warps) * 128; };
     float sum[V][4], dy[V][4], h[V][4];
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -215,7 +218,11 @@ __global__ void __launch_bounds__(W * 32) rmsnorm_backward_row(const BackArgs a)
     for (int i = 0; i < V; ++i) load_group<VEC>(h[i], a.h + row * a.cols, base(i), a.cols, lane);
     for (; row < a.rows; row += gridDim.x, turn ^= 1) {
         const int64_t o = row * a.cols, next = row + gridDim.x;
-        float u[V][4];
+        float g[V][4], u[V][4], hn[V][4];  // the residual path's gradient, then the result; dy w; the next h
+        if (a.dh) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) load_group<VEC>(g[i], a.dh + o, base(i), a.cols, lane);
+        }
         float along = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -228,34 +235,24 @@ __global__ void __launch_bounds__(W * 32) rmsnorm_backward_row(const BackArgs a)
                 sum[i][j] = fmaf(dy[i][j], h[i][j] * root, sum[i][j]);
             }
         }
-        float g[V][4];  // the residual path's gradient, then the result
-        if (a.dh) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) load_group<VEC>(g[i], a.dh + o, base(i), a.cols, lane);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) g[i][j] = 0.0f;
-        }
-        const float next_root = next < a.rows ? __ldg(a.rstd + next) : 0.0f;
+        float next_root = 0.0f;
         if (next < a.rows) {
 #pragma unroll
             for (int i = 0; i < V; ++i) load_group<VEC>(dy[i], a.dy + next * a.cols, base(i), a.cols, lane);
+#pragma unroll
+            for (int i = 0; i < V; ++i) load_group<VEC>(hn[i], a.h + next * a.cols, base(i), a.cols, lane);
+            next_root = __ldg(a.rstd + next);
         }
-        const float f = root * root * __fdiv_rn(block_sum<W>(along, sh[turn], warp, lane), (float)a.cols);
+        const float f = root * root * __fdiv_rn(block_sum(along, sh[turn], warp, lane, warps), (float)a.cols);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float d = root * fmaf(-h[i][j], f, u[i][j]);
                 g[i][j] = a.dh ? __fadd_rn(g[i][j], d) : d;
+                h[i][j] = hn[i][j];
             }
             store_group<VEC>(a.dx + o, g[i], base(i), a.cols, lane);
-        }
-        if (next < a.rows) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) load_group<VEC>(h[i], a.h + next * a.cols, base(i), a.cols, lane);
         }
         root = next_root;
     }
@@ -284,7 +281,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_backward_wide(const BackArgs a) 
 #pragma unroll
         for (int j = 0; j < 4; ++j) along = fmaf(dy[j] * w[j], h[j], along);
     }
-    const float f = root * root * __fdiv_rn(block_sum<32>(along, sh, warp, lane), (float)a.cols);
+    const float f = root * root * __fdiv_rn(block_sum(along, sh, warp, lane, 32), (float)a.cols);
 #pragma unroll 2
     for (int g = warp; g < groups; g += 32) {
         float dy[4], h[4], w[4], t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -333,11 +330,14 @@ __global__ void __launch_bounds__(256) rmsnorm_weight_sum(float* __restrict__ dw
 constexpr int kSms = 148;
 constexpr int kWideParts = 64;
 
-// Blocks of the backward pass: as many as run at once.
-int back_warps(int64_t cols) { return cols <= 2048 ? 4 : cols <= 4096 ? 8 : cols <= 8192 ? 16 : 0; }
+// Warps of a block of the backward pass (0: rows too wide for its registers), and its blocks: as many as run
+// at once (16 warps an SM by their registers).
+int back_warps(int64_t cols) {
+    const int64_t w = ((cols + 127) / 128 + kBackV - 1) / kBackV;
+    return w <= 16 ? (int)w : 0;
+}
 int64_t back_blocks(int64_t rows, int64_t cols) {
-    const int w = back_warps(cols);
-    const int64_t n = kSms * (w == 4 ? 4 : w == 8 ? 2 : 1);
+    const int64_t n = kSms * (16 / back_warps(cols));
     return rows < n ? rows : n;
 }
 
@@ -365,13 +365,9 @@ int run_norm(const NormArgs& a, int64_t rows, cudaStream_t st) {
 
 template <bool VEC>
 int run_back(const BackArgs& a, int64_t blocks, cudaStream_t st) {
-    const dim3 grid((unsigned)blocks);
-    switch (back_warps(a.cols)) {
-        case 4: return (int)launch_dep(rmsnorm_backward_row<4, 4, VEC>, grid, dim3(128), 0, st, a);
-        case 8: return (int)launch_dep(rmsnorm_backward_row<8, 4, VEC>, grid, dim3(256), 0, st, a);
-        case 16: return (int)launch_dep(rmsnorm_backward_row<16, 4, VEC>, grid, dim3(512), 0, st, a);
-        default: return (int)launch_dep(rmsnorm_backward_wide<VEC>, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
-    }
+    const int w = back_warps(a.cols);
+    if (!w) return (int)launch_dep(rmsnorm_backward_wide<VEC>, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+    return (int)launch_dep(rmsnorm_backward_row<VEC>, dim3((unsigned)blocks), dim3(32u * w), 0, st, a);
 }
 
 }  // namespace
@@ -394,8 +390,8 @@ extern "C" int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy
                                            cudaStream_t st, int* launches) {
     const BackArgs a{dx, dw ? (float*)scratch : nullptr, dy, h, w, rstd, dh, rows, (int)cols};
     *launches = 0;
-    int parts = (int)back_blocks(rows, cols), rc = 0;
-    if (dw && !back_warps(cols)) {  // before dx, which may lie over dy or h
+    int parts = back_warps(cols) ? (int)back_blocks(rows, cols) : 0, rc = 0;
+    if (dw && !parts) {  // before dx, which may lie over dy or h
         const int64_t cb = (cols + 255) / 256, per = (rows + kWideParts - 1) / kWideParts;
         parts = (int)((rows + per - 1) / per);
         rc = (int)launch_dep(rmsnorm_weight_part, dim3((unsigned)(cb * parts)), dim3(256), 0, st, a, cb, per);

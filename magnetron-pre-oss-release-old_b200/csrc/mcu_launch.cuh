@@ -33,5 +33,16 @@ cudaError_t launch_dep(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
     return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
+// Lets a kernel use more than 48 KB of dynamic shared memory: asked for once per kernel and device.
+template <typename K>
+cudaError_t allow_smem(K kern, int bytes, bool (&done)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done[dev])) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done[dev] = true;
+    return e;
+}
+
 }  // namespace
 #endif
