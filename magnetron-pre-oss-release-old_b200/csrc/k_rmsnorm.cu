@@ -322,11 +322,12 @@ __global__ void __launch_bounds__(256) rmsnorm_weight_part(const BackArgs a, int
     a.part[slice * a.cols + c] = t;
 }
 
-// dw = the sum of the partial sums, in their order: 32 columns a block, 8 warps of consecutive parts.
-__global__ void __launch_bounds__(256) rmsnorm_weight_sum(float* __restrict__ dw, const float* __restrict__ part, int parts, int cols) {
-    __shared__ float sh[8][32];
+// dw = the sum of the partial sums in a fixed order: 32 columns a block, a warp per share of the parts, then
+// a warp per column over the shares.
+__global__ void __launch_bounds__(1024) rmsnorm_weight_sum(float* __restrict__ dw, const float* __restrict__ part, int parts, int cols) {
+    __shared__ float sh[32][33];
     pdl_begin();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, per = (parts + 7) / 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, per = (parts + 31) / 32;
     float t = 0.0f;
     if (c < cols) {
 #pragma unroll 8
@@ -334,11 +335,8 @@ __global__ void __launch_bounds__(256) rmsnorm_weight_sum(float* __restrict__ dw
     }
     sh[warp][lane] = t;
     __syncthreads();
-    if (warp == 0 && c < cols) {
-#pragma unroll
-        for (int i = 1; i < 8; ++i) t += sh[i][lane];
-        dw[c] = t;
-    }
+    t = warp_sum_f(sh[lane][warp]);
+    if (lane == 0 && blockIdx.x * 32 + warp < cols) dw[blockIdx.x * 32 + warp] = t;
 }
 
 constexpr int kSms = 148;
@@ -351,8 +349,9 @@ int back_warps(int64_t cols) {
     return w <= 16 ? (int)w : 0;
 }
 int64_t back_blocks(int64_t rows, int64_t cols) {
-    const int64_t n = kSms * (16 / back_warps(cols));
-    return rows < n ? rows : n;
+    // (few rows: about four a block, or one where that leaves SMs idle, since every block adds a part to dw)
+    const int64_t all = kSms * (16 / back_warps(cols)), four = rows < kSms ? rows : rows / 4 > kSms ? rows / 4 : kSms;
+    return four < all ? four : all;
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -418,7 +417,7 @@ extern "C" int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy
         ++*launches;
     }
     if (!rc && dw) {
-        rc = (int)launch_dep(rmsnorm_weight_sum, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, st, dw, (const float*)a.part, parts, (int)cols);
+        rc = (int)launch_dep(rmsnorm_weight_sum, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, st, dw, (const float*)a.part, parts, (int)cols);
         ++*launches;
     }
     return rc;
