@@ -33,18 +33,6 @@ __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// 32 lanes x 32 columns of TMEM; the values are there after tmem_wait.
-__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr));
-}
 // 16 columns, waited for.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[32]) {
     asm volatile(
@@ -55,17 +43,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[32]) {
         : "r"(taddr)
         : "memory");
 }
-// Waits for this thread's TMEM loads; v is tied to the wait so that no use moves ahead of it.
-__device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
-                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
-                   "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
-                 :
-                 : "memory");
-}
-
 // One lane of a converged warp.  The narrow kernel's roles run as whole warps and elect the lane only around
 // the issue, so that waits, loop and descriptors stay warp-uniform: with a branch on the lane number around
 // the role each MMA took about 80 cycles to issue.
@@ -102,6 +79,12 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* bar0, uint32_t parity0, uin
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+__device__ __forceinline__ float lds1(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ void bar_named(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // On a give-up: the loads that this thread issued (up to load `it`) have to land before the block ends.
@@ -112,11 +95,11 @@ __device__ __forceinline__ void drain_loads(uint64_t* full, uint32_t it) {
 }
 
 // ---- large products: CTA pairs, 256 x 256 tiles, persistent
-constexpr int kPairThreads = 384;  // warpgroup 0: producer, MMA issuer, two idle warps; 1 and 2: epilogue
-// 128 * kPairCtrl + 256 * kPairEpi = 384 * kPairLaunch: the epilogue holds 128 sums a thread
-constexpr int kPairLaunch = 168, kPairCtrl = 40, kPairEpi = 232;
-static_assert(128 * kPairCtrl + 256 * kPairEpi == kPairThreads * kPairLaunch, "register split must match the launch");
-constexpr int kPanel = 8;  // groups of per-column scales staged at a time
+constexpr int kPairThreads = 512;  // warpgroup 0: producer, MMA issuer, two relays; 1: scales; 2 and 3: epilogue
+// 256 * kPairCtrl + 256 * kPairEpi = 512 * kPairLaunch: the epilogue holds 128 sums a thread
+constexpr int kPairLaunch = 128, kPairCtrl = 40, kPairEpi = 216;
+static_assert(kPairCtrl + kPairEpi == 2 * kPairLaunch, "register split must match the launch");
+constexpr int kPanel = 8;      // groups of scales staged at a time
 constexpr int kGroupRows = 8;  // 256-row blocks that sweep the columns together, so that operands stay in L2
 
 template <bool YROW>
@@ -125,9 +108,11 @@ struct PairCfg {
     static constexpr int HALF = 128 * 128;  // this CTA's rows of x, or its half of y's, one group
     static constexpr int STAGE = 2 * HALF;
     static constexpr int BARS = STAGES * STAGE;
-    static constexpr int SLOTS = BARS + 1024;              // 8 epilogue warps x 32 x 32 f32
-    static constexpr int PANEL = SLOTS + 8 * 4096;         // 2 halves x kPanel x 128 scales
-    static constexpr int SMEM = PANEL + (YROW ? 2 * kPanel * 128 * 4 : 0) + 1024;
+    static constexpr int SLOTS = BARS + 1024;                      // 8 epilogue warps x 32 x 16 f32
+    static constexpr int YS = YROW ? 256 : 2;                      // scales of y per group
+    static constexpr int PANEL = (128 + YS) * kPanel * 4;          // x's 128 rows, then y's
+    static constexpr int PANELS = SLOTS + 8 * 2048;                // two of them
+    static constexpr int SMEM = PANELS + 2 * PANEL + 1024;
     static_assert(SMEM <= 227 * 1024, "must fit shared memory");
 };
 
@@ -137,6 +122,17 @@ __device__ __forceinline__ void pair_tile(int t, int num_m, int num_n, int& mb, 
     nb = (t - g * per) / rows;
 }
 
+// What bounds it: the group-wise epilogue.  A group is 512 cycles of MMA; its 256 fused multiply-adds per
+// scheduler with their TMEM loads and the way accumulator -> relay -> warpgroup -> MMA issuer, 2 of them in
+// flight, take about 900, at clocks that the 1 kW limit holds near 1.4 GHz: 8192^3 in 0.56 ms (1.95 PFLOP/s)
+// for a few calls and 0.64 ms (1.7) back to back; the MMAs and loads alone took 0.40 and 0.46 ms.
+// Measured and not kept: four accumulators of 128 columns (MMAs of N = 128 reach 0.84 of the rate), 16
+// epilogue warps of 64 columns (more instructions, 0.67 ms), packed f32x2 multiply-adds (half the
+// instructions, the same pipe cycles, more register copies: 0.64 ms and up).
+//
+// The epilogue waits at a named barrier, never on an mbarrier: a polling loop among its 128 live sums made the
+// compiler copy half of them every group.  A relay warp per epilogue warpgroup polls the accumulator's mbarrier
+// (bounded) and joins the barrier; four more warps stage the scales, a panel of groups ahead.
 template <bool YROW>
 __global__ void __maxnreg__(kPairLaunch)
     gemm_e4m3_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
@@ -149,10 +145,12 @@ __global__ void __maxnreg__(kPairLaunch)
     uint64_t* empty = full + C::STAGES;
     uint64_t* acc_full = empty + C::STAGES;
     uint64_t* acc_empty = acc_full + 2;
-    uint64_t* drain = acc_empty + 2;
+    uint64_t* sc_full = acc_empty + 2;
+    uint64_t* sc_empty = sc_full + 2;
+    uint64_t* drain = sc_empty + 2;
     uint32_t* tmem_slot = (uint32_t*)(drain + 1);
     volatile int* gave_up = (volatile int*)(tmem_slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int num_m = (M + 255) >> 8, num_n = (N + 255) >> 8, tiles = num_m * num_n;
@@ -165,6 +163,8 @@ __global__ void __maxnreg__(kPairLaunch)
         for (int a = 0; a < 2; ++a) {
             mbar_init(&acc_full[a], 1);
             mbar_init(&acc_empty[a], 16);  // one arrival per epilogue warp of both CTAs
+            mbar_init(&sc_full[a], 128);
+            mbar_init(&sc_empty[a], 2);  // both relays
         }
         mbar_init(drain, 1);
         *gave_up = 0;
@@ -180,142 +180,180 @@ __global__ void __maxnreg__(kPairLaunch)
     pdl_begin();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp < 4) {
+    if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairCtrl));
-        if (warp == 0 && lane == 0) {  // ---- TMA producer
-            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_x) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_y) : "memory");
-            uint32_t it = 0;
+        if (warp == 0) {  // ---- TMA producer
+            uint32_t it = 0, s = 0, phase = 1;
             bool ok = true;
             for (int t = pair; ok && t < tiles; t += pairs) {
                 int mb, nb;
                 pair_tile(t, num_m, num_n, mb, nb);
+                const int xr = mb * 256 + (int)rank * 128, yr = nb * 256 + (int)rank * 128;
                 for (int g = 0; g < G; ++g, ++it) {
-                    const uint32_t s = it % C::STAGES;
-                    if (!(ok = mbar_wait(&empty[s], (it / C::STAGES & 1) ^ 1, ab, 11))) break;
-                    // both CTAs' loads complete on the leader's barrier, which expects both
-                    const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
-                    uint8_t* st = smem + s * C::STAGE;
-                    if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
-                    tma_load_2d_pair(&map_x, fb, st, g * 128, mb * 256 + (int)rank * 128);
-                    tma_load_2d_pair(&map_y, fb, st + C::HALF, g * 128, nb * 256 + (int)rank * 128);
+                    if (!(ok = warp_wait(&empty[s], phase, ab, 11))) break;
+                    if (elect_one()) {
+                        // both CTAs' loads complete on the leader's barrier, which expects both
+                        const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
+                        uint8_t* st = smem + s * C::STAGE;
+                        if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
+                        tma_load_2d_pair(&map_x, fb, st, g * 128, xr);
+                        tma_load_2d_pair(&map_y, fb, st + C::HALF, g * 128, yr);
+                    }
+                    __syncwarp();
+                    if (++s == C::STAGES) s = 0, phase ^= 1;
                 }
             }
-            if (!ok && rank == 0) drain_loads<C::STAGES>(full, it);
-        } else if (warp == 1 && lane == 0 && rank == 0) {  // ---- MMA issuer, for both CTAs
-            constexpr uint32_t idesc = idesc_f8(256, 256);
-            uint32_t it = 0;
+            if (!ok && rank == 0 && lane == 0) drain_loads<C::STAGES>(full, it);
+        } else if (warp == 1) {
+            if (rank == 0) {  // ---- MMA issuer, for both CTAs
+                constexpr uint32_t idesc = idesc_f8(256, 256);
+                const uint64_t first = sw_desc<128>(smem_u32(smem));
+                uint32_t it = 0, s = 0, phase = 0;
+                bool ok = true;
+                for (int t = pair; ok && t < tiles; t += pairs) {
+                    for (int g = 0; g < G; ++g, ++it) {
+                        const uint32_t b = it & 1;
+                        if (!(ok = warp_wait2(&acc_empty[b], (it >> 1 & 1) ^ 1, &full[s], phase, ab, 12))) break;
+                        tc_fence_after();
+                        const uint64_t dx = first + s * (C::STAGE >> 4), dy = dx + (C::HALF >> 4);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) umma_f8_pair(tmem + b * 256, dx + k * 2, dy + k * 2, idesc, k);
+                            umma_commit_pair(&acc_full[b]);
+                            umma_commit_pair(&empty[s]);
+                        }
+                        __syncwarp();
+                        if (++s == C::STAGES) s = 0, phase ^= 1;
+                    }
+                }
+            }
+        } else if (warp < 4) {  // ---- relay of epilogue warpgroup `half`
+            const int half = warp - 2;
+            uint32_t it = 0, pi = 0;
+            for (int t = pair; t < tiles; t += pairs) {
+                for (int g = 0; g < G; ++g, ++it) {
+                    const bool first = (g & (kPanel - 1)) == 0;
+                    // (a relay that gives up goes on without waiting, so that the named barriers stay matched)
+                    if (first) warp_wait(&sc_full[pi & 1], pi >> 1 & 1, ab, 20);
+                    warp_wait(&acc_full[it & 1], it >> 1 & 1, ab, 14);
+                    tc_fence_after();
+                    tc_fence_before();
+                    bar_named(1 + half, 160);
+                    if (first) {  // the warpgroup is past the panel before this one
+                        if (pi && lane == 0) mbar_arrive(&sc_empty[(pi & 1) ^ 1]);
+                        ++pi;
+                    }
+                }
+            }
+        } else {  // ---- scales: thread i brings x's row i of the CTA and y's columns i and i + 128
+            const int i = threadIdx.x - 128;
+            uint32_t pi = 0;
             bool ok = true;
             for (int t = pair; ok && t < tiles; t += pairs) {
-                for (int g = 0; g < G; ++g, ++it) {
-                    const uint32_t s = it % C::STAGES, b = it & 1;
-                    if (!(ok = mbar_wait(&acc_empty[b], (it >> 1 & 1) ^ 1, ab, 12))) break;
-                    if (!(ok = mbar_wait(&full[s], it / C::STAGES & 1, ab, 13))) break;
-                    tc_fence_after();
-                    const uint32_t base = smem_u32(smem + s * C::STAGE);
+                int mb, nb;
+                pair_tile(t, num_m, num_n, mb, nb);
+                const float* px = xs + (int64_t)min(mb * 256 + (int)rank * 128 + i, M - 1) * G;
+                const float* py0 = ys + (int64_t)(YROW ? min(nb * 256 + i, N - 1) : min(nb * 256 + (i & 1) * 128, N - 1) >> 7) * G;
+                const float* py1 = ys + (int64_t)min(nb * 256 + 128 + i, N - 1) * G;  // (scales per row only)
+                for (int g0 = 0; g0 < G; g0 += kPanel, ++pi) {
+                    const int n = min(kPanel, G - g0);
+                    float v[kPanel];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_f8_pair(tmem + b * 256, sw_desc<128>(base + k * 32), sw_desc<128>(base + C::HALF + k * 32), idesc, k);
-                    umma_commit_pair(&empty[s]);
-                    umma_commit_pair(&acc_full[b]);
+                    for (int k = 0; k < kPanel; ++k) v[k] = k < n ? __ldg(px + g0 + k) : 0.0f;
+                    if (!(ok = warp_wait(&sc_empty[pi & 1], (pi >> 1 & 1) ^ 1, ab, 19))) break;
+                    float* p = (float*)(smem + C::PANELS + (pi & 1) * C::PANEL);
+#pragma unroll
+                    for (int k = 0; k < kPanel; ++k) p[k * 128 + i] = v[k];
+                    p += 128 * kPanel;
+                    if constexpr (YROW) {
+#pragma unroll
+                        for (int k = 0; k < kPanel; ++k) v[k] = k < n ? __ldg(py0 + g0 + k) : 0.0f;
+#pragma unroll
+                        for (int k = 0; k < kPanel; ++k) p[k * 256 + i] = v[k];
+#pragma unroll
+                        for (int k = 0; k < kPanel; ++k) v[k] = k < n ? __ldg(py1 + g0 + k) : 0.0f;
+#pragma unroll
+                        for (int k = 0; k < kPanel; ++k) p[k * 256 + 128 + i] = v[k];
+                    } else if (i < 2 * n) {
+                        p[i] = __ldg(py0 + g0 + (i >> 1));
+                    }
+                    mbar_arrive(&sc_full[pi & 1]);
                 }
             }
         }
     } else {  // ---- epilogue: lane = row, warpgroup = half of the columns
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairEpi));
-        const int q = warp & 3, half = (warp >> 2) - 1;
-        const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        const uint32_t slot = smem_u32(smem + C::SLOTS + (warp - 4) * 4096);
-        float* panel = (float*)(smem + C::PANEL) + half * kPanel * 128;
-        const uint32_t free0 = mapa_rank(smem_u32(&acc_empty[0]), 0), free1 = mapa_rank(smem_u32(&acc_empty[1]), 0);
+        const int q = warp & 3, half = (warp >> 2) - 2;
+        const uint32_t src0 = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
+        const uint32_t slot = smem_u32(smem + C::SLOTS + (warp - 8) * 2048);
+        const uint32_t panels = smem_u32(smem + C::PANELS);
+        const uint32_t released = mapa_rank(smem_u32(&acc_empty[0]), 0);
         const bool vec = (N & 3) == 0 && ((uintptr_t)r & 15) == 0;
-        uint32_t it = 0;
-        bool ok = true;
+        uint32_t it = 0, pi = 0;
         for (int t = pair; t < tiles; t += pairs) {
             int mb, nb;
             pair_tile(t, num_m, num_n, mb, nb);
             const int row0 = mb * 256 + (int)rank * 128 + q * 32, col0 = nb * 256 + half * 128;
-            const float* px = xs + (int64_t)min(row0 + lane, M - 1) * G;
-            // per-block scales: one per group; per-row scales: thread i of the warpgroup fetches column i's
-            const float* py = ys + (int64_t)(YROW ? min(col0 + q * 32 + lane, N - 1) : min(col0, N - 1) >> 7) * G;
             float sum[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
-            float ax = __ldg(px), ay = YROW ? 0.0f : __ldg(py);
             for (int g = 0; g < G; ++g, ++it) {
-                const uint32_t b = it & 1;
-                float nx = 0.0f, ny = 0.0f;
-                if (g + 1 < G) {  // the next group's scales
-                    nx = __ldg(px + g + 1);
-                    if (!YROW) ny = __ldg(py + g + 1);
-                }
-                if (YROW && (g & (kPanel - 1)) == 0) {
-                    float p[kPanel];
-#pragma unroll
-                    for (int i = 0; i < kPanel; ++i) p[i] = g + i < G ? __ldg(py + g + i) : 0.0f;
-                    bar_named(1 + half, 128);  // the warpgroup is done with the old panel
-#pragma unroll
-                    for (int i = 0; i < kPanel; ++i) panel[i * 128 + q * 32 + lane] = p[i];
-                    bar_named(1 + half, 128);
-                }
-                // (a warp that gives up goes on without waiting, so that the named barriers stay matched)
-                ok &= mbar_wait(&acc_full[b], it >> 1 & 1, ab, 14);
+                const uint32_t panel = panels + ((pi + (g / kPanel)) & 1) * C::PANEL + (g & (kPanel - 1)) * 512;
+                const uint32_t src = src0 + (it & 1) * 256;
+                bar_named(1 + half, 160);
                 tc_fence_after();
-                const float sc = YROW ? ax : __fmul_rn(ax, ay);
-                const uint32_t src = tmem + lanes + b * 256 + half * 128;
-                const uint32_t pan = smem_u32(panel + (g & (kPanel - 1)) * 128);
-                uint32_t v[2][32];
-                tmem_ld32_start(src, v[0]);
+                float sc = lds1(panel + (q * 32 + lane) * 4);
+                const uint32_t py = panels + ((pi + (g / kPanel)) & 1) * C::PANEL + kPanel * 512 + (g & (kPanel - 1)) * C::YS * 4;
+                if (!YROW) sc = __fmul_rn(sc, lds1(py + half * 4));
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    tmem_wait(v[c & 1]);
-                    if (c < 3) {
-                        tmem_ld32_start(src + (c + 1) * 32, v[(c + 1) & 1]);
-                    } else {  // everything read: the accumulator goes back to the leader's MMA issuer
+                    uint32_t v[32];
+                    tmem_ld32(src + c * 32, v);
+                    if (c == 3) {  // everything is read: the accumulator goes back to the leader's MMA issuer
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(b ? free1 : free0);
+                        if (lane == 0) mbar_arrive_cluster(released + (it & 1) * 8);
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
-                        float4 s4 = make_float4(sc, sc, sc, sc);
+                        float4 s = make_float4(sc, sc, sc, sc);
                         if (YROW) {
-                            const float4 y4 = lds4(pan + (c * 32 + j) * 4);
-                            s4 = make_float4(__fmul_rn(sc, y4.x), __fmul_rn(sc, y4.y), __fmul_rn(sc, y4.z), __fmul_rn(sc, y4.w));
+                            const float4 y = lds4(py + (half * 128 + c * 32 + j) * 4);
+                            s = make_float4(__fmul_rn(sc, y.x), __fmul_rn(sc, y.y), __fmul_rn(sc, y.z), __fmul_rn(sc, y.w));
                         }
-                        sum[c * 32 + j] = __fmaf_rn(__uint_as_float(v[c & 1][j]), s4.x, sum[c * 32 + j]);
-                        sum[c * 32 + j + 1] = __fmaf_rn(__uint_as_float(v[c & 1][j + 1]), s4.y, sum[c * 32 + j + 1]);
-                        sum[c * 32 + j + 2] = __fmaf_rn(__uint_as_float(v[c & 1][j + 2]), s4.z, sum[c * 32 + j + 2]);
-                        sum[c * 32 + j + 3] = __fmaf_rn(__uint_as_float(v[c & 1][j + 3]), s4.w, sum[c * 32 + j + 3]);
+                        float* d = sum + c * 32 + j;
+                        d[0] = __fmaf_rn(__uint_as_float(v[j]), s.x, d[0]);
+                        d[1] = __fmaf_rn(__uint_as_float(v[j + 1]), s.y, d[1]);
+                        d[2] = __fmaf_rn(__uint_as_float(v[j + 2]), s.z, d[2]);
+                        d[3] = __fmaf_rn(__uint_as_float(v[j + 3]), s.w, d[3]);
                     }
                 }
-                ax = nx;
-                ay = ny;
             }
-            // 32 x 32 chunks through this warp's slot, so that rows leave as 128-byte stores
+            pi += (G + kPanel - 1) / kPanel;
+            // 32 x 16 chunks through this warp's slot, so that rows leave in pieces of 64 bytes
+            const bool ok = !*gave_up;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int col = col0 + c * 32;
+            for (int c = 0; c < 8; ++c) {
+                const int col = col0 + c * 16;
                 if (!ok || row0 >= M || col >= N) break;
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    sts4(slot + lane * 128 + (((j >> 2) ^ (lane & 7)) << 4), sum[c * 32 + j], sum[c * 32 + j + 1],
-                         sum[c * 32 + j + 2], sum[c * 32 + j + 3]);
+                for (int j = 0; j < 4; ++j)
+                    sts4(slot + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), sum[c * 16 + j * 4], sum[c * 16 + j * 4 + 1],
+                         sum[c * 16 + j * 4 + 2], sum[c * 16 + j * 4 + 3]);
                 __syncwarp();
                 if (vec) {
-                    const int cc = (lane & 7) * 4;
-#pragma unroll 1
-                    for (int i = 0; i < 8; ++i) {
-                        const int rr = 4 * i + (lane >> 3);
-                        const float4 o = lds4(slot + rr * 128 + (((cc >> 2) ^ (rr & 7)) << 4));
-                        if (row0 + rr < M && col + cc < N) __stcs((float4*)(r + (int64_t)(row0 + rr) * N + col + cc), o);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int rr = 8 * i + (lane >> 2), cc = lane & 3;
+                        const float4 o = lds4(slot + rr * 64 + ((cc ^ ((rr >> 1) & 3)) << 4));
+                        if (row0 + rr < M && col + cc * 4 < N) __stcs((float4*)(r + (int64_t)(row0 + rr) * N + col + cc * 4), o);
                     }
                 } else {
 #pragma unroll 1
-                    for (int rr = 0; rr < 32 && row0 + rr < M; ++rr) {
-                        float o;
-                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(o) : "r"(slot + rr * 128 + (((lane >> 2) ^ (rr & 7)) << 4) + (lane & 3) * 4) : "memory");
-                        if (col + lane < N) r[(int64_t)(row0 + rr) * N + col + lane] = o;
+                    for (int i = 0; i < 16; ++i) {
+                        const int rr = 2 * i + (lane >> 4), cc = lane & 15;
+                        const float o = lds1(slot + rr * 64 + (((cc >> 2) ^ ((rr >> 1) & 3)) << 4) + (cc & 3) * 4);
+                        if (row0 + rr < M && col + cc < N) r[(int64_t)(row0 + rr) * N + col + cc] = o;
                     }
                 }
                 __syncwarp();
@@ -594,12 +632,19 @@ int run_pair(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, cons
                   (int)G, status);
 }
 
+// CTAs per tile: up to 8, while they all run at once and have at least two groups each.
+template <int BN>
+int narrow_parts(int64_t tiles, int64_t G) {
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= sms() * NarrowCfg<BN>::PER_SM && G >= 4 * parts) parts *= 2;
+    return parts;
+}
+
 template <int BN>
 int run_narrow(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, const float* ys, float* r, int64_t M, int64_t N,
                int64_t G, int y_block, int* status, cudaStream_t st) {
     const int64_t tiles = (M + BN - 1) / BN * ((N + 127) / 128);
-    int parts = 1;  // CTAs per tile: up to 8, while they all run at once and have at least two groups each
-    while (parts < 8 && tiles * parts * 2 <= sms() * NarrowCfg<BN>::PER_SM && G >= 4 * parts) parts *= 2;
+    const int parts = narrow_parts<BN>(tiles, G);
     if (tiles * parts > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const int per = (int)((G + parts - 1) / parts);
     if (y_block)
@@ -609,14 +654,17 @@ int run_narrow(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, co
                   (int)N, (int)G, parts, per, status);
 }
 
-// Both kernels run in waves of the GPU: 148 tiles of 128 x 128 at a time, or 74 of 256 x 256.  A wave takes
-// 0.51 and 0.73 us a group of K with scales of y per block, 0.69 and 1.0 us with scales per row (N = 4096
-// and 14336, K = 4096 and 2500), so the pairs win where their larger tiles fill their last wave:
-// 512 x 4096 x 4096 16.8 us against 23.5, 1024 x 4096 x 4096 33.4 us against 23.5.
-bool pair_is_faster(int64_t M, int64_t N, int y_block) {
-    const int64_t narrow = (M + 127) / 128 * ((N + 127) / 128), pair = (M + 255) / 256 * ((N + 255) / 256);
-    const int64_t n = sms(), wn = (narrow + n - 1) / n, wp = (pair + n / 2 - 1) / (n / 2);
-    return wp * (y_block ? 73 : 100) < wn * (y_block ? 51 : 69);
+// Both kernels run in waves of the GPU: 148 tiles of 128 x 128 at a time, or 74 of 256 x 256.  Measured with
+// N = 4096 and 14336 and K = 256 to 8192: a narrow wave takes 4 us and 0.41 us a group of K (0.50 with
+// scales of y per row); the persistent pairs take 8.5 us in all and 0.46 us a group and wave (7.3 and 0.80).
+// So the pairs win once their larger tiles fill a wave: 512 x 4096 x 4096 takes 17 us narrow and 23 in
+// pairs, 1024 x 4096 x 4096 33 us narrow and 23 in pairs.
+bool pair_is_faster(int64_t M, int64_t N, int64_t G, int y_block) {
+    const int64_t narrow = (M + 127) / 128 * ((N + 127) / 128), pair = (M + 255) / 256 * ((N + 255) / 256), n = sms();
+    const int64_t parts = narrow_parts<128>(narrow, G), per = (G + parts - 1) / parts;
+    const int64_t tn = (narrow * parts + n - 1) / n * (400 + (y_block ? 41 : 50) * per);
+    const int64_t tp = (pair + n / 2 - 1) / (n / 2) * (y_block ? 46 : 80) * G + (y_block ? 850 : 730);
+    return tp < tn;
 }
 
 }  // namespace
@@ -625,7 +673,7 @@ extern "C" int mcu_launch_matmul_e4m3(float* r, const uint8_t* xq, const float* 
                                       const float* ys, int64_t M, int64_t K, int64_t N, int y_block, int* status,
                                       cudaStream_t st, int* launches) {
     const int64_t G = (K + 127) / 128, ld = G * 128;
-    const int bn = M <= 16 ? 16 : M <= 32 ? 32 : !pair_is_faster(M, N, y_block) ? 128 : 0;
+    const int bn = M <= 16 ? 16 : M <= 32 ? 32 : !pair_is_faster(M, N, G, y_block) ? 128 : 0;
     CUtensorMap mx, my;
     if (!e4m3_map(&mx, xq, M, ld, bn ? bn : 128) || !e4m3_map(&my, yq, N, ld, 128)) return (int)cudaErrorInvalidValue;
     *launches = 1;
