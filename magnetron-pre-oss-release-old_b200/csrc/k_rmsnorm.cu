@@ -64,6 +64,13 @@ __device__ __forceinline__ float block_sum(float v, float* sh, int warp, int lan
     return warp_sum_f(lane < warps ? sh[lane] : 0.0f);
 }
 
+// 1 / sqrt(a), the approximation's last bits put right by one Newton step.
+__device__ __forceinline__ float inv_sqrt(float a) {
+    const float r = rsqrtf(a), p = __fmul_rn(a, r), e = __fmaf_rn(a, r, -p);
+    const float n = __fmaf_rn(__fmaf_rn(-e, r, __fmaf_rn(-p, r, 1.0f)), 0.5f * r, r);
+    return isfinite(n) ? n : r;
+}
+
 struct NormArgs {
     float* y;
     uint8_t* q;
@@ -133,7 +140,7 @@ __global__ void __launch_bounds__(W * 32) rmsnorm_row(const NormArgs a) {
     for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) ss = fmaf(t[i][j], t[i][j], ss);
-    const float root = rsqrtf(__fdiv_rn(block_sum(ss, sh, warp, lane, W), (float)a.cols) + a.eps);
+    const float root = inv_sqrt(__fdiv_rn(block_sum(ss, sh, warp, lane, W), (float)a.cols) + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = root;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -169,7 +176,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_wide(const NormArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) ss = fmaf(t[j], t[j], ss);
     }
-    const float root = rsqrtf(__fdiv_rn(block_sum(ss, sh, warp, lane, 32), (float)a.cols) + a.eps);
+    const float root = inv_sqrt(__fdiv_rn(block_sum(ss, sh, warp, lane, 32), (float)a.cols) + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = root;
     for (int g = warp; g < groups; g += 32) {
         float t[4], w[4];

@@ -270,7 +270,9 @@ def test_rmsnorm_in_place_and_unaligned(rows, cols):
     px, pr, pw, py, ph = up(pad(x)), up(pad(res)), up(pad(w)), out(rows * cols + 2), out(rows * cols + 2)
     d.rmsnorm_rows(rows, cols, px.data_ptr + 4, pw.data_ptr + 4, EPS, residual=pr.data_ptr + 4, y=py.data_ptr + 4,
                    h=ph.data_ptr + 4)
-    assert np.array_equal(py.read()[1:-1], want_y) and np.array_equal(ph.read()[1:-1], want_h)
+    # a thread adds other columns of an unaligned row: both results are within norm_rel of the formula
+    assert np.all(np.abs(py.read()[1:-1] - want_y) <= 2 * norm_rel(cols) * np.abs(want_y))
+    assert np.array_equal(ph.read()[1:-1], want_h)
     assert np.isnan(py.read()[[0, -1]]).all()
 
 
