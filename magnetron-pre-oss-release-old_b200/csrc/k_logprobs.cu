@@ -144,7 +144,8 @@ struct Candidates {
     uint64_t pool[kWarps * kKeep];
     uint64_t list[kWarps][32];
     uint32_t group[64];  // maxima of 64 groups of threads over the first chunk
-    uint32_t least;      // orders below it are no candidates: the first chunk's bound, raised by full buffers
+    uint32_t first;      // the first chunk's bound
+    uint32_t least;      // the bound that full buffers gave
     int pooled;
 };
 
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
     const Row r = row_of(x + row * x_s1, cols);
     const int nvec = vectors_of(r), per = (nvec + parts - 1) / parts;
     const int v0 = min(rank * per, nvec), v1 = min(v0 + per, nvec);
-    if (TOP && threadIdx.x == 0) cand.pooled = 0;
+    if (TOP && threadIdx.x == 0) cand.pooled = 0, cand.least = 0;  // (seen by all after the first chunk's barriers)
 
     float m = -FLT_MAX, s = 0.0f, t = 0.0f;
     int held = 0;         // keys in this warp's buffer
@@ -260,10 +261,10 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
                 if (warp == 0) {
                     const uint32_t list = merge32(sort32(cand.group[lane], lane), sort32(cand.group[lane + 32], lane), lane);
                     const uint32_t least = __shfl_sync(0xffffffffu, list, top - 1);
-                    if (lane == 0) cand.least = least;
+                    if (lane == 0) cand.first = least;
                 }
                 __syncthreads();
-                const uint32_t least = cand.least;
+                const uint32_t least = cand.first;
                 if (__any_sync(0xffffffffu, big >= least)) {
 #pragma unroll
                     for (int i = 0; i < kVecs * 4; ++i) {

@@ -476,6 +476,30 @@ def test_logprobs_ties_and_signed_zeros():
         assert np.array_equal(got["top_id"], best(x, 32))
 
 
+@pytest.mark.parametrize("order", ["rising", "falling", "few values", "spikes late", "mostly masked"])
+def test_logprobs_top_of_awkward_rows(order):
+    """Rows that keep beating the bound, or tie with it, everywhere in the row."""
+    cols, k = 150003, 32
+    g = rng(21)
+    x = g.normal(0, 1, (3, cols)).astype(np.float32)
+    if order in ("rising", "falling"):
+        x = np.sort(x, axis=1)[:, ::1 if order == "rising" else -1]
+    elif order == "few values":
+        x = np.floor(x * 2)
+    elif order == "spikes late":
+        x[:, -2000:] += 10
+    else:
+        x[:] = -np.inf
+        x[0, [7, 90000, 140001]] = 1.0
+        x[1, 149000:149010] = 2.0
+        x[2, ::7] = -1.0
+    x = np.ascontiguousarray(np.repeat(x, 60, 0))  # one block a row as well as a cluster a row
+    for rows in (3 * 60, 3):
+        part = x[:: 180 // rows]
+        got = run_logprobs(part, np.zeros(rows, np.int32), k)
+        assert np.array_equal(got["top_id"], best(part, k))
+
+
 def test_logprobs_nan_inf_and_odd_ids():
     cols = 5000
     x = rng(15).normal(0, 1, (5, cols)).astype(np.float32)
