@@ -10,6 +10,7 @@
 #include <cooperative_groups.h>
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 #include "mcu_kernels.h"
 #include "mcu_launch.cuh"
 #include "mcu_lm.cuh"
@@ -23,6 +24,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFar = -1e30f;  // stands for d = -inf where it meets a factor of zero
 constexpr int kVecs = 4;        // float4 per thread and chunk
 constexpr int kMaxCluster = 8;  // CTAs that share a row
+constexpr int kSms = 148;
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
@@ -144,7 +146,7 @@ struct Candidates {
     uint64_t pool[kWarps * kKeep];
     uint64_t list[kWarps][32];
     uint32_t group[64];  // maxima of 64 groups of threads over the first chunk
-    uint32_t first;      // the first chunk's bound
+    uint32_t first;      // the bound that the groups gave
     uint32_t least;      // the bound that full buffers gave
     int pooled;
 };
@@ -161,11 +163,27 @@ __device__ __forceinline__ uint64_t best_of(const uint64_t* key, int n, int lane
     return best;
 }
 
+// The top-th largest maximum of 64 groups of threads, from each thread's; 0 if fewer have one.
+template <int T>
+__device__ __forceinline__ uint32_t group_bound(Candidates<T>& cand, uint32_t big, int top, int warp, int lane) {
+#pragma unroll
+    for (int o = 1; o < T / 64; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+    if (threadIdx.x % (T / 64) == 0) cand.group[threadIdx.x / (T / 64)] = big;
+    __syncthreads();
+    if (warp == 0) {
+        const uint32_t list = merge32(sort32(cand.group[lane], lane), sort32(cand.group[lane + 32], lane), lane);
+        const uint32_t least = __shfl_sync(0xffffffffu, list, top - 1);
+        if (lane == 0) cand.first = least;
+    }
+    __syncthreads();
+    return cand.first;
+}
+
 // One cluster of `parts` CTAs of T threads per row; each streams its part of the row once, 16 logits a
 // thread and chunk, the next chunk's loads issued before the present one is worked on.  Bound by HBM, 4
-// bytes a logit, without alternatives (4095 x 100003: 256 us, 6.4 TB/s); with 8 of them 300 to 330 us
-// (5.0 to 5.5 TB/s), the rest being the bound's two barriers a row and the chunks in which a candidate
-// shows.  Collecting candidates for the whole block, with a barrier a chunk, took 520 us.
+// bytes a logit: 4095 x 100003 takes 240 us without alternatives (6.8 TB/s) and 276 us with 8 of them (5.9),
+// the rest being the bound's barriers and the chunks in which a candidate shows.  Collecting candidates for
+// the whole block, with a barrier a chunk, took 520 us.
 //
 // Candidates: the top-th largest of 64 group maxima of the first chunk is a lower bound of the row's
 // top-th logit, so that about top (1.1 to 1.4 times) of the first chunk's logits pass it, and top / 8192
@@ -254,17 +272,7 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
                     for (int i = 0; i < kVecs * 4; ++i)
                         if (inside >> i & 1) big = max(big, order_of(v[i]));
                 }
-#pragma unroll
-                for (int o = 1; o < T / 64; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-                if (threadIdx.x % (T / 64) == 0) cand.group[threadIdx.x / (T / 64)] = big;
-                __syncthreads();
-                if (warp == 0) {
-                    const uint32_t list = merge32(sort32(cand.group[lane], lane), sort32(cand.group[lane + 32], lane), lane);
-                    const uint32_t least = __shfl_sync(0xffffffffu, list, top - 1);
-                    if (lane == 0) cand.first = least;
-                }
-                __syncthreads();
-                const uint32_t least = cand.first;
+                const uint32_t least = group_bound<T>(cand, big, top, warp, lane);
                 if (__any_sync(0xffffffffu, big >= least)) {
 #pragma unroll
                     for (int i = 0; i < kVecs * 4; ++i) {
@@ -283,6 +291,12 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
                         if (__any_sync(0xffffffffu, yes)) push(yes, v[i], i);
                     }
                 }
+            }
+            // four chunks on, the running maxima give a bound four times as sharp
+            if (base - v0 == 3 * T * kVecs && v1 - base > 4 * T * kVecs) {
+                const uint32_t least = group_bound<T>(cand, order_of(m), top, warp, lane);
+                // (the lowest value is also the maximum of a thread that has seen nothing above -inf)
+                if (least > order_of(-FLT_MAX)) exceed = max(exceed, least + (least < kOrderInf));
             }
             if (held > kKeep) {
                 __syncwarp();
@@ -442,13 +456,22 @@ extern "C" int mcu_launch_logprobs(float* logp, float* lse, float* entropy, floa
                                    const float* x, const int32_t* id, int64_t rows, int64_t cols, int64_t x_s1, int top,
                                    cudaStream_t st, int* launches) {
     *launches = 1;
-    if (cols <= 4096)  // short rows: small blocks
-        return top ? run_rows<128, true>(logp, lse, entropy, top_logp, top_id, x, id, rows, cols, x_s1, top, 1, st)
-                   : run_rows<128, false>(logp, lse, entropy, top_logp, top_id, x, id, rows, cols, x_s1, top, 1, st);
-    int parts = 1;  // few rows: up to 8 CTAs share one, at least a chunk of 8192 logits each
-    while (parts < kMaxCluster && rows * parts < 148 && cols >= 2 * 8192 * (int64_t)parts) parts *= 2;
-    return top ? run_rows<512, true>(logp, lse, entropy, top_logp, top_id, x, id, rows, cols, x_s1, top, parts, st)
-               : run_rows<512, false>(logp, lse, entropy, top_logp, top_id, x, id, rows, cols, x_s1, top, parts, st);
+    const auto go = [&](auto threads, int parts) {
+        constexpr int T = decltype(threads)::value;
+        return top ? run_rows<T, true>(logp, lse, entropy, top_logp, top_id, x, id, rows, cols, x_s1, top, parts, st)
+                   : run_rows<T, false>(logp, lse, entropy, top_logp, top_id, x, id, rows, cols, x_s1, top, parts, st);
+    };
+    // Few rows: blocks of 512 threads, up to 8 of them sharing a row, at least a chunk of 8192 logits each.
+    // Many: an SM's 1024 threads as small blocks, whose barriers and ends overlap better, yet not so small
+    // that the first chunk says little about the row: 4095 x 100003 with 8 alternatives takes 302, 276 and
+    // 351 us with 512, 256 and 128 threads, 8192 x 5000 with 5 takes 200, 118 and 83 us.
+    if (rows < kSms && cols > 2048) {
+        int parts = 1;
+        while (parts < kMaxCluster && rows * parts < kSms && cols >= 2 * 8192 * (int64_t)parts) parts *= 2;
+        return go(std::integral_constant<int, 512>(), parts);
+    }
+    if (cols > 8192) return go(std::integral_constant<int, 256>(), 1);
+    return go(std::integral_constant<int, 128>(), 1);
 }
 
 extern "C" int mcu_launch_logprobs_backward(float* dx, const float* x, const int32_t* id, const float* lse,

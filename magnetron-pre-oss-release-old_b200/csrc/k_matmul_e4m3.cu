@@ -632,11 +632,12 @@ int run_pair(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, cons
                   (int)G, status);
 }
 
-// CTAs per tile: up to 8, while they all run at once and have at least two groups each.
+// CTAs per tile: up to 8, while they all run at once and have at least four groups each
+// (K = 2048, N = 4096, M = 4: 4 CTAs 4.5 us, 8 of two groups 4.95).
 template <int BN>
 int narrow_parts(int64_t tiles, int64_t G) {
     int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= sms() * NarrowCfg<BN>::PER_SM && G >= 4 * parts) parts *= 2;
+    while (parts < 8 && tiles * parts * 2 <= sms() * NarrowCfg<BN>::PER_SM && G >= 8 * parts) parts *= 2;
     return parts;
 }
 
