@@ -185,13 +185,13 @@ __device__ __forceinline__ uint32_t group_bound(Candidates<T>& cand, uint32_t bi
 // the rest being the bound's barriers and the chunks in which a candidate shows.  Collecting candidates for
 // the whole block, with a barrier a chunk, took 520 us.
 //
-// Candidates: the top-th largest of 64 group maxima of the first chunk is a lower bound of the row's
-// top-th logit, so that about top (1.1 to 1.4 times) of the first chunk's logits pass it, and top / 8192
-// of all later ones (T = 512): a warp looks at single elements only where the maximum of a lane's 16
-// passes.  Later elements have higher columns than the at least `top` that reached the bound in the
-// first chunk, so they have to exceed it; a bound that a warp's full buffer gives has to be reached only,
-// since another warp may still be at lower columns.  The order in which candidates are found does not
-// matter: keys are distinct and sorted at the end.
+// Candidates: the top-th largest of 64 group maxima of the first chunk is a lower bound of the row's top-th
+// logit, so that little more than `top` of the first chunk's logits pass it, as many in each later chunk, and
+// from the fifth on, with the maxima of four, a quarter of that: a warp looks at single elements only where
+// the maximum of a lane's 16 passes.  Later elements have higher columns than the at least `top` that reached
+// the bound, so they have to exceed it; a bound that a warp's full buffer gives has to be reached only, since
+// another warp may still be at lower columns.  The order in which candidates are found does not matter: keys
+// are distinct and sorted at the end.
 template <int T, bool TOP>
 __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__ logp, float* __restrict__ lse,
                                                              float* __restrict__ entropy, float* __restrict__ top_logp,

@@ -79,6 +79,22 @@ __device__ __forceinline__ bool warp_wait2(uint64_t* bar0, uint32_t parity0, uin
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// Four f32 of shared memory times s, two packed multiplications (each product rounded to nearest as alone).
+__device__ __forceinline__ float4 lds4_times(uint32_t at, float s) {
+    float4 v;
+    asm volatile(
+        "{\n\t.reg .b64 a, b, s;\n\t"
+        "ld.shared.v2.b64 {a, b}, [%4];\n\t"
+        "mov.b64 s, {%5, %5};\n\t"
+        "mul.rn.f32x2 a, a, s;\n\t"
+        "mul.rn.f32x2 b, b, s;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t"
+        "mov.b64 {%2, %3}, b;\n\t}"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+        : "r"(at), "f"(s)
+        : "memory");
+    return v;
+}
 __device__ __forceinline__ float lds1(uint32_t a) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
@@ -317,10 +333,7 @@ __global__ void __maxnreg__(kPairLaunch)
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         float4 s = make_float4(sc, sc, sc, sc);
-                        if (YROW) {
-                            const float4 y = lds4(py + (half * 128 + c * 32 + j) * 4);
-                            s = make_float4(__fmul_rn(sc, y.x), __fmul_rn(sc, y.y), __fmul_rn(sc, y.z), __fmul_rn(sc, y.w));
-                        }
+                        if (YROW) s = lds4_times(py + (half * 128 + c * 32 + j) * 4, sc);
                         float* d = sum + c * 32 + j;
                         d[0] = __fmaf_rn(__uint_as_float(v[j]), s.x, d[0]);
                         d[1] = __fmaf_rn(__uint_as_float(v[j + 1]), s.y, d[1]);
