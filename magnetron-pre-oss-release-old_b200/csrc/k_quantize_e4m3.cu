@@ -60,21 +60,21 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, sh_top[0][i]);
-        const float sc = e4m3_scale(top), inv = __frcp_rn(sc);
-        if (threadIdx.x == 0) s[TRANSPOSE ? c0 / 128 * groups + r0 / 128 : r0 / 128 * groups + c0 / 128] = sc;
+        const E4m3Group gr = e4m3_group(top);
+        if (threadIdx.x == 0) s[TRANSPOSE ? c0 / 128 * groups + r0 / 128 : r0 / 128 * groups + c0 / 128] = gr.scale;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][j] *= inv;
+            for (int j = 0; j < 4; ++j) v[i][j] *= gr.factor;
     } else if constexpr (!TRANSPOSE) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const uint32_t top = __reduce_max_sync(
                 0xffffffffu, max(max(abs_bits(v[i][0]), abs_bits(v[i][1])), max(abs_bits(v[i][2]), abs_bits(v[i][3]))));
-            const float sc = e4m3_scale(top), inv = __frcp_rn(sc);
-            if (lane == 0 && r + i < rows) s[(int64_t)(r + i) * groups + c0 / 128] = sc;
+            const E4m3Group gr = e4m3_group(top);
+            if (lane == 0 && r + i < rows) s[(int64_t)(r + i) * groups + c0 / 128] = gr.scale;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][j] *= inv;
+            for (int j = 0; j < 4; ++j) v[i][j] *= gr.factor;
         }
     } else {
 #pragma unroll
@@ -90,10 +90,10 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = max(top, sh_top[i][col(j)]);
-            const float sc = e4m3_scale(top), inv = __frcp_rn(sc);
-            if (warp == 0 && c0 + col(j) < cols) s[(int64_t)(c0 + col(j)) * groups + r0 / 128] = sc;
+            const E4m3Group gr = e4m3_group(top);
+            if (warp == 0 && c0 + col(j) < cols) s[(int64_t)(c0 + col(j)) * groups + r0 / 128] = gr.scale;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i][j] *= inv;
+            for (int i = 0; i < 16; ++i) v[i][j] *= gr.factor;
         }
     }
     if constexpr (!TRANSPOSE) {

@@ -96,9 +96,9 @@ __device__ __forceinline__ void norm_group(const NormArgs& a, const float (&t)[4
     if (a.y) store_group<VEC>(a.y + o, v, g * 128, a.cols, lane);
     if (a.q) {
         const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3]))));
-        const float sc = e4m3_scale(top), inv = __frcp_rn(sc);
-        if (lane == 0) a.s[row * groups + g] = sc;
-        const uint32_t b = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+        const E4m3Group gr = e4m3_group(top);
+        if (lane == 0) a.s[row * groups + g] = gr.scale;
+        const uint32_t b = e4m3x4(v[0] * gr.factor, v[1] * gr.factor, v[2] * gr.factor, v[3] * gr.factor);
         uint8_t* q = a.q + (row * groups + g) * 128;
         if (VEC) {
             *(uint32_t*)(q + lane * 4) = b;

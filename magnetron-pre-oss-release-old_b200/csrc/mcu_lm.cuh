@@ -21,13 +21,16 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 // |v| as an integer whose order is the magnitude's, NaN above infinity: a maximum over these keeps NaN.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// A group's scale from the bits of its largest magnitude.  Values are multiplied by its reciprocal: that
-// rounds twice in f32 before e4m3 rounds, which moves about one value in 10^7 (those within 2^-23 of a tie)
-// to the neighbour that lies as near.  The corrected division (two fused multiply-adds a value) cost 4 to 15 %
-// of the kernels and still rounds once in f32.
-__device__ __forceinline__ float e4m3_scale(uint32_t amax_bits) {
-    const float a = __uint_as_float(amax_bits);
-    return __fdiv_rn(a < kE4m3Tiny ? kE4m3Tiny : a, kE4m3Max);
+// A group's scale amax / 448 and the factor 448 / amax of its values, from the bits of its largest
+// magnitude.  A value is rounded twice in f32 (the factor, the product) before e4m3 rounds it, which moves
+// about one in 10^7, those within 2^-23 of a tie, to the neighbour that lies as near.  The corrected division
+// (two fused multiply-adds a value) cost 4 to 15 % of the kernels and still rounds once in f32.
+struct E4m3Group {
+    float scale, factor;
+};
+__device__ __forceinline__ E4m3Group e4m3_group(uint32_t amax_bits) {
+    const float a = __uint_as_float(amax_bits), m = a < kE4m3Tiny ? kE4m3Tiny : a;
+    return E4m3Group{__fdiv_rn(m, kE4m3Max), __fdiv_rn(kE4m3Max, m)};
 }
 
 __device__ __forceinline__ float warp_sum_f(float v) {

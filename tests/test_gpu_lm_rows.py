@@ -79,8 +79,8 @@ def check_quantized(q, s, v, block, rel):
     assert np.all(np.abs(s - want) <= want * (rel + 2 * U))  # the maximum's own error, the division
     each = np.repeat(np.repeat(s.astype(np.float64), 128, 0)[:rows] if block else s.astype(np.float64), 128, 1)[:, :cols]
     t = v / each
-    # t = v * (1 / s): the value's error, the reciprocal's and the product's rounding, then half a step of
-    # the result (at the larger magnitude where rounding crosses a power of two)
+    # q is formed from v (448 / amax): the value's error, the factor's and the product's rounding and that of
+    # s here, then half a step of the result (at the larger magnitude where rounding crosses a power of two)
     slack = np.abs(t) * (rel + 3 * U)
     assert np.all(np.abs(VALUES[q[:, :cols]] - t) <= half_step(np.abs(t) + slack) + slack)
 
