@@ -266,8 +266,8 @@ MAG_CUDA_EXPORT int mag_cuda_img_draw_text(mag_compute_device_t* dvc, mag_tensor
  * infinite and itself NaN, and both reach every product that reads the group.
  *
  * Calls check their arguments before any work (MAG_CUDA_E_INVALID), take rows = 0 as nothing to do,
- * and may be captured into a CUDA graph of mag_cuda_stream: a captured call allocates nothing that
- * outlives the graph, and returns MAG_CUDA_E_INVALID for tensor storage that was never written or
+ * come from one host thread at a time, and may be captured into a CUDA graph of mag_cuda_stream after
+ * one eager call of the kind: a captured call allocates nothing that outlives the graph, and returns MAG_CUDA_E_INVALID for tensor storage that was never written or
  * has an asynchronous copy in flight (neither a pending clear nor a wait belongs in the graph).
  * Results depend on the inputs alone: sums are formed in a fixed order, without atomics. */
 #define MAG_CUDA_E4M3_ROW 0

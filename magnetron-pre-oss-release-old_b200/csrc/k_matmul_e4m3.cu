@@ -43,7 +43,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[32]) {
         : "r"(taddr)
         : "memory");
 }
-// One lane of a converged warp.  The narrow kernel's roles run as whole warps and elect the lane only around
+// One lane of a converged warp.  The producer and MMA roles run as whole warps and elect the lane only around
 // the issue, so that waits, loop and descriptors stay warp-uniform: with a branch on the lane number around
 // the role each MMA took about 80 cycles to issue.
 __device__ __forceinline__ bool elect_one() {

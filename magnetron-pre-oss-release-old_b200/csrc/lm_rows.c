@@ -19,10 +19,10 @@ static int bad_matrix(int64_t rows, int64_t cols) {
     return rows < 0 || rows >= MCU_MAX_DIM || cols < 1 || cols >= MCU_MAX_DIM || rows * cols > ((int64_t)1 << 42);
 }
 
-int64_t mag_cuda_e4m3_ld(int64_t cols) { return cols > 0 ? (cols + 127) / 128 * 128 : 0; }
+int64_t mag_cuda_e4m3_ld(int64_t cols) { return cols > 0 && cols < MCU_MAX_DIM ? (cols + 127) / 128 * 128 : 0; }
 
 int64_t mag_cuda_e4m3_scales(int64_t rows, int64_t cols, int group) {
-    if (rows <= 0 || cols <= 0 || (group != MAG_CUDA_E4M3_ROW && group != MAG_CUDA_E4M3_BLOCK)) return 0;
+    if (rows <= 0 || rows >= MCU_MAX_DIM || cols <= 0 || cols >= MCU_MAX_DIM || (group != MAG_CUDA_E4M3_ROW && group != MAG_CUDA_E4M3_BLOCK)) return 0;
     return (group == MAG_CUDA_E4M3_BLOCK ? (rows + 127) / 128 : rows) * (mag_cuda_e4m3_ld(cols) / 128);
 }
 

@@ -474,6 +474,8 @@ class Device:
     # matrices (a Tensor of shape (cols, rows)); e4m3 operands and int32 ids are raw bytes in Tensors.
     def e4m3(self, rows: int, cols: int, block: bool = False):
         """Storage of an e4m3 operand: its bytes [rows][e4m3_ld(cols)] and its scales."""
+        if rows < 1 or cols < 1:
+            raise ValueError(f"an e4m3 operand of {rows} x {cols} values")
         g = e4m3_ld(cols) // 128
         return self.tensor((32 * g, rows)), self.tensor((g, -(-rows // 128) if block else rows))
 

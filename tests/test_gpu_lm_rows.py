@@ -587,6 +587,81 @@ def test_logprobs_gradient_against_differences():
     assert abs(got.sum() - diff) <= 1e-5 * np.abs(got).sum()
 
 
+# ------------------------------------------------------------- offsets past 32 bits
+def test_offsets_past_32_bits():
+    """Matrices of more than 2^32 bytes (and 2^31 values): their last rows are right."""
+    import torch
+    d = device()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    dev = f"cuda:{d.ordinal}"
+    last = 3
+    # log probabilities: three rows 1.5 * 10^9 logits apart
+    cols, stride = 5000, 1_500_000_000
+    x = torch.empty(3 * stride, device=dev)
+    rows = torch.randn(3, cols, device=dev, generator=g)
+    for i in range(3):
+        x[i * stride:i * stride + cols] = rows[i]
+    ids = torch.tensor([1, 2, cols - 1], dtype=torch.int32, device=dev)
+    lse, logp, one = (torch.ones(3, device=dev) for _ in range(3))
+    torch.cuda.synchronize()
+    d.token_logprobs(3, cols, x.data_ptr(), ids.data_ptr(), logp=logp.data_ptr(), lse=lse.data_ptr(), x_stride=stride)
+    d.token_logprobs_backward(3, cols, x.data_ptr(), x.data_ptr(), ids.data_ptr(), lse.data_ptr(), None, one.data_ptr(),
+                              x_stride=stride, dx_stride=stride)
+    d.sync()
+    r64 = rows.double()
+    want = r64 - torch.logsumexp(r64, 1, keepdim=True)
+    assert torch.all((logp - want.gather(1, ids[:, None].long())[:, 0]).abs() <= 1e-5)
+    grad = -want.exp()
+    grad[torch.arange(3), ids.long()] += 1
+    for i in range(3):
+        assert torch.all((x[i * stride:i * stride + cols] - grad[i]).abs() <= 1e-5)
+    del x
+    # norm and quantiser: 2.2 * 10^9 values
+    n, c = 550_000, 4000
+    x = torch.randn(n, c, device=dev, generator=g)
+    w = torch.ones(c, device=dev)
+    q = torch.empty(n, MB.e4m3_ld(c), dtype=torch.uint8, device=dev)
+    s = torch.empty(n, MB.e4m3_ld(c) // 128, device=dev)
+    tail = x[-last:].double()
+    torch.cuda.synchronize()
+    d.rmsnorm_rows(n, c, x.data_ptr(), w.data_ptr(), EPS, y=x.data_ptr(), q=q.data_ptr(), q_scale=s.data_ptr())
+    d.sync()
+    v = (tail / (tail.square().mean(1, keepdim=True) + EPS).sqrt()).cpu().numpy()
+    assert np.all(np.abs(x[-last:].cpu().numpy() - v) <= np.abs(v) * norm_rel(c))
+    check_quantized(q[-last:].cpu().numpy(), s[-last:].cpu().numpy(), v, False, norm_rel(c))
+    q.zero_()
+    tail = x[-last:].cpu().numpy().astype(np.float64)
+    torch.cuda.synchronize()
+    d.quantize_e4m3(n, c, x.data_ptr(), q.data_ptr(), s.data_ptr())
+    d.sync()
+    check_quantized(q[-last:].cpu().numpy(), s[-last:].cpu().numpy(), tail, False, 0.0)
+    qt = torch.empty(c, MB.e4m3_ld(n), dtype=torch.uint8, device=dev)
+    st = torch.empty(c, MB.e4m3_ld(n) // 128, device=dev)
+    end = n // 128 * 128 - 256
+    col = x[end:, -last:].cpu().numpy().astype(np.float64).T
+    torch.cuda.synchronize()
+    d.quantize_e4m3(n, c, x.data_ptr(), qt.data_ptr(), st.data_ptr(), transpose=True)
+    d.sync()
+    check_quantized(qt[-last:, end:].cpu().numpy(), st[-last:, end // 128:].cpu().numpy(), col, False, 0.0)
+    del x, q, qt
+    # product: 70000 x 40000 results, by pairs, and 20 x 120 million by narrow tiles
+    for m, n in ((70_000, 40_000), (20, 120_000_000)):
+        xq, xs, xv = operand(last, 128, False, 30)
+        yq, ys, yv = operand(last, 128, False, 31)
+        bx, by = (torch.zeros(k, 128, dtype=torch.uint8, device=dev) for k in (m, n))
+        sx, sy = (torch.ones(k, 1, device=dev) for k in (m, n))
+        bx[-last:], by[-last:] = torch.from_numpy(xq).to(dev), torch.from_numpy(yq).to(dev)
+        sx[-last:], sy[-last:] = torch.from_numpy(xs).to(dev), torch.from_numpy(ys).to(dev)
+        r = torch.empty(m, n, device=dev)
+        torch.cuda.synchronize()
+        d.matmul_e4m3(m, 128, n, r.data_ptr(), bx.data_ptr(), sx.data_ptr(), by.data_ptr(), sy.data_ptr(), y_block=False)
+        d.sync()
+        assert np.all(np.abs(r[-last:, -last:].cpu().numpy() - xv @ yv.T) <= product_bound(xv, yv, 1))
+        assert not r[-last:, 1000:2000].any() and not r[:m - last, -last:].any()  # the rows of zeros
+        del bx, by, sx, sy, r
+    torch.cuda.empty_cache()
+
+
 # ---------------------------------------------------------------- as they are used
 def test_layer_and_loss_together():
     """One 8-bit layer with its norm, the loss on its logits, and both gradients of the layer."""

@@ -18,7 +18,7 @@ BIG = 1 << 31
 def test_operand_layout():
     for cols, ld in ((1, 128), (127, 128), (128, 128), (129, 256), (5000, 5120)):
         assert L.mag_cuda_e4m3_ld(cols) == MB.e4m3_ld(cols) == ld
-    assert L.mag_cuda_e4m3_ld(0) == 0 and L.mag_cuda_e4m3_ld(-5) == 0
+    assert L.mag_cuda_e4m3_ld(0) == 0 and L.mag_cuda_e4m3_ld(-5) == 0 and L.mag_cuda_e4m3_ld((1 << 63) - 1) == 0
     assert L.mag_cuda_e4m3_scales(5, 300, MB.E4M3_ROW) == 15
     assert L.mag_cuda_e4m3_scales(129, 300, MB.E4M3_BLOCK) == 6
     assert L.mag_cuda_e4m3_scales(5, 300, 2) == 0 and L.mag_cuda_e4m3_scales(-1, 300, 0) == 0
@@ -106,3 +106,6 @@ def test_python_refusals_raise():
         d.quantize_e4m3(4, 0, A, A, A)
     with pytest.raises(MB.CudaError):
         d.token_logprobs(4, 8, A, top=40, top_id=A)
+    for rows, cols in ((0, 5), (5, 0)):
+        with pytest.raises(ValueError):
+            d.e4m3(rows, cols)
