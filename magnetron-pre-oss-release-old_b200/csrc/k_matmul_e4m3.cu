@@ -392,7 +392,7 @@ __global__ void __maxnreg__(kPairLaunch)
 constexpr int kNarrowAcc = 4;     // accumulators, so that the MMAs run ahead of the epilogue
 constexpr int kNarrowPanel = 16;  // groups of x's scales staged at a time
 
-template <int BN>
+template <int BN, bool YROW>
 struct NarrowCfg {
     static constexpr int A = 128 * 128, B = BN * 128, STAGE = A + B;
     static constexpr int STAGES = BN == 32 ? 5 : 6;
@@ -400,18 +400,21 @@ struct NarrowCfg {
     static constexpr int EPI = BN >= 128 ? 16 : 4;  // epilogue warps: four quadrants of lanes, 16 or 32 columns each
     static constexpr int WC = BN * 4 / EPI;       // columns of a warp
     static constexpr int THREADS = 64 + 32 * EPI;
-    static constexpr int PANEL = STAGES * STAGE;  // kNarrowPanel x BN scales of x
-    static constexpr int BARS = PANEL + 16 * BN * 4;
+    // scales of y per row: staged like x's where the epilogue's warps are many; the few warps of a narrow tile
+    // fetch their own (4 x 4096 x 4096: 5.7 us, 6.9 staged; 100 x 4096 x 14336: 22.4 us, 18.9 staged)
+    static constexpr bool STAGE_Y = YROW && BN >= 128;
+    static constexpr int PANEL = STAGES * STAGE;  // kNarrowPanel x BN scales of x, then x 128 of y
+    static constexpr int BARS = PANEL + kNarrowPanel * (BN + (STAGE_Y ? 128 : 0)) * 4;
     static constexpr int SMEM = BARS + 512 + 1024;
     static constexpr int COLS = kNarrowAcc * BN;
     static_assert(PER_SM * SMEM <= 227 * 1024 && 128 * BN * 4 <= STAGES * STAGE, "must fit shared memory");
 };
 template <int BN, bool YROW>
-__global__ void __launch_bounds__(NarrowCfg<BN>::THREADS, NarrowCfg<BN>::PER_SM)
+__global__ void __launch_bounds__(NarrowCfg<BN, YROW>::THREADS, NarrowCfg<BN, YROW>::PER_SM)
     gemm_e4m3_narrow(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
                      const float* __restrict__ xs, const float* __restrict__ ys, float* __restrict__ r, int M, int N, int G,
                      int parts, int per, int* status) {
-    using C = NarrowCfg<BN>;
+    using C = NarrowCfg<BN, YROW>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* full = (uint64_t*)(smem + C::BARS);
@@ -493,35 +496,41 @@ __global__ void __launch_bounds__(NarrowCfg<BN>::THREADS, NarrowCfg<BN>::PER_SM)
         float sum[C::WC];  // this lane's row of y against the warp's rows of x
 #pragma unroll
         for (int j = 0; j < C::WC; ++j) sum[j] = 0.0f;
-        // x's scales, BN rows x 16 groups at a time (a block's scale of y already multiplied in), the next
-        // panel's values fetched one panel ahead
-        constexpr int PV = BN * kNarrowPanel / (32 * C::EPI);
-        float ahead[PV];
+        // the scales of x's BN rows (a block's scale of y already multiplied in) and of y's 128 rows, 16 groups
+        // at a time, fetched one panel ahead
+        constexpr int PX = BN * kNarrowPanel / (32 * C::EPI), PY = C::STAGE_Y ? 128 * kNarrowPanel / (32 * C::EPI) : 0;
+        float ahead[PX + PY];
         const auto fetch = [&](int it) {
 #pragma unroll
-            for (int i = 0; i < PV; ++i) {
+            for (int i = 0; i < PX; ++i) {
                 const int e = tid + i * 32 * C::EPI, m = m0 + e / kNarrowPanel, g = it + e % kNarrowPanel;
                 const bool in = m < M && g < ng;
                 ahead[i] = in ? __ldg(xs + (int64_t)m * G + g0 + g) : 0.0f;
                 if (!YROW && in) ahead[i] = __fmul_rn(ahead[i], __ldg(py + g));
             }
+#pragma unroll
+            for (int i = 0; i < PY; ++i) {
+                const int e = tid + i * 32 * C::EPI, y = n0 + e / kNarrowPanel, g = it + e % kNarrowPanel;
+                ahead[PX + i] = y < N && g < ng ? __ldg(ys + (int64_t)y * G + g0 + g) : 0.0f;
+            }
         };
         fetch(0);
-        float ay = YROW && ng > 0 ? __ldg(py) : 0.0f;
+        float own_y = YROW && !C::STAGE_Y && ng > 0 ? __ldg(py) : 1.0f;
         bool ready = false;
         for (uint32_t it = 0; it < (uint32_t)ng; ++it) {
             const uint32_t b = it % kNarrowAcc, ap = it / kNarrowAcc & 1;
             if ((it & (kNarrowPanel - 1)) == 0) {
                 if (it) bar_named(1, 32 * C::EPI);
 #pragma unroll
-                for (int i = 0; i < PV; ++i) {
-                    const int e = tid + i * 32 * C::EPI;
-                    panel[e % kNarrowPanel * BN + e / kNarrowPanel] = ahead[i];
+                for (int i = 0; i < PX + PY; ++i) {
+                    const int e = tid + (i < PX ? i : i - PX) * 32 * C::EPI, row = e / kNarrowPanel, g = e % kNarrowPanel;
+                    panel[i < PX ? g * BN + row : kNarrowPanel * BN + g * 128 + row] = ahead[i];
                 }
                 bar_named(1, 32 * C::EPI);
                 if (it + kNarrowPanel < (uint32_t)ng) fetch(it + kNarrowPanel);
             }
-            const float ny = YROW && it + 1 < (uint32_t)ng ? __ldg(py + it + 1) : 0.0f;
+            const float ay = C::STAGE_Y ? panel[kNarrowPanel * BN + (it & (kNarrowPanel - 1)) * 128 + q * 32 + lane] : own_y;
+            if (YROW && !C::STAGE_Y && it + 1 < (uint32_t)ng) own_y = __ldg(py + it + 1);
             // (a warp that gives up goes on without waiting, so that the named barriers stay matched)
             if (!ready) ok &= warp_wait(&acc_full[b], ap, ab, 18);
             tc_fence_after();
@@ -537,14 +546,13 @@ __global__ void __launch_bounds__(NarrowCfg<BN>::THREADS, NarrowCfg<BN>::PER_SM)
             ready = it + 1 < (uint32_t)ng && __all_sync(0xffffffffu, mbar_ready(&acc_full[(it + 1) % kNarrowAcc], (it + 1) / kNarrowAcc & 1));
 #pragma unroll
             for (int j = 0; j < C::WC; j += 4) {
-                const float4 x4 = lds4(pan + j * 4);
+                const float4 x4 = YROW ? lds4_times(pan + j * 4, ay) : lds4(pan + j * 4);
                 const uint32_t* w = v + j;
-                sum[j] = __fmaf_rn(__uint_as_float(w[0]), YROW ? __fmul_rn(ay, x4.x) : x4.x, sum[j]);
-                sum[j + 1] = __fmaf_rn(__uint_as_float(w[1]), YROW ? __fmul_rn(ay, x4.y) : x4.y, sum[j + 1]);
-                sum[j + 2] = __fmaf_rn(__uint_as_float(w[2]), YROW ? __fmul_rn(ay, x4.z) : x4.z, sum[j + 2]);
-                sum[j + 3] = __fmaf_rn(__uint_as_float(w[3]), YROW ? __fmul_rn(ay, x4.w) : x4.w, sum[j + 3]);
+                sum[j] = __fmaf_rn(__uint_as_float(w[0]), x4.x, sum[j]);
+                sum[j + 1] = __fmaf_rn(__uint_as_float(w[1]), x4.y, sum[j + 1]);
+                sum[j + 2] = __fmaf_rn(__uint_as_float(w[2]), x4.z, sum[j + 2]);
+                sum[j + 3] = __fmaf_rn(__uint_as_float(w[3]), x4.w, sum[j + 3]);
             }
-            ay = ny;
         }
         if (ok && parts == 1 && n < N) {
 #pragma unroll
@@ -650,7 +658,7 @@ int run_pair(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, cons
 template <int BN>
 int narrow_parts(int64_t tiles, int64_t G) {
     int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= sms() * NarrowCfg<BN>::PER_SM && G >= 8 * parts) parts *= 2;
+    while (parts < 8 && tiles * parts * 2 <= sms() * NarrowCfg<BN, false>::PER_SM && G >= 8 * parts) parts *= 2;
     return parts;
 }
 
@@ -662,21 +670,21 @@ int run_narrow(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, co
     if (tiles * parts > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const int per = (int)((G + parts - 1) / parts);
     if (y_block)
-        return launch<gemm_e4m3_narrow<BN, false>>(tiles * parts, NarrowCfg<BN>::THREADS, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
+        return launch<gemm_e4m3_narrow<BN, false>>(tiles * parts, NarrowCfg<BN, false>::THREADS, NarrowCfg<BN, false>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
                       (int)N, (int)G, parts, per, status);
-    return launch<gemm_e4m3_narrow<BN, true>>(tiles * parts, NarrowCfg<BN>::THREADS, NarrowCfg<BN>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
+    return launch<gemm_e4m3_narrow<BN, true>>(tiles * parts, NarrowCfg<BN, true>::THREADS, NarrowCfg<BN, true>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
                   (int)N, (int)G, parts, per, status);
 }
 
 // Both kernels run in waves of the GPU: 148 tiles of 128 x 128 at a time, or 74 of 256 x 256.  Measured with
-// N = 4096 and 14336 and K = 256 to 8192: a narrow wave takes 4 us and 0.41 us a group of K (0.50 with
+// N = 4096 and 14336 and K = 256 to 8192: a narrow wave takes 4 us and 0.41 us a group of K (0.47 with
 // scales of y per row); the persistent pairs take 8.5 us in all and 0.46 us a group and wave (7.3 and 0.80).
 // So the pairs win once their larger tiles fill a wave: 512 x 4096 x 4096 takes 17 us narrow and 23 in
 // pairs, 1024 x 4096 x 4096 33 us narrow and 23 in pairs.
 bool pair_is_faster(int64_t M, int64_t N, int64_t G, int y_block) {
     const int64_t narrow = (M + 127) / 128 * ((N + 127) / 128), pair = (M + 255) / 256 * ((N + 255) / 256), n = sms();
     const int64_t parts = narrow_parts<128>(narrow, G), per = (G + parts - 1) / parts;
-    const int64_t tn = (narrow * parts + n - 1) / n * (400 + (y_block ? 41 : 50) * per);
+    const int64_t tn = (narrow * parts + n - 1) / n * (400 + (y_block ? 41 : 47) * per);
     const int64_t tp = (pair + n / 2 - 1) / (n / 2) * (y_block ? 46 : 80) * G + (y_block ? 850 : 730);
     return tp < tn;
 }
