@@ -5,6 +5,7 @@
 #include "mcu_kernels.h"
 #include "mcu_launch.cuh"
 #include "mcu_lm.cuh"
+#include "mcu_tc.cuh"
 
 using namespace mcu;
 
@@ -197,7 +198,36 @@ struct BackArgs {
     const float* dh;
     int64_t rows;
     int cols;
+    int parts;    // blocks of a cluster, which share every row
+    int* status;  // of its bounded waits
 };
+
+constexpr int kBackV = 4;         // groups a warp
+constexpr int kBackWarps = 16;    // warps of a block at most
+constexpr int kBackAhead = 12;    // and of one that fetches dh a row ahead
+constexpr int kBackCluster = 8;   // blocks of a cluster at most
+
+// Sum over the warps of the cluster's blocks, the same on every thread: each warp sends its share to every
+// block's sh [parts][kBackWarps], counted on that block's mbarrier.  (A cluster barrier instead would wait for
+// the row's stores and loads as well: 4096 x 16384 takes 217 us so, 187 this way.)  Two arrays and mbarriers
+// take turns: whoever sends to one again has received what every warp sent after its last reading.
+__device__ __forceinline__ float cluster_sum(float v, float* sh, uint64_t* bar, uint32_t parity, int warp, int lane, int warps, int rank,
+                                             int parts, const Abort& ab) {
+    v = warp_sum_f(v);
+    if (threadIdx.x == 0) mbar_expect_tx(bar, (uint32_t)(parts * warps * 4));
+    if (lane < parts)
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(
+                         mapa_rank(smem_u32(sh + rank * kBackWarps + warp), lane)),
+                     "f"(v), "r"(mapa_rank(smem_u32(bar), lane))
+                     : "memory");
+    __syncwarp();
+    mbar_wait(bar, parity, ab, 24);
+    __syncwarp();
+    float t = 0.0f;
+    for (int i = lane; i < parts * kBackWarps; i += 32)
+        if (i % kBackWarps < warps) t += sh[i];
+    return warp_sum_f(t);
+}
 
 // A block goes through rows blockIdx.x, + grid, ...; a thread keeps the same columns in every row and so its
 // sums for the weight's gradient in registers.  The next row's dy and h are in flight during the row's
@@ -205,23 +235,38 @@ struct BackArgs {
 // (4099 x 5000 took 71 us, now 64).  Bound by HBM, 12 bytes read and 4 written a value: 8192 x 8192 runs at
 // 6.5 TB/s.  Rows that leave an SM with 9 to 12 warps keep too few bytes in flight that way; their blocks
 // have the registers to fetch dh a row ahead too (AHEAD: 57.5 us, 5.7 TB/s; two blocks an SM with half the
-// registers each spilled and took 66 us).
-constexpr int kBackV = 4;  // groups a warp
-
-template <bool VEC, bool AHEAD>
-__global__ void __launch_bounds__(AHEAD ? 384 : 512, 1) rmsnorm_backward_row(const BackArgs a) {
+// registers each spilled and took 66 us).  Rows that do not fit a block's registers (8192 columns) are shared
+// by a cluster (CLUSTER): 4096 x 12288 in 126 us, 6.4 TB/s; in two passes over the row and one for the weight's
+// gradient it took 281.
+template <bool VEC, bool AHEAD, bool CLUSTER>
+__global__ void __launch_bounds__(32 * (AHEAD ? kBackAhead : kBackWarps), 1) rmsnorm_backward_row(const BackArgs a) {
     constexpr int V = kBackV;
-    __shared__ float sh[2][16];
+    __shared__ float sh[2][kBackWarps * (CLUSTER ? kBackCluster : 1)];
+    __shared__ uint64_t bars[2];
+    __shared__ volatile int gave_up;
+    const Abort ab{&gave_up, a.status};
+    if (CLUSTER) {
+        if (threadIdx.x == 0) {
+            gave_up = 0;
+            mbar_init(&bars[0], 1);
+            mbar_init(&bars[1], 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
     pdl_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    const auto base = [&](int i) { return (warp + i * warps) * 128; };
+    const int parts = CLUSTER ? a.parts : 1, rank = CLUSTER ? (int)blockIdx.x % parts : 0;
+    const int first = CLUSTER ? (int)blockIdx.x / parts : (int)blockIdx.x, step = CLUSTER ? (int)gridDim.x / parts : (int)gridDim.x;
+    const auto base = [&](int i) { return ((rank * V + i) * warps + warp) * 128; };
     float sum[V][4], dy[V][4], h[V][4];
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) sum[i][j] = 0.0f;
-    int turn = 0;
-    int64_t row = blockIdx.x;
+    uint32_t turn = 0;
+    int64_t row = first;
     float root = __ldg(a.rstd + row);
 #pragma unroll
     for (int i = 0; i < V; ++i) load_group<VEC>(dy[i], a.dy + row * a.cols, base(i), a.cols, lane);
@@ -232,8 +277,9 @@ __global__ void __launch_bounds__(AHEAD ? 384 : 512, 1) rmsnorm_backward_row(con
 #pragma unroll
         for (int i = 0; i < V; ++i) load_group<VEC>(dh[AHEAD ? i : 0], a.dh + row * a.cols, base(i), a.cols, lane);
     }
-    for (; row < a.rows; row += gridDim.x, turn ^= 1) {
-        const int64_t o = row * a.cols, next = row + gridDim.x;
+    if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every block of the cluster runs
+    for (; row < a.rows; row += step, ++turn) {
+        const int64_t o = row * a.cols, next = row + step;
         float g[V][4], u[V][4], hn[V][4], gn[AHEAD ? V : 1][4];  // the residual path's gradient, then the result; dy w; the next h
         if (!AHEAD && a.dh) {
 #pragma unroll
@@ -263,7 +309,9 @@ __global__ void __launch_bounds__(AHEAD ? 384 : 512, 1) rmsnorm_backward_row(con
                 for (int i = 0; i < V; ++i) load_group<VEC>(gn[AHEAD ? i : 0], a.dh + next * a.cols, base(i), a.cols, lane);
             }
         }
-        const float f = root * root * __fdiv_rn(block_sum(along, sh[turn], warp, lane, warps), (float)a.cols);
+        const float all = CLUSTER ? cluster_sum(along, sh[turn & 1], &bars[turn & 1], turn >> 1 & 1, warp, lane, warps, rank, parts, ab)
+                                  : block_sum(along, sh[turn & 1], warp, lane, warps);
+        const float f = root * root * __fdiv_rn(all, (float)a.cols);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
 #pragma unroll
@@ -279,11 +327,12 @@ __global__ void __launch_bounds__(AHEAD ? 384 : 512, 1) rmsnorm_backward_row(con
     }
     if (a.part) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) store_group<VEC>(a.part + (int64_t)blockIdx.x * a.cols, sum[i], base(i), a.cols, lane);
+        for (int i = 0; i < V; ++i) store_group<VEC>(a.part + (int64_t)first * a.cols, sum[i], base(i), a.cols, lane);
     }
+    if (CLUSTER) cluster_sync();  // no block leaves while a peer may still send to it
 }
 
-// Rows that do not fit: dx in two passes over the row, dw's partial sums by columns over a share of rows.
+// Rows that do not fit a cluster either: dx in two passes over the row, dw's partial sums by columns over a share of rows.
 template <bool VEC>
 __global__ void __launch_bounds__(1024) rmsnorm_backward_wide(const BackArgs a) {
     __shared__ float sh[32];
@@ -349,13 +398,24 @@ __global__ void __launch_bounds__(1024) rmsnorm_weight_sum(float* __restrict__ d
 constexpr int kSms = 148;
 constexpr int kWideParts = 64;
 
-// Warps of a block of the backward pass (0: rows too wide for its registers), and its blocks: as many as run
-// at once (16 warps an SM by their registers).
+// Blocks that share a row in the backward pass: rows wider than a block's registers take an even number, since
+// clusters of three found no room when the kernel before left the SMs in an odd order (4096 x 16384: 253 us, 187
+// in twos).  Blocks of up to 12 warps, which fetch dh ahead, are the faster ones (4096 x 32768: 353 us in sixes,
+// 400 in fours), but not by enough to take four instead of two (194 us and 187).
+int back_parts(int64_t cols) {
+    if (cols <= kBackWarps * kBackV * 128) return 1;
+    int parts = 2;
+    while (parts < kBackCluster && cols > (int64_t)parts * (parts == 2 ? kBackWarps : kBackAhead) * kBackV * 128) parts += 2;
+    return parts;
+}
+// Warps of a block (0: rows too wide for a cluster's registers), and the rows in work at once: as many as the
+// GPU holds (16 warps an SM by their registers).
 int back_warps(int64_t cols) {
-    const int64_t w = ((cols + 127) / 128 + kBackV - 1) / kBackV;
-    return w <= 16 ? (int)w : 0;
+    const int64_t each = 128 * kBackV * back_parts(cols), w = (cols + each - 1) / each;
+    return w <= kBackWarps ? (int)w : 0;
 }
 int64_t back_blocks(int64_t rows, int64_t cols) {
+    if (back_parts(cols) > 1) return rows < kSms / back_parts(cols) ? rows : kSms / back_parts(cols);
     // (few rows: about four a block, or one where that leaves SMs idle, since every block adds a part to dw)
     const int64_t all = kSms * (16 / back_warps(cols)), four = rows < kSms ? rows : rows / 4 > kSms ? rows / 4 : kSms;
     return four < all ? four : all;
@@ -383,12 +443,37 @@ int run_norm(const NormArgs& a, int64_t rows, cudaStream_t st) {
     return go(rmsnorm_row<8, 8, VEC>, rows, 256, st, a);
 }
 
+// *blocks: the clusters wanted, lowered to those that the GPU holds at once.
+int run_back_cluster(void (*kern)(BackArgs), const BackArgs& a, int* blocks, int warps, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)(*blocks * a.parts));
+    cfg.blockDim = dim3(32u * warps);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;  // the query takes the cluster's shape only
+    int held = 0;
+    if (cudaOccupancyMaxActiveClusters(&held, kern, &cfg) != cudaSuccess || held <= 0) {
+        cudaGetLastError();
+        held = *blocks;  // no answer: clusters that do not fit wait for those that do
+    }
+    if (held < *blocks) *blocks = held;
+    cfg.gridDim = dim3((unsigned)(*blocks * a.parts));
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, kern, a);
+}
 template <bool VEC>
-int run_back(const BackArgs& a, int64_t blocks, cudaStream_t st) {
+int run_back(const BackArgs& a, int* blocks, cudaStream_t st) {
     const int w = back_warps(a.cols);
     if (!w) return (int)launch_dep(rmsnorm_backward_wide<VEC>, dim3((unsigned)a.rows), dim3(1024), 0, st, a);
-    return (int)launch_dep(w > 8 && w <= 12 ? rmsnorm_backward_row<VEC, true> : rmsnorm_backward_row<VEC, false>, dim3((unsigned)blocks),
-                           dim3(32u * w), 0, st, a);
+    if (a.parts > 1) return run_back_cluster(w <= kBackAhead ? rmsnorm_backward_row<VEC, true, true> : rmsnorm_backward_row<VEC, false, true>, a, blocks, w, st);
+    return (int)launch_dep(w > 8 && w <= kBackAhead ? rmsnorm_backward_row<VEC, true, false> : rmsnorm_backward_row<VEC, false, false>,
+                           dim3((unsigned)*blocks), dim3(32u * w), 0, st, a);
 }
 
 }  // namespace
@@ -408,8 +493,8 @@ extern "C" size_t mcu_rmsnorm_backward_scratch_bytes(int64_t rows, int64_t cols)
 
 extern "C" int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy, const float* h, const float* w,
                                            const float* rstd, const float* dh, int64_t rows, int64_t cols, void* scratch,
-                                           cudaStream_t st, int* launches) {
-    const BackArgs a{dx, dw ? (float*)scratch : nullptr, dy, h, w, rstd, dh, rows, (int)cols};
+                                           int* status, cudaStream_t st, int* launches) {
+    const BackArgs a{dx, dw ? (float*)scratch : nullptr, dy, h, w, rstd, dh, rows, (int)cols, back_parts(cols), status};
     *launches = 0;
     int parts = back_warps(cols) ? (int)back_blocks(rows, cols) : 0, rc = 0;
     if (dw && !parts) {  // before dx, which may lie over dy or h
@@ -419,8 +504,8 @@ extern "C" int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy
         ++*launches;
     }
     if (!rc) {
-        rc = cols % 4 == 0 && aligned16(dx) && aligned16(dy) && aligned16(h) && aligned16(w) && aligned16(dh) ? run_back<true>(a, parts, st)
-                                                                                                               : run_back<false>(a, parts, st);
+        rc = cols % 4 == 0 && aligned16(dx) && aligned16(dy) && aligned16(h) && aligned16(w) && aligned16(dh) ? run_back<true>(a, &parts, st)
+                                                                                                               : run_back<false>(a, &parts, st);
         ++*launches;
     }
     if (!rc && dw) {

@@ -92,7 +92,7 @@ int mag_cuda_rmsnorm_rows_backward_f32(mag_compute_device_t* dvc, float* dx, flo
     }
     rc = mcu_call_begin(&c, dvc, bufs, 7, dw ? mcu_rmsnorm_backward_scratch_bytes(rows, cols) : 0);
     if (rc) return rc;
-    rc = mcu_launch_rmsnorm_backward(dx, dw, dy, h, w, rstd, dh, rows, cols, c.scratch, c.stream, &k);
+    rc = mcu_launch_rmsnorm_backward(dx, dw, dy, h, w, rstd, dh, rows, cols, c.scratch, c.status, c.stream, &k);
     return mcu_call_end(&c, rc, k);
 }
 

@@ -137,7 +137,7 @@ int mcu_launch_rmsnorm(float* y, uint8_t* q, float* s, float* h, float* rstd, co
                        const float* w, float eps, int64_t rows, int64_t cols, cudaStream_t st, int* launches);
 size_t mcu_rmsnorm_backward_scratch_bytes(int64_t rows, int64_t cols);
 int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy, const float* h, const float* w,
-                                const float* rstd, const float* dh, int64_t rows, int64_t cols, void* scratch,
+                                const float* rstd, const float* dh, int64_t rows, int64_t cols, void* scratch, int* status,
                                 cudaStream_t st, int* launches);
 /* k_quantize_e4m3.cu */
 int mcu_launch_quantize_e4m3(uint8_t* q, float* s, const float* x, int64_t rows, int64_t cols, int block,

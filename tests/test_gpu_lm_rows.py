@@ -292,7 +292,7 @@ def test_rmsnorm_zero_and_nonfinite_rows():
     assert np.all(np.abs(a[[0, 4]] - 1 / math.sqrt(1.5)) <= norm_rel(cols))
 
 
-@pytest.mark.parametrize("rows,cols", NORMS + [(5000, 96), (33, 8192)])
+@pytest.mark.parametrize("rows,cols", NORMS + [(5000, 96), (33, 8192), (200, 9001), (300, 20000), (2, 65536), (3, 70001)])
 def test_rmsnorm_backward(rows, cols):
     d = device()
     g = rng(11, rows, cols)
