@@ -83,7 +83,9 @@ struct NormArgs {
     const float* w;
     float eps;
     int cols;
+    int parts;  // blocks of a cluster, which share a row
 };
+constexpr int kNormCluster = 8;  // at most
 
 // One group's outputs from its sums t.
 template <bool VEC>
@@ -112,21 +114,28 @@ __device__ __forceinline__ void norm_group(const NormArgs& a, const float (&t)[4
 
 // One block of W warps per row, the row held in registers (V groups a warp): one read and one write of
 // every value, bound by HBM where rows abound (8192 x 8192 with the residual and an e4m3 result: 149 us,
-// 5.9 TB/s, 0.90 of the copy rate) and by latency (loads, one barrier) where they are few.
-template <int W, int V, bool VEC>
+// 5.9 TB/s, 0.90 of the copy rate) and by latency (loads, one barrier) where they are few.  Rows wider than a
+// block's registers are shared by a cluster (CLUSTER), each block a span of the row and one meeting for the sum:
+// 4096 x 32768 takes 338 us, 5.2 TB/s (548 when a second pass read the row again), bound by the blocks that an
+// SM holds: four at 64 registers a thread (359 us with three at 80).
+template <int W, int V, bool VEC, bool CLUSTER = false>
 __global__ void __launch_bounds__(W * 32) rmsnorm_row(const NormArgs a) {
-    __shared__ float sh[W];
+    __shared__ float sh[W * (CLUSTER ? kNormCluster : 1)];
+    if (CLUSTER) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     pdl_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row = blockIdx.x, o = row * a.cols;
-    const int groups = (a.cols + 127) >> 7;
+    const int parts = CLUSTER ? a.parts : 1, rank = CLUSTER ? (int)blockIdx.x % parts : 0;
+    const int64_t row = CLUSTER ? blockIdx.x / (unsigned)parts : blockIdx.x, o = row * a.cols;
+    const int groups = (a.cols + 127) >> 7, span = CLUSTER ? (groups + parts - 1) / parts : groups;  // a block's groups
+    const int g0 = rank * span + warp, end = CLUSTER ? min(groups, (rank + 1) * span) : groups;
+    const int cols = CLUSTER ? min(a.cols, end * 128) : a.cols;
     float t[V][4], w[V][4];
 #pragma unroll
-    for (int i = 0; i < V; ++i) load_group<VEC>(t[i], a.x + o, (warp + i * W) * 128, a.cols, lane);
+    for (int i = 0; i < V; ++i) load_group<VEC>(t[i], a.x + o, (g0 + i * W) * 128, cols, lane);
     if (a.res) {
         float u[V][4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) load_group<VEC>(u[i], a.res + o, (warp + i * W) * 128, a.cols, lane);
+        for (int i = 0; i < V; ++i) load_group<VEC>(u[i], a.res + o, (g0 + i * W) * 128, cols, lane);
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
@@ -134,25 +143,39 @@ __global__ void __launch_bounds__(W * 32) rmsnorm_row(const NormArgs a) {
     }
     if (V <= 2) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) load_weight<VEC>(w[i], a.w, (warp + i * W) * 128, a.cols, lane);
+        for (int i = 0; i < V; ++i) load_weight<VEC>(w[i], a.w, (g0 + i * W) * 128, cols, lane);
     }
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) ss = fmaf(t[i][j], t[i][j], ss);
-    const float root = inv_sqrt(__fdiv_rn(block_sum(ss, sh, warp, lane, W), (float)a.cols) + a.eps);
-    if (a.rstd && threadIdx.x == 0) a.rstd[row] = root;
+    float all;
+    if (CLUSTER) {  // every warp leaves its share in each block's array
+        all = warp_sum_f(ss);
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every block of the cluster runs
+        if (lane < parts)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_rank(smem_u32(sh + rank * W + warp), lane)), "f"(all) : "memory");
+        __syncwarp();
+        cluster_sync();
+        all = 0.0f;
+        for (int i = lane; i < parts * W; i += 32) all += sh[i];
+        all = warp_sum_f(all);
+    } else {
+        all = block_sum(ss, sh, warp, lane, W);
+    }
+    const float root = inv_sqrt(__fdiv_rn(all, (float)a.cols) + a.eps);
+    if (a.rstd && threadIdx.x == 0 && rank == 0) a.rstd[row] = root;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int g = warp + i * W;
-        if (g >= groups) break;
-        if (V > 2) load_weight<VEC>(w[i], a.w, g * 128, a.cols, lane);
+        const int g = g0 + i * W;
+        if (g >= end) break;
+        if (V > 2) load_weight<VEC>(w[i], a.w, g * 128, cols, lane);
         norm_group<VEC>(a, t[i], w[i], root, row, g, groups, lane);
     }
 }
 
-// Rows that do not fit the registers: the second pass reads the row again (from L2).
+// Rows that do not fit a cluster's registers: the second pass reads the row again.
 template <bool VEC>
 __global__ void __launch_bounds__(1024) rmsnorm_wide(const NormArgs a) {
     __shared__ float sh[32];
@@ -423,13 +446,38 @@ int64_t back_blocks(int64_t rows, int64_t cols) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// A launch of clusters of `parts` blocks, as a programmatic dependent of the stream's previous kernel.
+struct ClusterLaunch {
+    cudaLaunchAttribute attr[2] = {};
+    cudaLaunchConfig_t cfg = {};
+    ClusterLaunch(dim3 grid, dim3 block, int parts, cudaStream_t st) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)parts;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = grid;
+        cfg.blockDim = block;
+        cfg.stream = st;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+    }
+};
+
 template <typename K>
 int go(K kern, int64_t grid, int threads, cudaStream_t st, const NormArgs& a) {
     return (int)launch_dep(kern, dim3((unsigned)grid), dim3((unsigned)threads), 0, st, a);
 }
 template <bool VEC>
-int run_norm(const NormArgs& a, int64_t rows, cudaStream_t st) {
+int run_norm(NormArgs& a, int64_t rows, cudaStream_t st) {
     const int groups = (a.cols + 127) / 128;
+    // wide rows: a cluster, except where 32 warps of one block are the quicker (300 x 16000: 12.6 us, 14.1 by two
+    // blocks; 4096 x 12288: 124 us, 135 by two)
+    if (groups <= 64 * kNormCluster && (groups > 128 || (groups > 96 && rows > 4 * kSms))) {
+        a.parts = (groups + 63) / 64;
+        ClusterLaunch l(dim3((unsigned)(rows * a.parts)), dim3(256), a.parts, st);
+        return (int)cudaLaunchKernelEx(&l.cfg, rmsnorm_row<8, 8, VEC, true>, (const NormArgs)a);
+    }
     // few rows: 32 warps share a row and each holds less of it
     if (groups > 64 || (rows <= 2 * kSms && groups > 8)) {
         if (groups <= 32) return go(rmsnorm_row<32, 1, VEC>, rows, 1024, st, a);
@@ -445,27 +493,17 @@ int run_norm(const NormArgs& a, int64_t rows, cudaStream_t st) {
 
 // *blocks: the clusters wanted, lowered to those that the GPU holds at once.
 int run_back_cluster(void (*kern)(BackArgs), const BackArgs& a, int* blocks, int warps, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)a.parts;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)(*blocks * a.parts));
-    cfg.blockDim = dim3(32u * warps);
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;  // the query takes the cluster's shape only
+    ClusterLaunch l(dim3((unsigned)(*blocks * a.parts)), dim3(32u * warps), a.parts, st);
     int held = 0;
-    if (cudaOccupancyMaxActiveClusters(&held, kern, &cfg) != cudaSuccess || held <= 0) {
+    l.cfg.numAttrs = 1;  // the query takes the cluster's shape only
+    if (cudaOccupancyMaxActiveClusters(&held, kern, &l.cfg) != cudaSuccess || held <= 0) {
         cudaGetLastError();
         held = *blocks;  // no answer: clusters that do not fit wait for those that do
     }
     if (held < *blocks) *blocks = held;
-    cfg.gridDim = dim3((unsigned)(*blocks * a.parts));
-    cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, kern, a);
+    l.cfg.gridDim = dim3((unsigned)(*blocks * a.parts));
+    l.cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&l.cfg, kern, a);
 }
 template <bool VEC>
 int run_back(const BackArgs& a, int* blocks, cudaStream_t st) {
@@ -481,7 +519,7 @@ int run_back(const BackArgs& a, int* blocks, cudaStream_t st) {
 extern "C" int mcu_launch_rmsnorm(float* y, uint8_t* q, float* s, float* h, float* rstd, const float* x,
                                   const float* res, const float* w, float eps, int64_t rows, int64_t cols,
                                   cudaStream_t st, int* launches) {
-    const NormArgs a{y, q, s, h, rstd, x, res, w, eps, (int)cols};
+    NormArgs a{y, q, s, h, rstd, x, res, w, eps, (int)cols, 1};
     *launches = 1;
     if (cols % 4 == 0 && aligned16(x) && aligned16(res) && aligned16(w) && aligned16(y) && aligned16(h)) return run_norm<true>(a, rows, st);
     return run_norm<false>(a, rows, st);
