@@ -409,7 +409,8 @@ def lp_tol(x, adds):
 
 
 LOGITS = [(1, 1, 1), (1, 5, 5), (4, 32, 32), (3, 33, 7), (2, 1000, 20), (5, 1023, 1), (3, 4097, 32), (300, 256, 4), (700, 1030, 0),
-          (5, 50001, 20), (1, 131072, 32), (9, 131072, 5), (2, 262147, 10), (160, 20000, 8), (1, 1000003, 32)]
+          (5, 50001, 20), (1, 131072, 32), (9, 131072, 5), (2, 262147, 10), (160, 20000, 8), (1, 1000003, 32),
+          (148, 66001, 3), (200, 5000, 20), (594, 65537, 2), (1200, 9000, 4)]
 
 
 @pytest.mark.parametrize("rows,cols,k", LOGITS)
