@@ -466,8 +466,8 @@ extern "C" int mcu_launch_logprobs(float* logp, float* lse, float* entropy, floa
     // 22.9 with one, 34 with 256 threads; 100 x 32000: 11.0 with one, 12.1 with two).
     // Many: an SM's 1024 threads as small blocks, whose barriers and ends overlap better, yet not so small
     // that the first chunk says little about the row: 4095 x 100003 with 8 alternatives takes 302, 276 and
-    // 351 us with 512, 256 and 128 threads, 8192 x 5000 with 5 takes 200, 118 and 83 us, 2048 x 12000 with 20
-    // takes 63, 42 and 38.  Long rows whose last wave would be short take the larger blocks (700 x 131072: 75 us, 84).
+    // 351 us with 512, 256 and 128 threads, 8192 x 5000 with 5 takes 200, 118 and 83 us, 8192 x 20000 with 20
+    // takes 196 and 182 us with 256 and 128, 8192 x 32000 250 and 239, 4096 x 50257 179 and 201.  Long rows whose last wave would be short take the larger blocks (700 x 131072: 75 us, 84).
     const auto waves = [&](int64_t blocks) { return (rows + kSms * blocks - 1) / (kSms * blocks); };  // of so many blocks an SM
     if (rows <= 2 * kSms && cols > (rows <= kSms ? 8192 : 16384)) {
         int parts = 1;
@@ -475,7 +475,7 @@ extern "C" int mcu_launch_logprobs(float* logp, float* lse, float* entropy, floa
         return go(std::integral_constant<int, 512>(), parts);
     }
     if (cols > 65536 && waves(2) * 4 <= waves(4) * 2 * 3) return go(std::integral_constant<int, 512>(), 1);
-    if (cols > (waves(8) > 1 ? 16384 : 8192) || (rows <= 2 * kSms && cols > 2048)) return go(std::integral_constant<int, 256>(), 1);
+    if (cols > (waves(8) > 1 ? 32768 : 8192) || (rows <= 2 * kSms && cols > 2048)) return go(std::integral_constant<int, 256>(), 1);
     return go(std::integral_constant<int, 128>(), 1);
 }
 
