@@ -152,7 +152,7 @@ struct Candidates {
 };
 
 // The best 32 of n keys, sorted over the lanes of the calling warp.
-__device__ __forceinline__ uint64_t best_of(const uint64_t* key, int n, int lane) {
+__device__ __noinline__ uint64_t best_of(const uint64_t* key, int n, int lane) {
     uint64_t best = 0;
     for (int i = 0; i < n; i += 32) {
         const uint64_t k = i + lane < n ? key[i + lane] : 0;
@@ -181,14 +181,15 @@ __device__ __forceinline__ uint32_t group_bound(Candidates<T>& cand, uint32_t bi
 
 // One cluster of `parts` CTAs of T threads per row; each streams its part of the row once, 16 logits a
 // thread and chunk, the next chunk's loads issued before the present one is worked on.  Bound by HBM, 4
-// bytes a logit: 4095 x 100003 takes 240 us without alternatives (6.8 TB/s) and 276 us with 8 of them (5.9),
-// the rest being the bound's barriers and the chunks in which a candidate shows.  Collecting candidates for
+// bytes a logit: 4095 x 100003 takes 240 us without alternatives (6.8 TB/s) and 268 us with 8 of them (6.1),
+// the rest being the bound's barriers, the chunks in which a candidate shows and, for rows of few chunks, misses of
+// the instruction cache (8192 x 4096: 28 us without alternatives, 56 with one).  Collecting candidates for
 // the whole block, with a barrier a chunk, took 520 us.
 //
 // Candidates: the top-th largest of 64 group maxima of the first chunk is a lower bound of the row's top-th
 // logit, so that little more than `top` of the first chunk's logits pass it, as many in each later chunk, and
 // from the fifth on, with the maxima of four, a quarter of that: a warp looks at single elements only where
-// the maximum of a lane's 16 passes.  Later elements have higher columns than the at least `top` that reached
+// the maximum of a lane's 16 passes, and then where that of four does.  Later elements have higher columns than the at least `top` that reached
 // the bound, so they have to exceed it; a bound that a warp's full buffer gives has to be reached only, since
 // another warp may still be at lower columns.  The order in which candidates are found does not matter: keys
 // are distinct and sorted at the end.
@@ -275,9 +276,14 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
                 const uint32_t least = group_bound<T>(cand, big, top, warp, lane);
                 if (__any_sync(0xffffffffu, big >= least)) {
 #pragma unroll
-                    for (int i = 0; i < kVecs * 4; ++i) {
-                        const bool yes = (inside >> i & 1) && order_of(v[i]) >= least;
-                        if (__any_sync(0xffffffffu, yes)) push(yes, v[i], i);
+                    for (int q = 0; q < kVecs * 4; q += 4) {
+                        const float top4 = fmaxf(fmaxf(v[q], v[q + 1]), fmaxf(v[q + 2], v[q + 3]));
+                        if (!__any_sync(0xffffffffu, order_of(top4) >= least || cs != cs)) continue;
+#pragma unroll
+                        for (int i = q; i < q + 4; ++i) {
+                            const bool yes = (inside >> i & 1) && order_of(v[i]) >= least;
+                            if (__any_sync(0xffffffffu, yes)) push(yes, v[i], i);
+                        }
                     }
                 }
                 exceed = least + (least < kOrderInf);
@@ -286,9 +292,14 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
                 const float least = order_value(min(max(exceed, *(volatile uint32_t*)&cand.least), kOrderInf));
                 if (__any_sync(0xffffffffu, !(cm < least) || cs != cs)) {
 #pragma unroll
-                    for (int i = 0; i < kVecs * 4; ++i) {  // (elements past the row are -inf, below any bound here)
-                        const bool yes = !(v[i] < least);
-                        if (__any_sync(0xffffffffu, yes)) push(yes, v[i], i);
+                    for (int q = 0; q < kVecs * 4; q += 4) {  // (elements past the row are -inf, below any bound here)
+                        const float top4 = fmaxf(fmaxf(v[q], v[q + 1]), fmaxf(v[q + 2], v[q + 3]));
+                        if (!__any_sync(0xffffffffu, !(top4 < least) || cs != cs)) continue;
+#pragma unroll
+                        for (int i = q; i < q + 4; ++i) {
+                            const bool yes = !(v[i] < least);
+                            if (__any_sync(0xffffffffu, yes)) push(yes, v[i], i);
+                        }
                     }
                 }
             }
@@ -321,8 +332,24 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
         at = __shfl_sync(0xffffffffu, at, 0);
         for (int i = lane; i < held; i += 32) cand.pool[at + i] = cand.key[warp][i];
         __syncthreads();
-        const int n = cand.pooled, lists = (n + 31) / 32;  // a list per 32 keys
-        if (warp < lists) {
+        const int n = cand.pooled;
+        const bool count = T == 512 && n <= 128;
+        const int lists = count ? 0 : (n + 31) / 32;  // a list per 32 keys
+        if (count) {
+            // where latency counts a key's place is the number of larger ones (no two are equal), which is no chain
+            // of exchanges (4 x 131072: 9.5 us, 9.9); it takes more instructions, which small blocks have no room for
+            if (warp * 32 < n) {
+                const int i = warp * 32 + lane;
+                const uint64_t k = i < n ? cand.pool[i] : 0;
+                int place = 0;
+#pragma unroll 8
+                for (int j = 0; j < n; ++j) place += cand.pool[j] > k;
+                if (i < n && place < 32) cand.list[0][place] = k;
+            }
+            if (n > 32) __syncthreads();
+            else __syncwarp();
+            if (warp == 0 && lane < n) list = cand.list[0][lane];
+        } else if (warp < lists) {
             for (int i = warp * 32; i < n; i += T) {
                 const uint64_t k = sort32(i + lane < n ? cand.pool[i + lane] : 0, lane);
                 list = i == warp * 32 ? k : merge32(list, k, lane);
