@@ -728,10 +728,9 @@ def test_layer_and_loss_together():
     assert np.abs(get(dg, k) - (u * t * r).sum(0)).max() <= 1e-5 * np.abs(u * t * r).sum(0).max()
 
 
-def graph_calls():
+def graph_calls(rows=40, k=384, n=600):
     """The calls of one small step, as closures over buffers that were written once."""
     d = device()
-    rows, k, n = 40, 384, 600
     g = rng(19)
     x, w = up(g.normal(0, 1, (rows, k))), up(g.normal(1, 0.2, k))
     y, h, rstd, dx, dw = out(rows, k), out(rows, k), out(rows), out(rows, k), out(k)
@@ -751,13 +750,14 @@ def graph_calls():
     return calls, x, [logits, logp, lse, ent, tl, ti, dl, dx, dw, y], (rows, k)
 
 
-def test_captured_and_replayed():
+@pytest.mark.parametrize("size", [(40, 384, 600), (6, 17000, 300)])
+def test_captured_and_replayed(size):
     """Two graphs of the same calls over their own buffers, replayed in turn on new inputs: equal to
     eager calls bit for bit, also after the device's scratch has been grown by other work."""
     import torch
     d = device()
     stream = torch.cuda.ExternalStream(d.stream, device=f"cuda:{d.ordinal}")
-    sets = [graph_calls() for _ in range(2)]
+    sets = [graph_calls(*size) for _ in range(2)]
     graphs = []
     for calls, _, _, _ in sets:
         for c in calls:
