@@ -397,7 +397,9 @@ struct NarrowCfg {
     static constexpr int A = 128 * 128, B = BN * 128, STAGE = A + B;
     static constexpr int STAGES = BN == 32 ? 5 : 6;
     static constexpr int PER_SM = BN <= 32 ? 2 : 1;
-    static constexpr int EPI = BN >= 128 ? 16 : 4;  // epilogue warps: four quadrants of lanes, 16 or 32 columns each
+    // epilogue warps: four quadrants of lanes, 16 or 32 columns each (BN = 64, N = 14336: 13.2 us with 16 warps, 13.4
+    // with 8; with scales of y per row, which each warp fetches, 16.5 and 14.5)
+    static constexpr int EPI = BN >= 128 ? 16 : BN == 64 ? (YROW ? 8 : 16) : 4;
     static constexpr int WC = BN * 4 / EPI;       // columns of a warp
     static constexpr int THREADS = 64 + 32 * EPI;
     // scales of y per row: staged like x's where the epilogue's warps are many; the few warps of a narrow tile
@@ -695,13 +697,14 @@ extern "C" int mcu_launch_matmul_e4m3(float* r, const uint8_t* xq, const float* 
                                       const float* ys, int64_t M, int64_t K, int64_t N, int y_block, int* status,
                                       cudaStream_t st, int* launches) {
     const int64_t G = (K + 127) / 128, ld = G * 128;
-    const int bn = M <= 16 ? 16 : M <= 32 ? 32 : !pair_is_faster(M, N, G, y_block) ? 128 : 0;
+    const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : !pair_is_faster(M, N, G, y_block) ? 128 : 0;
     CUtensorMap mx, my;
     if (!e4m3_map(&mx, xq, M, ld, bn ? bn : 128) || !e4m3_map(&my, yq, N, ld, 128)) return (int)cudaErrorInvalidValue;
     *launches = 1;
     switch (bn) {
         case 16: return run_narrow<16>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
         case 32: return run_narrow<32>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
+        case 64: return run_narrow<64>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
         case 128: return run_narrow<128>(mx, my, xs, ys, r, M, N, G, y_block, status, st);
         default:
             return y_block ? run_pair<false>(mx, my, xs, ys, r, M, N, G, status, st)

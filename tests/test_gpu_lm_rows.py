@@ -136,7 +136,8 @@ def product_bound(x, y, groups):
 PRODUCTS = [(1, 128, 8), (1, 100, 7), (1, 4096, 300), (2, 1, 1), (3, 129, 130), (4, 4096, 1024), (8, 512, 129), (9, 300, 257),
             (16, 1024, 384), (17, 640, 100), (31, 256, 1000), (33, 2000, 65), (64, 128, 512), (100, 1500, 700),
             (127, 384, 127), (128, 256, 128), (129, 1000, 513), (200, 4100, 260), (256, 512, 256), (257, 640, 1025),
-            (520, 1300, 771), (1030, 256, 40), (2100, 300, 2001), (5000, 128, 1030), (700, 1664, 5000), (300, 4096, 9000), (260, 256, 33000)]
+            (520, 1300, 771), (1030, 256, 40), (2100, 300, 2001), (5000, 128, 1030), (700, 1664, 5000), (300, 4096, 9000), (260, 256, 33000),
+            (48, 14336, 700), (64, 700, 20000), (40, 5000, 1300)]
 
 
 @pytest.mark.parametrize("block", [True, False])
