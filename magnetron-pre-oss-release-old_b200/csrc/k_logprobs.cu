@@ -181,7 +181,7 @@ __device__ __forceinline__ uint32_t group_bound(Candidates<T>& cand, uint32_t bi
 
 // One cluster of `parts` CTAs of T threads per row; each streams its part of the row once, 16 logits a
 // thread and chunk, the next chunk's loads issued before the present one is worked on.  Bound by HBM, 4
-// bytes a logit: 4095 x 100003 takes 240 us without alternatives (6.8 TB/s) and 268 us with 8 of them (6.1),
+// bytes a logit: 4095 x 100003 takes 240 us without alternatives (6.8 TB/s) and 266 us with 5 of them (6.2),
 // the rest being the bound's barriers, the chunks in which a candidate shows and, for rows of few chunks, misses of
 // the instruction cache (8192 x 4096: 28 us without alternatives, 56 with one).  Collecting candidates for
 // the whole block, with a barrier a chunk, took 520 us.
