@@ -187,12 +187,12 @@ __device__ __forceinline__ uint32_t group_bound(Candidates<T>& cand, uint32_t bi
 // the whole block, with a barrier a chunk, took 520 us.
 //
 // Candidates: the top-th largest of 64 group maxima of the first chunk is a lower bound of the row's top-th
-// logit, so that little more than `top` of the first chunk's logits pass it, as many in each later chunk, and
-// from the fifth on, with the maxima of four, a quarter of that: a warp looks at single elements only where
-// the maximum of a lane's 16 passes, and then where that of four does.  Later elements have higher columns than the at least `top` that reached
-// the bound, so they have to exceed it; a bound that a warp's full buffer gives has to be reached only, since
-// another warp may still be at lower columns.  The order in which candidates are found does not matter: keys
-// are distinct and sorted at the end.
+// logit, so that little more than `top` of the first chunk's logits pass it, as many in each later chunk,
+// and from the fifth on, with the maxima of four, a quarter of that: a warp looks at single elements only
+// where the maximum of a lane's 16 passes, and then where that of four does.  Later elements have higher
+// columns than the at least `top` that reached the bound, so they have to exceed it; a bound that a warp's
+// full buffer gives has to be reached only, since another warp may still be at lower columns.  The order in
+// which candidates are found does not matter: keys are distinct and sorted at the end.
 template <int T, bool TOP>
 __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__ logp, float* __restrict__ lse,
                                                              float* __restrict__ entropy, float* __restrict__ top_logp,
@@ -494,7 +494,8 @@ extern "C" int mcu_launch_logprobs(float* logp, float* lse, float* entropy, floa
     // Many: an SM's 1024 threads as small blocks, whose barriers and ends overlap better, yet not so small
     // that the first chunk says little about the row: 4095 x 100003 with 8 alternatives takes 302, 276 and
     // 351 us with 512, 256 and 128 threads, 8192 x 5000 with 5 takes 200, 118 and 83 us, 8192 x 20000 with 20
-    // takes 196 and 182 us with 256 and 128, 8192 x 32000 250 and 239, 4096 x 50257 179 and 201.  Long rows whose last wave would be short take the larger blocks (700 x 131072: 75 us, 84).
+    // takes 196 and 182 us with 256 and 128, 8192 x 32000 250 and 239, 4096 x 50257 179 and 201.  Long rows
+    // whose last wave would be short take the larger blocks (700 x 131072: 75 us, 84).
     const auto waves = [&](int64_t blocks) { return (rows + kSms * blocks - 1) / (kSms * blocks); };  // of so many blocks an SM
     if (rows <= 2 * kSms && cols > (rows <= kSms ? 8192 : 16384)) {
         int parts = 1;
