@@ -18,13 +18,15 @@ constexpr int kThreads = 256;  // 8 warps of 16 rows
 // joined by warp reductions and one exchange in shared memory.  Transposed, a lane's 16 rows of a column
 // are 16 neighbouring bytes of the result: they go through a 16 KB tile (16-byte pieces, exclusive-or
 // swizzled against bank conflicts) and leave as whole 128-byte rows.
-// Bound by HBM, 4 bytes read and 1 written a value: an 8192 x 4096 weight turned, in blocks, takes 28.8 us
-// (5.8 TB/s, 0.89 of the copy rate).
+// Bound by HBM, 4 bytes read and 1 written a value, with two conversions a value beside it: 8192 x 8192 in rows takes
+// 63 us (5.3 TB/s, 0.82 of the copy rate), an 8192 x 4096 weight turned, in blocks, 30.2 us (5.6 TB/s, 0.85).
+// A group's scale and factors are formed once: by lane i for the warp's row i, by thread n for the tile's column n.
 template <bool VEC, bool BLOCK, bool TRANSPOSE>
 __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict__ q, float* __restrict__ s,
                                                              const float* __restrict__ x, int rows, int cols, int col_tiles,
                                                              int64_t ld) {
     __shared__ uint32_t sh_top[TRANSPOSE && !BLOCK ? 8 : 1][TRANSPOSE && !BLOCK ? 128 : 8];
+    __shared__ float sh_group[3][TRANSPOSE && !BLOCK ? 128 : 1];
     __shared__ __align__(16) uint8_t tile[TRANSPOSE ? 128 * 128 : 16];
     pdl_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -49,6 +51,7 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict
         }
     }
     const int64_t groups = ld / 128;
+    E4m3Group gr;  // of the block; of row `lane` of the warp's; of the present column
     if constexpr (BLOCK) {
         uint32_t top = 0;
 #pragma unroll
@@ -60,23 +63,9 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, sh_top[0][i]);
-        const E4m3Group gr = e4m3_group(top);
+        gr = e4m3_group(top);
         if (threadIdx.x == 0) s[TRANSPOSE ? c0 / 128 * groups + r0 / 128 : r0 / 128 * groups + c0 / 128] = gr.scale;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][j] *= gr.factor;
-    } else if constexpr (!TRANSPOSE) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint32_t top = __reduce_max_sync(
-                0xffffffffu, max(max(abs_bits(v[i][0]), abs_bits(v[i][1])), max(abs_bits(v[i][2]), abs_bits(v[i][3]))));
-            const E4m3Group gr = e4m3_group(top);
-            if (lane == 0 && r + i < rows) s[(int64_t)(r + i) * groups + c0 / 128] = gr.scale;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][j] *= gr.factor;
-        }
-    } else {
+    } else if constexpr (TRANSPOSE) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             uint32_t top = 0;
@@ -85,22 +74,31 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict
             sh_top[warp][col(j)] = top;
         }
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        if (threadIdx.x < 128) {  // a column each
+            const int n = threadIdx.x;
             uint32_t top = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, sh_top[i][col(j)]);
-            const E4m3Group gr = e4m3_group(top);
-            if (warp == 0 && c0 + col(j) < cols) s[(int64_t)(c0 + col(j)) * groups + r0 / 128] = gr.scale;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i][j] *= gr.factor;
+            for (int i = 0; i < 8; ++i) top = max(top, sh_top[i][n]);
+            const E4m3Group g = e4m3_group(top);
+            sh_group[0][n] = g.scale;
+            sh_group[1][n] = g.low;
+            sh_group[2][n] = g.high;
+            if (c0 + n < cols) s[(int64_t)(c0 + n) * groups + r0 / 128] = g.scale;
         }
-    }
-    if constexpr (!TRANSPOSE) {
+        __syncthreads();
+    } else {
+        uint32_t mine = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            if (r + i >= rows) break;
-            const uint32_t b = e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3]);
+            const uint32_t top = __reduce_max_sync(
+                0xffffffffu, max(max(abs_bits(v[i][0]), abs_bits(v[i][1])), max(abs_bits(v[i][2]), abs_bits(v[i][3]))));
+            if (lane == i) mine = top;
+        }
+        gr = e4m3_group(mine);
+        if (lane < 16 && r + lane < rows) s[(int64_t)(r + lane) * groups + c0 / 128] = gr.scale;
+    }
+    if constexpr (!TRANSPOSE) {
+        const auto put = [&](int i, uint32_t b) {
             uint8_t* o = q + (int64_t)(r + i) * ld + c0;
             if (VEC) {
                 *(uint32_t*)(o + lane * 4) = b;
@@ -108,16 +106,35 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[col(j)] = (uint8_t)(b >> (8 * j));
             }
+        };
+        uint32_t open = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (r + i >= rows) break;  // (for the whole warp)
+            if constexpr (BLOCK) {
+                put(i, e4m3_quotients(gr, v[i][0], v[i][1], v[i][2], v[i][3]));
+            } else {
+                const E4m3Group g{0.0f, __shfl_sync(0xffffffffu, gr.low, i), __shfl_sync(0xffffffffu, gr.high, i)};
+                put(i, e4m3_try(g, v[i][0], v[i][1], v[i][2], v[i][3], &open));
+            }
+        }
+        if (!BLOCK && __any_sync(0xffffffffu, open)) {  // one warp of a hundred
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (r + i >= rows) break;
+                put(i, e4m3_divide(__shfl_sync(0xffffffffu, gr.scale, i), v[i][0], v[i][1], v[i][2], v[i][3]));
+            }
         }
     } else {
         const auto piece = [&](int n, int c) { return n * 128 + ((c ^ ((VEC ? n >> 2 : n) & 7)) << 4); };
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (!BLOCK) gr = E4m3Group{sh_group[0][col(j)], sh_group[1][col(j)], sh_group[2][col(j)]};
             uint4 b;
-            b.x = e4m3x4(v[0][j], v[1][j], v[2][j], v[3][j]);
-            b.y = e4m3x4(v[4][j], v[5][j], v[6][j], v[7][j]);
-            b.z = e4m3x4(v[8][j], v[9][j], v[10][j], v[11][j]);
-            b.w = e4m3x4(v[12][j], v[13][j], v[14][j], v[15][j]);
+            b.x = e4m3_quotients(gr, v[0][j], v[1][j], v[2][j], v[3][j]);
+            b.y = e4m3_quotients(gr, v[4][j], v[5][j], v[6][j], v[7][j]);
+            b.z = e4m3_quotients(gr, v[8][j], v[9][j], v[10][j], v[11][j]);
+            b.w = e4m3_quotients(gr, v[12][j], v[13][j], v[14][j], v[15][j]);
             *(uint4*)(tile + piece(col(j), warp)) = b;
         }
         __syncthreads();

@@ -101,7 +101,7 @@ __device__ __forceinline__ void norm_group(const NormArgs& a, const float (&t)[4
         const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3]))));
         const E4m3Group gr = e4m3_group(top);
         if (lane == 0) a.s[row * groups + g] = gr.scale;
-        const uint32_t b = e4m3x4(v[0] * gr.factor, v[1] * gr.factor, v[2] * gr.factor, v[3] * gr.factor);
+        const uint32_t b = e4m3_quotients(gr, v[0], v[1], v[2], v[3]);
         uint8_t* q = a.q + (row * groups + g) * 128;
         if (VEC) {
             *(uint32_t*)(q + lane * 4) = b;

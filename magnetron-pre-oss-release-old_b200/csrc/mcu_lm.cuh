@@ -21,16 +21,32 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 // |v| as an integer whose order is the magnitude's, NaN above infinity: a maximum over these keeps NaN.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// A group's scale amax / 448 and the factor 448 / amax of its values, from the bits of its largest
-// magnitude.  A value is rounded twice in f32 (the factor, the product) before e4m3 rounds it, which moves
-// about one in 10^7, those within 2^-23 of a tie, to the neighbour that lies as near.  The corrected division
-// (two fused multiply-adds a value) cost 4 to 15 % of the kernels and still rounds once in f32.
+// A group's scale s = a / 448 (a its largest magnitude, at least kE4m3Tiny), from the bits of that magnitude, and two
+// factors around 1 / s.  With d1, d2, d3 roundings of at most 2^-24 each, s = (a / 448)(1 + d1) and f = (448 / a)(1 + d2),
+// so 1 / s lies within f (1 +- 1.01 * 2^-23), and low and high = f (1 -+ 2^-22)(1 + d3) lie outside that.
 struct E4m3Group {
-    float scale, factor;
+    float scale, low, high;
 };
 __device__ __forceinline__ E4m3Group e4m3_group(uint32_t amax_bits) {
-    const float a = __uint_as_float(amax_bits), m = a < kE4m3Tiny ? kE4m3Tiny : a;
-    return E4m3Group{__fdiv_rn(m, kE4m3Max), __fdiv_rn(kE4m3Max, m)};
+    const float a = __uint_as_float(amax_bits), m = a < kE4m3Tiny ? kE4m3Tiny : a, f = __fdiv_rn(kE4m3Max, m);
+    return E4m3Group{__fdiv_rn(m, kE4m3Max), __fmul_rn(f, 1.0f - 0x1p-22f), __fmul_rn(f, 1.0f + 0x1p-22f)};
+}
+__device__ __forceinline__ uint32_t e4m3_divide(float scale, float a, float b, float c, float d) {
+    return e4m3x4(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale));
+}
+// Four values as bytes: each quotient v / s rounded to f32, then to e4m3.  Rounding keeps order, so where v low and
+// v high give the same byte the quotient gives it too; else (5 values of 10^6, those next to a tie) *open gets a bit,
+// and the quotients have to be formed.  Dividing every value instead: an 8192 x 4096 weight turned, in blocks, 37.9 us,
+// 30.2 so; one factor alone (27.9 us) moved one value of 3 * 10^6 to its other neighbour.
+__device__ __forceinline__ uint32_t e4m3_try(const E4m3Group& g, float a, float b, float c, float d, uint32_t* open) {
+    const uint32_t q = e4m3x4(a * g.low, b * g.low, c * g.low, d * g.low);
+    *open |= q ^ e4m3x4(a * g.high, b * g.high, c * g.high, d * g.high);
+    return q;
+}
+__device__ __forceinline__ uint32_t e4m3_quotients(const E4m3Group& g, float a, float b, float c, float d) {
+    uint32_t open = 0;
+    const uint32_t q = e4m3_try(g, a, b, c, d, &open);
+    return open ? e4m3_divide(g.scale, a, b, c, d) : q;
 }
 
 __device__ __forceinline__ float warp_sum_f(float v) {
