@@ -268,8 +268,11 @@ MAG_CUDA_EXPORT int mag_cuda_img_draw_text(mag_compute_device_t* dvc, mag_tensor
  *
  * Calls check their arguments before any work (MAG_CUDA_E_INVALID), take rows = 0 as nothing to do,
  * come from one host thread at a time, and may be captured into a CUDA graph of mag_cuda_stream after
- * one eager call of the kind: a captured call allocates nothing that outlives the graph, and returns MAG_CUDA_E_INVALID for tensor storage that was never written or
- * has an asynchronous copy in flight (neither a pending clear nor a wait belongs in the graph).
+ * one eager call of the kind: a captured call allocates nothing that outlives the graph, and returns
+ * MAG_CUDA_E_INVALID for tensor storage that was never written or has an asynchronous copy in flight (neither a
+ * pending clear nor a wait belongs in the graph).  Between replays on that stream the tensors may be cleared,
+ * written, read and copied asynchronously like any others: from the capture on, a clear of their storage is issued
+ * at once and the stream waits for their asynchronous copies as soon as those are queued.
  * Results depend on the inputs alone: sums are formed in a fixed order, without atomics. */
 #define MAG_CUDA_E4M3_ROW 0
 #define MAG_CUDA_E4M3_BLOCK 1

@@ -70,6 +70,7 @@ typedef struct mcu_block {
     uint8_t known_zero;   /* nothing has written the buffer since it was zeroed */
     uint8_t state;        /* 0 empty, 1 live, 2 deleted */
     uint8_t io_pending;   /* an async copy on the copy stream touches the buffer: io_ev marks its end */
+    uint8_t in_graph;     /* a call on it was captured by the caller: replays touch it without any bookkeeping */
     cudaEvent_t io_ev;
 } mcu_block;
 
@@ -151,6 +152,7 @@ static void tab_grow(mcu_device* d) {
         tab_insert(d, old[i].base, old[i].size, old[i].zero_pending, old[i].known_zero);
         mcu_block* nb = tab_find(d, old[i].base);
         nb->io_pending = old[i].io_pending;
+        nb->in_graph = old[i].in_graph;
         nb->io_ev = old[i].io_ev;
     }
     free(old);
@@ -161,7 +163,7 @@ static void tab_insert(mcu_device* d, uintptr_t base, size_t size, int zero_pend
     size_t i = hash_ptr(base, d->tab_cap);
     while (d->tab[i].state == 1) i = (i + 1) & (d->tab_cap - 1);
     if (d->tab[i].state == 0) d->tab_used++;
-    d->tab[i] = (mcu_block){base, size, (uint8_t)zero_pending, (uint8_t)known_zero, 1, 0, NULL};
+    d->tab[i] = (mcu_block){base, size, (uint8_t)zero_pending, (uint8_t)known_zero, 1, 0, 0, NULL};
     d->tab_live++;
 }
 
@@ -239,7 +241,7 @@ static void sto_set(mag_storage_buffer* sto, size_t offs, uint8_t x) {
     if (offs == 0 && x == 0 && !d->eager_zero && !d->managed && !d->capturing) {
         mcu_block* b = tab_find(d, sto->base);
         io_wait(d, b);
-        if (b) {
+        if (b && !b->in_graph) { /* (a replay neither issues a pending clear nor takes it back) */
             b->zero_pending = b->known_zero = 1;
             return;
         }
@@ -743,6 +745,12 @@ int mcu_call_begin(mcu_call* c, mag_compute_device_t* dvc, const mcu_buf* bufs, 
         if (c->prev_device != d->ordinal) cudaSetDevice(c->prev_device);
         return rc;
     }
+    if (captured) {
+        for (int i = 0; i < n; ++i) {
+            mcu_block* b = bufs[i].p ? tab_find_containing(d, (uintptr_t)bufs[i].p) : NULL;
+            if (b) b->in_graph = 1;
+        }
+    }
     for (int i = 0; i < n; ++i)
         if (bufs[i].p && !bufs[i].out) ext_in(d, bufs[i].p);
     for (int i = 0; i < n; ++i)
@@ -972,7 +980,8 @@ static int io_async(mag_compute_device_t* dvc, mag_tensor_t* t, void* host, size
                            : cudaMemcpyAsync(host, (const void*)b->base, bytes, cudaMemcpyDeviceToHost, d->copy_stream);
     if (e != cudaSuccess) return (int)e;
     MCU_CHECK(cudaEventRecord(b->io_ev, d->copy_stream));
-    b->io_pending = 1;
+    if (b->in_graph) MCU_CHECK(cudaStreamWaitEvent(d->stream, b->io_ev, 0)); /* a replay waits for nothing else */
+    else b->io_pending = 1;
     return 0;
 }
 

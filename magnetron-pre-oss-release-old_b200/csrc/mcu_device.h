@@ -26,7 +26,8 @@ typedef struct mcu_buf {
 } mcu_buf;
 /* One call on the device's stream: makes the device current, books the buffers and finds scratch.
  * While the stream is being captured the scratch is the graph's own (allocated and freed by nodes of
- * it), and buffers that need a clear or a wait first are refused.  mcu_call_end undoes both and
+ * it), buffers that need a clear or a wait first are refused, and the buffers' later clears and
+ * asynchronous copies are put on the stream at once, since a replay does not look for them.  mcu_call_end undoes both and
  * returns rc, or the error that ending met. */
 typedef struct mcu_call {
     mag_compute_device_t* dvc;
