@@ -131,6 +131,12 @@ def _operand(g, rows, cols, block):
 
 
 def prepare(case, seed):
+    if own:
+        # The memory is torch's: from here on torch works on the library's stream, as in a program that has both, so
+        # that a call follows what torch still writes and torch's next work follows the call.
+        stream = torch.cuda.ExternalStream(_dev().stream, device=f"cuda:{_dev().ordinal}")
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
     g = _generator(seed)
     op = case["op"]
     s = dict(case)
