@@ -261,10 +261,10 @@ MAG_CUDA_EXPORT int mag_cuda_img_draw_text(mag_compute_device_t* dvc, mag_tensor
  *      MAG_CUDA_E4M3_ROW    [rows][G]             the group is 1 x 128 (activations, gradients)
  *      MAG_CUDA_E4M3_BLOCK  [ceil(rows / 128)][G] the group is 128 x 128 (weights)
  * and stands for s * q.  q must be 16-byte aligned.  With a = max(amax, 2^-100), amax a group's
- * largest magnitude, its scale is s = a / 448, and q is v / s rounded to f32 and then to the nearest e4m3
- * value (ties to even), so a group of zeros has zero bytes and a small scale; a NaN in a group makes the whole
- * group NaN, an infinity makes its scale
- * infinite and itself NaN, and both reach every product that reads the group.
+ * largest magnitude, its scale is s = a / 448 (in f32, a times 1 / 448), and q is v / s rounded to f32 and
+ * then to the nearest e4m3 value (ties to even), so a group of zeros has zero bytes and a small scale; a NaN
+ * in a group makes the whole group NaN, an infinity makes its scale infinite and itself NaN, and both reach
+ * every product that reads the group.
  *
  * Calls check their arguments before any work (MAG_CUDA_E_INVALID), take rows = 0 as nothing to do,
  * come from one host thread at a time, and may be captured into a CUDA graph of mag_cuda_stream after

@@ -21,15 +21,16 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 // |v| as an integer whose order is the magnitude's, NaN above infinity: a maximum over these keeps NaN.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// A group's scale s = a / 448 (a its largest magnitude, at least kE4m3Tiny), from the bits of that magnitude, and two
-// factors around 1 / s.  With d1, d2, d3 roundings of at most 2^-24 each, s = (a / 448)(1 + d1) and f = (448 / a)(1 + d2),
-// so 1 / s lies within f (1 +- 1.01 * 2^-23), and low and high = f (1 -+ 2^-22)(1 + d3) lie outside that.
+// A group's scale s, a / 448 (a its largest magnitude, at least kE4m3Tiny) by a multiplication, from the bits of that
+// magnitude, and two factors around 1 / s.  With u = 2^-24, c = 1 / 448 as f32 holds it is (1 / 448)(1 + 0.75 u), so that
+// s = a c (1 + d1) = (a / 448)(1 + d), |d| <= 1.76 u.  f = (448 / a)(1 + d2), hence 1 / s lies within f (1 +- 2.8 u), and
+// low and high = f (1 -+ 4 u)(1 + d3) lie outside that (d1, d2, d3 are single roundings, at most u).
 struct E4m3Group {
     float scale, low, high;
 };
 __device__ __forceinline__ E4m3Group e4m3_group(uint32_t amax_bits) {
     const float a = __uint_as_float(amax_bits), m = a < kE4m3Tiny ? kE4m3Tiny : a, f = __fdiv_rn(kE4m3Max, m);
-    return E4m3Group{__fdiv_rn(m, kE4m3Max), __fmul_rn(f, 1.0f - 0x1p-22f), __fmul_rn(f, 1.0f + 0x1p-22f)};
+    return E4m3Group{__fmul_rn(m, 1.0f / kE4m3Max), __fmul_rn(f, 1.0f - 0x1p-22f), __fmul_rn(f, 1.0f + 0x1p-22f)};
 }
 __device__ __forceinline__ uint32_t e4m3_divide(float scale, float a, float b, float c, float d) {
     return e4m3x4(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale));

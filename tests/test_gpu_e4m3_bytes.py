@@ -1,7 +1,7 @@
 """The bytes of e4m3 operands and the bits of their products on the GPU, compared for equality.
 
-A group's scale is s = f32(a / 448) and a byte is the e4m3 value nearest to the quotient v / s as f32
-rounds it, ties to even.  Division and both roundings are IEEE's, so numpy gives the same bits."""
+A group's scale is s = f32(a f32(1 / 448)) and a byte is the e4m3 value nearest to the quotient v / s as f32
+rounds it, ties to even.  Both operations and roundings are IEEE's, so numpy gives the same bits."""
 import numpy as np
 import pytest
 
@@ -50,7 +50,7 @@ def quantized(v, block):
     p[:rows, :cols] = v
     with np.errstate(all="ignore"):
         top = np.abs(p.reshape(n, 128 if block else 1, ld // 128, 128)).max((1, 3))
-        s = np.maximum(top, TINY) / np.float32(448)
+        s = np.maximum(top, TINY) * (np.float32(1) / np.float32(448))
         each = np.repeat(np.repeat(s, 128, 0)[:rows] if block else s, 128, 1)
         q = to_e4m3(p[:rows] / each)
     q[:, cols:] = 0
@@ -67,7 +67,7 @@ def near_ties(rows, seed):
     """Rows of groups whose other values lie at and next to the midpoints of neighbouring e4m3 values."""
     g = np.random.default_rng([0xE4, seed])
     top = np.exp(g.normal(0, 8, rows)).astype(np.float32)
-    s = top / np.float32(448)
+    s = top * (np.float32(1) / np.float32(448))
     mid = (VALUES[:0x7E].astype(np.float64) + VALUES[1:0x7F]) / 2
     v = (mid[None, :] * s[:, None].astype(np.float64)).astype(np.float32)
     v = (v.view(np.int32) + g.integers(-2, 3, v.shape)).astype(np.int32).view(np.float32)
