@@ -131,7 +131,7 @@ def _operand(g, rows, cols, block):
 
 
 def prepare(case, seed):
-    if own:
+    if own and torch.cuda.current_stream().cuda_stream != _dev().stream:
         # The memory is torch's: from here on torch works on the library's stream, as in a program that has both, so
         # that a call follows what torch still writes and torch's next work follows the call.
         stream = torch.cuda.ExternalStream(_dev().stream, device=f"cuda:{_dev().ordinal}")
