@@ -12,6 +12,9 @@ namespace {
 
 constexpr int kThreads = 256;  // 8 warps of 16 rows
 
+// Masks the first n bytes of a word.  (Bytes past the matrix are zero, also in a group that a NaN makes NaN.)
+__device__ __forceinline__ uint32_t first_bytes(int n) { return n >= 4 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << (8 * n)) - 1; }
+
 // One block per 128 x 128 tile of x, in registers: a warp holds 16 of the tile's rows, a lane four of its
 // columns (VEC: neighbours, one 16-byte load a row; else 32 apart, four 4-byte loads), all loads issued
 // before the first use.  Largest magnitudes are taken over a lane's columns or rows in registers and
@@ -98,7 +101,11 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict
         if (lane < 16 && r + lane < rows) s[(int64_t)(r + lane) * groups + c0 / 128] = gr.scale;
     }
     if constexpr (!TRANSPOSE) {
+        uint32_t keep = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) keep |= c0 + col(j) < cols ? 0xFFu << (8 * j) : 0u;
         const auto put = [&](int i, uint32_t b) {
+            b &= keep;
             uint8_t* o = q + (int64_t)(r + i) * ld + c0;
             if (VEC) {
                 *(uint32_t*)(o + lane * 4) = b;
@@ -135,6 +142,12 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict
             b.y = e4m3_quotients(gr, v[4][j], v[5][j], v[6][j], v[7][j]);
             b.z = e4m3_quotients(gr, v[8][j], v[9][j], v[10][j], v[11][j]);
             b.w = e4m3_quotients(gr, v[12][j], v[13][j], v[14][j], v[15][j]);
+            if (r + 16 > rows) {
+                b.x &= first_bytes(rows - r);
+                b.y &= first_bytes(rows - r - 4);
+                b.z &= first_bytes(rows - r - 8);
+                b.w &= first_bytes(rows - r - 12);
+            }
             *(uint4*)(tile + piece(col(j), warp)) = b;
         }
         __syncthreads();

@@ -98,10 +98,17 @@ __device__ __forceinline__ void norm_group(const NormArgs& a, const float (&t)[4
     for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(__fmul_rn(t[j], root), w[j]);
     if (a.y) store_group<VEC>(a.y + o, v, g * 128, a.cols, lane);
     if (a.q) {
+        // past the row's end zero, whatever the root (0 times infinity) and the group (NaN)
+        uint32_t keep = 0xFFFFFFFFu;
+        if (g * 128 + 128 > a.cols) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (g * 128 + lane_col<VEC>(lane, j) >= a.cols) v[j] = 0.0f, keep &= ~(0xFFu << (8 * j));
+        }
         const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3]))));
         const E4m3Group gr = e4m3_group(top);
         if (lane == 0) a.s[row * groups + g] = gr.scale;
-        const uint32_t b = e4m3_quotients(gr, v[0], v[1], v[2], v[3]);
+        const uint32_t b = keep & e4m3_quotients(gr, v[0], v[1], v[2], v[3]);
         uint8_t* q = a.q + (row * groups + g) * 128;
         if (VEC) {
             *(uint32_t*)(q + lane * 4) = b;

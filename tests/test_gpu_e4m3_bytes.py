@@ -113,3 +113,45 @@ def test_norm_quantizes_its_own_result(rows, cols):
     want, ws = quantized(y.read().reshape(rows, cols), False)
     assert np.array_equal(s.read().view(np.uint32), ws.reshape(-1).view(np.uint32))
     assert same_bytes(get_bytes(q, rows, want.shape[1]), want)
+
+
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("block", [False, True])
+@pytest.mark.parametrize("rows,cols", [(7, 300), (7, 301), (140, 141), (130, 17)])
+def test_padding_of_groups_with_nan_and_inf(rows, cols, block, transpose):
+    """Bytes past the columns are zero whatever the group holds; its own bytes and scales are the rule's."""
+    d = device()
+    v = np.random.default_rng([0xE6, rows, cols]).normal(0, 1, (rows, cols)).astype(np.float32)
+    v[1, cols - 1] = np.nan
+    v[3, cols - 2] = np.inf
+    v[rows - 1, 0] = -np.inf
+    v[5] = 0
+    want, ws = quantized(v, block)
+    x = np.ascontiguousarray(v.T if transpose else v)
+    q, s = d.e4m3(rows, cols, block)
+    filled(q)
+    d.quantize_e4m3(*x.shape, up(x), q, s, block=block, transpose=transpose)
+    got = get_bytes(q, rows, want.shape[1])
+    assert not got[:, cols:].any()
+    assert same_bytes(got, want)
+    assert np.array_equal(s.read(), ws.reshape(-1), equal_nan=True)
+
+
+@pytest.mark.parametrize("cols", [300, 301, 9001, 20001])
+def test_padding_of_norms_without_a_finite_root(cols):
+    """eps = 0: a row of zeros has 0 * inf, one whose squares underflow t * inf; rows with NaN and infinity."""
+    d = device()
+    x = np.ones((5, cols), np.float32)
+    x[0] = 0
+    x[1] = 1e-25
+    x[2, cols - 1] = np.nan
+    x[3, 2] = np.inf
+    t, (q, s) = up(x), d.e4m3(5, cols)
+    filled(q)
+    d.rmsnorm_rows(5, cols, t, up(np.ones(cols)), 0.0, q=q, q_scale=s)
+    got, sc = get_bytes(q, 5, MB.e4m3_ld(cols)), s.read().reshape(5, -1)
+    assert not got[:, cols:].any()
+    assert np.all((got[:3, :cols] & 0x7F) == 0x7F) and np.isnan(sc[[0, 2]]).all() and np.isposinf(sc[1]).all()
+    # the root of a row with an infinity is 0: the infinity gives NaN, which takes its group, the others give 0
+    assert np.all((got[3, :128] & 0x7F) == 0x7F) and not (got[3, 128:] & 0x7F).any()
+    assert np.all(got[4, :cols] == 0x7E) and np.isfinite(sc[4]).all()
