@@ -410,6 +410,9 @@ __global__ void __launch_bounds__(T, 1024 / T) logprobs_rows(float* __restrict__
 // Four vectors a thread of one row's chunk; bound by HBM, 8 bytes a logit (2048 x 65600: 168 us, 6.4 TB/s).
 constexpr int kBackThreads = 256;
 constexpr int kBackVecs = 4;
+// The least log probability that counts: e^d is 0 in f32 from -104 on, and 0 times a distance bounded here is 0 for
+// gradients of the entropy up to 2^120 (with kFar for a bound it was 0 times infinity from 3.4e8 on).
+constexpr float kGone = -128.0f;
 
 __global__ void __launch_bounds__(kBackThreads) logprobs_backward(float* dx, const float* x, const int32_t* __restrict__ id,
                                                                   const float* __restrict__ lse,
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kBackThreads) logprobs_backward(float* dx, con
     const float ge = g_entropy ? g_entropy[row] : 0.0f, en = g_entropy ? entropy[row] : 0.0f;
     const auto grad = [&](float v, int64_t c) {
         const float d = v - l, e = exp2_fast(d * kLog2e);
-        const float r = -e * fmaf(ge, fmaxf(d, kFar) + en, g);
+        const float r = -e * fmaf(ge, fmaxf(d, kGone) + en, g);
         return none ? 0.0f : c == hot ? r + g : r;
     };
     const int off = (int)((uintptr_t)p >> 2) & 3;
