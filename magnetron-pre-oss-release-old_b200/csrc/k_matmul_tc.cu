@@ -1419,13 +1419,6 @@ bool make_bias_map(CUtensorMap* m, const float* bias, int64_t M, int64_t N) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// MAG_CUDA_TC_TEST_STALL=1 makes the GEMM's first wait one that never completes (read at each
-// launch): a test of the bounded waits and the status word without any fault.
-int test_stall() {
-    const char* e = getenv("MAG_CUDA_TC_TEST_STALL");
-    return e && e[0] == '1';
-}
-
 template <bool FUSED, bool F16, bool PAIR, int RB = ROW_BYTES>
 int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const CUtensorMap& d,
                 const CUtensorMap& bias, float* r, int64_t M, int64_t N, int64_t kp, int* status, const Epi& epi,

@@ -230,6 +230,7 @@ struct BackArgs {
     int cols;
     int parts;    // blocks of a cluster, which share every row
     int* status;  // of its bounded waits
+    int stall;    // a test of them: nobody sends in the first row
 };
 
 constexpr int kBackV = 4;         // groups a warp
@@ -240,23 +241,28 @@ constexpr int kBackCluster = 8;   // blocks of a cluster at most
 // Sum over the warps of the cluster's blocks, the same on every thread: each warp sends its share to every
 // block's sh [parts][kBackWarps], counted on that block's mbarrier.  (A cluster barrier instead would wait for
 // the row's stores and loads as well: 4096 x 16384 takes 217 us so, 187 this way.)  Two arrays and mbarriers
-// take turns: whoever sends to one again has received what every warp sent after its last reading.
-__device__ __forceinline__ float cluster_sum(float v, float* sh, uint64_t* bar, uint32_t parity, int warp, int lane, int warps, int rank,
-                                             int parts, const Abort& ab) {
+// take turns: whoever sends to one again has received what every warp sent after its last reading.  False, for the
+// whole warp, when a wait gave up: the warp then leaves the rows, so that no mbarrier is armed again whose phase is
+// not complete, and its peers, which get nothing more from it, run out of theirs and follow.
+__device__ __forceinline__ bool cluster_sum(float v, float* all, float* sh, uint64_t* bar, uint32_t parity, int warp, int lane, int warps,
+                                            int rank, int parts, const Abort& ab, bool send) {
     v = warp_sum_f(v);
     if (threadIdx.x == 0) mbar_expect_tx(bar, (uint32_t)(parts * warps * 4));
-    if (lane < parts)
+    if (lane < parts && send)
         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(
                          mapa_rank(smem_u32(sh + rank * kBackWarps + warp), lane)),
                      "f"(v), "r"(mapa_rank(smem_u32(bar), lane))
                      : "memory");
+    // one lane polls: 32 that give up take 32 times as long, half a second each
+    uint32_t ok = 1;
+    if (lane == 0) ok = mbar_wait(bar, parity, ab, 24);
     __syncwarp();
-    mbar_wait(bar, parity, ab, 24);
-    __syncwarp();
+    if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
     float t = 0.0f;
     for (int i = lane; i < parts * kBackWarps; i += 32)
         if (i % kBackWarps < warps) t += sh[i];
-    return warp_sum_f(t);
+    *all = warp_sum_f(t);
+    return true;
 }
 
 // A block goes through rows blockIdx.x, + grid, ...; a thread keeps the same columns in every row and so its
@@ -339,8 +345,13 @@ __global__ void __launch_bounds__(32 * (AHEAD ? kBackAhead : kBackWarps), 1) rms
                 for (int i = 0; i < V; ++i) load_group<VEC>(gn[AHEAD ? i : 0], a.dh + next * a.cols, base(i), a.cols, lane);
             }
         }
-        const float all = CLUSTER ? cluster_sum(along, sh[turn & 1], &bars[turn & 1], turn >> 1 & 1, warp, lane, warps, rank, parts, ab)
-                                  : block_sum(along, sh[turn & 1], warp, lane, warps);
+        float all;
+        if (CLUSTER) {
+            if (!cluster_sum(along, &all, sh[turn & 1], &bars[turn & 1], turn >> 1 & 1, warp, lane, warps, rank, parts, ab, !a.stall || turn))
+                break;
+        } else {
+            all = block_sum(along, sh[turn & 1], warp, lane, warps);
+        }
         const float f = root * root * __fdiv_rn(all, (float)a.cols);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -359,7 +370,11 @@ __global__ void __launch_bounds__(32 * (AHEAD ? kBackAhead : kBackWarps), 1) rms
 #pragma unroll
         for (int i = 0; i < V; ++i) store_group<VEC>(a.part + (int64_t)first * a.cols, sum[i], base(i), a.cols, lane);
     }
-    if (CLUSTER) cluster_sync();  // no block leaves while a peer may still send to it
+    if (CLUSTER) {
+        cluster_sync();  // no block leaves while a peer may still send to it
+        if (threadIdx.x == 0 && gave_up)  // and none that did not wait for what was sent before it has had time to land
+            for (int i = 0; i < 1024; ++i) __nanosleep(64);
+    }
 }
 
 // Rows that do not fit a cluster either: dx in two passes over the row, dw's partial sums by columns over a share of rows.
@@ -539,7 +554,7 @@ extern "C" size_t mcu_rmsnorm_backward_scratch_bytes(int64_t rows, int64_t cols)
 extern "C" int mcu_launch_rmsnorm_backward(float* dx, float* dw, const float* dy, const float* h, const float* w,
                                            const float* rstd, const float* dh, int64_t rows, int64_t cols, void* scratch,
                                            int* status, cudaStream_t st, int* launches) {
-    const BackArgs a{dx, dw ? (float*)scratch : nullptr, dy, h, w, rstd, dh, rows, (int)cols, back_parts(cols), status};
+    const BackArgs a{dx, dw ? (float*)scratch : nullptr, dy, h, w, rstd, dh, rows, (int)cols, back_parts(cols), status, test_stall()};
     *launches = 0;
     int parts = back_warps(cols) ? (int)back_blocks(rows, cols) : 0, rc = 0;
     if (dw && !parts) {  // before dx, which may lie over dy or h

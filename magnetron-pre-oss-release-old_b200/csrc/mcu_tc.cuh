@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 #include <cstdint>
+#include <cstdlib>
 #include "mcu_launch.cuh"
 
 namespace {
@@ -148,6 +149,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
           "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// MAG_CUDA_TC_TEST_STALL=1 makes the first wait of a kernel with bounded waits one that never completes (read at
+// each launch, tests only).
+int test_stall() {
+    const char* e = getenv("MAG_CUDA_TC_TEST_STALL");
+    return e && e[0] == '1';
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
