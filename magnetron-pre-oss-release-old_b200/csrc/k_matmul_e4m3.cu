@@ -153,7 +153,7 @@ template <bool YROW>
 __global__ void __maxnreg__(kPairLaunch)
     gemm_e4m3_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
                    const float* __restrict__ xs, const float* __restrict__ ys, float* __restrict__ r, int M, int N, int G,
-                   int* status) {
+                   int* status, int stall) {
     using C = PairCfg<YROW>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -200,7 +200,8 @@ __global__ void __maxnreg__(kPairLaunch)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairCtrl));
         if (warp == 0) {  // ---- TMA producer
             uint32_t it = 0, s = 0, phase = 1;
-            bool ok = true;
+            // stall, a test of the bounded waits: one for a phase that nothing completes, ahead of every load
+            bool ok = !stall || warp_wait(&empty[0], 0, ab, 11);
             for (int t = pair; ok && t < tiles; t += pairs) {
                 int mb, nb;
                 pair_tile(t, num_m, num_n, mb, nb);
@@ -374,7 +375,7 @@ __global__ void __maxnreg__(kPairLaunch)
         }
     }
     __syncthreads();
-    if (warp == 1 && lane == 0 && rank == 0 && *gave_up) {  // MMAs in flight end before the accumulators go
+    if (warp == 1 && rank == 0 && *gave_up && elect_one()) {  // MMAs in flight end before the accumulators go
         umma_commit_pair_local(drain);
         for (uint32_t i = 0; i < kWaitLimit && !mbar_test(drain, 0); ++i) __nanosleep(64);
     }
@@ -415,7 +416,7 @@ template <int BN, bool YROW>
 __global__ void __launch_bounds__(NarrowCfg<BN, YROW>::THREADS, NarrowCfg<BN, YROW>::PER_SM)
     gemm_e4m3_narrow(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
                      const float* __restrict__ xs, const float* __restrict__ ys, float* __restrict__ r, int M, int N, int G,
-                     int parts, int per, int* status) {
+                     int parts, int per, int* status, int stall) {
     using C = NarrowCfg<BN, YROW>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -458,7 +459,8 @@ __global__ void __launch_bounds__(NarrowCfg<BN, YROW>::THREADS, NarrowCfg<BN, YR
 
     if (warp == 0) {  // ---- TMA producer
         uint32_t s = 0, phase = 1;
-        for (int g = g0; g < g1; ++g) {
+        if (stall) ok = warp_wait(&empty[0], 0, ab, 15);  // (as in the pairs)
+        for (int g = g0; ok && g < g1; ++g) {
             if (!(ok = warp_wait(&empty[s], phase, ab, 15))) break;
             if (elect_one()) {
                 mbar_expect_tx(&full[s], C::STAGE);
@@ -589,7 +591,7 @@ __global__ void __launch_bounds__(NarrowCfg<BN, YROW>::THREADS, NarrowCfg<BN, YR
         cluster_sync();  // a CTA's sums stay until every peer has read them
     }
     if (warp == 1) {
-        if (lane == 0 && *gave_up) {
+        if (*gave_up && elect_one()) {
             umma_commit(drain);
             for (uint32_t i = 0; i < kWaitLimit && !mbar_test(drain, 0); ++i) __nanosleep(64);
         }
@@ -652,7 +654,7 @@ int run_pair(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, cons
     if (tiles > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const int64_t pairs = tiles < sms() / 2 ? tiles : sms() / 2;
     return launch<gemm_e4m3_pair<YROW>>(2 * pairs, kPairThreads, PairCfg<YROW>::SMEM, 2, st, mx, my, xs, ys, r, (int)M, (int)N,
-                  (int)G, status);
+                  (int)G, status, test_stall());
 }
 
 // CTAs per tile: up to 8, while they all run at once and have at least four groups each
@@ -673,9 +675,9 @@ int run_narrow(const CUtensorMap& mx, const CUtensorMap& my, const float* xs, co
     const int per = (int)((G + parts - 1) / parts);
     if (y_block)
         return launch<gemm_e4m3_narrow<BN, false>>(tiles * parts, NarrowCfg<BN, false>::THREADS, NarrowCfg<BN, false>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
-                      (int)N, (int)G, parts, per, status);
+                      (int)N, (int)G, parts, per, status, test_stall());
     return launch<gemm_e4m3_narrow<BN, true>>(tiles * parts, NarrowCfg<BN, true>::THREADS, NarrowCfg<BN, true>::SMEM, parts, st, mx, my, xs, ys, r, (int)M,
-                  (int)N, (int)G, parts, per, status);
+                  (int)N, (int)G, parts, per, status, test_stall());
 }
 
 // Both kernels run in waves of the GPU: 148 tiles of 128 x 128 at a time, or 74 of 256 x 256.  Measured with

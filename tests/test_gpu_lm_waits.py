@@ -51,3 +51,20 @@ def test_norm_backward_of_wide_rows(rows, cols):
     dy, h = (up(g.normal(0, 1, (rows, cols))) for _ in range(2))
     w, rstd, dx, dw = up(g.normal(1, 0.2, cols)), up(np.ones(rows)), up(np.zeros((rows, cols))), up(np.zeros(cols))
     stalled(lambda: d.rmsnorm_rows_backward(rows, cols, dx, dw, dy, h, w, rstd), [dx, dw])
+
+
+# narrow tiles of 16, 32, 64 and 128 rows of x, K whole and split over clusters; pairs
+@pytest.mark.parametrize("block", [True, False])
+@pytest.mark.parametrize("m,k,n", [(4, 4096, 256), (4, 300, 1000), (20, 2048, 130), (20, 128, 4096), (60, 4096, 512), (60, 256, 700),
+                                   (100, 4096, 600), (100, 200, 2000), (1024, 256, 4096), (1000, 2500, 4000)])
+def test_matmul_e4m3(m, k, n, block):
+    d = device()
+    g = np.random.default_rng([0x6F, m, k, n])
+
+    def operand(rows, blocks):
+        q = np.zeros((rows, MB.e4m3_ld(k)), np.uint8)
+        q[:, :k] = g.integers(0, 0x7F, (rows, k))
+        return up(q.view(np.float32)), up(g.uniform(0.5, 2, (-(-rows // 128) if blocks else rows, MB.e4m3_ld(k) // 128)))
+
+    (xq, xs), (yq, ys), r = operand(m, False), operand(n, block), d.tensor((n, m))
+    stalled(lambda: d.matmul_e4m3(m, k, n, r, xq, xs, yq, ys, y_block=block), [r])
