@@ -155,3 +155,28 @@ def test_padding_of_norms_without_a_finite_root(cols):
     # the root of a row with an infinity is 0: the infinity gives NaN, which takes its group, the others give 0
     assert np.all((got[3, :128] & 0x7F) == 0x7F) and not (got[3, 128:] & 0x7F).any()
     assert np.all(got[4, :cols] == 0x7E) and np.isfinite(sc[4]).all()
+
+
+@pytest.mark.parametrize("block", [True, False])
+@pytest.mark.parametrize("m,k,n", [(2, 512, 64), (20, 512, 96), (60, 300, 200), (140, 512, 300), (700, 640, 5000)])
+def test_products_of_whole_numbers_are_exact(m, k, n, block):
+    """0, +-1, 2, 3 and scales of powers of two: every product and sum is a whole number below 2^24 times a
+    power of two, so f32 holds it whatever the order, and the result is equal bit for bit."""
+    d = device()
+    g = np.random.default_rng([0xE7, m])
+    codes = np.array([0x00, 0x38, 0x40, 0x44, 0xB8, 0xC0], np.uint8)
+    ld = MB.e4m3_ld(k)
+
+    def operand(rows, blocks):
+        q = np.zeros((rows, ld), np.uint8)
+        q[:, :k] = codes[g.integers(0, len(codes), (rows, k))]
+        s = 2.0 ** g.integers(0, 3, (-(-rows // 128) if blocks else rows, ld // 128))
+        full = np.repeat(s, 128, 0)[:rows] if blocks else s
+        return q, s.astype(np.float32), VALUES[q].astype(np.float64) * np.repeat(full, 128, 1)
+
+    xq, xs, x = operand(m, False)
+    yq, ys, y = operand(n, block)
+    r = d.tensor((n, m))
+    d.matmul_e4m3(m, k, n, r, up(xq.view(np.float32)), up(xs), up(yq.view(np.float32)), up(ys), y_block=block)
+    want = x @ y.T  # at most 640 * 9 * 16, exact
+    assert np.array_equal(r.read().reshape(m, n), want.astype(np.float32))

@@ -127,3 +127,40 @@ def test_a_replay_waits_for_uploads_and_downloads():
     d.copies_sync()
     assert np.array_equal(got.numpy(), second)
     assert np.array_equal(y.read(), first)
+
+
+def test_a_graph_keeps_its_scratch_when_the_device_grows_its_own():
+    """A device of its own, whose scratch is 1 MiB after the small call: the larger one needs 148 parts of 4096
+    columns, 2.4 MB, so the scratch moves; what it held is allocated again and overwritten."""
+    d = MB.Device()
+    try:
+        g = np.random.default_rng(0x6C)
+
+        def buffers(rows, cols):
+            t = [d.tensor((rows * cols,)) for _ in range(3)] + [d.tensor((cols,)) for _ in range(2)] + [d.tensor((rows,))]
+            for b in t:
+                b.write(g.normal(1, 0.3, b.numel).astype(np.float32))
+            return t  # dx, dy, h, dw, w, rstd
+
+        def backward(rows, cols, t):
+            d.rmsnorm_rows_backward(rows, cols, t[0], t[3], t[1], t[2], t[4], t[5])
+
+        small, large = buffers(300, 512), buffers(300, 4096)
+        replay = capture(d, [lambda: backward(300, 512, small)])
+        want = [small[i].read() for i in (0, 3)]
+        backward(300, 4096, large)
+        d.sync()
+        fill = [d.tensor((1 << 16,)) for _ in range(16)]  # 4 MiB from the pool that took the old scratch back
+        for t in fill:
+            t.write(np.full(t.numel, np.nan, np.float32))
+        for i in (0, 3):
+            small[i].write(np.full(small[i].numel, np.nan, np.float32))
+        replay()
+        d.sync()
+        for i, a in zip((0, 3), want):
+            assert np.array_equal(small[i].read(), a)
+        for t in fill:
+            assert np.isnan(t.read()).all()
+        del replay, small, large, fill
+    finally:
+        d.close()
