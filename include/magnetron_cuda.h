@@ -287,7 +287,8 @@ MAG_CUDA_EXPORT int mag_cuda_quantize_e4m3(mag_compute_device_t* dvc, uint8_t* q
                                            int64_t rows, int64_t cols, int group, int transpose);
 /* r [M][N] = x y^T for e4m3 operands x (M x K, ROW groups) and y (N x K, y_group groups), both with
  * K along their rows: r[m][n] = sum over groups g of xs[m][g] ys[n or n/128][g] (sum over k in g of
- * xq[m][k] yq[n][k]), groups added in f32 with rounding to nearest.  With the operands swapped and
+ * xq[m][k] yq[n][k]), groups added in f32 with rounding to nearest.  The two scales are multiplied first, in f32,
+ * where their product should be a normal number.  With the operands swapped and
  * transposed by mag_cuda_quantize_e4m3 the same call gives both gradients of a layer: dX = dY W^T
  * (W [K][N] quantised without transpose, BLOCK) and dW = X^T dY (both transposed, ROW).
  * M, N < 2^31 - 256; K < 2^31 - 256. */
@@ -299,7 +300,8 @@ MAG_CUDA_EXPORT int mag_cuda_matmul_e4m3(mag_compute_device_t* dvc, float* r, co
  * Outputs, each optional (null) except that y or q must be there: y = v in f32; q and s = v as an
  * e4m3 operand with ROW groups (both or neither); h = t (the next layer's residual, and what the
  * backward pass reads); rstd [rows].  h and y may each be x or residual (not the same one).
- * The sum of squares is formed in f32 per thread over at most cols / 128 values and joined in f32. */
+ * The sum of squares is formed in f32, per thread over at most max(4, cols / 128) values, and joined in f32: a
+ * |t| above 1.8e19 makes it infinite and rstd zero. */
 MAG_CUDA_EXPORT int mag_cuda_rmsnorm_rows_f32(mag_compute_device_t* dvc, float* y, uint8_t* q, float* s, float* h,
                                               float* rstd, const float* x, const float* residual, const float* w,
                                               float eps, int64_t rows, int64_t cols);

@@ -181,9 +181,9 @@ __device__ __forceinline__ uint32_t group_bound(Candidates<T>& cand, uint32_t bi
 
 // One cluster of `parts` CTAs of T threads per row; each streams its part of the row once, 16 logits a
 // thread and chunk, the next chunk's loads issued before the present one is worked on.  Bound by HBM, 4
-// bytes a logit: 4095 x 100003 takes 240 us without alternatives (6.8 TB/s) and 266 us with 5 of them (6.2),
+// bytes a logit: 4095 x 100003 takes 247 us without alternatives (6.6 TB/s) and 298 us with 8 of them (5.5),
 // the rest being the bound's barriers, the chunks in which a candidate shows and, for rows of few chunks, misses of
-// the instruction cache (8192 x 4096: 28 us without alternatives, 56 with one).  Collecting candidates for
+// the instruction cache (8192 x 4096: 29 us without alternatives, 67 with five).  Collecting candidates for
 // the whole block, with a barrier a chunk, took 520 us.
 //
 // Candidates: the top-th largest of 64 group maxima of the first chunk is a lower bound of the row's top-th
@@ -495,10 +495,10 @@ extern "C" int mcu_launch_logprobs(float* logp, float* lse, float* entropy, floa
     // logits each, or eight where they share an SM (148 x 131072 with 20 alternatives: 21.0 us with two parts,
     // 22.9 with one, 34 with 256 threads; 100 x 32000: 11.0 with one, 12.1 with two).
     // Many: an SM's 1024 threads as small blocks, whose barriers and ends overlap better, yet not so small
-    // that the first chunk says little about the row: 4095 x 100003 with 8 alternatives takes 302, 276 and
-    // 351 us with 512, 256 and 128 threads, 8192 x 5000 with 5 takes 200, 118 and 83 us, 8192 x 20000 with 20
-    // takes 196 and 182 us with 256 and 128, 8192 x 32000 250 and 239, 4096 x 50257 179 and 201.  Long rows
-    // whose last wave would be short take the larger blocks (700 x 131072: 75 us, 84).
+    // that the first chunk says little about the row: on the device 4095 x 100003 with 8 alternatives takes 311, 289
+    // and 354 us with 512, 256 and 128 threads, 8192 x 5000 with 5 takes 192, 106 and 78 us, 8192 x 20000 with 20
+    // takes 209 and 179 us with 256 and 128, 8192 x 32000 248 and 231, 4096 x 50257 175 and 200.  Long rows
+    // whose last wave would be short take the larger blocks (700 x 131072: 73 us, 82).
     const auto waves = [&](int64_t blocks) { return (rows + kSms * blocks - 1) / (kSms * blocks); };  // of so many blocks an SM
     if (rows <= 2 * kSms && cols > (rows <= kSms ? 8192 : 16384)) {
         int parts = 1;

@@ -141,7 +141,7 @@ __device__ __forceinline__ void pair_tile(int t, int num_m, int num_n, int& mb, 
 // What bounds it: the group-wise epilogue.  A group is 512 cycles of MMA; its 256 fused multiply-adds per
 // scheduler with their TMEM loads and the way accumulator -> relay -> warpgroup -> MMA issuer, 2 of them in
 // flight, take about 900, at clocks that the 1 kW limit holds near 1.4 GHz: 8192^3 in 0.56 ms (1.95 PFLOP/s)
-// for a few calls and 0.64 ms (1.7) back to back; the MMAs and loads alone took 0.40 and 0.46 ms.
+// for a few calls and 0.63 ms (1.75) back to back; the MMAs and loads alone took 0.40 and 0.46 ms.
 // Measured and not kept: four accumulators of 128 columns (MMAs of N = 128 reach 0.84 of the rate), 16
 // epilogue warps of 64 columns (more instructions, 0.67 ms), packed f32x2 multiply-adds (half the
 // instructions, the same pipe cycles, more register copies: 0.64 ms and up).

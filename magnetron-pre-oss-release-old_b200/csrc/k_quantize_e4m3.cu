@@ -22,7 +22,7 @@ __device__ __forceinline__ uint32_t first_bytes(int n) { return n >= 4 ? 0xFFFFF
 // are 16 neighbouring bytes of the result: they go through a 16 KB tile (16-byte pieces, exclusive-or
 // swizzled against bank conflicts) and leave as whole 128-byte rows.
 // Bound by HBM, 4 bytes read and 1 written a value, with two conversions a value beside it: 8192 x 8192 in rows takes
-// 63 us (5.3 TB/s, 0.82 of the copy rate), an 8192 x 4096 weight turned, in blocks, 30.2 us (5.6 TB/s, 0.85).
+// 63 us (5.3 TB/s, 0.82 of the copy rate), an 8192 x 4096 weight turned, in blocks, 31.4 us (5.3 TB/s, 0.82).
 // A group's scale and factors are formed once: by lane i for the warp's row i, by thread n for the tile's column n.
 template <bool VEC, bool BLOCK, bool TRANSPOSE>
 __global__ void __launch_bounds__(kThreads, 2) quantize_tile(uint8_t* __restrict__ q, float* __restrict__ s,

@@ -120,11 +120,12 @@ __device__ __forceinline__ void norm_group(const NormArgs& a, const float (&t)[4
 }
 
 // One block of W warps per row, the row held in registers (V groups a warp): one read and one write of
-// every value, bound by HBM where rows abound (8192 x 8192 with the residual and an e4m3 result: 149 us,
-// 5.9 TB/s, 0.90 of the copy rate) and by latency (loads, one barrier) where they are few.  Rows wider than a
+// every value, bound by HBM where rows abound (8192 x 8192 with the residual and an e4m3 result: 154 us,
+// 5.7 TB/s, 0.87 of the copy rate) and by latency (loads, one barrier) where they are few.  Rows wider than a
 // block's registers are shared by a cluster (CLUSTER), each block a span of the row and one meeting for the sum:
-// 4096 x 32768 takes 338 us, 5.2 TB/s (548 when a second pass read the row again), bound by the blocks that an
-// SM holds: four at 64 registers a thread (359 us with three at 80).
+// 4096 x 32768 takes 348 us, 5.0 TB/s (before the e4m3 bytes were decided by two factors 338, and 548 when a second
+// pass read the row again), bound by the blocks that an SM holds: four at 64 registers a thread (three at 80 took 6 %
+// more).
 template <int W, int V, bool VEC, bool CLUSTER = false>
 __global__ void __launch_bounds__(W * 32) rmsnorm_row(const NormArgs a) {
     __shared__ float sh[W * (CLUSTER ? kNormCluster : 1)];
@@ -240,7 +241,7 @@ constexpr int kBackCluster = 8;   // blocks of a cluster at most
 
 // Sum over the warps of the cluster's blocks, the same on every thread: each warp sends its share to every
 // block's sh [parts][kBackWarps], counted on that block's mbarrier.  (A cluster barrier instead would wait for
-// the row's stores and loads as well: 4096 x 16384 takes 217 us so, 187 this way.)  Two arrays and mbarriers
+// the row's stores and loads as well: 4096 x 16384 takes 217 us so, 188 this way.)  Two arrays and mbarriers
 // take turns: whoever sends to one again has received what every warp sent after its last reading.  False, for the
 // whole warp, when a wait gave up: the warp then leaves the rows, so that no mbarrier is armed again whose phase is
 // not complete, and its peers, which get nothing more from it, run out of theirs and follow.
@@ -268,9 +269,9 @@ __device__ __forceinline__ bool cluster_sum(float v, float* all, float* sh, uint
 // A block goes through rows blockIdx.x, + grid, ...; a thread keeps the same columns in every row and so its
 // sums for the weight's gradient in registers.  The next row's dy and h are in flight during the row's
 // reduction, which has one barrier: with h loaded after the row's stores instead, every row waited for it
-// (4099 x 5000 took 71 us, now 64).  Bound by HBM, 12 bytes read and 4 written a value: 8192 x 8192 runs at
+// (4099 x 5000 took 71 us, then 64).  Bound by HBM, 12 bytes read and 4 written a value: 8192 x 8192 runs at
 // 6.5 TB/s.  Rows that leave an SM with 9 to 12 warps keep too few bytes in flight that way; their blocks
-// have the registers to fetch dh a row ahead too (AHEAD: 57.5 us, 5.7 TB/s; two blocks an SM with half the
+// have the registers to fetch dh a row ahead too (AHEAD: 58 us, 5.6 TB/s; two blocks an SM with half the
 // registers each spilled and took 66 us).  Rows that do not fit a block's registers (8192 columns) are shared
 // by a cluster (CLUSTER): 4096 x 12288 in 126 us, 6.4 TB/s; in two passes over the row and one for the weight's
 // gradient it took 281.
@@ -445,7 +446,7 @@ constexpr int kWideParts = 64;
 
 // Blocks that share a row in the backward pass: rows wider than a block's registers take an even number, since
 // clusters of three found no room when the kernel before left the SMs in an odd order (4096 x 16384: 253 us, 187
-// in twos).  Blocks of up to 12 warps, which fetch dh ahead, are the faster ones (4096 x 32768: 353 us in sixes,
+// in twos).  Blocks of up to 12 warps, which fetch dh ahead, are the faster ones (4096 x 32768: 356 us in sixes,
 // 400 in fours), but not by enough to take four instead of two (194 us and 187).
 int back_parts(int64_t cols) {
     if (cols <= kBackWarps * kBackV * 128) return 1;

@@ -37,8 +37,8 @@ __device__ __forceinline__ uint32_t e4m3_divide(float scale, float a, float b, f
 }
 // Four values as bytes: each quotient v / s rounded to f32, then to e4m3.  Rounding keeps order, so where v low and
 // v high give the same byte the quotient gives it too; else (5 values of 10^6, those next to a tie) *open gets a bit,
-// and the quotients have to be formed.  Dividing every value instead: an 8192 x 4096 weight turned, in blocks, 37.9 us,
-// 30.2 so; one factor alone (27.9 us) moved one value of 3 * 10^6 to its other neighbour.
+// and the quotients have to be formed.  On the device an 8192 x 4096 weight turned, in blocks, takes 30.4 us so, 37.9
+// when every value is divided, and 27.9 by one factor alone, which moved one value of 3 * 10^6 to its other neighbour.
 __device__ __forceinline__ uint32_t e4m3_try(const E4m3Group& g, float a, float b, float c, float d, uint32_t* open) {
     const uint32_t q = e4m3x4(a * g.low, b * g.low, c * g.low, d * g.low);
     *open |= q ^ e4m3x4(a * g.high, b * g.high, c * g.high, d * g.high);
