@@ -335,6 +335,88 @@ MAG_CUDA_EXPORT int mag_cuda_token_logprobs_backward_f32(mag_compute_device_t* d
                                                          const float* g_logp, const float* g_entropy, int64_t rows,
                                                          int64_t cols, int64_t x_s1, int64_t dx_s1);
 
+/* ---- language-model attention: head norm and rotation, an 8-bit paged cache, attention over it ----
+ * (no counterpart in the reference)
+ *
+ * A head row is head_dim consecutive f32 values; the heads of a token lie one after another, tokens at a
+ * stride of x_s1 values (at least heads * head_dim), so that queries, keys and values may be parts of one
+ * row of a fused projection.  Calls check, order, capture and count as those of the section above; what lies on
+ * the device (positions, slots, tables, lengths) is checked by the kernels, which skip what is out of range.
+ * Sums are formed in f32 in a fixed order, without atomics. */
+
+/* The position's rotation of the first rot values of a head (rot a multiple of 8, at most head_dim; the rest
+ * pass): pair p < rot / 2 turns by the angle pos[row] * inv_freq[p],
+ *   (a, b) -> magnitude (a cos - b sin, b cos + a sin),
+ * the pair being values (p, p + rot / 2), or with interleaved != 0 values (2 p, 2 p + 1).  Angles are formed and
+ * reduced in f64: positions of any int32 value keep their turn's fraction.  Scaled rotations (linear, by
+ * wavelength, with a magnitude) lie in the table and the magnitude. */
+typedef struct mag_cuda_rotation {
+    const int32_t* pos;    /* [rows], device */
+    const float* inv_freq; /* [rot / 2], device */
+    int32_t rot;           /* 0: no rotation, pos and inv_freq are not read */
+    int32_t interleaved;
+    float magnitude;
+} mag_cuda_rotation;
+
+/* y = rotated(normed(x)) of rows x heads head rows.  With w [head_dim] (null: no norm) a head row becomes
+ * x rstd w, rstd = 1 / sqrt(mean(x^2) + eps), which goes to rstd [rows][heads] if that is not null (it wants w).
+ * rotation may be null.  y may be x when the strides are equal.  head_dim: a multiple of 8 from 8 to 256. */
+MAG_CUDA_EXPORT int mag_cuda_rotate_heads_f32(mag_compute_device_t* dvc, float* y, float* rstd, const float* x,
+                                              const float* w, float eps, const mag_cuda_rotation* rotation,
+                                              int64_t rows, int64_t heads, int64_t head_dim, int64_t x_s1,
+                                              int64_t y_s1);
+/* Its gradient: with u = the transposed rotation of dy (magnitude included), from x, w and rstd of the forward call,
+ *   dx = rstd (u w - x rstd^2 mean(u w x)),   dw [head_dim] = sum over rows and heads of u x rstd
+ * (dw null: not wanted; zero for rows = 0).  Without a norm (w null) dx = u, and x, rstd and dw are null.
+ * dx may be dy or x when the strides are equal. */
+MAG_CUDA_EXPORT int mag_cuda_rotate_heads_backward_f32(mag_compute_device_t* dvc, float* dx, float* dw, const float* dy,
+                                                       const float* x, const float* w, const float* rstd,
+                                                       const mag_cuda_rotation* rotation, int64_t rows, int64_t heads,
+                                                       int64_t head_dim, int64_t dx_s1, int64_t dy_s1, int64_t x_s1);
+
+/* A paged cache of keys and values.  Slot s is token s % page_size of page s / page_size; a head row of a slot is
+ * head_dim e4m3 bytes and one scale s, formed as an e4m3 operand's group is (s = max(amax, 2^-100) / 448), except that
+ * a row with a NaN or an infinity has zero bytes and the scale NaN: no byte is ever NaN.
+ * head_dim: a multiple of 16 from 16 to 128; page_size: a power of two from 16 to 1024; pages * page_size < 2^31.
+ * All four arrays are 16-byte aligned. */
+typedef struct mag_cuda_kv_cache {
+    uint8_t* k;     /* [pages][heads][page_size][head_dim] */
+    uint8_t* v;
+    float* k_scale; /* [pages][heads][page_size] */
+    float* v_scale;
+    int32_t pages, heads, head_dim, page_size;
+} mag_cuda_kv_cache;
+/* Writes rows of keys (normed by k_w unless that is null, then rotated) and of values to their slots [rows], and in
+ * the same pass q_out = rotated(normed(q)) for q_heads query heads, normed by q_w (q and q_out null: none; else both,
+ * q_out may be q when the strides are equal).  A slot outside 0 .. pages * page_size - 1 takes no key and value (a row of
+ * padding); its queries are written.  Slots of one call that are not outside are all different, else what those slots
+ * hold afterwards is not defined. */
+MAG_CUDA_EXPORT int mag_cuda_kv_write(mag_compute_device_t* dvc, const mag_cuda_kv_cache* cache, const int32_t* slot,
+                                      const float* k, const float* v, const float* k_w, float* q_out, const float* q,
+                                      const float* q_w, float eps, const mag_cuda_rotation* rotation, int64_t rows,
+                                      int64_t q_heads, int64_t k_s1, int64_t v_s1, int64_t q_s1, int64_t q_out_s1);
+/* The keys and values of slots [rows] in f32 (k or v may be null, not both); zeros for a slot outside the cache. */
+MAG_CUDA_EXPORT int mag_cuda_kv_read(mag_compute_device_t* dvc, const mag_cuda_kv_cache* cache, float* k, float* v,
+                                     const int32_t* slot, int64_t rows, int64_t k_s1, int64_t v_s1);
+/* Attention of new tokens over the cache.  Sequence i has the query rows start[i] .. start[i + 1] - 1 (start [seqs + 1],
+ * not falling, within 0 .. rows) and length[i] cached tokens, its new ones among them as the last; token j lies in slot
+ * j % page_size of page table[i * table_s1 + j / page_size].  Query head h reads kv head h / (q_heads / heads), where
+ * q_heads is a multiple of the cache's heads.  With n new tokens, row t (0 .. n - 1) is at position
+ * p = length - n + t and sees the tokens j with j <= p, j > p - window (window 0: no such limit) and a table entry within
+ * 0 .. pages - 1:
+ *   out = sum_j softmax_j(scale q . k_j) v_j,   lse [rows][q_heads] = log sum_j exp(scale q . k_j)  (null: not wanted).
+ * A row that sees nothing has out 0 and lse -inf.  A NaN or an infinity in a query, or a NaN scale of a key or value,
+ * reaches the rows that see it and no other.  Rows outside start[0] .. start[seqs] keep what out and lse hold, and so do rows of
+ * a sequence past its first max_new (an upper bound of n that the caller knows on the host); lengths are taken as at most
+ * table_s1 * page_size and at least 0.
+ * Products are formed on the tensor cores from f16 halves of the queries and the probabilities (22 bits each; the cache's
+ * values are exact), sums and statistics in f32.  scale: finite, not negative. */
+MAG_CUDA_EXPORT int mag_cuda_attention_paged_f32(mag_compute_device_t* dvc, float* out, float* lse, const float* q,
+                                                 const mag_cuda_kv_cache* cache, const int32_t* table,
+                                                 const int32_t* start, const int32_t* length, int64_t seqs,
+                                                 int64_t table_s1, int64_t rows, int64_t max_new, int64_t q_heads,
+                                                 float scale, int64_t window, int64_t q_s1, int64_t out_s1);
+
 /* ---- allocation-free entry point (no counterpart in the reference) ----
  * R[M,N] = X[M,K] Y[K,N] for 1 <= M <= 16, the same split-K kernels as
  * mag_cuda_matmul_f32 uses for such shapes, but it never allocates: for callers

@@ -65,13 +65,6 @@ __device__ __forceinline__ float block_sum(float v, float* sh, int warp, int lan
     return warp_sum_f(lane < warps ? sh[lane] : 0.0f);
 }
 
-// 1 / sqrt(a), the approximation's last bits put right by one Newton step.
-__device__ __forceinline__ float inv_sqrt(float a) {
-    const float r = rsqrtf(a), p = __fmul_rn(a, r), e = __fmaf_rn(a, r, -p);
-    const float n = __fmaf_rn(__fmaf_rn(-e, r, __fmaf_rn(-p, r, 1.0f)), 0.5f * r, r);
-    return isfinite(n) ? n : r;
-}
-
 struct NormArgs {
     float* y;
     uint8_t* q;

@@ -6,18 +6,9 @@
 #include "magnetron_cuda.h"
 #include "mcu_device.h"
 #include "mcu_kernels.h"
+#include "mcu_args.h"
 
 #include <math.h>
-
-#define MCU_MAX_DIM (((int64_t)1 << 31) - 256)
-
-static int odd4(const void* p) { return ((uintptr_t)p & 3) != 0; }
-static int odd16(const void* p) { return ((uintptr_t)p & 15) != 0; }
-
-/* Row counts and widths that the kernels index (their product stays far below 2^63). */
-static int bad_matrix(int64_t rows, int64_t cols) {
-    return rows < 0 || rows >= MCU_MAX_DIM || cols < 1 || cols >= MCU_MAX_DIM || rows * cols > ((int64_t)1 << 42);
-}
 
 int64_t mag_cuda_e4m3_ld(int64_t cols) { return cols > 0 && cols < MCU_MAX_DIM ? (cols + 127) / 128 * 128 : 0; }
 

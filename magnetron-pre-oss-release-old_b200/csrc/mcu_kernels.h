@@ -10,6 +10,7 @@
 #include <stdint.h>
 #include <stddef.h>
 #include <cuda_runtime_api.h>
+#include "magnetron_cuda.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -152,6 +153,38 @@ int mcu_launch_logprobs(float* logp, float* lse, float* entropy, float* top_logp
 int mcu_launch_logprobs_backward(float* dx, const float* x, const int32_t* id, const float* lse, const float* entropy,
                                  const float* g_logp, const float* g_entropy, int64_t rows, int64_t cols, int64_t x_s1,
                                  int64_t dx_s1, cudaStream_t st, int* launches);
+
+/* k_heads.cu: the rotation's rot is 0 where there is none; the backward pass needs
+ * mcu_rotate_heads_backward_scratch_bytes of scratch when dw is set.  q_heads = 0: no queries. */
+int mcu_launch_rotate_heads(float* y, float* rstd, const float* x, const float* w, float eps, const mag_cuda_rotation* rot,
+                            int64_t rows, int64_t heads, int64_t head_dim, int64_t x_s1, int64_t y_s1, cudaStream_t st,
+                            int* launches);
+size_t mcu_rotate_heads_backward_scratch_bytes(int64_t rows, int64_t heads, int64_t head_dim);
+int mcu_launch_rotate_heads_backward(float* dx, float* dw, const float* dy, const float* x, const float* w, const float* rstd,
+                                     const mag_cuda_rotation* rot, int64_t rows, int64_t heads, int64_t head_dim,
+                                     int64_t dx_s1, int64_t dy_s1, int64_t x_s1, void* scratch, cudaStream_t st,
+                                     int* launches);
+int mcu_launch_kv_write(const mag_cuda_kv_cache* cache, const int32_t* slot, const float* k, const float* v, const float* k_w,
+                        float* q_out, const float* q, const float* q_w, float eps, const mag_cuda_rotation* rot, int64_t rows,
+                        int64_t q_heads, int64_t k_s1, int64_t v_s1, int64_t q_s1, int64_t q_out_s1, cudaStream_t st,
+                        int* launches);
+int mcu_launch_kv_read(const mag_cuda_kv_cache* cache, float* k, float* v, const int32_t* slot, int64_t rows, int64_t k_s1,
+                       int64_t v_s1, cudaStream_t st, int* launches);
+/* k_attention.cu: one call's arguments as in magnetron_cuda.h (window below 2^31 + 1). */
+typedef struct mcu_attention {
+    float* out;
+    float* lse;
+    const float* q;
+    mag_cuda_kv_cache cache;
+    const int32_t* table;
+    const int32_t* start;
+    const int32_t* length;
+    int64_t seqs, table_s1, rows, max_new, q_heads;
+    float scale;
+    int64_t window, q_s1, out_s1;
+} mcu_attention;
+size_t mcu_attention_scratch_bytes(const mcu_attention* a);
+int mcu_launch_attention(const mcu_attention* a, void* scratch, int* status, cudaStream_t st, int* launches);
 
 #ifdef __cplusplus
 }

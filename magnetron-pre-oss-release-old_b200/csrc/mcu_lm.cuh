@@ -1,4 +1,4 @@
-// Device helpers of the language-model row kernels (norm, e4m3 quantiser and product, log probabilities).
+// Device helpers of the language-model row kernels (norms, e4m3 quantiser and product, cache, log probabilities).
 #ifndef MCU_LM_CUH
 #define MCU_LM_CUH
 #include <cstdint>
@@ -54,6 +54,13 @@ __device__ __forceinline__ float warp_sum_f(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+}
+
+// 1 / sqrt(a), the approximation's last bits put right by one Newton step.
+__device__ __forceinline__ float inv_sqrt(float a) {
+    const float r = rsqrtf(a), p = __fmul_rn(a, r), e = __fmaf_rn(a, r, -p);
+    const float n = __fmaf_rn(__fmaf_rn(-e, r, __fmaf_rn(-p, r, 1.0f)), 0.5f * r, r);
+    return isfinite(n) ? n : r;
 }
 
 }  // namespace mcu

@@ -142,6 +142,11 @@ def load_library(path: str = LIB_PATH):
         "mag_cuda_rmsnorm_rows_backward_f32": ([vp] * 8 + [i64, i64], C.c_int),
         "mag_cuda_token_logprobs_f32": ([vp] * 8 + [i64, i64, i64, C.c_int], C.c_int),
         "mag_cuda_token_logprobs_backward_f32": ([vp] * 8 + [i64, i64, i64, i64], C.c_int),
+        "mag_cuda_rotate_heads_f32": ([vp] * 5 + [C.c_float, vp] + [i64] * 5, C.c_int),
+        "mag_cuda_rotate_heads_backward_f32": ([vp] * 8 + [i64] * 6, C.c_int),
+        "mag_cuda_kv_write": ([vp] * 9 + [C.c_float, vp] + [i64] * 6, C.c_int),
+        "mag_cuda_kv_read": ([vp] * 5 + [i64] * 3, C.c_int),
+        "mag_cuda_attention_paged_f32": ([vp] * 8 + [i64] * 5 + [C.c_float] + [i64] * 3, C.c_int),
         "mag_cuda_fill_uniform_pcg_f32": ([vp, vp, i64, C.c_float, C.c_float, C.POINTER(C.c_uint64), C.c_uint64],
                                           C.c_int),
         "mag_cuda_fill_normal_pcg_f32": ([vp, vp, i64, C.c_float, C.c_float, C.POINTER(C.c_uint64), C.c_uint64],
@@ -300,6 +305,21 @@ def e4m3_values() -> np.ndarray:
     return np.where(b & 0x80, -v, v).astype(np.float32)
 
 
+def rope_frequencies(rot: int, base: float = 10000.0, *, factor: float = 1.0, original: int = 0, low: float = 1.0,
+                     high: float = 32.0) -> np.ndarray:
+    """The inv_freq table of a Rotation: pair p turns by base^(-2 p / rot) a position.  factor > 1 stretches it for
+    contexts that much longer: every pair alike, or with original (the context it was trained on) by wavelength: pairs
+    that turn at least `high` times in the original context keep their frequency, those that turn at most `low` times
+    are slowed by the whole factor, and between the two the frequencies are mixed linearly."""
+    if rot < 0 or rot % 2 or not base > 0 or not factor > 0 or original < 0 or not 0 <= low < high:
+        raise ValueError("rope_frequencies: rot even, base and factor above 0, 0 <= low < high")
+    f = base ** (-np.arange(0, rot, 2, dtype=np.float64) / max(rot, 1))
+    keep = np.zeros_like(f)
+    if original:
+        keep = np.clip((original * f / (2.0 * np.pi) - low) / (high - low), 0.0, 1.0)
+    return (f * keep + f / factor * (1.0 - keep)).astype(np.float32)
+
+
 # ------------------------------------------------------------------- tensors
 class Tensor:
     """One ``mag_tensor_t`` owned by Python, with storage from the device."""
@@ -384,6 +404,39 @@ class Tensor:
                 self.free()
         except Exception:
             pass
+
+
+class RotationStruct(C.Structure):
+    """mag_cuda_rotation"""
+    _fields_ = [("pos", C.c_void_p), ("inv_freq", C.c_void_p), ("rot", C.c_int32), ("interleaved", C.c_int32),
+                ("magnitude", C.c_float)]
+
+
+class KvCacheStruct(C.Structure):
+    """mag_cuda_kv_cache"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("pages", C.c_int32),
+                ("heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32)]
+
+
+class Rotation:
+    """The turn of the first rot values of each head by its row's position: pos (int32, a row's position) and
+    inv_freq (rope_frequencies) are Tensors or device addresses."""
+
+    def __init__(self, pos, inv_freq, rot: int, *, interleaved: bool = False, magnitude: float = 1.0):
+        self.pos, self.inv_freq = pos, inv_freq
+        self.c = RotationStruct(address(pos), address(inv_freq), rot, int(interleaved), magnitude)
+        self.ptr = C.addressof(self.c)
+
+
+class KvCache:
+    """A paged cache of e4m3 keys and values with a scale per token and head: k, v [pages][heads][page_size][head_dim],
+    k_scale, v_scale [pages][heads][page_size], Tensors (Device.kv_cache) or device addresses."""
+
+    def __init__(self, k, v, k_scale, v_scale, pages: int, heads: int, head_dim: int, page_size: int):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.heads, self.head_dim, self.page_size = pages, heads, head_dim, page_size
+        self.c = KvCacheStruct(address(k), address(v), address(k_scale), address(v_scale), pages, heads, head_dim, page_size)
+        self.ptr = C.addressof(self.c)
 
 
 class Device:
@@ -525,6 +578,63 @@ class Device:
             self.p, address(dx), address(x), address(ids), address(lse), address(entropy), address(g_logp),
             address(g_entropy), rows, cols, cols if x_stride is None else x_stride,
             cols if dx_stride is None else dx_stride), "token_logprobs_backward")
+
+    # ---- language-model attention.  Strides (of rows, in values) default to the heads' own width.
+    def kv_cache(self, pages: int, heads: int, head_dim: int, page_size: int) -> KvCache:
+        """A paged cache in this device's storage; slots that were never written hold zeros."""
+        if min(pages, heads) < 1 or head_dim % 16 or not 16 <= head_dim <= 128 or page_size & (page_size - 1) or not 16 <= page_size <= 1024:
+            raise ValueError(f"a cache of {pages} pages of {page_size} tokens, {heads} heads of {head_dim} values")
+        n = pages * heads * page_size
+        k, v = (self.tensor((n * head_dim // 4,)) for _ in range(2))
+        return KvCache(k, v, self.tensor((n,)), self.tensor((n,)), pages, heads, head_dim, page_size)
+
+    def rotate_heads(self, rows: int, heads: int, head_dim: int, y, x, *, w=None, eps: float = 1e-6, rstd=None,
+                     rotation: Rotation | None = None, x_stride: int | None = None, y_stride: int | None = None):
+        """y = x with each head normed (w) and rotated; rstd [rows][heads] for the backward pass."""
+        n = heads * head_dim
+        check(self.L.mag_cuda_rotate_heads_f32(self.p, address(y), address(rstd), address(x), address(w), eps,
+                                               rotation.ptr if rotation else None, rows, heads, head_dim,
+                                               n if x_stride is None else x_stride, n if y_stride is None else y_stride),
+              "rotate_heads")
+
+    def rotate_heads_backward(self, rows: int, heads: int, head_dim: int, dx, dw, dy, *, x=None, w=None, rstd=None,
+                              rotation: Rotation | None = None, dx_stride: int | None = None,
+                              dy_stride: int | None = None, x_stride: int | None = None):
+        """dx and dw of rotate_heads, from the gradient dy of y."""
+        n = heads * head_dim
+        check(self.L.mag_cuda_rotate_heads_backward_f32(
+            self.p, address(dx), address(dw), address(dy), address(x), address(w), address(rstd),
+            rotation.ptr if rotation else None, rows, heads, head_dim, n if dx_stride is None else dx_stride,
+            n if dy_stride is None else dy_stride, n if x_stride is None else x_stride), "rotate_heads_backward")
+
+    def kv_write(self, cache: KvCache, rows: int, slot, k, v, *, k_w=None, q=None, q_out=None, q_heads: int = 0, q_w=None,
+                 eps: float = 1e-6, rotation: Rotation | None = None, k_stride: int | None = None,
+                 v_stride: int | None = None, q_stride: int | None = None, q_out_stride: int | None = None):
+        """Keys (normed by k_w, rotated) and values of rows into their slots; q_out = q normed by q_w and rotated."""
+        n, m = cache.heads * cache.head_dim, q_heads * cache.head_dim
+        check(self.L.mag_cuda_kv_write(
+            self.p, cache.ptr, address(slot), address(k), address(v), address(k_w), address(q_out), address(q),
+            address(q_w), eps, rotation.ptr if rotation else None, rows, q_heads, n if k_stride is None else k_stride,
+            n if v_stride is None else v_stride, m if q_stride is None else q_stride,
+            m if q_out_stride is None else q_out_stride), "kv_write")
+
+    def kv_read(self, cache: KvCache, rows: int, slot, *, k=None, v=None, k_stride: int | None = None,
+                v_stride: int | None = None):
+        """The keys and values of slots in f32."""
+        n = cache.heads * cache.head_dim
+        check(self.L.mag_cuda_kv_read(self.p, cache.ptr, address(k), address(v), address(slot), rows,
+                                      n if k_stride is None else k_stride, n if v_stride is None else v_stride),
+              "kv_read")
+
+    def attention_paged(self, cache: KvCache, rows: int, q_heads: int, out, q, table, start, length, seqs: int,
+                        table_stride: int, *, max_new: int, scale: float, window: int = 0, lse=None,
+                        q_stride: int | None = None, out_stride: int | None = None):
+        """out = attention of the rows of sequence i, start[i] .. start[i + 1] - 1, over its length[i] cached tokens."""
+        n = q_heads * cache.head_dim
+        check(self.L.mag_cuda_attention_paged_f32(
+            self.p, address(out), address(lse), address(q), cache.ptr, address(table), address(start), address(length),
+            seqs, table_stride, rows, max_new, q_heads, scale, window, n if q_stride is None else q_stride,
+            n if out_stride is None else out_stride), "attention_paged")
 
     # ---- .magnetron storage (mag_tensor_save / mag_tensor_load, magnetron/magnetron.c:2931-2977)
     def save(self, path: str, tensors):
