@@ -1,13 +1,383 @@
 // k_attention.cu - attention of new tokens over the paged e4m3 cache (mag_cuda_attention_paged_f32).
 #include <cuda_runtime.h>
 #include <cstdint>
-#include "mcu_kernels.h"
-#include "mcu_launch.cuh"
-#include "mcu_lm.cuh"
+#include "mcu_attention.cuh"
 
 using namespace mcu;
 
 namespace {
+
+// ------------------------------------------------------------ few rows: single tokens and short runs of them
+//
+// The rows of one kv head (new tokens x query heads of the group) are at most 16 here, so the cache's bytes bound the
+// work: each is read once, by one warp, for all rows.  A block works through its share of all (sequence, kv head) items'
+// units of 128 tokens; a warp takes every eighth group of 16 tokens, four groups in flight by cp.async in a ring of its
+// own, and keeps its own running maximum, sum and output.  The block's warps are joined in shared memory when an item
+// ends, blocks that share an item by attention_join.
+//
+// Products run on mma.sync m16n8k16 (f16, f32 sums): e4m3 bytes become f16 in registers, exactly.  Queries and
+// probabilities are split in two f16, high and low.  Up to 8 rows (STACK) the halves are rows 0-7 and 8-15 of one
+// operand, so that the split costs no instruction and a thread finds both halves' results in its own registers.
+// The order of a product's inner index is free, so it is chosen such that a thread's operands are 16 consecutive bytes
+// of a row of keys (inner index: the head's values) and of four rows of values (columns: the head's values).
+constexpr int kFewWarps = 8, kFewStages = 4;
+constexpr int kGroup = 16;               // tokens of a warp's step; pages hold a multiple
+constexpr int kFlush = 16;               // groups between two flushes: the tensor core's sums lose up to a step each
+constexpr float kTop = 15.0f;            // probabilities are formed as 2^kTop p: their f16 halves keep 22 bits down to 2^-18
+
+template <int DP>
+struct FewCfg {
+    static constexpr int STAGE = 2 * kGroup * DP + 2 * kGroup * 4;  // keys, values, their scales
+    static constexpr int RING = kFewStages * STAGE;
+};
+template <int DP, bool STACK>
+struct FewSmem {
+    static constexpr int VALS = (STACK ? DP / 4 : DP / 2);  // outputs a thread holds
+    static constexpr int SUMS = FewCfg<DP>::RING * kFewWarps;
+    static constexpr int STATS = SUMS + kFewWarps * 32 * VALS * 4;  // [warp][16] of (m, l), then [warp] of the values' unit
+    static constexpr int BYTES = STATS + kFewWarps * 16 * 8 + kFewWarps * 4;
+    static_assert(Share<16, DP, 32 * kFewWarps>::SMEM <= SUMS, "the search for work takes the rings' room");
+};
+
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+template <int DP, bool STACK>
+__global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
+    using C = FewCfg<DP>;
+    using S = FewSmem<DP, STACK>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int KI = DP / 64;      // 16-byte pieces of a key a thread holds
+    constexpr int NT = DP / 8;       // column tiles of the output
+    constexpr int VB = DP / 8;       // bytes of a row of values a thread holds
+    constexpr int QF = STACK ? 1 : 2;
+    constexpr int NR = STACK ? 1 : 2;  // rows a thread works on: g, and g + 8
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const uint32_t ring = smem_addr(smem) + warp * C::RING;
+    float4* sums = (float4*)(smem + S::SUMS) + warp * 8 * S::VALS;  // [VALS / 4][32]
+    float2* stats = (float2*)(smem + S::STATS);
+    float* units = (float*)(stats + kFewWarps * 16);
+        pdl_begin();
+
+    Share<16, DP, 32 * kFewWarps> sh;
+    if (!sh.find(a, (int64_t*)smem)) return;
+    if (a.dim != DP) {  // columns past the head's stay zero: no copy writes them
+        for (int i = lane; i < C::RING / 16; i += 32) *(uint4*)(smem + warp * C::RING + 16 * i) = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+    }
+    while (sh.more()) {
+        const Item it = sh.item(a);
+        const int rows = it.rows;
+        // ---- queries: operand fragments and each row's factor to log2 units
+        uint32_t qf[QF][4 * KI][4];
+        float rf[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int row = g + 8 * r;
+            float x[KI][16];
+            uint32_t top = 0;
+            const bool live = row < rows;
+            const float* p = a.q + (int64_t)(it.row0 + (live ? row / a.group : 0)) * a.q_s1 +
+                             (int64_t)(it.head * a.group + (live ? row % a.group : 0)) * a.dim;
+#pragma unroll
+            for (int i = 0; i < KI; ++i) {
+                const int d = 64 * i + 16 * c;
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const float4 t = live && d < a.dim ? load4(p + d + 4 * v, a.q_vec) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    x[i][4 * v] = t.x, x[i][4 * v + 1] = t.y, x[i][4 * v + 2] = t.z, x[i][4 * v + 3] = t.w;
+                }
+#pragma unroll
+                for (int v = 0; v < 16; ++v) top = max(top, abs_bits(x[i][v]));
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float up = query_unit(top);
+            rf[r] = a.scale * kLog2e / up;
+#pragma unroll
+            for (int i = 0; i < KI; ++i)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    uint32_t h0, l0, h1, l1;
+                    split2(x[i][4 * s] * up, x[i][4 * s + 1] * up, h0, l0);
+                    split2(x[i][4 * s + 2] * up, x[i][4 * s + 3] * up, h1, l1);
+                    if (STACK) {
+                        qf[0][4 * i + s][0] = h0, qf[0][4 * i + s][1] = l0, qf[0][4 * i + s][2] = h1, qf[0][4 * i + s][3] = l1;
+                    } else {
+                        qf[0][4 * i + s][r] = h0, qf[0][4 * i + s][2 + r] = h1;
+                        qf[QF - 1][4 * i + s][r] = l0, qf[QF - 1][4 * i + s][2 + r] = l1;
+                    }
+                }
+        }
+        // ---- what each row sees, and what all rows do
+        int first[NR], last[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int row = g + 8 * r;
+            last[r] = row < rows ? it.pos + row / a.group : -1;
+            first[r] = a.window && last[r] >= a.window ? last[r] - a.window + 1 : 0;
+        }
+        const int all_last = it.pos, all_first = it.top_first;  // tokens within are seen by every row
+
+        float o[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        float m[NR], mrf[NR], l[NR], fade[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, mrf[r] = kNone, l[r] = 0.0f, fade[r] = 1.0f;
+        float unit = kLeastUnit, per_unit = 1.0f / kLeastUnit;
+#pragma unroll
+        for (int e = 0; e < S::VALS / 4; ++e) sums[e * 32 + lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+        const int g0 = it.from * 8 + warp, g1 = min(it.to * 8, (it.high - it.base + kGroup - 1) / kGroup), steps = g0 < g1 ? (g1 - g0 + 7) / 8 : 0;
+        const int32_t* table = a.table + (int64_t)it.seq * a.table_s1;
+        int page = steps > 0 ? table[(it.base + kGroup * g0) >> a.page_log] : -1;
+        uint32_t there = 0;  // bit s: the group in stage s has a page
+        int issued = 0;
+        auto issue = [&]() {
+            if (issued < steps) {
+                const int j0 = it.base + kGroup * (g0 + 8 * issued), st = issued & (kFewStages - 1);
+                const bool ok = (uint32_t)page < (uint32_t)a.pages;
+                there = (there & ~(1u << st)) | ((uint32_t)ok << st);
+                if (ok) {
+                    const int64_t at = ((((int64_t)page * a.heads) + it.head) << a.page_log) + (j0 & ((1 << a.page_log) - 1));
+                    const uint32_t dst = ring + st * C::STAGE;
+                    constexpr int PR = 512 / DP;  // rows of one copy of the warp
+                    const int r0 = lane / (DP / 16), ch = lane % (DP / 16);
+#pragma unroll
+                    for (int i = 0; i < kGroup / PR; ++i) {
+                        const int row = r0 + PR * i, j = j0 + row;
+                        const bool in = j >= it.low && j < it.high;
+                        if (16 * ch < a.dim) {
+                            copy16(dst + row * DP + 16 * key_chunk<DP>(ch, row), a.k + (at + row) * a.dim + 16 * ch, in);
+                            copy16(dst + kGroup * DP + row * DP + 16 * value_chunk<DP>(ch, row), a.v + (at + row) * a.dim + 16 * ch, in);
+                        }
+                    }
+                    if (lane < 8) copy16(dst + 2 * kGroup * DP + 16 * lane, (lane < 4 ? a.ks : a.vs) + at + 4 * (lane & 3), true);
+                }
+                if (issued + 1 < steps) page = table[(j0 + 8 * kGroup) >> a.page_log];
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ++issued;
+        };
+        auto flush = [&]() {
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int e = 0; e < DP / 16; ++e) {  // half of the columns, four tiles
+                    float4 t = sums[(r * (DP / 16) + e) * 32 + lane];
+                    const int half = e / (DP / 32), j = 4 * (e % (DP / 32));
+                    float v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = STACK ? o[j + k][half] + o[j + k][2 + half] : o[j + k][2 * r + half];
+                    t.x = fmaf(t.x, fade[r], v[0]), t.y = fmaf(t.y, fade[r], v[1]), t.z = fmaf(t.z, fade[r], v[2]), t.w = fmaf(t.w, fade[r], v[3]);
+                    sums[(r * (DP / 16) + e) * 32 + lane] = t;
+                }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) fade[r] = 1.0f;
+        };
+#pragma unroll
+        for (int s = 0; s < kFewStages - 1; ++s) issue();
+        for (int i = 0; i < steps; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
+            __syncwarp();
+            const int st = i & (kFewStages - 1), j0 = it.base + kGroup * (g0 + 8 * i);
+            const bool has = there >> st & 1;
+            issue();
+            if (!has) continue;  // (the same for the whole warp)
+            const uint32_t at = ring + st * C::STAGE;
+            // ---- logits of 16 tokens: tiles of 8, the inner index in the order of the thread's bytes
+            float s[2][4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+#pragma unroll
+                for (int p = 0; p < KI; ++p) {
+                    const uint4 w = lds128(at + (8 * t + g) * DP + 16 * key_chunk<DP>(4 * p + c, 8 * t + g));
+                    const uint32_t b[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t b0 = f16_of_e4m3(b[k]), b1 = f16_of_e4m3(b[k] >> 16);
+#pragma unroll
+                        for (int f = 0; f < QF; ++f) mma16(s[t], qf[f][4 * p + k], b0, b1);
+                    }
+                }
+            }
+            float ks[4], vs[4];
+            {
+                const float2 k0 = lds64(at + 2 * kGroup * DP + 8 * c), k1 = lds64(at + 2 * kGroup * DP + 32 + 8 * c);
+                const float2 v0 = lds64(at + 2 * kGroup * DP + 64 + 8 * c), v1 = lds64(at + 2 * kGroup * DP + 96 + 8 * c);
+                ks[0] = k0.x, ks[1] = k0.y, ks[2] = k1.x, ks[3] = k1.y, vs[0] = v0.x, vs[1] = v0.y, vs[2] = v1.x, vs[3] = v1.y;
+            }
+            const bool edge = j0 < all_first || j0 + kGroup - 1 > all_last;
+            float t[NR][4];
+            bool seen[NR][4];
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float raw = STACK ? s[k >> 1][k & 1] + s[k >> 1][2 + (k & 1)] : s[k >> 1][2 * r + (k & 1)];
+                    t[r][k] = raw * ks[k];
+                    seen[r][k] = true;
+                }
+            if (edge) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int j = j0 + 8 * (k >> 1) + 2 * c + (k & 1);
+                    if (j < it.low || j >= it.high) vs[k] = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        seen[r][k] = j >= first[r] && j <= last[r];
+                        if (!seen[r][k]) t[r][k] = -INFINITY;
+                    }
+                }
+            }
+            // ---- the running maxima and the values' unit, where one of them grows
+            bool grows = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                grows |= vs[k] > unit;
+#pragma unroll
+                for (int r = 0; r < NR; ++r) grows |= t[r][k] > m[r];
+            }
+            if (__any_sync(0xffffffffu, grows)) {
+                float v = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+                float shrink = 1.0f;
+                if (v > unit && v < kLargestScale) {
+                    const float next = unit_above(v);
+                    shrink = unit / next;
+                    unit = next, per_unit = 1.0f / next;
+                }
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    float x = fmaxf(fmaxf(t[r][0], t[r][1]), fmaxf(t[r][2], t[r][3]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                    float f = 1.0f;
+                    if (x > m[r]) {
+                        const float next = fmaf(x, rf[r], -kTop);
+                        f = exp2_f(mrf[r] - next);
+                        m[r] = x, mrf[r] = next;
+                        l[r] *= f;
+                    }
+                    f *= shrink;
+                    fade[r] *= f;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        o[j][2 * r] *= f, o[j][2 * r + 1] *= f;
+                        if (STACK) o[j][2] *= f, o[j][3] *= f;
+                    }
+                }
+            }
+            // ---- probabilities, times their values' scales in the unit, as operand fragments
+            uint32_t pf[QF][4];
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                float w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float p = exp2_f(fmaf(t[r][k], rf[r], -mrf[r]));
+                    if (!seen[r][k]) p = 0.0f;
+                    l[r] += p;
+                    w[k] = seen[r][k] ? p * (vs[k] * per_unit) : 0.0f;
+                }
+                uint32_t h0, l0, h1, l1;
+                split2(w[0], w[1], h0, l0);
+                split2(w[2], w[3], h1, l1);
+                if (STACK) {
+                    pf[0][0] = h0, pf[0][1] = l0, pf[0][2] = h1, pf[0][3] = l1;
+                } else {
+                    pf[0][r] = h0, pf[0][2 + r] = h1;
+                    pf[QF - 1][r] = l0, pf[QF - 1][2 + r] = l1;
+                }
+            }
+            // ---- output: 16 tokens are the inner index, a thread holds VB bytes of the four rows of its tokens
+            uint32_t b[4][VB / 4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int row = 8 * (k >> 1) + 2 * c + (k & 1);
+                const uint32_t va = at + kGroup * DP + row * DP;
+                if (DP == 128) {
+                    const uint4 w = lds128(va + 16 * value_chunk<DP>(g, row));
+                    b[k][0] = w.x, b[k][1] = w.y, b[k][VB / 4 - 2] = w.z, b[k][VB / 4 - 1] = w.w;
+                } else {
+                    const float2 w = lds64(va + 16 * value_chunk<DP>(g >> 1, row) + 8 * (g & 1));
+                    b[k][0] = __float_as_uint(w.x), b[k][1] = __float_as_uint(w.y);
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < VB / 4; ++w)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t x = __byte_perm(b[0][w], b[1][w], h ? 0x7362 : 0x5140), y = __byte_perm(b[2][w], b[3][w], h ? 0x7362 : 0x5140);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t b0 = f16_of_e4m3(k ? x >> 16 : x), b1 = f16_of_e4m3(k ? y >> 16 : y);
+#pragma unroll
+                        for (int f = 0; f < QF; ++f) mma16(o[4 * w + 2 * h + k], pf[f], b0, b1);
+                    }
+                }
+            if ((i & (kFlush - 1)) == kFlush - 1) flush();
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        flush();
+        // ---- the block's warps joined
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (c == 0) stats[warp * 16 + g + 8 * r] = make_float2(mrf[r], l[r]);
+        }
+        if (lane == 0) units[warp] = unit;
+        __syncthreads();
+        for (int x = threadIdx.x; x < 8 * S::VALS; x += 32 * kFewWarps) {
+            const int e = x >> 5, ln = x & 31, r = e / (DP / 16), row = (ln >> 2) + 8 * r;
+            const int half = e % (DP / 16) / (DP / 32), j = 4 * (e % (DP / 32)), d = VB * (2 * (ln & 3) + half) + j;
+            if (row >= rows || d >= a.dim) continue;
+            float top = kNone, total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, stats[w * 16 + row].x);
+            float f[kFewWarps];
+#pragma unroll
+            for (int w = 0; w < kFewWarps; ++w) {
+                const float2 st = stats[w * 16 + row];
+                f[w] = exp2_f(st.x - top);
+                total = fmaf(st.y, f[w], total);
+            }
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kFewWarps; ++w) {
+                const float4 t = ((float4*)(smem + S::SUMS))[w * 8 * S::VALS + x];
+                const float k = f[w] * inv * units[w];
+                v.x = fmaf(t.x, k, v.x), v.y = fmaf(t.y, k, v.y), v.z = fmaf(t.z, k, v.z), v.w = fmaf(t.w, k, v.w);
+            }
+            put_out(a, sh, it, row, d, v, top, total);
+        }
+        __syncthreads();
+        sh.advance(a, it);
+    }
+}
+
+template <int DP, bool STACK>
+int run_few(const AttnArgs& a, cudaStream_t st) {
+    static bool done[64];
+    constexpr int bytes = FewSmem<DP, STACK>::BYTES;
+    const cudaError_t e = allow_smem(attention_few<DP, STACK>, bytes, done);
+    if (e != cudaSuccess) return (int)e;
+    return (int)launch_dep(attention_few<DP, STACK>, dim3((unsigned)a.blocks), dim3(32 * kFewWarps), bytes, st, a);
+}
 
 __device__ __forceinline__ float4 e4m3_values(uint32_t b) {
     uint32_t lo, hi;
@@ -67,15 +437,38 @@ __global__ void __launch_bounds__(128) attention_rows(mcu_attention a) {
     if (a.lse && lane == 0) a.lse[row * a.q_heads + head] = l == 0.0f ? -INFINITY : m + logf(l);
 }
 
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+constexpr int kSms = 148;
+constexpr int kFewRows = 16;
+int padded(const mcu_attention* a) { return a->cache.head_dim <= 64 ? 64 : 128; }
+
 }  // namespace
 
 extern "C" size_t mcu_attention_scratch_bytes(const mcu_attention* a) {
-    (void)a;
-    return 0;
+    return (size_t)(2 * kSms * part_floats(kFewRows, padded(a))) * 4;
 }
 
-extern "C" int mcu_launch_attention(const mcu_attention* a, void* scratch, int* status, cudaStream_t st, int* launches) {
-    (void)scratch, (void)status;
-    *launches = 1;
-    return (int)launch_dep(attention_rows, dim3((unsigned)((a->rows * a->q_heads + 3) / 4)), dim3(128), 0, st, *a);
+extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, int* status, cudaStream_t st, int* launches) {
+    const int group = (int)(c->q_heads / c->cache.heads);
+    if (c->max_new * group > kFewRows) {
+        *launches = 1;
+        return (int)launch_dep(attention_rows, dim3((unsigned)((c->rows * c->q_heads + 3) / 4)), dim3(128), 0, st, *c);
+    }
+    AttnArgs a = {};
+    a.out = c->out, a.lse = c->lse, a.q = c->q, a.k = c->cache.k, a.v = c->cache.v, a.ks = c->cache.k_scale, a.vs = c->cache.v_scale;
+    a.table = c->table, a.start = c->start, a.length = c->length, a.table_s1 = c->table_s1, a.q_s1 = c->q_s1, a.out_s1 = c->out_s1;
+    a.parts = (float*)scratch, a.status = status, a.seqs = (int)c->seqs, a.rows = (int)c->rows, a.max_new = (int)c->max_new;
+    a.heads = c->cache.heads, a.group = group, a.dim = c->cache.head_dim, a.pages = c->cache.pages;
+    while ((1 << a.page_log) < c->cache.page_size) ++a.page_log;
+    a.window = c->window >= ((int64_t)1 << 31) - 1 ? 0 : (int)c->window;
+    a.longest = (int)(c->table_s1 * c->cache.page_size);
+    a.least = 1, a.most = kFewRows, a.blocks = kSms, a.scale = c->scale;
+    a.q_vec = aligned16(c->q) && !(c->q_s1 & 3), a.out_vec = aligned16(c->out) && !(c->out_s1 & 3);
+    const bool stack = c->max_new * group <= 8, wide = a.dim > 64;
+    int rc = wide ? stack ? run_few<128, true>(a, st) : run_few<128, false>(a, st) : stack ? run_few<64, true>(a, st) : run_few<64, false>(a, st);
+    if (rc) return rc;
+    *launches = 2;
+    const dim3 grid(a.blocks, kFewRows / 4);
+    return (int)(wide ? launch_dep(attention_join<16, 128>, grid, dim3(128), 0, st, a) : launch_dep(attention_join<16, 64>, grid, dim3(128), 0, st, a));
 }

@@ -130,7 +130,7 @@ int mag_cuda_attention_paged_f32(mag_compute_device_t* dvc, float* out, float* l
                                  const int32_t* length, int64_t seqs, int64_t table_s1, int64_t rows, int64_t max_new,
                                  int64_t q_heads, float scale, int64_t window, int64_t q_s1, int64_t out_s1) {
     if (!dvc || !out || !q || bad_cache(cache) || !table || !start || !length || bad_matrix(seqs, table_s1) ||
-        table_s1 * cache->page_size >= ((int64_t)1 << 31) || max_new < 0 || max_new >= MCU_MAX_DIM || q_heads % cache->heads ||
+        table_s1 * cache->page_size >= MCU_MAX_DIM || max_new < 0 || max_new >= MCU_MAX_DIM || q_heads % cache->heads ||
         bad_heads(rows, q_heads, cache->head_dim, q_s1) || bad_heads(rows, q_heads, cache->head_dim, out_s1) || !(scale >= 0.0f) ||
         isinf(scale) || window < 0 || out == q || odd4(out) || odd4(lse) || odd4(q) || odd4(table) || odd4(start) || odd4(length))
         return MAG_CUDA_E_INVALID;

@@ -1,0 +1,364 @@
+// Pieces that the attention kernels share: how blocks share the work, what an item is, and where its output goes.
+#ifndef MCU_ATTENTION_CUH
+#define MCU_ATTENTION_CUH
+#include <cuda_runtime.h>
+#include <cstdint>
+#include "mcu_kernels.h"
+#include "mcu_launch.cuh"
+#include "mcu_lm.cuh"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+constexpr float kNone = -3.0e38f;               // the maximum of no logits: finite, so that differences of it stay numbers
+constexpr float kLeastUnit = 0x1p-120f;         // unit of the values' scales before any was seen (the least scale is 2^-109)
+constexpr float kLargestScale = 0x1p126f;       // a scale that is no number or not finite does not set the unit
+constexpr int kUnitTokens = 128;                // tokens of a unit of work
+
+struct AttnArgs {
+    float *out, *lse;
+    const float* q;
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    const int32_t *table, *start, *length;
+    int64_t table_s1, q_s1, out_s1;
+    float* parts;  // two slots a block, of part_floats() floats
+    int* status;
+    int seqs, rows, max_new, heads, group, dim, pages, page_log, window;
+    int longest;             // tokens that a sequence's table has room for
+    int least, most;         // the rows of a kv head (new tokens x group) of the sequences that this launch takes
+    int blocks, q_vec, out_vec, stall;
+    float scale;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 lds64(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load4(const float* p, int vec) {
+    if (vec) return *(const float4*)p;
+    return make_float4(p[0], p[1], p[2], p[3]);
+}
+__device__ __forceinline__ float exp2_f(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void store_row(const AttnArgs& a, int64_t row, int head, int d, float4 v) {
+    float* p = a.out + row * a.out_s1 + (int64_t)head * a.dim + d;
+    if (a.out_vec) {
+        *(float4*)p = v;
+    } else {
+        p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
+    }
+}
+// Two e4m3 bytes (the low ones of x) as two f16, exactly.
+__device__ __forceinline__ uint32_t f16_of_e4m3(uint32_t x) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)x));
+    return r;
+}
+// a and b as f16 pairs (a low): high = the nearest f16, low = the nearest f16 of what is left, 22 bits together.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& high, uint32_t& low) {
+    asm("{\n\t.reg .b16 x, y;\n\t.reg .f32 u, v;\n\t"
+        "cvt.rn.f16x2.f32 %0, %3, %2;\n\t"
+        "mov.b32 {x, y}, %0;\n\t"
+        "cvt.f32.f16 u, x;\n\t"
+        "cvt.f32.f16 v, y;\n\t"
+        "sub.f32 u, %2, u;\n\t"
+        "sub.f32 v, %3, v;\n\t"
+        "cvt.rn.f16x2.f32 %1, v, u;\n\t}"
+        : "=&r"(high), "=r"(low)
+        : "f"(a), "f"(b));
+}
+// The power of two that takes a query row of largest magnitude `top` (its bits) to 2^13 .. 2^14, where both halves of a
+// value have their bits; 1 for a row of zeros or with a NaN or infinity.
+__device__ __forceinline__ float query_unit(uint32_t top) {
+    const int e = (int)(top >> 23);
+    return e == 0 || e == 255 ? 1.0f : __uint_as_float((uint32_t)min(254, 127 + 127 + 13 - e) << 23);
+}
+// The least power of two above v (v finite, positive, below 2^126).
+__device__ __forceinline__ float unit_above(float v) { return __uint_as_float((__float_as_uint(v) & 0x7F800000u) + 0x00800000u); }
+
+// Where a piece of 16 bytes of a staged row of keys or values lies within its row, so that the lanes that read
+// together find other banks.
+template <int DP>
+__device__ __forceinline__ int key_chunk(int ch, int row) {
+    return DP == 128 ? ch ^ 4 * (row & 1) : ch;
+}
+template <int DP>
+__device__ __forceinline__ int value_chunk(int ch, int row) {
+    return DP == 128 ? ch ^ (row & 6) : ch ^ (row >> 1 & 3);
+}
+
+// One item: up to MAX rows (new token, query head of the group) of a sequence and kv head, and this block's part of the
+// tokens that they see.  Row r of the item is row first_row + r of the sequence's rows, of token (first_row + r) / group.
+struct Item {
+    int seq, head, rows, first_row;
+    int row0;             // the sequence's first row of q and out
+    int pos;              // position of the sequence's first new token (negative where it is not in the cache)
+    int low, high, base;  // tokens that any row sees; base = low rounded down to whole groups of 16
+    int top_first;        // the first token that all rows see
+    int units, from, to;  // units of 128 tokens from base, and this block's
+};
+
+// Tokens that the rows [first_row, first_row + rows) of a sequence see together.
+struct Seq {
+    int row0, n, take, length;  // take: rows of q that are taken (at most max_new)
+    __device__ Seq(const AttnArgs& a, int s) {
+        row0 = min(max(a.start[s], 0), a.rows);
+        const int end = min(max(a.start[s + 1], row0), a.rows);
+        n = end - row0;
+        take = min(n, a.max_new);
+        length = min(max(a.length[s], 0), a.longest);
+        const int64_t rows = (int64_t)take * a.group;
+        if (rows < a.least || rows > a.most) take = 0;
+    }
+};
+__device__ __forceinline__ int first_seen(const AttnArgs& a, int pos) { return a.window && pos >= a.window ? pos - a.window + 1 : 0; }
+
+template <int MAX>
+__device__ __forceinline__ int64_t tiles_of(const AttnArgs& a, const Seq& q) {
+    return ((int64_t)q.take * a.group + MAX - 1) / MAX;
+}
+// Tokens and units of tile t of a sequence: at least one unit, so that rows that see nothing are written.
+template <int MAX>
+__device__ __forceinline__ int span_of(const AttnArgs& a, const Seq& q, int64_t t, int& low, int& high) {
+    const int tok0 = (int)(t * MAX / a.group), tok1 = (int)(min(t * MAX + MAX, (int64_t)q.take * a.group) - 1) / a.group;
+    const int p0 = q.length - q.n + tok0, p1 = q.length - q.n + tok1;
+    low = first_seen(a, p0), high = p1 + 1;
+    if (high <= low) low = high = 0;
+    return max(1, (high - (low & ~15) + kUnitTokens - 1) / kUnitTokens);
+}
+
+// A slot of a block's part of an item: 8 ints (1 if it begins an item that ends elsewhere, the item's head, rows, first row,
+// row0, last block), then maximum and sum of each row, then its rows of output.
+__host__ __device__ constexpr int64_t part_floats(int max, int dp) { return 8 + 2 * max + (int64_t)max * dp; }
+__device__ __forceinline__ float* part_slot(const AttnArgs& a, int max, int dp, int64_t block, int which) {
+    return a.parts + (2 * block + which) * part_floats(max, dp);
+}
+
+// A block's share of all units, in the order sequence, kv head, tile, tokens: equal shares, so that ragged lengths load
+// the GPU evenly whatever the lengths are, which only the device knows.  An item that a share's end cuts is joined from its
+// parts afterwards.  THREADS threads of the block call every member together.
+template <int MAX, int DP, int THREADS>
+struct Share {
+    static constexpr int SEQS = 1024;  // sequences looked at together
+    static constexpr int SMEM = SEQS * 8 + 32 * 8 + 32;
+    int64_t total, at, left, blocks, tile;
+    int seq, head, off;
+
+    // Units of one kv head of sequence s.  MAX = 16: one tile, each thread another sequence; else a warp's lanes share the tiles.
+    __device__ static int64_t seq_units(const AttnArgs& a, int s, bool by_warp) {
+        const Seq q(a, s);
+        const int64_t n = tiles_of<MAX>(a, q);
+        int64_t u = 0;
+        int lo, hi;
+        for (int64_t t = by_warp ? threadIdx.x & 31 : 0; t < n; t += by_warp ? 32 : 1) u += span_of<MAX>(a, q, t, lo, hi);
+        if (by_warp)
+#pragma unroll
+            for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+        return u;
+    }
+    // Fills sh[0 .. SEQS) with the units of sequences from `first`; returns this thread's sum of its run of them, its
+    // exclusive prefix and the sum of all.
+    __device__ void chunk(const AttnArgs& a, int first, int64_t* sh, int64_t& mine, int64_t& before, int64_t& all) const {
+        constexpr int RUN = SEQS / THREADS;
+        int64_t* warps = sh + SEQS;
+        const int n = min(SEQS, a.seqs - first), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        __syncthreads();
+        if (MAX <= 16) {
+            for (int i = threadIdx.x; i < n; i += THREADS) sh[i] = seq_units(a, first + i, false) * a.heads;
+        } else {
+            for (int i = warp; i < n; i += THREADS / 32) {
+                const int64_t u = seq_units(a, first + i, true);
+                if (lane == 0) sh[i] = u * a.heads;
+            }
+        }
+        __syncthreads();
+        mine = 0;
+#pragma unroll
+        for (int i = 0; i < RUN; ++i)
+            if (threadIdx.x * RUN + i < n) mine += sh[threadIdx.x * RUN + i];
+        int64_t inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
+        }
+        if (lane == 31) warps[warp] = inc;
+        __syncthreads();
+        before = inc - mine, all = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) before += warps[w];
+            all += warps[w];
+        }
+    }
+    // Finds the block's first item; false when the block has no work.  sh: SMEM bytes of shared memory.
+    __device__ bool find(const AttnArgs& a, int64_t* sh) {
+        constexpr int RUN = SEQS / THREADS;
+        int64_t* found = sh + SEQS + 32;
+        int64_t mine = 0, before = 0, all = 0;
+        if (threadIdx.x == 0) *(int*)slot(a, 0) = *(int*)slot(a, 1) = 0;
+        total = 0;
+        for (int s = 0; s < a.seqs; s += SEQS) {
+            chunk(a, s, sh, mine, before, all);
+            total += all;
+        }
+        blocks = min((int64_t)gridDim.x, total);  // each has a unit at least, so that an item's parts lie in consecutive blocks
+        if (blockIdx.x >= blocks) return false;
+        at = total * blockIdx.x / blocks;
+        left = total * (blockIdx.x + 1) / blocks - at;
+        int64_t run = 0;
+        for (int s = 0; s < a.seqs; s += SEQS) {
+            if (a.seqs > SEQS) chunk(a, s, sh, mine, before, all);
+            if (at >= run + before && at < run + before + mine) {
+                int64_t x = at - run - before;
+                int i = threadIdx.x * RUN;
+                for (; x >= sh[i]; ++i) x -= sh[i];
+                found[0] = s + i, found[1] = x, found[2] = sh[i] / a.heads;
+            }
+            run += all;
+            if (at < run) break;
+        }
+        __syncthreads();
+        seq = (int)found[0];
+        const int64_t x = found[1], per = found[2];
+        head = (int)(x / per);
+        int64_t rest = x - head * per;
+        tile = 0;
+        if (MAX > 16) {  // (each warp for itself)
+            const Seq q(a, seq);
+            const int64_t n = tiles_of<MAX>(a, q);
+            const int lane = threadIdx.x & 31;
+            for (;; tile += 32) {
+                int lo, hi;
+                const int64_t u = tile + lane < n ? span_of<MAX>(a, q, tile + lane, lo, hi) : 0;
+                int64_t inc = u;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += t;
+                }
+                const uint32_t past = __ballot_sync(0xffffffffu, inc > rest);
+                if (past) {
+                    const int i = __ffs((int)past) - 1;
+                    tile += i;
+                    rest -= __shfl_sync(0xffffffffu, inc - u, i);
+                    break;
+                }
+                rest -= __shfl_sync(0xffffffffu, inc, 31);
+                if (tile + 32 >= n) break;  // (not reached: the sequence's units hold the unit looked for)
+            }
+        }
+        off = (int)rest;
+        __syncthreads();
+        return true;
+    }
+    __device__ bool more() const { return left > 0; }
+    __device__ Item item(const AttnArgs& a) const {
+        const Seq q(a, seq);
+        Item it;
+        it.seq = seq, it.head = head, it.row0 = q.row0;
+        it.first_row = (int)(tile * MAX);
+        it.rows = (int)min((int64_t)MAX, (int64_t)q.take * a.group - it.first_row);
+        it.pos = q.length - q.n;
+        it.units = span_of<MAX>(a, q, tile, it.low, it.high);
+        it.base = it.low & ~15;
+        it.top_first = first_seen(a, it.pos + (it.first_row + it.rows - 1) / a.group);
+        it.from = off;
+        it.to = (int)min((int64_t)it.units, off + left);
+        return it;
+    }
+    __device__ void advance(const AttnArgs& a, const Item& it) {
+        at += it.to - it.from, left -= it.to - it.from, off = 0;
+        if (left <= 0) return;
+        if (MAX > 16) {
+            ++tile;
+            if (tile < tiles_of<MAX>(a, Seq(a, seq))) return;
+        }
+        tile = 0;
+        if (++head < a.heads) return;
+        head = 0;
+        while (++seq < a.seqs)
+            if (Seq(a, seq).take) return;
+        left = 0;  // (not reached: the shares add up to all units)
+    }
+    // The block that holds the last unit of the item that begins at unit `at`.
+    __device__ int last_block(const Item& it) const {
+        const int64_t end = at - it.from + it.units;
+        return (int)((end * blocks + total - 1) / total) - 1;
+    }
+    __device__ static float* slot(const AttnArgs& a, int which) { return part_slot(a, MAX, DP, blockIdx.x, which); }
+};
+
+// Four values of an item's row from column d on, normed by the sum `total` of 2^(logit - top): to out, with the row's lse, where
+// the block has the whole item, else to the block's slot.
+template <int MAX, int DP, int THREADS>
+__device__ __forceinline__ void put_out(const AttnArgs& a, const Share<MAX, DP, THREADS>& sh, const Item& it, int row, int d, float4 v,
+                                        float top, float total) {
+    if (it.from == 0 && it.to == it.units) {
+        const int r = it.first_row + row, token = r / a.group, head = it.head * a.group + r % a.group;
+        store_row(a, it.row0 + token, head, d, v);
+        if (d == 0 && a.lse) a.lse[(int64_t)(it.row0 + token) * a.heads * a.group + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+        return;
+    }
+    float* p = sh.slot(a, it.from == 0);
+    if (d == 0) {
+        p[8 + 2 * row] = top, p[9 + 2 * row] = total;
+        if (row == 0 && it.from == 0) {
+            int* m = (int*)p;
+            m[1] = it.head, m[2] = it.rows, m[3] = it.first_row, m[4] = it.row0, m[5] = sh.last_block(it), m[0] = 1;
+        }
+    }
+    *(float4*)(p + 8 + 2 * MAX + row * DP + d) = v;
+}
+
+// Items whose units several blocks had: blockIdx.x is the block that began it, a warp takes a row.  The parts' weights are
+// their sums times 2^(top - the highest top); parts are added in the blocks' order.
+template <int MAX, int DP>
+__global__ void __launch_bounds__(128) attention_join(AttnArgs a) {
+    pdl_begin();
+    const int* m = (const int*)part_slot(a, MAX, DP, blockIdx.x, 1);
+    if (!m[0]) return;
+    const int row = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= m[2]) return;
+    const int parts = m[5] - (int)blockIdx.x + 1, r = m[3] + row, head = m[1] * a.group + r % a.group;
+    const int64_t to = m[4] + r / a.group;
+    float top = kNone, total = 0.0f;
+    for (int p = lane; p < parts; p += 32) top = fmaxf(top, part_slot(a, MAX, DP, blockIdx.x + p, p == 0)[8 + 2 * row]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p0 = 0; p0 < parts; p0 += 32) {
+        float w = 0.0f;
+        if (p0 + lane < parts) {
+            const float* p = part_slot(a, MAX, DP, blockIdx.x + p0 + lane, p0 + lane == 0) + 8 + 2 * row;
+            w = p[1] * exp2_f(p[0] - top);
+        }
+        const int n = min(32, parts - p0);
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float k = __shfl_sync(0xffffffffu, w, i);
+            total += k;
+            if (4 * lane < DP) {
+                const float4 t = *(const float4*)(part_slot(a, MAX, DP, blockIdx.x + p0 + i, p0 + i == 0) + 8 + 2 * MAX + row * DP + 4 * lane);
+                v.x = fmaf(k, t.x, v.x), v.y = fmaf(k, t.y, v.y), v.z = fmaf(k, t.z, v.z), v.w = fmaf(k, t.w, v.w);
+            }
+        }
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    if (4 * lane < a.dim) store_row(a, to, head, 4 * lane, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    if (lane == 0 && a.lse) a.lse[to * a.heads * a.group + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+}
+
+}  // namespace
+#endif
