@@ -2,6 +2,7 @@
 #include <cuda_runtime.h>
 #include <cstdint>
 #include "mcu_attention.cuh"
+#include "mcu_attention_tiles.cuh"
 
 using namespace mcu;
 
@@ -23,7 +24,6 @@ namespace {
 constexpr int kFewWarps = 8, kFewStages = 4;
 constexpr int kGroup = 16;               // tokens of a warp's step; pages hold a multiple
 constexpr int kFlush = 16;               // groups between two flushes: the tensor core's sums lose up to a step each
-constexpr float kTop = 15.0f;            // probabilities are formed as 2^kTop p: their f16 halves keep 22 bits down to 2^-18
 
 template <int DP>
 struct FewCfg {
@@ -129,9 +129,9 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
         float o[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        float m[NR], mrf[NR], l[NR], fade[NR];
+        float m[NR], l[NR], fade[NR];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, mrf[r] = kNone, l[r] = 0.0f, fade[r] = 1.0f;
+        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f, fade[r] = 1.0f;
         float unit = kLeastUnit, per_unit = 1.0f / kLeastUnit;
 #pragma unroll
         for (int e = 0; e < S::VALS / 4; ++e) sums[e * 32 + lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -266,9 +266,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
                     float f = 1.0f;
                     if (x > m[r]) {
-                        const float next = fmaf(x, rf[r], -kTop);
-                        f = exp2_f(mrf[r] - next);
-                        m[r] = x, mrf[r] = next;
+                        f = m[r] == -INFINITY ? 0.0f : exp2_f((m[r] - x) * rf[r]);
+                        m[r] = x;
                         l[r] *= f;
                     }
                     f *= shrink;
@@ -287,7 +286,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
                 float w[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    float p = exp2_f(fmaf(t[r][k], rf[r], -mrf[r]));
+                    float p = exp2_f(fmaf(t[r][k] - m[r], rf[r], kTop));
                     if (!seen[r][k]) p = 0.0f;
                     l[r] += p;
                     w[k] = seen[r][k] ? p * (vs[k] * per_unit) : 0.0f;
@@ -337,7 +336,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
         for (int r = 0; r < NR; ++r) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (c == 0) stats[warp * 16 + g + 8 * r] = make_float2(mrf[r], l[r]);
+            if (c == 0) stats[warp * 16 + g + 8 * r] = make_float2(top_of(m[r], rf[r]), l[r]);
         }
         if (lane == 0) units[warp] = unit;
         __syncthreads();
@@ -376,85 +375,40 @@ int run_few(const AttnArgs& a, cudaStream_t st) {
     constexpr int bytes = FewSmem<DP, STACK>::BYTES;
     const cudaError_t e = allow_smem(attention_few<DP, STACK>, bytes, done);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_dep(attention_few<DP, STACK>, dim3((unsigned)a.blocks), dim3(32 * kFewWarps), bytes, st, a);
+    const int rc = (int)launch_dep(attention_few<DP, STACK>, dim3((unsigned)a.blocks), dim3(32 * kFewWarps), bytes, st, a);
+    if (rc) return rc;
+    return (int)launch_dep(attention_join<16, DP>, dim3((unsigned)a.blocks, 4), dim3(128), 0, st, a);
 }
-
-__device__ __forceinline__ float4 e4m3_values(uint32_t b) {
-    uint32_t lo, hi;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)b));
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(b >> 16)));
-    float4 r;
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(lo));
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(r.z), "=f"(r.w) : "r"(hi));
-    return r;
-}
-
-// A warp takes one head of one row and goes through its keys with the running maximum and sum.
-__global__ void __launch_bounds__(128) attention_rows(mcu_attention a) {
-    pdl_begin();
-    const int lane = threadIdx.x & 31;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), row = item / a.q_heads;
-    const int head = (int)(item - row * a.q_heads), dim = a.cache.head_dim, page = a.cache.page_size;
-    if (row >= a.rows) return;
-    int64_t seq = 0, s0 = 0, s1 = 0;
-    for (; seq < a.seqs; ++seq) {
-        s0 = min(max((int64_t)a.start[seq], (int64_t)0), a.rows);
-        s1 = min(max((int64_t)a.start[seq + 1], s0), a.rows);
-        if (row >= s0 && row < s1) break;
-    }
-    if (seq == a.seqs || row - s0 >= a.max_new) return;
-    const int64_t length = min(max((int64_t)a.length[seq], (int64_t)0), a.table_s1 * page);
-    const int64_t pos = length - (s1 - s0) + (row - s0), lo = a.window ? max(pos - a.window + 1, (int64_t)0) : 0;
-    const int kv = head / (int)(a.q_heads / a.cache.heads);
-    float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o = q;
-    if (4 * lane < dim) {
-        const float* p = a.q + row * a.q_s1 + (int64_t)head * dim + 4 * lane;
-        q = make_float4(p[0], p[1], p[2], p[3]);
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int64_t j = lo; j <= pos; ++j) {
-        const int pg = a.table[seq * a.table_s1 + j / page];
-        if ((uint32_t)pg >= (uint32_t)a.cache.pages) continue;
-        const int64_t at = ((int64_t)pg * a.cache.heads + kv) * page + j % page;
-        float4 k = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = k;
-        if (4 * lane < dim) {
-            k = e4m3_values(*(const uint32_t*)(a.cache.k + at * dim + 4 * lane));
-            v = e4m3_values(*(const uint32_t*)(a.cache.v + at * dim + 4 * lane));
-        }
-        const float vs = a.cache.v_scale[at];
-        const float x = warp_sum_f(fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)))) * a.cache.k_scale[at] * a.scale;
-        const float mn = fmaxf(m, x), f = m == mn ? 1.0f : expf(m - mn), p = x == -INFINITY ? 0.0f : expf(x - mn);
-        l = fmaf(l, f, p);
-        o.x = fmaf(o.x, f, p * (v.x * vs)), o.y = fmaf(o.y, f, p * (v.y * vs));
-        o.z = fmaf(o.z, f, p * (v.z * vs)), o.w = fmaf(o.w, f, p * (v.w * vs));
-        m = mn;
-    }
-    const float r = l == 0.0f ? 0.0f : 1.0f / l;
-    if (4 * lane < dim) {
-        float* p = a.out + row * a.out_s1 + (int64_t)head * dim + 4 * lane;
-        p[0] = o.x * r, p[1] = o.y * r, p[2] = o.z * r, p[3] = o.w * r;
-    }
-    if (a.lse && lane == 0) a.lse[row * a.q_heads + head] = l == 0.0f ? -INFINITY : m + logf(l);
-}
-
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int kSms = 148;
 constexpr int kFewRows = 16;
 int padded(const mcu_attention* a) { return a->cache.head_dim <= 64 ? 64 : 128; }
 
+// The kernels of a call.  Sequences of up to `few` rows of a kv head go to attention_few; the host knows an upper bound of
+// new tokens only, so above it the other kernel takes what is longer, and both are launched unless every sequence may have
+// the bound (a full rectangle of rows).
+struct Forms {
+    int few;
+    bool tiles;
+};
+Forms forms_of(const mcu_attention* a) {
+    const int64_t group = a->q_heads / a->cache.heads, most = a->max_new * group;
+    if (most <= kFewRows) return Forms{most <= 8 ? 8 : kFewRows, false};
+    if (a->rows == a->seqs * a->max_new) return Forms{0, true};
+    return Forms{group <= 8 ? 8 : group <= kFewRows ? kFewRows : 0, true};
+}
+
 }  // namespace
 
 extern "C" size_t mcu_attention_scratch_bytes(const mcu_attention* a) {
-    return (size_t)(2 * kSms * part_floats(kFewRows, padded(a))) * 4;
+    const Forms f = forms_of(a);
+    return (size_t)(2 * kSms * ((f.few ? part_floats(kFewRows, padded(a)) : 0) + (f.tiles ? part_floats(kTileRows, padded(a)) : 0))) * 4;
 }
 
 extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, int* status, cudaStream_t st, int* launches) {
     const int group = (int)(c->q_heads / c->cache.heads);
-    if (c->max_new * group > kFewRows) {
-        *launches = 1;
-        return (int)launch_dep(attention_rows, dim3((unsigned)((c->rows * c->q_heads + 3) / 4)), dim3(128), 0, st, *c);
-    }
+    const Forms f = forms_of(c);
     AttnArgs a = {};
     a.out = c->out, a.lse = c->lse, a.q = c->q, a.k = c->cache.k, a.v = c->cache.v, a.ks = c->cache.k_scale, a.vs = c->cache.v_scale;
     a.table = c->table, a.start = c->start, a.length = c->length, a.table_s1 = c->table_s1, a.q_s1 = c->q_s1, a.out_s1 = c->out_s1;
@@ -463,12 +417,22 @@ extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, int* 
     while ((1 << a.page_log) < c->cache.page_size) ++a.page_log;
     a.window = c->window >= ((int64_t)1 << 31) - 1 ? 0 : (int)c->window;
     a.longest = (int)(c->table_s1 * c->cache.page_size);
-    a.least = 1, a.most = kFewRows, a.blocks = kSms, a.scale = c->scale;
+    a.blocks = kSms, a.scale = c->scale, a.stall = test_stall();
     a.q_vec = aligned16(c->q) && !(c->q_s1 & 3), a.out_vec = aligned16(c->out) && !(c->out_s1 & 3);
-    const bool stack = c->max_new * group <= 8, wide = a.dim > 64;
-    int rc = wide ? stack ? run_few<128, true>(a, st) : run_few<128, false>(a, st) : stack ? run_few<64, true>(a, st) : run_few<64, false>(a, st);
-    if (rc) return rc;
-    *launches = 2;
-    const dim3 grid(a.blocks, kFewRows / 4);
-    return (int)(wide ? launch_dep(attention_join<16, 128>, grid, dim3(128), 0, st, a) : launch_dep(attention_join<16, 64>, grid, dim3(128), 0, st, a));
+    const bool wide = a.dim > 64;
+    int rc = 0;
+    *launches = 0;
+    if (f.tiles) {
+        a.least = f.few + 1, a.most = 0x7fffffff;
+        rc = wide ? run_tiles<128>(a, st) : run_tiles<64>(a, st);
+        *launches += 2;
+        a.parts += 2 * kSms * part_floats(kTileRows, padded(c));
+    }
+    if (!rc && f.few) {
+        a.least = 1, a.most = f.few;
+        const bool stack = f.few <= 8;
+        rc = wide ? stack ? run_few<128, true>(a, st) : run_few<128, false>(a, st) : stack ? run_few<64, true>(a, st) : run_few<64, false>(a, st);
+        *launches += 2;
+    }
+    return rc;
 }

@@ -11,6 +11,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 constexpr float kNone = -3.0e38f;               // the maximum of no logits: finite, so that differences of it stay numbers
+constexpr float kTop = 15.0f;                   // probabilities are formed as 2^kTop p: their f16 halves keep 22 bits down to 2^-18
 constexpr float kLeastUnit = 0x1p-120f;         // unit of the values' scales before any was seen (the least scale is 2^-109)
 constexpr float kLargestScale = 0x1p126f;       // a scale that is no number or not finite does not set the unit
 constexpr int kUnitTokens = 128;                // tokens of a unit of work
@@ -59,6 +60,8 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int64_t row, int he
         p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
     }
 }
+// The logarithm (base 2) of the probabilities' unit where the highest logit is m, in units of rf; kNone for no logits.
+__device__ __forceinline__ float top_of(float m, float rf) { return m == -INFINITY ? kNone : fmaf(m, rf, -kTop); }
 // Two e4m3 bytes (the low ones of x) as two f16, exactly.
 __device__ __forceinline__ uint32_t f16_of_e4m3(uint32_t x) {
     uint32_t r;
