@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float raw = STACK ? s[k >> 1][k & 1] + s[k >> 1][2 + (k & 1)] : s[k >> 1][2 * r + (k & 1)];
-                    t[r][k] = raw * ks[k];
+                    t[r][k] = __fmul_rn(raw, ks[k]);
                     seen[r][k] = true;
                 }
             if (edge) {

@@ -14,26 +14,44 @@ using namespace mcu;
 //   S = Qh K^T + Ql K^T,   O = Ph V + Pl V,
 // Q and P as two f16 (22 bits), K and V exact in f16.  Both left operands lie in TMEM, where a product's rate does not hang on
 // two operands' shared-memory reads: 2 x 128 columns of S, over which P is written in place, 128 of O, 128 of Q.  O starts
-// from zero for every 128 tokens and is added in registers in f32 (rounded to nearest), times the step of the running maximum and
+// from zero for every 128 tokens and is added in registers in f32 (rounded to nearest), times the step of the row's reference and
 // the unit of the tile's value scales: no accumulator is ever rescaled, and the tensor core's truncating sums stay short.
 //   warps 0-7    softmax: warp w has the rows 32 (w & 3) .. and half w / 4 of the tokens and of the output's columns
 //   warps 8-11   loaders: e4m3 from the pages through registers to f16 tiles (128-byte swizzle), scales, valid tokens
 //   warp 12      issues the products: S of tile j + 1 before O of tile j, so that softmax runs under them
+//   warp 13      plans: puts the block's items into a ring, so that the others find theirs without global loads
+// Probabilities are 2^kTileTop relative to a reference that need not be the row's maximum: their f16 halves leave room for 7
+// powers of two above it.  A tile is formed with the reference as it is; where the sum of a thread's 64 probabilities is
+// below 2^16 (it bounds each of them) that stands, else the pair of warps that share the rows finds the maximum, moves the reference
+// there and forms the tile again.  After a row's first tile that is rare, and a separate pass for the maximum is saved.
 constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 512;
-constexpr int kTileLaunch = 128, kSoftRegs = 176, kLoadRegs = 112, kIssueRegs = 48;
+constexpr int kTileLaunch = 128, kSoftRegs = 184, kLoadRegs = 96, kIssueRegs = 48;
 static_assert(2 * kSoftRegs + kLoadRegs + kIssueRegs == 4 * kTileLaunch, "register split must match the launch");
+constexpr float kTileTop = 9.0f;
+constexpr float kTileSum = 65000.0f;  // below the largest f16
+constexpr int kItems = 4;             // items in the planner's ring
+
+// What the roles need of an item, as the planner leaves it; rows = 0: no more.
+struct __align__(16) TileItem {
+    int rows, n, row0, first_row;        // n: tiles of 128 tokens
+    int pos, all_first, all_last, head;  // every row sees the tokens all_first .. all_last
+    int low, high, first, seq;           // first: the first token of the first tile
+    int whole, begins, last_block, pad;
+};
+static_assert(sizeof(TileItem) == 64, "four 16-byte pieces");
 
 template <int DP>
 struct TileCfg {
-    static constexpr int BLOCKS = DP / 64;                  // column blocks of 64 f16
+    static constexpr int BLOCKS = DP / 64;                   // column blocks of 64 f16
     static constexpr int TILE = BLOCKS * kTileTokens * 128;  // bytes of a K or V tile
     static constexpr int K = 0, V = 2 * TILE;
     static constexpr int SCALES = 4 * TILE;                  // 4 x {keys' scales, values' ratios, valid tokens, unit}
     static constexpr int SLOT = 2 * kTileTokens * 4 + 32;
-    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][2][128]
-    static constexpr int SUMS = MAXIMA + 2 * 2 * 128 * 4;    // [2][128]
+    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][128]
+    static constexpr int SUMS = MAXIMA + 2 * 128 * 4;        // [2][128]
     static constexpr int TOPS = SUMS + 2 * 128 * 4;          // [2][4] of the loaders
-    static constexpr int BARS = TOPS + 32;
+    static constexpr int ITEMS = TOPS + 32;
+    static constexpr int BARS = ITEMS + kItems * 64;
     static constexpr int SMEM = BARS + 256 + 1024;
     static constexpr uint32_t S_COL = 0, O_COL = 256, Q_COL = 384;
     static_assert(Share<kTileRows, DP, kTileThreads>::SMEM <= SCALES, "the search for work takes the tiles' room");
@@ -54,6 +72,19 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const 
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 __device__ __forceinline__ void bar_named(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+// A barrier that also says whether any of its threads came with true.
+__device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(id), "r"(threads), "r"((uint32_t)mine)
+        : "memory");
+    return any != 0;
+}
 
 // D (+)= A B with A (f16) in TMEM; one thread.
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -73,12 +104,6 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, uint32_t lead) {
            (uint64_t)2 << 61;
 }
 
-__device__ __forceinline__ void tmem_load32(uint32_t taddr, float (&v)[32]) {
-    uint32_t u[32];
-    tmem_ld32(taddr, u);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]),
@@ -88,10 +113,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
 }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ float4 lds128f(uint32_t a) {
-    const uint4 v = lds128(a);
-    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-}
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -102,9 +123,93 @@ __device__ __forceinline__ float lds32(uint32_t a) {
 }
 __device__ __forceinline__ void sts32(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
 
-// 128 tokens of an item: how many of its units hold any.
-__device__ __forceinline__ int item_tiles(const Item& it) {
-    return max(0, min(it.to, (it.high - it.base + kTileTokens - 1) / kTileTokens) - it.from);
+// Pairs of f32 in one instruction, each rounded as alone.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_of(uint32_t a, uint32_t b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// (not volatile: scales are read after the barrier that the tile's start waits for, and may be read early within the tile)
+__device__ __forceinline__ void lds_pairs(uint32_t a, uint64_t& x, uint64_t& y) {
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "r"(a));
+}
+// As split2, for a pair.
+__device__ __forceinline__ void split_pair(uint64_t w, uint32_t& high, uint32_t& low) {
+    asm("{\n\t.reg .b16 x, y;\n\t.reg .f32 a, b, u, v;\n\t.reg .b64 h, d;\n\t"
+        "mov.b64 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.f32 %0, b, a;\n\t"
+        "mov.b32 {x, y}, %0;\n\t"
+        "cvt.f32.f16 u, x;\n\t"
+        "cvt.f32.f16 v, y;\n\t"
+        "sub.f32 u, a, u;\n\t"
+        "sub.f32 v, b, v;\n\t"
+        "cvt.rn.f16x2.f32 %1, v, u;\n\t}"
+        : "=&r"(high), "=r"(low)
+        : "l"(w));
+}
+
+// 32 columns of S at taddr to probabilities times their values' ratios, as f16 halves; *sum gains the probabilities.
+// CARE: tokens whose bit in `seen` is not set have none, and a logit is rounded before the reference is taken from it, so
+// that the two are equal where they should be (unrounded they differ by up to 2^-24 of the logit: of no account while that is
+// small).
+template <bool CARE>
+__device__ __forceinline__ void tile_chunk(uint32_t taddr, uint32_t ks, uint32_t vs, uint64_t minus_m, uint64_t rf, uint32_t seen,
+                                           uint32_t* high, uint32_t* low, uint64_t* sum) {
+    const uint64_t top = pair_of(kTileTop, kTileTop);
+    uint32_t v[32];
+    tmem_ld32(taddr, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        uint64_t kk[2], vv[2];
+        lds_pairs(ks + 16 * k, kk[0], kk[1]);
+        lds_pairs(vs + 16 * k, vv[0], vv[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = 4 * k + 2 * h;
+            float x, y;
+            uint64_t t;
+            if (CARE) {  // (one by one: packed, the compiler joins the two roundings)
+                float k0, k1, m0, m1;
+                unpair(kk[h], k0, k1);
+                unpair(minus_m, m0, m1);
+                t = pair_of(__fadd_rn(__fmul_rn(__uint_as_float(v[e]), k0), m0), __fadd_rn(__fmul_rn(__uint_as_float(v[e + 1]), k1), m1));
+            } else {
+                t = fma2(pair_of(v[e], v[e + 1]), kk[h], minus_m);
+            }
+            unpair(fma2(t, rf, top), x, y);
+            x = exp2_f(x), y = exp2_f(y);
+            if (CARE) x = seen >> e & 1 ? x : 0.0f, y = seen >> (e + 1) & 1 ? y : 0.0f;
+            const uint64_t p = pair_of(x, y);
+            *sum = add2(*sum, p);
+            uint64_t w = mul2(p, vv[h]);
+            if (CARE) {
+                unpair(w, x, y);
+                w = pair_of(seen >> e & 1 ? x : 0.0f, seen >> (e + 1) & 1 ? y : 0.0f);
+            }
+            split_pair(w, high[2 * k + h], low[2 * k + h]);
+        }
+    }
 }
 
 template <int DP>
@@ -123,7 +228,9 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     uint64_t* o_free = o_full + 1;
     uint64_t* q_full = o_free + 1;
     uint64_t* drain = q_full + 1;
-    uint32_t* tmem_slot = (uint32_t*)(drain + 1);
+    uint64_t* i_full = drain + 1;  // kItems each
+    uint64_t* i_free = i_full + kItems;
+    uint32_t* tmem_slot = (uint32_t*)(i_free + kItems);
     volatile int* gave_up = (volatile int*)(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const Abort ab{gave_up, a.status};
@@ -137,6 +244,10 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             mbar_init(&p_full[i], 256);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&sc_full[i], 128);
+        for (int i = 0; i < kItems; ++i) {
+            mbar_init(&i_full[i], 1);
+            mbar_init(&i_free[i], 13);  // a lane of each softmax and loader warp and of the issuer
+        }
         mbar_init(o_full, 1);
         mbar_init(o_free, 256);
         mbar_init(q_full, 256);
@@ -158,6 +269,25 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     const bool work = sh.find(a, (int64_t*)smem);
     __syncthreads();
 
+    // Item i of the block's, once the planner has it there.  The warps that meet at named barriers (id, threads; 0: none) end
+    // together: a barrier tells whether any of them saw that a wait was given up.
+    const uint32_t ring = smem_u32(smem + C::ITEMS);
+    auto item = [&](uint32_t i, int id, int threads) {
+        warp_wait(&i_full[i & (kItems - 1)], i / kItems & 1, ab, 41);
+        TileItem it;
+        int* w = (int*)&it;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint4 v = lds128(ring + (i & (kItems - 1)) * 64 + 16 * k);
+            w[4 * k] = (int)v.x, w[4 * k + 1] = (int)v.y, w[4 * k + 2] = (int)v.z, w[4 * k + 3] = (int)v.w;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&i_free[i & (kItems - 1)]);
+        const bool over = *gave_up != 0;
+        if (threads ? bar_any(id, threads, over) : __any_sync(0xffffffffu, over)) it.rows = 0;
+        return it;
+    };
+
     if (!work) {
         // nothing to do but to free TMEM
     } else if (warp < 8) {  // ---- softmax
@@ -165,160 +295,197 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         constexpr int HD = DP / 2;  // this thread's columns of the output and values of a query
         const int half = warp >> 2, row = 32 * (warp & 3) + lane, pair = 1 + (warp & 3);
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t scales = smem_u32(smem + C::SCALES), maxima = smem_u32(smem + C::MAXIMA), sums = smem_u32(smem + C::SUMS);
-        uint32_t t = 0;  // tiles done
-        while (sh.more()) {
-            const Item it = sh.item(a);
-            const int n = item_tiles(it), r = it.first_row + row;
+        const uint32_t scales = smem_u32(smem + C::SCALES) + 64 * half * 4, maxima = smem_u32(smem + C::MAXIMA), sums = smem_u32(smem + C::SUMS);
+        // The query's half row of an item, in TMEM as two f16 (the products that read the last item's are done: their S was
+        // waited for); returns the factor that takes S to log2 units.
+        auto query = [&](const TileItem& it) {
+            const int r = it.first_row + row;
             const bool live = row < it.rows;
-            float rf = 0.0f;
-            if (n) {  // the query's half row, in TMEM as two f16 (products that read the last item's are done: their S was waited for)
-                const float* p = a.q + (int64_t)(it.row0 + (live ? r / a.group : 0)) * a.q_s1 +
-                                 (int64_t)(it.head * a.group + (live ? r % a.group : 0)) * a.dim + HD * half;
-                float x[HD];
-                uint32_t top = 0;
+            const float* p = a.q + (int64_t)(it.row0 + (live ? r / a.group : 0)) * a.q_s1 +
+                             (int64_t)(it.head * a.group + (live ? r % a.group : 0)) * a.dim + HD * half;
+            float x[HD];
+            uint32_t top = 0;
+            if (a.q_vec) {
 #pragma unroll
                 for (int i = 0; i < HD / 4; ++i) {
-                    const float4 v = live && HD * half + 4 * i < a.dim ? load4(p + 4 * i, a.q_vec) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    const float4 v = live && HD * half + 4 * i < a.dim ? *(const float4*)(p + 4 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
                 }
+            } else {
 #pragma unroll
-                for (int i = 0; i < HD; ++i) top = max(top, abs_bits(x[i]));
-                sts32(sums + (half * 128 + row) * 4, __uint_as_float(top));
-                bar_named(pair, 64);
-                top = max(top, __float_as_uint(lds32(sums + ((half ^ 1) * 128 + row) * 4)));
-                const float up = query_unit(top);
-                rf = a.scale * kLog2e / up;
-#pragma unroll
-                for (int i = 0; i < HD / 32; ++i) {
-                    uint32_t h[16], l[16];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) split2(x[32 * i + 2 * k] * up, x[32 * i + 2 * k + 1] * up, h[k], l[k]);
-                    tmem_st16(tmem + lanes + C::Q_COL + HD / 2 * half + 16 * i, h);
-                    tmem_st16(tmem + lanes + C::Q_COL + DP / 2 + HD / 2 * half + 16 * i, l);
-                }
-                tmem_st_done();
-                tc_fence_before();
-                mbar_arrive(q_full);
+                for (int i = 0; i < HD; ++i) x[i] = live && HD * half + i < a.dim ? p[i] : 0.0f;
             }
-            const int last = live ? it.pos + r / a.group : -1, first = a.window && last >= a.window ? last - a.window + 1 : 0;
-            const int all_last = it.pos + it.first_row / a.group, all_first = it.top_first;
-            float o[HD];
 #pragma unroll
-            for (int i = 0; i < HD; ++i) o[i] = 0.0f;
+            for (int i = 0; i < HD; ++i) top = max(top, abs_bits(x[i]));
+            sts32(sums + (half * 128 + row) * 4, __uint_as_float(top));
+            bar_named(pair, 64);
+            top = max(top, __float_as_uint(lds32(sums + ((half ^ 1) * 128 + row) * 4)));
+            bar_named(pair, 64);
+            const float up = query_unit(top);
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+                uint32_t h[16], l[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) split2(x[32 * i + 2 * k] * up, x[32 * i + 2 * k + 1] * up, h[k], l[k]);
+                tmem_st16(tmem + lanes + C::Q_COL + HD / 2 * half + 16 * i, h);
+                tmem_st16(tmem + lanes + C::Q_COL + DP / 2 + HD / 2 * half + 16 * i, l);
+            }
+            tmem_st_done();
+            tc_fence_before();
+            mbar_arrive(q_full);
+            return a.scale * kLog2e / up;
+        };
+        uint32_t t = 0, i = 0;  // tiles done, items
+        TileItem it = item(0, pair, 64);
+        float rf = it.rows && it.n ? query(it) : 0.0f;
+        while (it.rows) {
+            const int r = it.first_row + row;
+            const bool live = row < it.rows;
+            const int last = live ? it.pos + r / a.group : -1, first = a.window && last >= a.window ? last - a.window + 1 : 0;
+            const uint64_t rf2 = pair_of(rf, rf);
+            uint64_t o[HD / 2];
+#pragma unroll
+            for (int k = 0; k < HD / 2; ++k) o[k] = 0;
             float m = -INFINITY, l = 0.0f, fade = 1.0f, unit = 0.0f;
+            bool wild = false;  // a row's logits are large for the unrounded form
             // O of tile x joins the sums: waits for it, and hands the columns back
             auto add = [&](uint32_t x) {
+                if (__any_sync(0xffffffffu, fade != 1.0f)) {
+                    const uint64_t f = pair_of(fade, fade);
+#pragma unroll
+                    for (int k = 0; k < HD / 2; ++k) o[k] = mul2(o[k], f);
+                }
+                const uint64_t u = pair_of(unit, unit);
                 warp_wait(o_full, x & 1, ab, 31);
                 tc_fence_after();
-                float v[32];
 #pragma unroll
-                for (int i = 0; i < HD / 32; ++i) {
-                    tmem_load32(tmem + lanes + C::O_COL + HD * half + 32 * i, v);
-                    if (i == HD / 32 - 1) {
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(tmem + lanes + C::O_COL + HD * half + 32 * c, v);
+                    if (c == HD / 32 - 1) {
                         tc_fence_before();
                         mbar_arrive(o_free);
                     }
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[32 * i + k] = fmaf(v[k], unit, o[32 * i + k] * fade);
+                    for (int k = 0; k < 16; ++k) o[16 * c + k] = fma2(pair_of(v[2 * k], v[2 * k + 1]), u, o[16 * c + k]);
                 }
             };
-            for (int j = 0; j < n; ++j, ++t) {
-                const uint32_t slot = scales + (t & 3) * C::SLOT;
-                const int j0 = it.base + kTileTokens * (it.from + j) + 64 * half;
+            for (int j = 0; j < it.n; ++j, ++t) {
+                const uint32_t slot = scales + (t & 3) * C::SLOT;  // (this half's scales)
                 warp_wait(&sc_full[t & 3], t >> 2 & 1, ab, 32);
+                const int j0 = it.first + kTileTokens * j;
+                const uint4 ok = lds128(slot - 64 * half * 4 + 2 * kTileTokens * 4);
+                const float next_unit = lds32(slot - 64 * half * 4 + 2 * kTileTokens * 4 + 16);
+                // not all tokens seen by all rows
+                const bool edge = j0 < it.all_first || j0 + kTileTokens - 1 > it.all_last || (ok.x & ok.y & ok.z & ok.w) != 0xffffffffu;
+                uint32_t seen0 = half ? ok.z : ok.x, seen1 = half ? ok.w : ok.y;
+                if (edge) {
+                    const int lo = first - j0 - 64 * half, hi = last - j0 - 64 * half;  // tokens lo .. hi of this half's
+                    const int a0 = max(lo, 0), b0 = min(hi, 31), a1 = max(lo - 32, 0), b1 = min(hi - 32, 31);
+                    seen0 &= a0 > b0 ? 0u : (0xffffffffu << a0) & (0xffffffffu >> (31 - b0));
+                    seen1 &= a1 > b1 ? 0u : (0xffffffffu << a1) & (0xffffffffu >> (31 - b1));
+                }
                 warp_wait(&s_full[t & 1], t >> 1 & 1, ab, 33);
                 tc_fence_after();
                 const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 64 * half;
-                float s[64];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float v[32];
-                    tmem_load32(sc + 32 * i, v);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float4 ks = lds128f(slot + (64 * half + 32 * i + 4 * k) * 4);
-                        s[32 * i + 4 * k] = v[4 * k] * ks.x, s[32 * i + 4 * k + 1] = v[4 * k + 1] * ks.y;
-                        s[32 * i + 4 * k + 2] = v[4 * k + 2] * ks.z, s[32 * i + 4 * k + 3] = v[4 * k + 3] * ks.w;
+                uint32_t h[32], lo[32];
+                float step = 1.0f, mine = 0.0f;
+                auto form = [&]() {
+                    const uint64_t mm = pair_of(-m, -m);
+                    uint64_t sum = 0;
+                    if (edge || wild) {
+                        tile_chunk<true>(sc, slot, slot + kTileTokens * 4, mm, rf2, seen0, h, lo, &sum);
+                        tile_chunk<true>(sc + 32, slot + 128, slot + kTileTokens * 4 + 128, mm, rf2, seen1, h + 16, lo + 16, &sum);
+                    } else {
+                        tile_chunk<false>(sc, slot, slot + kTileTokens * 4, mm, rf2, 0u, h, lo, &sum);
+                        tile_chunk<false>(sc + 32, slot + 128, slot + kTileTokens * 4 + 128, mm, rf2, 0u, h + 16, lo + 16, &sum);
                     }
-                }
-                // valid tokens of the tile, and whether every row sees them all
-                const uint4 ok = lds128(slot + 2 * kTileTokens * 4);
-                const int tile0 = j0 - 64 * half;
-                const bool edge = tile0 < all_first || tile0 + kTileTokens - 1 > all_last || (ok.x & ok.y & ok.z & ok.w) != 0xffffffffu;
-                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-                if (edge) {
+                    float x, y;
+                    unpair(sum, x, y);
+                    mine = x + y;
+                };
+                for (int again = 0;; ++again) {
+                    form();
+                    if (again || !bar_any(pair, 64, !(mine < kTileSum))) break;
+                    // the rows' maxima of the tile, of both halves
+                    float x = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(sc + 32 * c, v);
+                        const uint32_t seen = c ? seen1 : seen0;
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) {  // tokens first .. last of the 32 from j0 + 32 w
-                        const int lo = max(first - j0 - 32 * w, 0), hi = min(last - j0 - 32 * w, 31);
-                        const uint32_t range = lo > hi ? 0u : (0xffffffffu << lo) & (0xffffffffu >> (31 - hi));
-                        seen[w] = range & (half ? (w ? ok.w : ok.z) : (w ? ok.y : ok.x));
-                    }
-#pragma unroll
-                    for (int k = 0; k < 64; ++k)
-                        if (!(seen[k >> 5] >> (k & 31) & 1)) s[k] = -INFINITY;
-                }
-                float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
-#pragma unroll
-                for (int k = 0; k < 64; k += 4) x0 = fmaxf(x0, s[k]), x1 = fmaxf(x1, s[k + 1]), x2 = fmaxf(x2, s[k + 2]), x3 = fmaxf(x3, s[k + 3]);
-                float x = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
-                sts32(maxima + (((t & 1) * 2 + half) * 128 + row) * 4, x);
-                bar_named(pair, 64);
-                x = fmaxf(x, lds32(maxima + (((t & 1) * 2 + (half ^ 1)) * 128 + row) * 4));
-                float step = 1.0f;
-                if (x > m) {
-                    step = m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
-                    m = x;
-                    l *= step;
-                }
-                const float next_unit = lds32(slot + 2 * kTileTokens * 4 + 16);
-                float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t h[16], lo[16];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float4 vs = lds128f(slot + (kTileTokens + 64 * half + 32 * i + 4 * k) * 4);
-                        float p[4], w[4];
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            p[q] = exp2_f(fmaf(s[32 * i + 4 * k + q] - m, rf, kTop));
-                            if (edge && !(seen[i] >> (4 * k + q) & 1)) p[q] = 0.0f;
+                        for (int k = 0; k < 32; ++k) {
+                            const float y = __fmul_rn(__uint_as_float(v[k]), lds32(slot + 128 * c + 4 * k));
+                            if (seen >> k & 1) x = fmaxf(x, y);
                         }
-                        l0 += p[0] + p[1], l1 += p[2] + p[3];
-                        w[0] = p[0] * vs.x, w[1] = p[1] * vs.y, w[2] = p[2] * vs.z, w[3] = p[3] * vs.w;
-                        if (edge) {
-#pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                if (!(seen[i] >> (4 * k + q) & 1)) w[q] = 0.0f;
-                        }
-                        split2(w[0], w[1], h[2 * k], lo[2 * k]);
-                        split2(w[2], w[3], h[2 * k + 1], lo[2 * k + 1]);
                     }
-                    tmem_st16(sc + 32 * i, h);
-                    tmem_st16(sc + 32 * i + 16, lo);
+                    sts32(maxima + (half * 128 + row) * 4, x);
+                    bar_named(pair, 64);
+                    x = fmaxf(x, lds32(maxima + ((half ^ 1) * 128 + row) * 4));
+                    if (x > m) {
+                        step = m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
+                        m = x;
+                        l *= step;
+                    }
+                    wild = __any_sync(0xffffffffu, fabsf(m * rf) > 0x1p14f);
                 }
-                l += l0 + l1;
+                l += mine;
+                tmem_st16(sc, h);
+                tmem_st16(sc + 16, lo);
+                tmem_st16(sc + 32, h + 16);
+                tmem_st16(sc + 48, lo + 16);
                 tmem_st_done();
                 tc_fence_before();
                 mbar_arrive(&p_full[t & 1]);
                 if (j) add(t - 1);
                 fade = step, unit = next_unit;
             }
-            if (n) add(t - 1);
+            // the next item's queries before this one's last product is waited for
+            const TileItem next = item(++i, pair, 64);
+            const float next_rf = next.rows && next.n ? query(next) : 0.0f;
+            if (it.n) add(t - 1);
             sts32(sums + (half * 128 + row) * 4, l);
             bar_named(pair, 64);
             l += lds32(sums + ((half ^ 1) * 128 + row) * 4);
             bar_named(pair, 64);
             if (live) {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const float k = inv * 0x1p15f;
+                const float k = l == 0.0f ? 0.0f : 0x1p16f / l;  // (units are kept 2^-16 of theirs: no sum of theirs overflows)
+                const float top = m == -INFINITY ? kNone : fmaf(m, rf, -kTileTop);
+                const int head = it.head * a.group + r % a.group;
+                const int64_t token = it.row0 + r / a.group;
+                float* dst;
+                bool vec = true;
+                if (it.whole) {
+                    dst = a.out + token * a.out_s1 + (int64_t)head * a.dim, vec = a.out_vec;
+                    if (a.lse && half == 0) a.lse[token * a.heads * a.group + head] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
+                } else {
+                    float* p = part_slot(a, kTileRows, DP, blockIdx.x, it.begins);
+                    dst = p + 8 + 2 * kTileRows + row * DP;
+                    if (half == 0) {
+                        p[8 + 2 * row] = top, p[9 + 2 * row] = l;
+                        if (row == 0 && it.begins) {
+                            int* w = (int*)p;
+                            w[1] = it.head, w[2] = it.rows, w[3] = it.first_row, w[4] = it.row0, w[5] = it.last_block, w[0] = 1;
+                        }
+                    }
+                }
+                dst += HD * half;
 #pragma unroll
-                for (int i = 0; i < HD / 4; ++i)
-                    if (HD * half + 4 * i < a.dim)
-                        put_out(a, sh, it, row, HD * half + 4 * i, make_float4(o[4 * i] * k, o[4 * i + 1] * k, o[4 * i + 2] * k, o[4 * i + 3] * k), top_of(m, rf), l);
+                for (int c = 0; c < HD / 4; ++c) {
+                    if (HD * half + 4 * c >= a.dim) break;
+                    float4 v;
+                    unpair(o[2 * c], v.x, v.y);
+                    unpair(o[2 * c + 1], v.z, v.w);
+                    v.x *= k, v.y *= k, v.z *= k, v.w *= k;
+                    if (vec) {
+                        *(float4*)(dst + 4 * c) = v;
+                    } else {
+                        dst[4 * c] = v.x, dst[4 * c + 1] = v.y, dst[4 * c + 2] = v.z, dst[4 * c + 3] = v.w;
+                    }
+                }
             }
-            sh.advance(a, it);
+            it = next, rf = next_rf;
         }
     } else if (warp < 12) {  // ---- loaders
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
@@ -327,101 +494,103 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         const int tid = threadIdx.x - 256, r0 = tid / CH, ch = tid % CH, lw = warp - 8;
         const uint32_t kt = smem_u32(smem + C::K), vt = smem_u32(smem + C::V), scales = smem_u32(smem + C::SCALES);
         const uint32_t tops = smem_u32(smem + C::TOPS);
-        const uint32_t first_at = (uint32_t)(ch >> 2) * (kTileTokens * 128);
+        // the two pieces of f16 that 16 bytes of e4m3 become; that of the other parity first where another lane of the row
+        // stores the same banks
+        const int odd = ch >> 2 & 1;
+        const uint32_t piece = (uint32_t)(ch >> 2) * (kTileTokens * 128) + r0 * 128;
+        const uint32_t at0 = piece + ((2 * (ch & 3) + odd) ^ (r0 & 7)) * 16, at1 = piece + ((2 * (ch & 3) + 1 - odd) ^ (r0 & 7)) * 16;
+        static_assert(STEP % 8 == 0, "a thread's rows have one place in the swizzle");
         uint32_t t = 0;
         if (a.stall) warp_wait(&k_empty[0], 0, ab, 34);  // a test of the bounded waits: nothing completes this phase
-        // 16 bytes of e4m3 to two pieces of f16, that of the other parity first where another lane of the row stores the same banks
-        auto put = [&](uint32_t tile, int row, uint4 v) {
-            const uint32_t b[4] = {v.x, v.y, v.z, v.w};
-            uint32_t f[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[2 * i] = f16_of_e4m3(b[i]), f[2 * i + 1] = f16_of_e4m3(b[i] >> 16);
-            const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
-            const int odd = ch >> 2 & 1, c0 = 2 * (ch & 3);
-            const uint32_t at = tile + first_at + row * 128;
-            sts128(at + ((c0 + odd) ^ (row & 7)) * 16, odd ? hi : lo);
-            sts128(at + ((c0 + 1 - odd) ^ (row & 7)) * 16, odd ? lo : hi);
+        auto put = [&](uint32_t tile, int i, uint4 v) {
+            const uint4 lo = make_uint4(f16_of_e4m3(v.x), f16_of_e4m3(v.x >> 16), f16_of_e4m3(v.y), f16_of_e4m3(v.y >> 16));
+            const uint4 hi = make_uint4(f16_of_e4m3(v.z), f16_of_e4m3(v.z >> 16), f16_of_e4m3(v.w), f16_of_e4m3(v.w >> 16));
+            sts128(tile + at0 + i * (STEP * 128), odd ? hi : lo);
+            sts128(tile + at1 + i * (STEP * 128), odd ? lo : hi);
         };
-        while (sh.more()) {
-            const Item it = sh.item(a);
-            const int n = item_tiles(it);
+        for (uint32_t i = 0;; ++i) {
+            const TileItem it = item(i, 5, 128);
+            if (!it.rows) break;
             const int32_t* table = a.table + (int64_t)it.seq * a.table_s1;
             uint4 kv[PER], vv[PER];
             float ks = 0.0f, vs = 0.0f;
             bool in = false;
-            int pages = -1;  // lane g: the page of group g (16 tokens) of the tile to load
+            int page = -1;      // lane g & 7: the page of group g (16 tokens) of the next tile
+            int64_t slot0 = 0;  // and the group's first slot in the cache's arrays, or -1, of the tile at hand
             auto look = [&](int j) {
-                const int at = it.base + kTileTokens * (it.from + j) + 16 * (lane & 7);
-                pages = j < n && at < it.high ? table[at >> a.page_log] : -1;
+                const int at = it.first + kTileTokens * j + 16 * (lane & 7);
+                page = j < it.n && at < it.high ? table[at >> a.page_log] : -1;
             };
-            // the slot of row `row` of tile j and whether it has one that any row of the item sees
-            auto where = [&](int j, int row, bool& there) {
-                const int tok = it.base + kTileTokens * (it.from + j) + row;
-                const int pg = __shfl_sync(0xffffffffu, pages, row >> 4);
-                there = (uint32_t)pg < (uint32_t)a.pages && tok >= it.low && tok < it.high;
-                return there ? (((((int64_t)pg * a.heads) + it.head) << a.page_log) + (tok & ((1 << a.page_log) - 1))) : (int64_t)0;
+            auto turn_to = [&](int j) {
+                const int at = it.first + kTileTokens * j + 16 * (lane & 7);
+                slot0 = (uint32_t)page < (uint32_t)a.pages ? ((((int64_t)page * a.heads) + it.head) << a.page_log) + (at & ((1 << a.page_log) - 1)) : (int64_t)-1;
             };
             auto fetch = [&](int j, const uint8_t* from, uint4 (&to)[PER]) {
+                const int tok = it.first + kTileTokens * j + r0;
+                from += (int64_t)(r0 & 15) * a.dim + 16 * ch;
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    bool there;
-                    const int64_t at = where(j, r0 + STEP * i, there);
-                    to[i] = there && 16 * ch < a.dim ? __ldg((const uint4*)(from + at * a.dim + 16 * ch)) : make_uint4(0, 0, 0, 0);
+                for (int k = 0; k < PER; ++k) {
+                    const int64_t s = __shfl_sync(0xffffffffu, slot0, (STEP * k + r0) >> 4);
+                    const bool there = s >= 0 && tok + STEP * k >= it.low && tok + STEP * k < it.high && 16 * ch < a.dim;
+                    to[k] = there ? __ldg((const uint4*)(from + s * a.dim)) : make_uint4(0, 0, 0, 0);
                 }
             };
             auto fetch_scales = [&](int j) {
-                const int64_t at = where(j, tid, in);
-                ks = in ? __ldg(a.ks + at) : 0.0f, vs = in ? __ldg(a.vs + at) : 0.0f;
+                const int tok = it.first + kTileTokens * j + tid;
+                const int64_t s = __shfl_sync(0xffffffffu, slot0, tid >> 4);
+                in = s >= 0 && tok >= it.low && tok < it.high;
+                ks = in ? __ldg(a.ks + s + (tid & 15)) : 0.0f, vs = in ? __ldg(a.vs + s + (tid & 15)) : 0.0f;
             };
-            if (n) {
+            if (it.n) {
                 look(0);
+                turn_to(0);
                 fetch(0, a.k, kv);
                 fetch_scales(0);
                 fetch(0, a.v, vv);
             }
-            for (int j = 0; j < n; ++j, ++t) {
+            for (int j = 0; j < it.n; ++j, ++t) {
                 look(j + 1);
                 // scales: the unit is the least power of two above the tile's largest
-                const bool number = vs < kLargestScale;
-                float top = number ? vs : 0.0f;
+                float top = vs < kLargestScale ? vs : 0.0f;
 #pragma unroll
                 for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 const uint32_t bits = __ballot_sync(0xffffffffu, in);
                 if (lane == 0) sts32(tops + ((t & 1) * 4 + lw) * 4, top);
                 warp_wait(&k_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 34);
                 bar_named(5, 128);
-                const float4 all = lds128f(tops + (t & 1) * 16);
-                const float unit = unit_above(fmaxf(fmaxf(fmaxf(all.x, all.y), fmaxf(all.z, all.w)), kLeastUnit));
+                const uint4 all = lds128(tops + (t & 1) * 16);
+                const float unit = unit_above(fmaxf(fmaxf(fmaxf(__uint_as_float(all.x), __uint_as_float(all.y)),
+                                                          fmaxf(__uint_as_float(all.z), __uint_as_float(all.w))), kLeastUnit));
                 const uint32_t slot = scales + (t & 3) * C::SLOT;
                 sts32(slot + tid * 4, ks);
                 sts32(slot + (kTileTokens + tid) * 4, vs * (1.0f / unit));
                 if (lane == 0) sts32(slot + (2 * kTileTokens + lw) * 4, __uint_as_float(bits));
-                if (tid == 0) sts32(slot + (2 * kTileTokens + 4) * 4, unit * 0x1p-15f);
+                if (tid == 0) sts32(slot + (2 * kTileTokens + 4) * 4, unit * 0x1p-16f);
                 mbar_arrive(&sc_full[t & 3]);
 #pragma unroll
-                for (int i = 0; i < PER; ++i) put(kt + (t & 1) * C::TILE, r0 + STEP * i, kv[i]);
+                for (int k = 0; k < PER; ++k) put(kt + (t & 1) * C::TILE, k, kv[k]);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&k_full[t & 1]);
-                if (j + 1 < n) {
+                turn_to(j + 1);
+                if (j + 1 < it.n) {
                     fetch(j + 1, a.k, kv);
                     fetch_scales(j + 1);
                 }
                 warp_wait(&v_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 35);
 #pragma unroll
-                for (int i = 0; i < PER; ++i) put(vt + (t & 1) * C::TILE, r0 + STEP * i, vv[i]);
+                for (int k = 0; k < PER; ++k) put(vt + (t & 1) * C::TILE, k, vv[k]);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&v_full[t & 1]);
-                if (j + 1 < n) fetch(j + 1, a.v, vv);
+                if (j + 1 < it.n) fetch(j + 1, a.v, vv);
             }
-            sh.advance(a, it);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         if (warp == 12) {  // ---- issuer
-            const int steps = (a.dim + 15) / 16;
+            const int steps = a.dim / 16;
             const uint32_t is = idesc_f16(kTileTokens, 0), io = idesc_f16(a.dim, 1);
             const uint64_t k0 = tile_desc(smem_u32(smem + C::K), 16), v0 = tile_desc(smem_u32(smem + C::V), kTileTokens * 128);
-            uint32_t t = 0, items = 0;
+            uint32_t t = 0, queries = 0;
             bool ok = true;
             auto logits = [&](uint32_t x) {
                 ok = ok && warp_wait(&k_full[x & 1], x >> 1 & 1, ab, 36);
@@ -437,33 +606,30 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 }
                 __syncwarp();
             };
-            while (ok && sh.more()) {
-                const Item it = sh.item(a);
-                const int n = item_tiles(it);
-                if (n) {
-                    ok = warp_wait(q_full, items++ & 1, ab, 37);
+            for (uint32_t i = 0; ok; ++i) {
+                const TileItem it = item(i, 0, 0);
+                if (!it.rows) break;
+                if (!it.n) continue;
+                ok = warp_wait(q_full, queries++ & 1, ab, 37);
+                tc_fence_after();
+                logits(t);
+                for (int j = 0; ok && j < it.n; ++j, ++t) {
+                    if (j + 1 < it.n) logits(t + 1);
+                    ok = ok && warp_wait(&v_full[t & 1], t >> 1 & 1, ab, 38);
+                    ok = ok && warp_wait(&p_full[t & 1], t >> 1 & 1, ab, 39);
+                    ok = ok && (t == 0 || warp_wait(o_free, (t - 1) & 1, ab, 40));
                     tc_fence_after();
-                    logits(t);
-                    for (int j = 0; ok && j < n; ++j, ++t) {
-                        if (j + 1 < n) logits(t + 1);
-                        ok = ok && warp_wait(&v_full[t & 1], t >> 1 & 1, ab, 38);
-                        ok = ok && warp_wait(&p_full[t & 1], t >> 1 & 1, ab, 39);
-                        ok = ok && (t == 0 || warp_wait(o_free, (t - 1) & 1, ab, 40));
-                        tc_fence_after();
-                        if (ok && elect_one()) {
-                            const uint32_t p = tmem + C::S_COL + 128 * (t & 1);
-                            const uint64_t b = v0 + (uint64_t)((t & 1) * (C::TILE >> 4));
-                            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                                for (int s = 0; s < 8; ++s)
-                                    umma_ts(tmem + C::O_COL, p + 32 * (s >> 1) + 8 * (s & 1) + 16 * h, b + s * (2048 >> 4), io, h + s);
-                            umma_commit(&v_empty[t & 1]);
-                            umma_commit(o_full);
-                        }
-                        __syncwarp();
+                    if (ok && elect_one()) {
+                        const uint32_t p = tmem + C::S_COL + 128 * (t & 1);
+                        const uint64_t b = v0 + (uint64_t)((t & 1) * (C::TILE >> 4));
+                        for (int h = 0; h < 2; ++h)
+                            for (int s = 0; s < 8; ++s)
+                                umma_ts(tmem + C::O_COL, p + 32 * (s >> 1) + 8 * (s & 1) + 16 * h, b + s * (2048 >> 4), io, h + s);
+                        umma_commit(&v_empty[t & 1]);
+                        umma_commit(o_full);
                     }
+                    __syncwarp();
                 }
-                sh.advance(a, it);
             }
             // products in flight end before TMEM is freed
             if (elect_one()) umma_commit(drain);
@@ -471,6 +637,31 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             if (lane == 0)
                 for (uint32_t i = 0; i < kWaitLimit && !mbar_test(drain, 0); ++i) __nanosleep(64);
             __syncwarp();
+        } else if (warp == 13) {  // ---- planner
+            for (uint32_t i = 0;; ++i) {
+                TileItem p = {};
+                const bool more = sh.more();
+                if (more) {
+                    const Item it = sh.item(a);
+                    p.rows = it.rows, p.row0 = it.row0, p.first_row = it.first_row;
+                    p.n = max(0, min(it.to, (it.high - it.base + kTileTokens - 1) / kTileTokens) - it.from);
+                    p.pos = it.pos, p.all_first = it.top_first, p.all_last = it.pos + it.first_row / a.group, p.head = it.head;
+                    p.low = it.low, p.high = it.high, p.first = it.base + kTileTokens * it.from, p.seq = it.seq;
+                    p.whole = it.from == 0 && it.to == it.units, p.begins = it.from == 0, p.last_block = sh.last_block(it);
+                    sh.advance(a, it);
+                }
+                const bool ok = warp_wait(&i_free[i & (kItems - 1)], (i / kItems & 1) ^ 1, ab, 42);
+                if (lane == 0) {
+                    const int* w = (const int*)&p;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        sts128(ring + (i & (kItems - 1)) * 64 + 16 * k,
+                               make_uint4((uint32_t)w[4 * k], (uint32_t)w[4 * k + 1], (uint32_t)w[4 * k + 2], (uint32_t)w[4 * k + 3]));
+                    mbar_arrive(&i_full[i & (kItems - 1)]);
+                }
+                __syncwarp();
+                if (!ok || !more) break;
+            }
         }
     }
     tc_fence_before();

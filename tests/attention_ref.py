@@ -61,8 +61,9 @@ def attention(q, k, v, scale, n, length, window, ok=None):
                 # are added like the logits, 2 x 64 instructions between two flushes into f32 sums, one flush per 128 to
                 # 1024 tokens and part; the exponential and the division take a few more.
                 add = (2 * 64 + len(vv) / 128 + 40) * 2 * U
-                # A weight is a sum of two f16 of at most 2^15: multiples of 2^-24, so off by up to 2^-40 of the largest, times
-                # e4m3 values of up to 448 of a scale at most twice the largest one (2^9 of 448 s, of which |v| may be 2^-3).
-                tol[t, h] = (np.abs(vv).T @ e) / total * (2 * ds + add) + 2.0 ** -36 * len(vv) * np.abs(vv).max() / total
+                # A weight is a sum of two f16, multiples of 2^-24 where the largest weight is 2^15 (few rows) or 2^9 (many): off by
+                # up to 2^-25 / 2^9 = 2^-34 of the largest, times e4m3 values of up to 448 of a unit at most twice the largest
+                # scale (2^10 scales, while the largest |v| may be as little as 2^6 of them): 2^-30 of the largest |v|.
+                tol[t, h] = (np.abs(vv).T @ e) / total * (2 * ds + add) + 2.0 ** -30 * len(vv) * np.abs(vv).max() / total
                 ltol[t, h] = ds + add + 2 * U * abs(lse[t, h])
     return out, lse, tol, ltol
