@@ -116,12 +116,6 @@ __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ float lds32(uint32_t a) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ void sts32(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
 
 // Pairs of f32 in one instruction, each rounded as alone.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
@@ -150,10 +144,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// (not volatile: scales are read after the barrier that the tile's start waits for, and may be read early within the tile)
-__device__ __forceinline__ void lds_pairs(uint32_t a, uint64_t& x, uint64_t& y) {
-    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "r"(a));
-}
 // As split2, for a pair.
 __device__ __forceinline__ void split_pair(uint64_t w, uint32_t& high, uint32_t& low) {
     asm("{\n\t.reg .b16 x, y;\n\t.reg .f32 a, b, u, v;\n\t.reg .b64 h, d;\n\t"
@@ -169,40 +159,36 @@ __device__ __forceinline__ void split_pair(uint64_t w, uint32_t& high, uint32_t&
         : "l"(w));
 }
 
-// 32 columns of S at taddr to probabilities times their values' ratios, as f16 halves; *sum gains the probabilities.
-// CARE: tokens whose bit in `seen` is not set have none, and a logit is rounded before the reference is taken from it, so
-// that the two are equal where they should be (unrounded they differ by up to 2^-24 of the logit: of no account while that is
-// small).
+// 32 columns of S to probabilities times their values' ratios, as f16 halves; *sum gains the probabilities.  Tokens that are
+// not to be seen have come as -inf.
+// CARE: for scales that are no numbers and for logits that are large.  Tokens whose bit in `seen` is not set have no part,
+// whatever their scales are, and a logit is rounded before the reference is taken from it, so that the two are equal where they
+// should be (unrounded they differ by up to 2^-24 of the logit: of no account while that is small).
 template <bool CARE>
-__device__ __forceinline__ void tile_chunk(uint32_t taddr, uint32_t ks, uint32_t vs, uint64_t minus_m, uint64_t rf, uint32_t seen,
+__device__ __forceinline__ void tile_chunk(const uint32_t (&v)[32], const ulonglong2* ks, const ulonglong2* vs, float m, uint64_t rf, uint32_t seen,
                                            uint32_t* high, uint32_t* low, uint64_t* sum) {
-    const uint64_t top = pair_of(kTileTop, kTileTop);
-    uint32_t v[32];
-    tmem_ld32(taddr, v);
+    const uint64_t top = pair_of(kTileTop, kTileTop), minus_m = pair_of(-m, -m);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        uint64_t kk[2], vv[2];
-        lds_pairs(ks + 16 * k, kk[0], kk[1]);
-        lds_pairs(vs + 16 * k, vv[0], vv[1]);
+        const ulonglong2 kk = ks[k], vv = vs[k];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int e = 4 * k + 2 * h;
+            const uint64_t kp = h ? kk.y : kk.x, vp = h ? vv.y : vv.x;
             float x, y;
             uint64_t t;
             if (CARE) {  // (one by one: packed, the compiler joins the two roundings)
-                float k0, k1, m0, m1;
-                unpair(kk[h], k0, k1);
-                unpair(minus_m, m0, m1);
-                t = pair_of(__fadd_rn(__fmul_rn(__uint_as_float(v[e]), k0), m0), __fadd_rn(__fmul_rn(__uint_as_float(v[e + 1]), k1), m1));
+                unpair(kp, x, y);
+                t = pair_of(__fadd_rn(__fmul_rn(__uint_as_float(v[e]), x), -m), __fadd_rn(__fmul_rn(__uint_as_float(v[e + 1]), y), -m));
             } else {
-                t = fma2(pair_of(v[e], v[e + 1]), kk[h], minus_m);
+                t = fma2(pair_of(v[e], v[e + 1]), kp, minus_m);
             }
             unpair(fma2(t, rf, top), x, y);
             x = exp2_f(x), y = exp2_f(y);
             if (CARE) x = seen >> e & 1 ? x : 0.0f, y = seen >> (e + 1) & 1 ? y : 0.0f;
             const uint64_t p = pair_of(x, y);
             *sum = add2(*sum, p);
-            uint64_t w = mul2(p, vv[h]);
+            uint64_t w = mul2(p, vp);
             if (CARE) {
                 unpair(w, x, y);
                 w = pair_of(seen >> e & 1 ? x : 0.0f, seen >> (e + 1) & 1 ? y : 0.0f);
@@ -216,7 +202,7 @@ template <int DP>
 __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     using C = TileCfg<DP>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     uint64_t* k_full = (uint64_t*)(smem + C::BARS);
     uint64_t* k_empty = k_full + 2;
     uint64_t* v_full = k_empty + 2;
@@ -278,7 +264,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         int* w = (int*)&it;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const uint4 v = lds128(ring + (i & (kItems - 1)) * 64 + 16 * k);
+            const uint4 v = ((const uint4*)(smem + C::ITEMS))[4 * (i & (kItems - 1)) + k];
             w[4 * k] = (int)v.x, w[4 * k + 1] = (int)v.y, w[4 * k + 2] = (int)v.z, w[4 * k + 3] = (int)v.w;
         }
         __syncwarp();
@@ -295,87 +281,140 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         constexpr int HD = DP / 2;  // this thread's columns of the output and values of a query
         const int half = warp >> 2, row = 32 * (warp & 3) + lane, pair = 1 + (warp & 3);
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t scales = smem_u32(smem + C::SCALES) + 64 * half * 4, maxima = smem_u32(smem + C::MAXIMA), sums = smem_u32(smem + C::SUMS);
-        // The query's half row of an item, in TMEM as two f16 (the products that read the last item's are done: their S was
-        // waited for); returns the factor that takes S to log2 units.
-        auto query = [&](const TileItem& it) {
-            const int r = it.first_row + row;
-            const bool live = row < it.rows;
-            const float* p = a.q + (int64_t)(it.row0 + (live ? r / a.group : 0)) * a.q_s1 +
-                             (int64_t)(it.head * a.group + (live ? r % a.group : 0)) * a.dim + HD * half;
-            float x[HD];
-            uint32_t top = 0;
-            if (a.q_vec) {
+        float* maxima = (float*)(smem + C::MAXIMA);
+        float* sums = (float*)(smem + C::SUMS);
+        uint32_t t = 0;  // tiles done
+        // The item at hand: its rows' reference and sum, output, the factor that takes S to log2 units.
+        TileItem it = {};
+        uint64_t o[HD / 2];
+        float m = -INFINITY, l = 0.0f, rf = 0.0f, fade = 1.0f, unit = 0.0f;
+        // O of the last tile joins the sums: waits for it, and hands the columns back
+        auto add_tile = [&](uint32_t x) {
+            if (__any_sync(0xffffffffu, fade != 1.0f)) {
+                const uint64_t f = pair_of(fade, fade);
 #pragma unroll
-                for (int i = 0; i < HD / 4; ++i) {
-                    const float4 v = live && HD * half + 4 * i < a.dim ? *(const float4*)(p + 4 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+                for (int k = 0; k < HD / 2; ++k) o[k] = mul2(o[k], f);
+            }
+            const uint64_t u = pair_of(unit, unit);
+            warp_wait(o_full, x & 1, ab, 31);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t v[32];
+                tmem_ld32(tmem + lanes + C::O_COL + HD * half + 32 * c, v);
+                if (c == HD / 32 - 1) {
+                    tc_fence_before();
+                    mbar_arrive(o_free);
                 }
-            } else {
 #pragma unroll
-                for (int i = 0; i < HD; ++i) x[i] = live && HD * half + i < a.dim ? p[i] : 0.0f;
+                for (int k = 0; k < 16; ++k) o[16 * c + k] = fma2(pair_of(v[2 * k], v[2 * k + 1]), u, o[16 * c + k]);
             }
-#pragma unroll
-            for (int i = 0; i < HD; ++i) top = max(top, abs_bits(x[i]));
-            sts32(sums + (half * 128 + row) * 4, __uint_as_float(top));
-            bar_named(pair, 64);
-            top = max(top, __float_as_uint(lds32(sums + ((half ^ 1) * 128 + row) * 4)));
-            bar_named(pair, 64);
-            const float up = query_unit(top);
-#pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {
-                uint32_t h[16], l[16];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) split2(x[32 * i + 2 * k] * up, x[32 * i + 2 * k + 1] * up, h[k], l[k]);
-                tmem_st16(tmem + lanes + C::Q_COL + HD / 2 * half + 16 * i, h);
-                tmem_st16(tmem + lanes + C::Q_COL + DP / 2 + HD / 2 * half + 16 * i, l);
-            }
-            tmem_st_done();
-            tc_fence_before();
-            mbar_arrive(q_full);
-            return a.scale * kLog2e / up;
         };
-        uint32_t t = 0, i = 0;  // tiles done, items
-        TileItem it = item(0, pair, 64);
-        float rf = it.rows && it.n ? query(it) : 0.0f;
-        while (it.rows) {
-            const int r = it.first_row + row;
-            const bool live = row < it.rows;
-            const int last = live ? it.pos + r / a.group : -1, first = a.window && last >= a.window ? last - a.window + 1 : 0;
-            const uint64_t rf2 = pair_of(rf, rf);
-            uint64_t o[HD / 2];
+#pragma unroll 1
+        for (uint32_t i = 0;; ++i) {
+            const TileItem next = item(i, pair, 64);
+            float next_rf = 0.0f;
+            if (next.rows && next.n) {
+                // the next item's queries, as two f16 in TMEM (the products that read the last item's are done: their S was
+                // waited for), before the last product of the item at hand is waited for
+                const int r = next.first_row + row;
+                const bool live = row < next.rows;
+                const float* p = a.q + (int64_t)(next.row0 + (live ? r / a.group : 0)) * a.q_s1 +
+                                 (int64_t)(next.head * a.group + (live ? r % a.group : 0)) * a.dim + HD * half;
+                float x[HD];
+                uint32_t top = 0;
+                if (a.q_vec) {
 #pragma unroll
-            for (int k = 0; k < HD / 2; ++k) o[k] = 0;
-            float m = -INFINITY, l = 0.0f, fade = 1.0f, unit = 0.0f;
-            bool wild = false;  // a row's logits are large for the unrounded form
-            // O of tile x joins the sums: waits for it, and hands the columns back
-            auto add = [&](uint32_t x) {
-                if (__any_sync(0xffffffffu, fade != 1.0f)) {
-                    const uint64_t f = pair_of(fade, fade);
+                    for (int k = 0; k < HD / 4; ++k) {
+                        const float4 v = live && HD * half + 4 * k < a.dim ? *(const float4*)(p + 4 * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
+                    }
+                } else {
 #pragma unroll
-                    for (int k = 0; k < HD / 2; ++k) o[k] = mul2(o[k], f);
+                    for (int k = 0; k < HD; ++k) x[k] = live && HD * half + k < a.dim ? p[k] : 0.0f;
                 }
-                const uint64_t u = pair_of(unit, unit);
-                warp_wait(o_full, x & 1, ab, 31);
-                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < HD; ++k) top = max(top, abs_bits(x[k]));
+                sums[half * 128 + row] = __uint_as_float(top);
+                bar_named(pair, 64);
+                top = max(top, __float_as_uint(sums[(half ^ 1) * 128 + row]));
+                bar_named(pair, 64);
+                const float up = query_unit(top);
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(tmem + lanes + C::O_COL + HD * half + 32 * c, v);
-                    if (c == HD / 32 - 1) {
-                        tc_fence_before();
-                        mbar_arrive(o_free);
-                    }
+                    uint32_t h[16], lo[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[16 * c + k] = fma2(pair_of(v[2 * k], v[2 * k + 1]), u, o[16 * c + k]);
+                    for (int k = 0; k < 16; ++k) split2(x[32 * c + 2 * k] * up, x[32 * c + 2 * k + 1] * up, h[k], lo[k]);
+                    tmem_st16(tmem + lanes + C::Q_COL + HD / 2 * half + 16 * c, h);
+                    tmem_st16(tmem + lanes + C::Q_COL + DP / 2 + HD / 2 * half + 16 * c, lo);
                 }
-            };
+                tmem_st_done();
+                tc_fence_before();
+                mbar_arrive(q_full);
+                next_rf = a.scale * kLog2e / up;
+            }
+            if (it.rows) {  // the item at hand is complete but for its last tile's output
+                if (it.n) add_tile(t - 1);
+                sums[half * 128 + row] = l;
+                bar_named(pair, 64);
+                l += sums[(half ^ 1) * 128 + row];
+                bar_named(pair, 64);
+                if (row < it.rows) {
+                    const int r = it.first_row + row;
+                    const float k = l == 0.0f ? 0.0f : 0x1p16f / l;  // (units are kept 2^-16 of theirs: no sum of theirs overflows)
+                    const float top = m == -INFINITY ? kNone : fmaf(m, rf, -kTileTop);
+                    float* dst;
+                    bool vec = true;
+                    if (it.whole) {
+                        const int head = it.head * a.group + r % a.group;
+                        const int64_t token = it.row0 + r / a.group;
+                        dst = a.out + token * a.out_s1 + (int64_t)head * a.dim, vec = a.out_vec;
+                        if (a.lse && half == 0) a.lse[token * a.heads * a.group + head] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
+                    } else {
+                        float* p = part_slot(a, kTileRows, DP, blockIdx.x, it.begins);
+                        dst = p + 8 + 2 * kTileRows + row * DP;
+                        if (half == 0) {
+                            p[8 + 2 * row] = top, p[9 + 2 * row] = l;
+                            if (row == 0 && it.begins) {
+                                int* w = (int*)p;
+                                w[1] = it.head, w[2] = it.rows, w[3] = it.first_row, w[4] = it.row0, w[5] = it.last_block, w[0] = 1;
+                            }
+                        }
+                    }
+                    dst += HD * half;
+                    const uint64_t kk = pair_of(k, k);
+#pragma unroll
+                    for (int c = 0; c < HD / 4; ++c) {
+                        float4 v;
+                        unpair(mul2(o[2 * c], kk), v.x, v.y);
+                        unpair(mul2(o[2 * c + 1], kk), v.z, v.w);
+                        if (HD * half + 4 * c >= a.dim) continue;
+                        if (vec) {
+                            *(float4*)(dst + 4 * c) = v;
+                        } else {
+                            dst[4 * c] = v.x, dst[4 * c + 1] = v.y, dst[4 * c + 2] = v.z, dst[4 * c + 3] = v.w;
+                        }
+                    }
+                }
+            }
+            if (!next.rows) break;
+            it = next, rf = next_rf;
+            const int last = row < it.rows ? it.pos + (it.first_row + row) / a.group : -1;
+            const int first = a.window && last >= a.window ? last - a.window + 1 : 0;
+            const uint64_t rf2 = pair_of(rf, rf);
+#pragma unroll
+            for (int k = 0; k < HD / 2; ++k) o[k] = 0;
+            m = -INFINITY, l = 0.0f, fade = 1.0f, unit = 0.0f;
+            bool wild = __any_sync(0xffffffffu, !(rf >= 0x1p-126f));  // a row's logits want the careful form
+#pragma unroll 1
             for (int j = 0; j < it.n; ++j, ++t) {
-                const uint32_t slot = scales + (t & 3) * C::SLOT;  // (this half's scales)
+                const uint8_t* slot = smem + C::SCALES + (t & 3) * C::SLOT;
+                const ulonglong2* ks = (const ulonglong2*)(slot + 64 * half * 4);
+                const ulonglong2* vs = (const ulonglong2*)(slot + (kTileTokens + 64 * half) * 4);
                 warp_wait(&sc_full[t & 3], t >> 2 & 1, ab, 32);
                 const int j0 = it.first + kTileTokens * j;
-                const uint4 ok = lds128(slot - 64 * half * 4 + 2 * kTileTokens * 4);
-                const float next_unit = lds32(slot - 64 * half * 4 + 2 * kTileTokens * 4 + 16);
+                const uint4 ok = *(const uint4*)(slot + 2 * kTileTokens * 4);
+                const float2 more = *(const float2*)(slot + 2 * kTileTokens * 4 + 16);  // unit, and 0 where a scale is no number
                 // not all tokens seen by all rows
                 const bool edge = j0 < it.all_first || j0 + kTileTokens - 1 > it.all_last || (ok.x & ok.y & ok.z & ok.w) != 0xffffffffu;
                 uint32_t seen0 = half ? ok.z : ok.x, seen1 = half ? ok.w : ok.y;
@@ -389,46 +428,54 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 tc_fence_after();
                 const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 64 * half;
                 uint32_t h[32], lo[32];
-                float step = 1.0f, mine = 0.0f;
-                auto form = [&]() {
-                    const uint64_t mm = pair_of(-m, -m);
+                float step = 1.0f, mine;
+#pragma unroll 1
+                for (int again = 0;; ++again) {
+                    const float ref = m == -INFINITY ? 0.0f : m;
                     uint64_t sum = 0;
-                    if (edge || wild) {
-                        tile_chunk<true>(sc, slot, slot + kTileTokens * 4, mm, rf2, seen0, h, lo, &sum);
-                        tile_chunk<true>(sc + 32, slot + 128, slot + kTileTokens * 4 + 128, mm, rf2, seen1, h + 16, lo + 16, &sum);
-                    } else {
-                        tile_chunk<false>(sc, slot, slot + kTileTokens * 4, mm, rf2, 0u, h, lo, &sum);
-                        tile_chunk<false>(sc + 32, slot + 128, slot + kTileTokens * 4 + 128, mm, rf2, 0u, h + 16, lo + 16, &sum);
+                    const bool care = wild || more.y == 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(sc + 32 * c, v);
+                        if (care) {
+                            tile_chunk<true>(v, ks + 8 * c, vs + 8 * c, ref, rf2, c ? seen1 : seen0, h + 16 * c, lo + 16 * c, &sum);
+                        } else {
+                            if (edge) {
+#pragma unroll
+                                for (int k = 0; k < 32; ++k)
+                                    if (!((c ? seen1 : seen0) >> k & 1)) v[k] = 0xff800000u;
+                            }
+                            tile_chunk<false>(v, ks + 8 * c, vs + 8 * c, ref, rf2, 0u, h + 16 * c, lo + 16 * c, &sum);
+                        }
                     }
                     float x, y;
                     unpair(sum, x, y);
                     mine = x + y;
-                };
-                for (int again = 0;; ++again) {
-                    form();
-                    if (again || !bar_any(pair, 64, !(mine < kTileSum))) break;
+                    if (again || !bar_any(pair, 64, !(mine < kTileSum) || (m == -INFINITY && (seen0 | seen1)))) break;
                     // the rows' maxima of the tile, of both halves
-                    float x = -INFINITY;
+                    x = -INFINITY;
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {
                         uint32_t v[32];
                         tmem_ld32(sc + 32 * c, v);
                         const uint32_t seen = c ? seen1 : seen0;
+                        const float* kf = (const float*)(ks + 8 * c);
 #pragma unroll
                         for (int k = 0; k < 32; ++k) {
-                            const float y = __fmul_rn(__uint_as_float(v[k]), lds32(slot + 128 * c + 4 * k));
+                            y = __fmul_rn(__uint_as_float(v[k]), kf[k]);
                             if (seen >> k & 1) x = fmaxf(x, y);
                         }
                     }
-                    sts32(maxima + (half * 128 + row) * 4, x);
+                    maxima[half * 128 + row] = x;
                     bar_named(pair, 64);
-                    x = fmaxf(x, lds32(maxima + ((half ^ 1) * 128 + row) * 4));
+                    x = fmaxf(x, maxima[(half ^ 1) * 128 + row]);
                     if (x > m) {
                         step = m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
                         m = x;
                         l *= step;
                     }
-                    wild = __any_sync(0xffffffffu, fabsf(m * rf) > 0x1p14f);
+                    wild = wild || __any_sync(0xffffffffu, fabsf(m * rf) > 0x1p14f);
                 }
                 l += mine;
                 tmem_st16(sc, h);
@@ -438,151 +485,113 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 tmem_st_done();
                 tc_fence_before();
                 mbar_arrive(&p_full[t & 1]);
-                if (j) add(t - 1);
-                fade = step, unit = next_unit;
+                if (j) add_tile(t - 1);
+                fade = step, unit = more.x;
             }
-            // the next item's queries before this one's last product is waited for
-            const TileItem next = item(++i, pair, 64);
-            const float next_rf = next.rows && next.n ? query(next) : 0.0f;
-            if (it.n) add(t - 1);
-            sts32(sums + (half * 128 + row) * 4, l);
-            bar_named(pair, 64);
-            l += lds32(sums + ((half ^ 1) * 128 + row) * 4);
-            bar_named(pair, 64);
-            if (live) {
-                const float k = l == 0.0f ? 0.0f : 0x1p16f / l;  // (units are kept 2^-16 of theirs: no sum of theirs overflows)
-                const float top = m == -INFINITY ? kNone : fmaf(m, rf, -kTileTop);
-                const int head = it.head * a.group + r % a.group;
-                const int64_t token = it.row0 + r / a.group;
-                float* dst;
-                bool vec = true;
-                if (it.whole) {
-                    dst = a.out + token * a.out_s1 + (int64_t)head * a.dim, vec = a.out_vec;
-                    if (a.lse && half == 0) a.lse[token * a.heads * a.group + head] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
-                } else {
-                    float* p = part_slot(a, kTileRows, DP, blockIdx.x, it.begins);
-                    dst = p + 8 + 2 * kTileRows + row * DP;
-                    if (half == 0) {
-                        p[8 + 2 * row] = top, p[9 + 2 * row] = l;
-                        if (row == 0 && it.begins) {
-                            int* w = (int*)p;
-                            w[1] = it.head, w[2] = it.rows, w[3] = it.first_row, w[4] = it.row0, w[5] = it.last_block, w[0] = 1;
-                        }
-                    }
-                }
-                dst += HD * half;
-#pragma unroll
-                for (int c = 0; c < HD / 4; ++c) {
-                    if (HD * half + 4 * c >= a.dim) break;
-                    float4 v;
-                    unpair(o[2 * c], v.x, v.y);
-                    unpair(o[2 * c + 1], v.z, v.w);
-                    v.x *= k, v.y *= k, v.z *= k, v.w *= k;
-                    if (vec) {
-                        *(float4*)(dst + 4 * c) = v;
-                    } else {
-                        dst[4 * c] = v.x, dst[4 * c + 1] = v.y, dst[4 * c + 2] = v.z, dst[4 * c + 3] = v.w;
-                    }
-                }
-            }
-            it = next, rf = next_rf;
         }
     } else if (warp < 12) {  // ---- loaders
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         constexpr int CH = DP / 16, PER = kTileTokens * CH / 128;  // pieces of 16 bytes of a row, and of a thread
         constexpr int STEP = 128 / CH;                             // rows between a thread's pieces
         const int tid = threadIdx.x - 256, r0 = tid / CH, ch = tid % CH, lw = warp - 8;
-        const uint32_t kt = smem_u32(smem + C::K), vt = smem_u32(smem + C::V), scales = smem_u32(smem + C::SCALES);
-        const uint32_t tops = smem_u32(smem + C::TOPS);
+        uint32_t* tops = (uint32_t*)(smem + C::TOPS);
         // the two pieces of f16 that 16 bytes of e4m3 become; that of the other parity first where another lane of the row
         // stores the same banks
         const int odd = ch >> 2 & 1;
         const uint32_t piece = (uint32_t)(ch >> 2) * (kTileTokens * 128) + r0 * 128;
-        const uint32_t at0 = piece + ((2 * (ch & 3) + odd) ^ (r0 & 7)) * 16, at1 = piece + ((2 * (ch & 3) + 1 - odd) ^ (r0 & 7)) * 16;
+        uint8_t* at0 = smem + piece + ((2 * (ch & 3) + odd) ^ (r0 & 7)) * 16;
+        uint8_t* at1 = smem + piece + ((2 * (ch & 3) + 1 - odd) ^ (r0 & 7)) * 16;
         static_assert(STEP % 8 == 0, "a thread's rows have one place in the swizzle");
-        uint32_t t = 0;
         if (a.stall) warp_wait(&k_empty[0], 0, ab, 34);  // a test of the bounded waits: nothing completes this phase
-        auto put = [&](uint32_t tile, int i, uint4 v) {
-            const uint4 lo = make_uint4(f16_of_e4m3(v.x), f16_of_e4m3(v.x >> 16), f16_of_e4m3(v.y), f16_of_e4m3(v.y >> 16));
-            const uint4 hi = make_uint4(f16_of_e4m3(v.z), f16_of_e4m3(v.z >> 16), f16_of_e4m3(v.w), f16_of_e4m3(v.w >> 16));
-            sts128(tile + at0 + i * (STEP * 128), odd ? hi : lo);
-            sts128(tile + at1 + i * (STEP * 128), odd ? lo : hi);
+        auto put = [&](uint32_t tile, const uint4 (&x)[PER]) {
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                const uint4 v = x[k];
+                const uint4 lo = make_uint4(f16_of_e4m3(v.x), f16_of_e4m3(v.x >> 16), f16_of_e4m3(v.y), f16_of_e4m3(v.y >> 16));
+                const uint4 hi = make_uint4(f16_of_e4m3(v.z), f16_of_e4m3(v.z >> 16), f16_of_e4m3(v.w), f16_of_e4m3(v.w >> 16));
+                *(uint4*)(at0 + tile + k * (STEP * 128)) = odd ? hi : lo;
+                *(uint4*)(at1 + tile + k * (STEP * 128)) = odd ? lo : hi;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
-        for (uint32_t i = 0;; ++i) {
-            const TileItem it = item(i, 5, 128);
-            if (!it.rows) break;
-            const int32_t* table = a.table + (int64_t)it.seq * a.table_s1;
-            uint4 kv[PER], vv[PER];
-            float ks = 0.0f, vs = 0.0f;
-            bool in = false;
-            int page = -1;      // lane g & 7: the page of group g (16 tokens) of the next tile
-            int64_t slot0 = 0;  // and the group's first slot in the cache's arrays, or -1, of the tile at hand
-            auto look = [&](int j) {
-                const int at = it.first + kTileTokens * j + 16 * (lane & 7);
-                page = j < it.n && at < it.high ? table[at >> a.page_log] : -1;
-            };
-            auto turn_to = [&](int j) {
+        uint4 kv[PER], vv[PER];
+        float ks = 0.0f, vs = 0.0f;
+        bool in = false;
+        TileItem it = {};
+        int j = -1;          // the tile of the item that the registers are filled for
+        int page = -1;       // lane g & 7: the page of group g (16 tokens) of the tile after
+        int64_t slot0 = -1;  // the group's first slot in the cache's arrays, or -1, of the tile
+        auto look = [&](int x) {
+            const int at = it.first + kTileTokens * x + 16 * (lane & 7);
+            page = x < it.n && at < it.high ? a.table[(int64_t)it.seq * a.table_s1 + (at >> a.page_log)] : -1;
+        };
+        auto fetch = [&](const uint8_t* from, uint4 (&to)[PER]) {
+            const int tok = it.first + kTileTokens * j + r0;
+            from += (int64_t)(r0 & 15) * a.dim + 16 * ch;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                const int64_t s = __shfl_sync(0xffffffffu, slot0, (STEP * k + r0) >> 4);
+                const bool there = s >= 0 && tok + STEP * k >= it.low && tok + STEP * k < it.high && 16 * ch < a.dim;
+                to[k] = there ? __ldg((const uint4*)(from + s * a.dim)) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        // Tile t goes from registers to shared memory, each half followed by the loads of the next tile's, which may be another
+        // item's.
+        bool have = false, more = true;
+        uint32_t items = 0;
+#pragma unroll 1
+        for (uint32_t t = 0; more || have;) {
+            if (have) {
+                // scales: the unit is the least power of two above the tile's largest
+                const bool number = vs < kLargestScale;
+                float top = number ? vs : 0.0f;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const uint32_t bits = __ballot_sync(0xffffffffu, in);
+                const bool bad = __any_sync(0xffffffffu, !number || !(fabsf(ks) < INFINITY));
+                if (lane == 0) tops[(t & 1) * 4 + lw] = abs_bits(top) | (bad ? 0x80000000u : 0u);
+                warp_wait(&k_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 34);
+                bar_named(5, 128);
+                const uint4 all = *(const uint4*)(tops + (t & 1) * 4);
+                const uint32_t largest = max(max(all.x & 0x7FFFFFFFu, all.y & 0x7FFFFFFFu), max(all.z & 0x7FFFFFFFu, all.w & 0x7FFFFFFFu));
+                const float unit = unit_above(fmaxf(__uint_as_float(largest), kLeastUnit));
+                float* slot = (float*)(smem + C::SCALES + (t & 3) * C::SLOT);
+                slot[tid] = ks == 0.0f ? 0x1p-126f : ks;  // (so that -inf times it is -inf)
+                slot[kTileTokens + tid] = vs * (1.0f / unit);
+                if (lane == 0) slot[2 * kTileTokens + lw] = __uint_as_float(bits);
+                if (tid == 0) slot[2 * kTileTokens + 4] = unit * 0x1p-16f, slot[2 * kTileTokens + 5] = (all.x | all.y | all.z | all.w) >> 31 ? 0.0f : 1.0f;
+                mbar_arrive(&sc_full[t & 3]);
+                put(C::K + (t & 1) * C::TILE, kv);
+                mbar_arrive(&k_full[t & 1]);
+            }
+            // the next tile
+            ++j;
+            if (j >= it.n) {
+                do {
+                    it = item(items++, 5, 128);
+                } while (it.rows && !it.n);
+                more = it.rows != 0;
+                j = 0;
+                look(0);
+            }
+            if (more) {
                 const int at = it.first + kTileTokens * j + 16 * (lane & 7);
                 slot0 = (uint32_t)page < (uint32_t)a.pages ? ((((int64_t)page * a.heads) + it.head) << a.page_log) + (at & ((1 << a.page_log) - 1)) : (int64_t)-1;
-            };
-            auto fetch = [&](int j, const uint8_t* from, uint4 (&to)[PER]) {
-                const int tok = it.first + kTileTokens * j + r0;
-                from += (int64_t)(r0 & 15) * a.dim + 16 * ch;
-#pragma unroll
-                for (int k = 0; k < PER; ++k) {
-                    const int64_t s = __shfl_sync(0xffffffffu, slot0, (STEP * k + r0) >> 4);
-                    const bool there = s >= 0 && tok + STEP * k >= it.low && tok + STEP * k < it.high && 16 * ch < a.dim;
-                    to[k] = there ? __ldg((const uint4*)(from + s * a.dim)) : make_uint4(0, 0, 0, 0);
-                }
-            };
-            auto fetch_scales = [&](int j) {
+                look(j + 1);
+                fetch(a.k, kv);
                 const int tok = it.first + kTileTokens * j + tid;
                 const int64_t s = __shfl_sync(0xffffffffu, slot0, tid >> 4);
                 in = s >= 0 && tok >= it.low && tok < it.high;
                 ks = in ? __ldg(a.ks + s + (tid & 15)) : 0.0f, vs = in ? __ldg(a.vs + s + (tid & 15)) : 0.0f;
-            };
-            if (it.n) {
-                look(0);
-                turn_to(0);
-                fetch(0, a.k, kv);
-                fetch_scales(0);
-                fetch(0, a.v, vv);
             }
-            for (int j = 0; j < it.n; ++j, ++t) {
-                look(j + 1);
-                // scales: the unit is the least power of two above the tile's largest
-                float top = vs < kLargestScale ? vs : 0.0f;
-#pragma unroll
-                for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const uint32_t bits = __ballot_sync(0xffffffffu, in);
-                if (lane == 0) sts32(tops + ((t & 1) * 4 + lw) * 4, top);
-                warp_wait(&k_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 34);
-                bar_named(5, 128);
-                const uint4 all = lds128(tops + (t & 1) * 16);
-                const float unit = unit_above(fmaxf(fmaxf(fmaxf(__uint_as_float(all.x), __uint_as_float(all.y)),
-                                                          fmaxf(__uint_as_float(all.z), __uint_as_float(all.w))), kLeastUnit));
-                const uint32_t slot = scales + (t & 3) * C::SLOT;
-                sts32(slot + tid * 4, ks);
-                sts32(slot + (kTileTokens + tid) * 4, vs * (1.0f / unit));
-                if (lane == 0) sts32(slot + (2 * kTileTokens + lw) * 4, __uint_as_float(bits));
-                if (tid == 0) sts32(slot + (2 * kTileTokens + 4) * 4, unit * 0x1p-16f);
-                mbar_arrive(&sc_full[t & 3]);
-#pragma unroll
-                for (int k = 0; k < PER; ++k) put(kt + (t & 1) * C::TILE, k, kv[k]);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&k_full[t & 1]);
-                turn_to(j + 1);
-                if (j + 1 < it.n) {
-                    fetch(j + 1, a.k, kv);
-                    fetch_scales(j + 1);
-                }
+            if (have) {
                 warp_wait(&v_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 35);
-#pragma unroll
-                for (int k = 0; k < PER; ++k) put(vt + (t & 1) * C::TILE, k, vv[k]);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                put(C::V + (t & 1) * C::TILE, vv);
                 mbar_arrive(&v_full[t & 1]);
-                if (j + 1 < it.n) fetch(j + 1, a.v, vv);
+                ++t;
             }
+            if (more) fetch(a.v, vv);
+            have = more;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
