@@ -20,15 +20,12 @@ using namespace mcu;
 //   warps 8-11   loaders: e4m3 from the pages through registers to f16 tiles (128-byte swizzle), scales, valid tokens
 //   warp 12      issues the products: S of tile j + 1 before O of tile j, so that softmax runs under them
 //   warp 13      plans: puts the block's items into a ring, so that the others find theirs without global loads
-// Probabilities are 2^kTileTop relative to a reference that need not be the row's maximum: their f16 halves leave room for 7
-// powers of two above it.  A tile is formed with the reference as it is; where the sum of a thread's 64 probabilities is
-// below 2^16 (it bounds each of them) that stands, else the pair of warps that share the rows finds the maximum, moves the reference
-// there and forms the tile again.  After a row's first tile that is rare, and a separate pass for the maximum is saved.
+// A tile's logits are read twice, for the rows' maxima and for the probabilities, in loops of 32 columns that are not unrolled:
+// the loops of all roles have to fit the SM's instruction cache together (unrolled, with the probabilities formed in one pass
+// against a reference that moved when it had to, a third of its requests missed and a tile took three times as long).
 constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 512;
-constexpr int kTileLaunch = 128, kSoftRegs = 184, kLoadRegs = 96, kIssueRegs = 48;
+constexpr int kTileLaunch = 128, kSoftRegs = 168, kLoadRegs = 128, kIssueRegs = 48;
 static_assert(2 * kSoftRegs + kLoadRegs + kIssueRegs == 4 * kTileLaunch, "register split must match the launch");
-constexpr float kTileTop = 9.0f;
-constexpr float kTileSum = 65000.0f;  // below the largest f16
 constexpr int kItems = 4;             // items in the planner's ring
 
 // What the roles need of an item, as the planner leaves it; rows = 0: no more.
@@ -47,10 +44,11 @@ struct TileCfg {
     static constexpr int K = 0, V = 2 * TILE;
     static constexpr int SCALES = 4 * TILE;                  // 4 x {keys' scales, values' ratios, valid tokens, unit}
     static constexpr int SLOT = 2 * kTileTokens * 4 + 32;
-    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][128]
-    static constexpr int SUMS = MAXIMA + 2 * 128 * 4;        // [2][128]
+    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][2][128]
+    static constexpr int SUMS = MAXIMA + 2 * 2 * 128 * 4;    // [2][128]
     static constexpr int TOPS = SUMS + 2 * 128 * 4;          // [2][4] of the loaders
-    static constexpr int ITEMS = TOPS + 32;
+    static constexpr int PLACES = TOPS + 32;                 // [8] of the loaders
+    static constexpr int ITEMS = PLACES + 64;
     static constexpr int BARS = ITEMS + kItems * 64;
     static constexpr int SMEM = BARS + 256 + 1024;
     static constexpr uint32_t S_COL = 0, O_COL = 256, Q_COL = 384;
@@ -144,6 +142,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // As split2, for a pair.
 __device__ __forceinline__ void split_pair(uint64_t w, uint32_t& high, uint32_t& low) {
     asm("{\n\t.reg .b16 x, y;\n\t.reg .f32 a, b, u, v;\n\t.reg .b64 h, d;\n\t"
@@ -167,7 +170,7 @@ __device__ __forceinline__ void split_pair(uint64_t w, uint32_t& high, uint32_t&
 template <bool CARE>
 __device__ __forceinline__ void tile_chunk(const uint32_t (&v)[32], const ulonglong2* ks, const ulonglong2* vs, float m, uint64_t rf, uint32_t seen,
                                            uint32_t* high, uint32_t* low, uint64_t* sum) {
-    const uint64_t top = pair_of(kTileTop, kTileTop), minus_m = pair_of(-m, -m);
+    const uint64_t top = pair_of(kTop, kTop), minus_m = pair_of(-m, -m);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const ulonglong2 kk = ks[k], vv = vs[k];
@@ -362,7 +365,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 if (row < it.rows) {
                     const int r = it.first_row + row;
                     const float k = l == 0.0f ? 0.0f : 0x1p16f / l;  // (units are kept 2^-16 of theirs: no sum of theirs overflows)
-                    const float top = m == -INFINITY ? kNone : fmaf(m, rf, -kTileTop);
+                    const float top = m == -INFINITY ? kNone : fmaf(m, rf, -kTop);
                     float* dst;
                     bool vec = true;
                     if (it.whole) {
@@ -405,7 +408,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < HD / 2; ++k) o[k] = 0;
             m = -INFINITY, l = 0.0f, fade = 1.0f, unit = 0.0f;
-            bool wild = __any_sync(0xffffffffu, !(rf >= 0x1p-126f));  // a row's logits want the careful form
+            const bool wild = !(rf >= 0x1p-126f);  // a row's logits want the careful form
 #pragma unroll 1
             for (int j = 0; j < it.n; ++j, ++t) {
                 const uint8_t* slot = smem + C::SCALES + (t & 3) * C::SLOT;
@@ -427,61 +430,60 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 warp_wait(&s_full[t & 1], t >> 1 & 1, ab, 33);
                 tc_fence_after();
                 const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 64 * half;
-                uint32_t h[32], lo[32];
-                float step = 1.0f, mine;
+                // the rows' maxima, of both halves
+                float x = -INFINITY;
 #pragma unroll 1
-                for (int again = 0;; ++again) {
-                    const float ref = m == -INFINITY ? 0.0f : m;
-                    uint64_t sum = 0;
-                    const bool care = wild || more.y == 0.0f;
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(sc + 32 * c, v);
+                    float y = -INFINITY, z = -INFINITY;
+                    const uint32_t seen = c ? seen1 : seen0;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(sc + 32 * c, v);
-                        if (care) {
-                            tile_chunk<true>(v, ks + 8 * c, vs + 8 * c, ref, rf2, c ? seen1 : seen0, h + 16 * c, lo + 16 * c, &sum);
-                        } else {
-                            if (edge) {
+                    for (int k = 0; k < 8; ++k) {
+                        const ulonglong2 kk = ks[8 * c + k];
+                        float p[4];
+                        unpair(mul2(pair_of(v[4 * k], v[4 * k + 1]), kk.x), p[0], p[1]);
+                        unpair(mul2(pair_of(v[4 * k + 2], v[4 * k + 3]), kk.y), p[2], p[3]);
+                        if (edge) {
 #pragma unroll
-                                for (int k = 0; k < 32; ++k)
-                                    if (!((c ? seen1 : seen0) >> k & 1)) v[k] = 0xff800000u;
-                            }
-                            tile_chunk<false>(v, ks + 8 * c, vs + 8 * c, ref, rf2, 0u, h + 16 * c, lo + 16 * c, &sum);
+                            for (int q = 0; q < 4; ++q) p[q] = seen >> (4 * k + q) & 1 ? p[q] : -INFINITY;
                         }
+                        y = max3(y, p[0], p[1]), z = max3(z, p[2], p[3]);
                     }
-                    float x, y;
-                    unpair(sum, x, y);
-                    mine = x + y;
-                    if (again || !bar_any(pair, 64, !(mine < kTileSum) || (m == -INFINITY && (seen0 | seen1)))) break;
-                    // the rows' maxima of the tile, of both halves
-                    x = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(sc + 32 * c, v);
-                        const uint32_t seen = c ? seen1 : seen0;
-                        const float* kf = (const float*)(ks + 8 * c);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            y = __fmul_rn(__uint_as_float(v[k]), kf[k]);
-                            if (seen >> k & 1) x = fmaxf(x, y);
-                        }
-                    }
-                    maxima[half * 128 + row] = x;
-                    bar_named(pair, 64);
-                    x = fmaxf(x, maxima[(half ^ 1) * 128 + row]);
-                    if (x > m) {
-                        step = m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
-                        m = x;
-                        l *= step;
-                    }
-                    wild = wild || __any_sync(0xffffffffu, fabsf(m * rf) > 0x1p14f);
+                    x = max3(x, y, z);
                 }
-                l += mine;
-                tmem_st16(sc, h);
-                tmem_st16(sc + 16, lo);
-                tmem_st16(sc + 32, h + 16);
-                tmem_st16(sc + 48, lo + 16);
+                maxima[((t & 1) * 2 + half) * 128 + row] = x;
+                bar_named(pair, 64);
+                x = fmaxf(x, maxima[((t & 1) * 2 + (half ^ 1)) * 128 + row]);
+                float step = 1.0f;
+                if (x > m) {
+                    step = m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
+                    m = x;
+                    l *= step;
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;
+                const bool care = __any_sync(0xffffffffu, wild || more.y == 0.0f || !(fabsf(ref * rf) <= 0x1p14f));
+                uint64_t sum = 0;
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t v[32], h[16], lo[16];
+                    tmem_ld32(sc + 32 * c, v);
+                    const uint32_t seen = c ? seen1 : seen0;
+                    if (care) {
+                        tile_chunk<true>(v, ks + 8 * c, vs + 8 * c, ref, rf2, seen, h, lo, &sum);
+                    } else {
+                        if (edge) {
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) v[k] = seen >> k & 1 ? v[k] : 0xff800000u;
+                        }
+                        tile_chunk<false>(v, ks + 8 * c, vs + 8 * c, ref, rf2, 0u, h, lo, &sum);
+                    }
+                    tmem_st16(sc + 32 * c, h);
+                    tmem_st16(sc + 32 * c + 16, lo);
+                }
+                float y;
+                unpair(sum, x, y);
+                l += x + y;
                 tmem_st_done();
                 tc_fence_before();
                 mbar_arrive(&p_full[t & 1]);
@@ -493,14 +495,16 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         constexpr int CH = DP / 16, PER = kTileTokens * CH / 128;  // pieces of 16 bytes of a row, and of a thread
         constexpr int STEP = 128 / CH;                             // rows between a thread's pieces
-        const int tid = threadIdx.x - 256, r0 = tid / CH, ch = tid % CH, lw = warp - 8;
+        // Eight lanes that store 16 bytes each have four pieces of two neighbouring rows, whose places in the swizzle differ by one:
+        // no two have the same banks.
+        const int tid = threadIdx.x - 256, lw = warp - 8;
+        const int ch = CH == 8 ? (lane & 3) | (lane >> 1 & 4) : lane & 3;
+        const int r0 = CH == 8 ? 4 * lw + (lane >> 2 & 1) + (lane >> 3 & 2) : 8 * lw + (lane >> 2);
         uint32_t* tops = (uint32_t*)(smem + C::TOPS);
-        // the two pieces of f16 that 16 bytes of e4m3 become; that of the other parity first where another lane of the row
-        // stores the same banks
-        const int odd = ch >> 2 & 1;
+        int64_t* places = (int64_t*)(smem + C::PLACES);
         const uint32_t piece = (uint32_t)(ch >> 2) * (kTileTokens * 128) + r0 * 128;
-        uint8_t* at0 = smem + piece + ((2 * (ch & 3) + odd) ^ (r0 & 7)) * 16;
-        uint8_t* at1 = smem + piece + ((2 * (ch & 3) + 1 - odd) ^ (r0 & 7)) * 16;
+        uint8_t* at0 = smem + piece + ((2 * (ch & 3)) ^ (r0 & 7)) * 16;
+        uint8_t* at1 = smem + piece + ((2 * (ch & 3) + 1) ^ (r0 & 7)) * 16;
         static_assert(STEP % 8 == 0, "a thread's rows have one place in the swizzle");
         if (a.stall) warp_wait(&k_empty[0], 0, ab, 34);  // a test of the bounded waits: nothing completes this phase
         auto put = [&](uint32_t tile, const uint4 (&x)[PER]) {
@@ -509,8 +513,8 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 const uint4 v = x[k];
                 const uint4 lo = make_uint4(f16_of_e4m3(v.x), f16_of_e4m3(v.x >> 16), f16_of_e4m3(v.y), f16_of_e4m3(v.y >> 16));
                 const uint4 hi = make_uint4(f16_of_e4m3(v.z), f16_of_e4m3(v.z >> 16), f16_of_e4m3(v.w), f16_of_e4m3(v.w >> 16));
-                *(uint4*)(at0 + tile + k * (STEP * 128)) = odd ? hi : lo;
-                *(uint4*)(at1 + tile + k * (STEP * 128)) = odd ? lo : hi;
+                *(uint4*)(at0 + tile + k * (STEP * 128)) = lo;
+                *(uint4*)(at1 + tile + k * (STEP * 128)) = hi;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
@@ -520,19 +524,22 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         TileItem it = {};
         int j = -1;          // the tile of the item that the registers are filled for
         int page = -1;       // lane g & 7: the page of group g (16 tokens) of the tile after
-        int64_t slot0 = -1;  // the group's first slot in the cache's arrays, or -1, of the tile
+        uint32_t rows = 0;   // of the thread's pieces, those that exist
+        bool some = false;   // not all of the warp's do
         auto look = [&](int x) {
             const int at = it.first + kTileTokens * x + 16 * (lane & 7);
             page = x < it.n && at < it.high ? a.table[(int64_t)it.seq * a.table_s1 + (at >> a.page_log)] : -1;
         };
+        // (a piece that does not exist is read from the cache's first slot and cleared)
+        const int64_t own = (int64_t)(r0 & 15) * a.dim + (16 * ch < a.dim ? 16 * ch : 0);
         auto fetch = [&](const uint8_t* from, uint4 (&to)[PER]) {
-            const int tok = it.first + kTileTokens * j + r0;
-            from += (int64_t)(r0 & 15) * a.dim + 16 * ch;
+            from += own;
 #pragma unroll
-            for (int k = 0; k < PER; ++k) {
-                const int64_t s = __shfl_sync(0xffffffffu, slot0, (STEP * k + r0) >> 4);
-                const bool there = s >= 0 && tok + STEP * k >= it.low && tok + STEP * k < it.high && 16 * ch < a.dim;
-                to[k] = there ? __ldg((const uint4*)(from + s * a.dim)) : make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < PER; ++k) to[k] = __ldg((const uint4*)(from + places[(STEP * k + r0) >> 4]));
+            if (some) {
+#pragma unroll
+                for (int k = 0; k < PER; ++k)
+                    if (!(rows >> k & 1)) to[k] = make_uint4(0, 0, 0, 0);
             }
         };
         // Tile t goes from registers to shared memory, each half followed by the loads of the next tile's, which may be another
@@ -575,14 +582,29 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 look(0);
             }
             if (more) {
-                const int at = it.first + kTileTokens * j + 16 * (lane & 7);
-                slot0 = (uint32_t)page < (uint32_t)a.pages ? ((((int64_t)page * a.heads) + it.head) << a.page_log) + (at & ((1 << a.page_log) - 1)) : (int64_t)-1;
+                const int tok = it.first + kTileTokens * j;
+                const bool exists = (uint32_t)page < (uint32_t)a.pages;
+                const int at = tok + 16 * (lane & 7);
+                const int64_t slot0 = exists ? ((((int64_t)page * a.heads) + it.head) << a.page_log) + (at & ((1 << a.page_log) - 1)) : (int64_t)0;
+                bar_named(5, 128);  // (the last tile's places have been read)
+                if (lw == 0 && lane < 8) places[lane] = slot0 * a.dim;
+                const uint32_t groups = __ballot_sync(0xffffffffu, exists) & 0xffu;
+                const int64_t s = __shfl_sync(0xffffffffu, slot0, tid >> 4) + (tid & 15);
+                in = (groups >> (tid >> 4) & 1) && tok + tid >= it.low && tok + tid < it.high;
+                ks = __ldg(a.ks + s), vs = __ldg(a.vs + s);
+                if (!in) ks = vs = 0.0f;
+                some = groups != 0xffu || tok < it.low || tok + kTileTokens > it.high || a.dim != DP;
+                if (some) {
+                    rows = 0;
+#pragma unroll
+                    for (int k = 0; k < PER; ++k) {
+                        const int r = STEP * k + r0;
+                        rows |= (uint32_t)((groups >> (r >> 4) & 1) && tok + r >= it.low && tok + r < it.high && 16 * ch < a.dim) << k;
+                    }
+                }
                 look(j + 1);
+                bar_named(5, 128);
                 fetch(a.k, kv);
-                const int tok = it.first + kTileTokens * j + tid;
-                const int64_t s = __shfl_sync(0xffffffffu, slot0, tid >> 4);
-                in = s >= 0 && tok >= it.low && tok < it.high;
-                ks = in ? __ldg(a.ks + s + (tid & 15)) : 0.0f, vs = in ? __ldg(a.vs + s + (tid & 15)) : 0.0f;
             }
             if (have) {
                 warp_wait(&v_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 35);
