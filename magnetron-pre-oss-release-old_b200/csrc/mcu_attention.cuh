@@ -43,6 +43,12 @@ __device__ __forceinline__ float2 lds64(uint32_t a) {
     asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ float4 load4(const float* p, int vec) {
     if (vec) return *(const float4*)p;
     return make_float4(p[0], p[1], p[2], p[3]);
@@ -173,7 +179,7 @@ struct Share {
     // Fills sh[0 .. SEQS) with the units of sequences from `first`; returns this thread's sum of its run of them, its
     // exclusive prefix and the sum of all.
     __device__ void chunk(const AttnArgs& a, int first, int64_t* sh, int64_t& mine, int64_t& before, int64_t& all) const {
-        constexpr int RUN = SEQS / THREADS;
+        constexpr int RUN = (SEQS + THREADS - 1) / THREADS;
         int64_t* warps = sh + SEQS;
         const int n = min(SEQS, a.seqs - first), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         __syncthreads();
@@ -207,7 +213,7 @@ struct Share {
     }
     // Finds the block's first item; false when the block has no work.  sh: SMEM bytes of shared memory.
     __device__ bool find(const AttnArgs& a, int64_t* sh) {
-        constexpr int RUN = SEQS / THREADS;
+        constexpr int RUN = (SEQS + THREADS - 1) / THREADS;
         int64_t* found = sh + SEQS + 32;
         int64_t mine = 0, before = 0, all = 0;
         if (threadIdx.x == 0) *(int*)slot(a, 0) = *(int*)slot(a, 1) = 0;

@@ -16,16 +16,17 @@ using namespace mcu;
 // two operands' shared-memory reads: 2 x 128 columns of S, over which P is written in place, 128 of O, 128 of Q.  O starts
 // from zero for every 128 tokens and is added in registers in f32 (rounded to nearest), times the step of the row's reference and
 // the unit of the tile's value scales: no accumulator is ever rescaled, and the tensor core's truncating sums stay short.
-//   warps 0-7    softmax: warp w has the rows 32 (w & 3) .. and half w / 4 of the tokens and of the output's columns
-//   warps 8-11   loaders: e4m3 from the pages through registers to f16 tiles (128-byte swizzle), scales, valid tokens
-//   warp 12      issues the products: S of tile j + 1 before O of tile j, so that softmax runs under them
-//   warp 13      plans: puts the block's items into a ring, so that the others find theirs without global loads
-// A tile's logits are read twice, for the rows' maxima and for the probabilities, in loops of 32 columns that are not unrolled:
-// the loops of all roles have to fit the SM's instruction cache together (unrolled, with the probabilities formed in one pass
-// against a reference that moved when it had to, a third of its requests missed and a tile took three times as long).
-constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 512;
-constexpr int kTileLaunch = 128, kSoftRegs = 168, kLoadRegs = 128, kIssueRegs = 48;
-static_assert(2 * kSoftRegs + kLoadRegs + kIssueRegs == 4 * kTileLaunch, "register split must match the launch");
+//   warps 0-15   softmax: warp w has the rows 32 (w & 3) .. and quarter w / 4 of the tokens and of the output's columns
+//   warps 16-19  loaders: e4m3 from the pages by cp.async, two tiles ahead, then to f16 tiles (128-byte swizzle)
+//   warp 20      issues the products: S of tile j + 1 before O of tile j, so that softmax runs under them
+//   warp 21      plans: puts the block's items into a ring, so that the others find theirs without global loads
+// What bounds it is the softmax's instructions, about 13 for two logits, not the products (2 x 1024 cycles a tile): four warps a
+// scheduler hide its latencies (two took 1.36 ms for the prompts below, unrolled for all columns 2.2 ms: the loops of all roles have to
+// fit the SM's instruction cache together).
+constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 768;
+constexpr int kTileLaunch = 80, kSoftRegs = 96, kLoadRegs = 56, kIssueRegs = 40;
+static_assert(4 * kSoftRegs + kLoadRegs + kIssueRegs == 6 * kTileLaunch, "register split must match the launch");
+constexpr int kSoftWarps = 16, kSoftThreads = 32 * kSoftWarps;
 constexpr int kItems = 4;             // items in the planner's ring
 
 // What the roles need of an item, as the planner leaves it; rows = 0: no more.
@@ -42,17 +43,20 @@ struct TileCfg {
     static constexpr int BLOCKS = DP / 64;                   // column blocks of 64 f16
     static constexpr int TILE = BLOCKS * kTileTokens * 128;  // bytes of a K or V tile
     static constexpr int K = 0, V = 2 * TILE;
-    static constexpr int SCALES = 4 * TILE;                  // 4 x {keys' scales, values' ratios, valid tokens, unit}
+    static constexpr int RAW = 4 * TILE;                     // [2] of keys, then values, as loaded: each thread's own pieces
+    static constexpr int RAW_TILE = TILE / 2;
+    static constexpr int RAW_SCALES = RAW + 4 * RAW_TILE;    // [2][2][128]
+    static constexpr int SCALES = RAW_SCALES + 2 * 2 * kTileTokens * 4;  // 4 x {keys' scales, values' ratios, valid tokens, unit}
     static constexpr int SLOT = 2 * kTileTokens * 4 + 32;
-    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][2][128]
-    static constexpr int SUMS = MAXIMA + 2 * 2 * 128 * 4;    // [2][128]
-    static constexpr int TOPS = SUMS + 2 * 128 * 4;          // [2][4] of the loaders
+    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][4][128]
+    static constexpr int SUMS = MAXIMA + 2 * 4 * 128 * 4;    // [4][128]
+    static constexpr int TOPS = SUMS + 4 * 128 * 4;          // [2][4] of the loaders
     static constexpr int PLACES = TOPS + 32;                 // [8] of the loaders
     static constexpr int ITEMS = PLACES + 64;
     static constexpr int BARS = ITEMS + kItems * 64;
     static constexpr int SMEM = BARS + 256 + 1024;
     static constexpr uint32_t S_COL = 0, O_COL = 256, Q_COL = 384;
-    static_assert(Share<kTileRows, DP, kTileThreads>::SMEM <= SCALES, "the search for work takes the tiles' room");
+    static_assert(Share<kTileRows, DP, kTileThreads>::SMEM <= RAW, "the search for work takes the tiles' room");
     static_assert(SMEM <= 227 * 1024, "must fit shared memory");
 };
 
@@ -61,9 +65,10 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// The whole warp waits, polled by one lane.  The __syncwarp holds the other lanes back: a shuffle whose result is not
-// used does not.
+// The whole warp waits: looks once together, then one lane polls.  (The __syncwarp holds the other lanes back; a shuffle
+// whose result is not used does not.)
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
+    if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
     uint32_t ok = 1;
     if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, ab, code);
     __syncwarp();
@@ -108,6 +113,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
         "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
         "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+          "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -162,45 +180,6 @@ __device__ __forceinline__ void split_pair(uint64_t w, uint32_t& high, uint32_t&
         : "l"(w));
 }
 
-// 32 columns of S to probabilities times their values' ratios, as f16 halves; *sum gains the probabilities.  Tokens that are
-// not to be seen have come as -inf.
-// CARE: for scales that are no numbers and for logits that are large.  Tokens whose bit in `seen` is not set have no part,
-// whatever their scales are, and a logit is rounded before the reference is taken from it, so that the two are equal where they
-// should be (unrounded they differ by up to 2^-24 of the logit: of no account while that is small).
-template <bool CARE>
-__device__ __forceinline__ void tile_chunk(const uint32_t (&v)[32], const ulonglong2* ks, const ulonglong2* vs, float m, uint64_t rf, uint32_t seen,
-                                           uint32_t* high, uint32_t* low, uint64_t* sum) {
-    const uint64_t top = pair_of(kTop, kTop), minus_m = pair_of(-m, -m);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const ulonglong2 kk = ks[k], vv = vs[k];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int e = 4 * k + 2 * h;
-            const uint64_t kp = h ? kk.y : kk.x, vp = h ? vv.y : vv.x;
-            float x, y;
-            uint64_t t;
-            if (CARE) {  // (one by one: packed, the compiler joins the two roundings)
-                unpair(kp, x, y);
-                t = pair_of(__fadd_rn(__fmul_rn(__uint_as_float(v[e]), x), -m), __fadd_rn(__fmul_rn(__uint_as_float(v[e + 1]), y), -m));
-            } else {
-                t = fma2(pair_of(v[e], v[e + 1]), kp, minus_m);
-            }
-            unpair(fma2(t, rf, top), x, y);
-            x = exp2_f(x), y = exp2_f(y);
-            if (CARE) x = seen >> e & 1 ? x : 0.0f, y = seen >> (e + 1) & 1 ? y : 0.0f;
-            const uint64_t p = pair_of(x, y);
-            *sum = add2(*sum, p);
-            uint64_t w = mul2(p, vp);
-            if (CARE) {
-                unpair(w, x, y);
-                w = pair_of(seen >> e & 1 ? x : 0.0f, seen >> (e + 1) & 1 ? y : 0.0f);
-            }
-            split_pair(w, high[2 * k + h], low[2 * k + h]);
-        }
-    }
-}
-
 template <int DP>
 __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     using C = TileCfg<DP>;
@@ -230,21 +209,21 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             mbar_init(&v_full[i], 128);
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 256);
+            mbar_init(&p_full[i], kSoftThreads);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&sc_full[i], 128);
         for (int i = 0; i < kItems; ++i) {
             mbar_init(&i_full[i], 1);
-            mbar_init(&i_free[i], 13);  // a lane of each softmax and loader warp and of the issuer
+            mbar_init(&i_free[i], kSoftWarps + 5);  // a lane of each softmax and loader warp and of the issuer
         }
         mbar_init(o_full, 1);
-        mbar_init(o_free, 256);
-        mbar_init(q_full, 256);
+        mbar_init(o_free, kSoftThreads);
+        mbar_init(q_full, kSoftThreads);
         mbar_init(drain, 1);
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 20) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -279,43 +258,42 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
 
     if (!work) {
         // nothing to do but to free TMEM
-    } else if (warp < 8) {  // ---- softmax
+    } else if (warp < kSoftWarps) {  // ---- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-        constexpr int HD = DP / 2;  // this thread's columns of the output and values of a query
-        const int half = warp >> 2, row = 32 * (warp & 3) + lane, pair = 1 + (warp & 3);
+        constexpr int QD = DP / 4;  // this thread's columns of the output and values of a query
+        const int quarter = warp >> 2, row = 32 * (warp & 3) + lane, group = 1 + (warp & 3);
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        float* maxima = (float*)(smem + C::MAXIMA);
+        float* maxima = (float*)(smem + C::MAXIMA);  // the four warps of a row meet here
         float* sums = (float*)(smem + C::SUMS);
         uint32_t t = 0;  // tiles done
-        // The item at hand: its rows' reference and sum, output, the factor that takes S to log2 units.
+        // The item at hand: its rows' maximum and sum, output, the factor that takes S to log2 units.
         TileItem it = {};
-        uint64_t o[HD / 2];
+        uint64_t o[QD / 2];
         float m = -INFINITY, l = 0.0f, rf = 0.0f, fade = 1.0f, unit = 0.0f;
         // O of the last tile joins the sums: waits for it, and hands the columns back
         auto add_tile = [&](uint32_t x) {
             if (__any_sync(0xffffffffu, fade != 1.0f)) {
                 const uint64_t f = pair_of(fade, fade);
 #pragma unroll
-                for (int k = 0; k < HD / 2; ++k) o[k] = mul2(o[k], f);
+                for (int k = 0; k < QD / 2; ++k) o[k] = mul2(o[k], f);
             }
             const uint64_t u = pair_of(unit, unit);
             warp_wait(o_full, x & 1, ab, 31);
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                uint32_t v[32];
-                tmem_ld32(tmem + lanes + C::O_COL + HD * half + 32 * c, v);
-                if (c == HD / 32 - 1) {
-                    tc_fence_before();
-                    mbar_arrive(o_free);
-                }
-#pragma unroll
-                for (int k = 0; k < 16; ++k) o[16 * c + k] = fma2(pair_of(v[2 * k], v[2 * k + 1]), u, o[16 * c + k]);
+            uint32_t v[QD];
+            if constexpr (QD == 32) {
+                tmem_ld32(tmem + lanes + C::O_COL + QD * quarter, v);
+            } else {
+                tmem_ld16(tmem + lanes + C::O_COL + QD * quarter, v);
             }
+            tc_fence_before();
+            mbar_arrive(o_free);
+#pragma unroll
+            for (int k = 0; k < QD / 2; ++k) o[k] = fma2(pair_of(v[2 * k], v[2 * k + 1]), u, o[k]);
         };
 #pragma unroll 1
         for (uint32_t i = 0;; ++i) {
-            const TileItem next = item(i, pair, 64);
+            const TileItem next = item(i, group, 128);
             float next_rf = 0.0f;
             if (next.rows && next.n) {
                 // the next item's queries, as two f16 in TMEM (the products that read the last item's are done: their S was
@@ -323,60 +301,64 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 const int r = next.first_row + row;
                 const bool live = row < next.rows;
                 const float* p = a.q + (int64_t)(next.row0 + (live ? r / a.group : 0)) * a.q_s1 +
-                                 (int64_t)(next.head * a.group + (live ? r % a.group : 0)) * a.dim + HD * half;
-                float x[HD];
+                                 (int64_t)(next.head * a.group + (live ? r % a.group : 0)) * a.dim + QD * quarter;
+                float x[QD];
                 uint32_t top = 0;
                 if (a.q_vec) {
 #pragma unroll
-                    for (int k = 0; k < HD / 4; ++k) {
-                        const float4 v = live && HD * half + 4 * k < a.dim ? *(const float4*)(p + 4 * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int k = 0; k < QD / 4; ++k) {
+                        const float4 v = live && QD * quarter + 4 * k < a.dim ? *(const float4*)(p + 4 * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
                     }
                 } else {
 #pragma unroll
-                    for (int k = 0; k < HD; ++k) x[k] = live && HD * half + k < a.dim ? p[k] : 0.0f;
+                    for (int k = 0; k < QD; ++k) x[k] = live && QD * quarter + k < a.dim ? p[k] : 0.0f;
                 }
 #pragma unroll
-                for (int k = 0; k < HD; ++k) top = max(top, abs_bits(x[k]));
-                sums[half * 128 + row] = __uint_as_float(top);
-                bar_named(pair, 64);
-                top = max(top, __float_as_uint(sums[(half ^ 1) * 128 + row]));
-                bar_named(pair, 64);
+                for (int k = 0; k < QD; ++k) top = max(top, abs_bits(x[k]));
+                sums[quarter * 128 + row] = __uint_as_float(top);
+                bar_named(group, 128);
+#pragma unroll
+                for (int k = 1; k < 4; ++k) top = max(top, __float_as_uint(sums[(quarter ^ k) * 128 + row]));
+                bar_named(group, 128);
                 const float up = query_unit(top);
+                uint32_t h[QD / 2], lo[QD / 2];
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    uint32_t h[16], lo[16];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) split2(x[32 * c + 2 * k] * up, x[32 * c + 2 * k + 1] * up, h[k], lo[k]);
-                    tmem_st16(tmem + lanes + C::Q_COL + HD / 2 * half + 16 * c, h);
-                    tmem_st16(tmem + lanes + C::Q_COL + DP / 2 + HD / 2 * half + 16 * c, lo);
+                for (int k = 0; k < QD / 2; ++k) split2(x[2 * k] * up, x[2 * k + 1] * up, h[k], lo[k]);
+                const uint32_t at = tmem + lanes + C::Q_COL + QD / 2 * quarter;
+                if constexpr (QD == 32) {
+                    tmem_st16(at, h);
+                    tmem_st16(at + DP / 2, lo);
+                } else {
+                    tmem_st8(at, h);
+                    tmem_st8(at + DP / 2, lo);
                 }
                 tmem_st_done();
                 tc_fence_before();
                 mbar_arrive(q_full);
-                next_rf = a.scale * kLog2e / up;
+                next_rf = fmaxf(a.scale * kLog2e / up, 0x1p-126f);  // (above zero, so that -inf times it is -inf)
             }
             if (it.rows) {  // the item at hand is complete but for its last tile's output
                 if (it.n) add_tile(t - 1);
-                sums[half * 128 + row] = l;
-                bar_named(pair, 64);
-                l += sums[(half ^ 1) * 128 + row];
-                bar_named(pair, 64);
+                sums[quarter * 128 + row] = l;
+                bar_named(group, 128);
+                l = (sums[row] + sums[128 + row]) + (sums[256 + row] + sums[384 + row]);
+                bar_named(group, 128);
                 if (row < it.rows) {
                     const int r = it.first_row + row;
                     const float k = l == 0.0f ? 0.0f : 0x1p16f / l;  // (units are kept 2^-16 of theirs: no sum of theirs overflows)
-                    const float top = m == -INFINITY ? kNone : fmaf(m, rf, -kTop);
+                    const float top = top_of(m, rf);
                     float* dst;
                     bool vec = true;
                     if (it.whole) {
                         const int head = it.head * a.group + r % a.group;
                         const int64_t token = it.row0 + r / a.group;
                         dst = a.out + token * a.out_s1 + (int64_t)head * a.dim, vec = a.out_vec;
-                        if (a.lse && half == 0) a.lse[token * a.heads * a.group + head] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
+                        if (a.lse && quarter == 0) a.lse[token * a.heads * a.group + head] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
                     } else {
                         float* p = part_slot(a, kTileRows, DP, blockIdx.x, it.begins);
                         dst = p + 8 + 2 * kTileRows + row * DP;
-                        if (half == 0) {
+                        if (quarter == 0) {
                             p[8 + 2 * row] = top, p[9 + 2 * row] = l;
                             if (row == 0 && it.begins) {
                                 int* w = (int*)p;
@@ -384,14 +366,14 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                             }
                         }
                     }
-                    dst += HD * half;
+                    dst += QD * quarter;
                     const uint64_t kk = pair_of(k, k);
 #pragma unroll
-                    for (int c = 0; c < HD / 4; ++c) {
+                    for (int c = 0; c < QD / 4; ++c) {
                         float4 v;
                         unpair(mul2(o[2 * c], kk), v.x, v.y);
                         unpair(mul2(o[2 * c + 1], kk), v.z, v.w);
-                        if (HD * half + 4 * c >= a.dim) continue;
+                        if (QD * quarter + 4 * c >= a.dim) continue;
                         if (vec) {
                             *(float4*)(dst + 4 * c) = v;
                         } else {
@@ -404,184 +386,180 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             it = next, rf = next_rf;
             const int last = row < it.rows ? it.pos + (it.first_row + row) / a.group : -1;
             const int first = a.window && last >= a.window ? last - a.window + 1 : 0;
-            const uint64_t rf2 = pair_of(rf, rf);
+            const uint64_t rf2 = pair_of(rf, rf), top2 = pair_of(kTop, kTop);
 #pragma unroll
-            for (int k = 0; k < HD / 2; ++k) o[k] = 0;
+            for (int k = 0; k < QD / 2; ++k) o[k] = 0;
             m = -INFINITY, l = 0.0f, fade = 1.0f, unit = 0.0f;
-            const bool wild = !(rf >= 0x1p-126f);  // a row's logits want the careful form
 #pragma unroll 1
             for (int j = 0; j < it.n; ++j, ++t) {
                 const uint8_t* slot = smem + C::SCALES + (t & 3) * C::SLOT;
-                const ulonglong2* ks = (const ulonglong2*)(slot + 64 * half * 4);
-                const ulonglong2* vs = (const ulonglong2*)(slot + (kTileTokens + 64 * half) * 4);
+                const ulonglong2* ks = (const ulonglong2*)(slot + 32 * quarter * 4);
+                const ulonglong2* vs = (const ulonglong2*)(slot + (kTileTokens + 32 * quarter) * 4);
                 warp_wait(&sc_full[t & 3], t >> 2 & 1, ab, 32);
                 const int j0 = it.first + kTileTokens * j;
                 const uint4 ok = *(const uint4*)(slot + 2 * kTileTokens * 4);
-                const float2 more = *(const float2*)(slot + 2 * kTileTokens * 4 + 16);  // unit, and 0 where a scale is no number
-                // not all tokens seen by all rows
-                const bool edge = j0 < it.all_first || j0 + kTileTokens - 1 > it.all_last || (ok.x & ok.y & ok.z & ok.w) != 0xffffffffu;
-                uint32_t seen0 = half ? ok.z : ok.x, seen1 = half ? ok.w : ok.y;
-                if (edge) {
-                    const int lo = first - j0 - 64 * half, hi = last - j0 - 64 * half;  // tokens lo .. hi of this half's
-                    const int a0 = max(lo, 0), b0 = min(hi, 31), a1 = max(lo - 32, 0), b1 = min(hi - 32, 31);
-                    seen0 &= a0 > b0 ? 0u : (0xffffffffu << a0) & (0xffffffffu >> (31 - b0));
-                    seen1 &= a1 > b1 ? 0u : (0xffffffffu << a1) & (0xffffffffu >> (31 - b1));
-                }
+                const float next_unit = *(const float*)(slot + 2 * kTileTokens * 4 + 16);
                 warp_wait(&s_full[t & 1], t >> 1 & 1, ab, 33);
                 tc_fence_after();
-                const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 64 * half;
-                // the rows' maxima, of both halves
-                float x = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(sc + 32 * c, v);
-                    float y = -INFINITY, z = -INFINITY;
-                    const uint32_t seen = c ? seen1 : seen0;
+                const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 32 * quarter;
+                uint32_t v[32];
+                tmem_ld32(sc, v);
+                uint64_t s[16];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const ulonglong2 kk = ks[8 * c + k];
-                        float p[4];
-                        unpair(mul2(pair_of(v[4 * k], v[4 * k + 1]), kk.x), p[0], p[1]);
-                        unpair(mul2(pair_of(v[4 * k + 2], v[4 * k + 3]), kk.y), p[2], p[3]);
-                        if (edge) {
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) p[q] = seen >> (4 * k + q) & 1 ? p[q] : -INFINITY;
-                        }
-                        y = max3(y, p[0], p[1]), z = max3(z, p[2], p[3]);
-                    }
-                    x = max3(x, y, z);
+                for (int k = 0; k < 8; ++k) {
+                    const ulonglong2 kk = ks[k];
+                    s[2 * k] = mul2(pair_of(v[4 * k], v[4 * k + 1]), kk.x);
+                    s[2 * k + 1] = mul2(pair_of(v[4 * k + 2], v[4 * k + 3]), kk.y);
                 }
-                maxima[((t & 1) * 2 + half) * 128 + row] = x;
-                bar_named(pair, 64);
-                x = fmaxf(x, maxima[((t & 1) * 2 + (half ^ 1)) * 128 + row]);
+                // not all tokens seen by all rows
+                if (j0 < it.all_first || j0 + kTileTokens - 1 > it.all_last || (ok.x & ok.y & ok.z & ok.w) != 0xffffffffu) {
+                    const int lo = max(first - j0 - 32 * quarter, 0), hi = min(last - j0 - 32 * quarter, 31);  // those of this quarter
+                    const uint32_t bits = quarter & 2 ? (quarter & 1 ? ok.w : ok.z) : (quarter & 1 ? ok.y : ok.x);
+                    const uint32_t seen = lo > hi ? 0u : bits & (0xffffffffu << lo) & (0xffffffffu >> (31 - hi));
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        float x, y;
+                        unpair(s[k], x, y);
+                        s[k] = pair_of(seen >> (2 * k) & 1 ? x : -INFINITY, seen >> (2 * k + 1) & 1 ? y : -INFINITY);
+                    }
+                }
+                // the rows' maxima
+                float x = -INFINITY, y = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                    float p, q;
+                    unpair(s[k], p, q);
+                    x = max3(x, p, q);
+                    unpair(s[k + 1], p, q);
+                    y = max3(y, p, q);
+                }
+                float* mine = maxima + (t & 1) * 512 + row;
+                mine[quarter * 128] = fmaxf(x, y);
+                bar_named(group, 128);
+                x = fmaxf(fmaxf(mine[0], mine[128]), fmaxf(mine[256], mine[384]));
                 float step = 1.0f;
                 if (x > m) {
                     step = m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
                     m = x;
                     l *= step;
                 }
-                const float ref = m == -INFINITY ? 0.0f : m;
-                const bool care = __any_sync(0xffffffffu, wild || more.y == 0.0f || !(fabsf(ref * rf) <= 0x1p14f));
+                const float ref = m == -INFINITY ? 0.0f : -m;
+                const uint64_t ref2 = pair_of(ref, ref);
                 uint64_t sum = 0;
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t v[32], h[16], lo[16];
-                    tmem_ld32(sc + 32 * c, v);
-                    const uint32_t seen = c ? seen1 : seen0;
-                    if (care) {
-                        tile_chunk<true>(v, ks + 8 * c, vs + 8 * c, ref, rf2, seen, h, lo, &sum);
-                    } else {
-                        if (edge) {
+                uint32_t h[16], lo[16];
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = seen >> k & 1 ? v[k] : 0xff800000u;
-                        }
-                        tile_chunk<false>(v, ks + 8 * c, vs + 8 * c, ref, rf2, 0u, h, lo, &sum);
+                for (int k = 0; k < 8; ++k) {
+                    const ulonglong2 vv = vs[k];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        unpair(fma2(add2(s[2 * k + q], ref2), rf2, top2), x, y);
+                        const uint64_t p = pair_of(exp2_f(x), exp2_f(y));
+                        sum = add2(sum, p);
+                        split_pair(mul2(p, q ? vv.y : vv.x), h[2 * k + q], lo[2 * k + q]);
                     }
-                    tmem_st16(sc + 32 * c, h);
-                    tmem_st16(sc + 32 * c + 16, lo);
                 }
-                float y;
+                tmem_st16(sc, h);
+                tmem_st16(sc + 16, lo);
                 unpair(sum, x, y);
                 l += x + y;
                 tmem_st_done();
                 tc_fence_before();
                 mbar_arrive(&p_full[t & 1]);
                 if (j) add_tile(t - 1);
-                fade = step, unit = more.x;
+                fade = step, unit = next_unit;
             }
         }
-    } else if (warp < 12) {  // ---- loaders
+    } else if (warp < kSoftWarps + 4) {  // ---- loaders
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         constexpr int CH = DP / 16, PER = kTileTokens * CH / 128;  // pieces of 16 bytes of a row, and of a thread
         constexpr int STEP = 128 / CH;                             // rows between a thread's pieces
         // Eight lanes that store 16 bytes each have four pieces of two neighbouring rows, whose places in the swizzle differ by one:
         // no two have the same banks.
-        const int tid = threadIdx.x - 256, lw = warp - 8;
+        const int tid = threadIdx.x - kSoftThreads, lw = warp - kSoftWarps;
         const int ch = CH == 8 ? (lane & 3) | (lane >> 1 & 4) : lane & 3;
         const int r0 = CH == 8 ? 4 * lw + (lane >> 2 & 1) + (lane >> 3 & 2) : 8 * lw + (lane >> 2);
         uint32_t* tops = (uint32_t*)(smem + C::TOPS);
         int64_t* places = (int64_t*)(smem + C::PLACES);
+        const uint32_t raw = smem_u32(smem + C::RAW) + tid * 16;
+        const uint32_t raw_scales = smem_u32(smem + C::RAW_SCALES) + tid * 4;
         const uint32_t piece = (uint32_t)(ch >> 2) * (kTileTokens * 128) + r0 * 128;
         uint8_t* at0 = smem + piece + ((2 * (ch & 3)) ^ (r0 & 7)) * 16;
         uint8_t* at1 = smem + piece + ((2 * (ch & 3) + 1) ^ (r0 & 7)) * 16;
         static_assert(STEP % 8 == 0, "a thread's rows have one place in the swizzle");
         if (a.stall) warp_wait(&k_empty[0], 0, ab, 34);  // a test of the bounded waits: nothing completes this phase
-        auto put = [&](uint32_t tile, const uint4 (&x)[PER]) {
-#pragma unroll
+        // a thread's pieces of keys (0) or values (1) of the tile in stage st: as they came, to f16
+        auto put = [&](int st, int which) {
+            asm volatile("cp.async.wait_group 3;" ::: "memory");
+            const uint8_t* from = smem + C::RAW + (2 * which + st) * C::RAW_TILE + tid * 16;
+            const uint32_t tile = (2 * which + st) * C::TILE;
+#pragma unroll 2
             for (int k = 0; k < PER; ++k) {
-                const uint4 v = x[k];
-                const uint4 lo = make_uint4(f16_of_e4m3(v.x), f16_of_e4m3(v.x >> 16), f16_of_e4m3(v.y), f16_of_e4m3(v.y >> 16));
-                const uint4 hi = make_uint4(f16_of_e4m3(v.z), f16_of_e4m3(v.z >> 16), f16_of_e4m3(v.w), f16_of_e4m3(v.w >> 16));
-                *(uint4*)(at0 + tile + k * (STEP * 128)) = lo;
-                *(uint4*)(at1 + tile + k * (STEP * 128)) = hi;
+                const uint4 v = *(const uint4*)(from + k * 2048);
+                *(uint4*)(at0 + tile + k * (STEP * 128)) =
+                    make_uint4(f16_of_e4m3(v.x), f16_of_e4m3(v.x >> 16), f16_of_e4m3(v.y), f16_of_e4m3(v.y >> 16));
+                *(uint4*)(at1 + tile + k * (STEP * 128)) =
+                    make_uint4(f16_of_e4m3(v.z), f16_of_e4m3(v.z >> 16), f16_of_e4m3(v.w), f16_of_e4m3(v.w >> 16));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
-        uint4 kv[PER], vv[PER];
-        float ks = 0.0f, vs = 0.0f;
-        bool in = false;
         TileItem it = {};
-        int j = -1;          // the tile of the item that the registers are filled for
-        int page = -1;       // lane g & 7: the page of group g (16 tokens) of the tile after
-        uint32_t rows = 0;   // of the thread's pieces, those that exist
-        bool some = false;   // not all of the warp's do
+        int j = -1;             // the tile of the item that is being loaded
+        int page = -1;          // lane g & 7: the page of group g (16 tokens) of the tile after
+        uint32_t rows = 0;      // of the thread's pieces, those that exist
+        uint32_t ins = 0;       // whether the thread's token exists, of the last tiles (bit 0: the last one loaded)
+        const int64_t own = (int64_t)(r0 & 15) * a.dim + (16 * ch < a.dim ? 16 * ch : 0);
         auto look = [&](int x) {
             const int at = it.first + kTileTokens * x + 16 * (lane & 7);
             page = x < it.n && at < it.high ? a.table[(int64_t)it.seq * a.table_s1 + (at >> a.page_log)] : -1;
         };
-        // (a piece that does not exist is read from the cache's first slot and cleared)
-        const int64_t own = (int64_t)(r0 & 15) * a.dim + (16 * ch < a.dim ? 16 * ch : 0);
-        auto fetch = [&](const uint8_t* from, uint4 (&to)[PER]) {
+        auto fetch = [&](const uint8_t* from, int st, int which) {
             from += own;
-#pragma unroll
-            for (int k = 0; k < PER; ++k) to[k] = __ldg((const uint4*)(from + places[(STEP * k + r0) >> 4]));
-            if (some) {
-#pragma unroll
-                for (int k = 0; k < PER; ++k)
-                    if (!(rows >> k & 1)) to[k] = make_uint4(0, 0, 0, 0);
-            }
+            const uint32_t to = raw + (2 * which + st) * C::RAW_TILE;
+#pragma unroll 2
+            for (int k = 0; k < PER; ++k) copy16(to + k * 2048, from + places[(STEP * k + r0) >> 4], rows >> k & 1);
         };
-        // Tile t goes from registers to shared memory, each half followed by the loads of the next tile's, which may be another
-        // item's.
-        bool have = false, more = true;
-        uint32_t items = 0;
+        // Two tiles are on their way while one goes to f16; the tiles of the block's items follow one another.
+        bool more = true;
+        uint32_t items = 0, left = 0;  // left: tiles on their way
 #pragma unroll 1
-        for (uint32_t t = 0; more || have;) {
+        for (uint32_t t = 0, x = 0; more || left; ++x) {  // x: the tile to load
+            const bool have = left == 2 || !more;  // tile t is to be put
             if (have) {
-                // scales: the unit is the least power of two above the tile's largest
-                const bool number = vs < kLargestScale;
-                float top = number ? vs : 0.0f;
-#pragma unroll
-                for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const uint32_t bits = __ballot_sync(0xffffffffu, in);
-                const bool bad = __any_sync(0xffffffffu, !number || !(fabsf(ks) < INFINITY));
-                if (lane == 0) tops[(t & 1) * 4 + lw] = abs_bits(top) | (bad ? 0x80000000u : 0u);
                 warp_wait(&k_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 34);
+                put((int)(t & 1), 0);
+                mbar_arrive(&k_full[t & 1]);
+                // scales: the unit is the least power of two above the tile's largest
+                const float* rs = (const float*)(smem + C::RAW_SCALES) + (t & 1) * 2 * kTileTokens + tid;
+                const bool in = ins >> (left - 1) & 1;
+                float ks = in ? rs[0] : 0.0f, vs = in ? rs[kTileTokens] : 0.0f;
+                if (!(vs < kLargestScale) || !(fabsf(ks) < INFINITY)) ks = __uint_as_float(0x7FFFFFFFu), vs = 0.0f;  // who sees it is lost
+                uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(vs));
+                const uint32_t bits = __ballot_sync(0xffffffffu, in);
+                if (lane == 0) tops[(t & 1) * 4 + lw] = top;
                 bar_named(5, 128);
                 const uint4 all = *(const uint4*)(tops + (t & 1) * 4);
-                const uint32_t largest = max(max(all.x & 0x7FFFFFFFu, all.y & 0x7FFFFFFFu), max(all.z & 0x7FFFFFFFu, all.w & 0x7FFFFFFFu));
-                const float unit = unit_above(fmaxf(__uint_as_float(largest), kLeastUnit));
+                const float unit = unit_above(fmaxf(__uint_as_float(max(max(all.x, all.y), max(all.z, all.w))), kLeastUnit));
                 float* slot = (float*)(smem + C::SCALES + (t & 3) * C::SLOT);
-                slot[tid] = ks == 0.0f ? 0x1p-126f : ks;  // (so that -inf times it is -inf)
+                slot[tid] = ks;
                 slot[kTileTokens + tid] = vs * (1.0f / unit);
                 if (lane == 0) slot[2 * kTileTokens + lw] = __uint_as_float(bits);
-                if (tid == 0) slot[2 * kTileTokens + 4] = unit * 0x1p-16f, slot[2 * kTileTokens + 5] = (all.x | all.y | all.z | all.w) >> 31 ? 0.0f : 1.0f;
+                if (tid == 0) slot[2 * kTileTokens + 4] = unit * 0x1p-16f;
                 mbar_arrive(&sc_full[t & 3]);
-                put(C::K + (t & 1) * C::TILE, kv);
-                mbar_arrive(&k_full[t & 1]);
             }
             // the next tile
-            ++j;
-            if (j >= it.n) {
-                do {
-                    it = item(items++, 5, 128);
-                } while (it.rows && !it.n);
-                more = it.rows != 0;
-                j = 0;
-                look(0);
-            }
             if (more) {
+                ++j;
+                if (j >= it.n) {
+                    do {
+                        it = item(items++, 5, 128);
+                    } while (it.rows && !it.n);
+                    more = it.rows != 0;
+                    j = 0;
+                    look(0);
+                }
+            }
+            const bool load = more;
+            if (load) {
                 const int tok = it.first + kTileTokens * j;
                 const bool exists = (uint32_t)page < (uint32_t)a.pages;
                 const int at = tok + 16 * (lane & 7);
@@ -590,34 +568,40 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 if (lw == 0 && lane < 8) places[lane] = slot0 * a.dim;
                 const uint32_t groups = __ballot_sync(0xffffffffu, exists) & 0xffu;
                 const int64_t s = __shfl_sync(0xffffffffu, slot0, tid >> 4) + (tid & 15);
-                in = (groups >> (tid >> 4) & 1) && tok + tid >= it.low && tok + tid < it.high;
-                ks = __ldg(a.ks + s), vs = __ldg(a.vs + s);
-                if (!in) ks = vs = 0.0f;
-                some = groups != 0xffu || tok < it.low || tok + kTileTokens > it.high || a.dim != DP;
-                if (some) {
-                    rows = 0;
+                const bool in = (groups >> (tid >> 4) & 1) && tok + tid >= it.low && tok + tid < it.high;
+                ins = ins << 1 | in;
+                const uint32_t to = raw_scales + (x & 1) * (2 * kTileTokens * 4);
+                copy4(to, a.ks + s);
+                copy4(to + kTileTokens * 4, a.vs + s);
+                rows = 16 * ch < a.dim ? 0xffu : 0u;
+                if (groups != 0xffu || tok < it.low || tok + kTileTokens > it.high) {
 #pragma unroll
                     for (int k = 0; k < PER; ++k) {
                         const int r = STEP * k + r0;
-                        rows |= (uint32_t)((groups >> (r >> 4) & 1) && tok + r >= it.low && tok + r < it.high && 16 * ch < a.dim) << k;
+                        if (!(groups >> (r >> 4) & 1) || tok + r < it.low || tok + r >= it.high) rows &= ~(1u << k);
                     }
                 }
                 look(j + 1);
                 bar_named(5, 128);
-                fetch(a.k, kv);
+                fetch(a.k, (int)(x & 1), 0);
             }
+            asm volatile("cp.async.commit_group;" ::: "memory");
             if (have) {
                 warp_wait(&v_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 35);
-                put(C::V + (t & 1) * C::TILE, vv);
+                put((int)(t & 1), 1);
                 mbar_arrive(&v_full[t & 1]);
-                ++t;
+                ++t, --left;
             }
-            if (more) fetch(a.v, vv);
-            have = more;
+            if (load) {
+                fetch(a.v, (int)(x & 1), 1);
+                ++left;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        if (warp == 12) {  // ---- issuer
+        if (warp == 20) {  // ---- issuer
             const int steps = a.dim / 16;
             const uint32_t is = idesc_f16(kTileTokens, 0), io = idesc_f16(a.dim, 1);
             const uint64_t k0 = tile_desc(smem_u32(smem + C::K), 16), v0 = tile_desc(smem_u32(smem + C::V), kTileTokens * 128);
@@ -668,7 +652,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             if (lane == 0)
                 for (uint32_t i = 0; i < kWaitLimit && !mbar_test(drain, 0); ++i) __nanosleep(64);
             __syncwarp();
-        } else if (warp == 13) {  // ---- planner
+        } else if (warp == 21) {  // ---- planner
             for (uint32_t i = 0;; ++i) {
                 TileItem p = {};
                 const bool more = sh.more();
@@ -697,7 +681,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 20) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
     }
