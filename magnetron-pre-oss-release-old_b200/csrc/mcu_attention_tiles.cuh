@@ -24,7 +24,7 @@ using namespace mcu;
 // scheduler hide its latencies (two took 1.36 ms for the prompts below, unrolled for all columns 2.2 ms: the loops of all roles have to
 // fit the SM's instruction cache together).
 constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 768;
-constexpr int kTileLaunch = 80, kSoftRegs = 96, kLoadRegs = 56, kIssueRegs = 40;
+constexpr int kTileLaunch = 80, kSoftRegs = 88, kLoadRegs = 80, kIssueRegs = 48;
 static_assert(4 * kSoftRegs + kLoadRegs + kIssueRegs == 6 * kTileLaunch, "register split must match the launch");
 constexpr int kSoftWarps = 16, kSoftThreads = 32 * kSoftWarps;
 constexpr int kItems = 4;             // items in the planner's ring
@@ -492,13 +492,15 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             asm volatile("cp.async.wait_group 3;" ::: "memory");
             const uint8_t* from = smem + C::RAW + (2 * which + st) * C::RAW_TILE + tid * 16;
             const uint32_t tile = (2 * which + st) * C::TILE;
-#pragma unroll 2
+            uint4 v[PER];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) v[k] = *(const uint4*)(from + k * 2048);
+#pragma unroll
             for (int k = 0; k < PER; ++k) {
-                const uint4 v = *(const uint4*)(from + k * 2048);
                 *(uint4*)(at0 + tile + k * (STEP * 128)) =
-                    make_uint4(f16_of_e4m3(v.x), f16_of_e4m3(v.x >> 16), f16_of_e4m3(v.y), f16_of_e4m3(v.y >> 16));
+                    make_uint4(f16_of_e4m3(v[k].x), f16_of_e4m3(v[k].x >> 16), f16_of_e4m3(v[k].y), f16_of_e4m3(v[k].y >> 16));
                 *(uint4*)(at1 + tile + k * (STEP * 128)) =
-                    make_uint4(f16_of_e4m3(v.z), f16_of_e4m3(v.z >> 16), f16_of_e4m3(v.w), f16_of_e4m3(v.w >> 16));
+                    make_uint4(f16_of_e4m3(v[k].z), f16_of_e4m3(v[k].z >> 16), f16_of_e4m3(v[k].w), f16_of_e4m3(v[k].w >> 16));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
@@ -515,8 +517,11 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         auto fetch = [&](const uint8_t* from, int st, int which) {
             from += own;
             const uint32_t to = raw + (2 * which + st) * C::RAW_TILE;
-#pragma unroll 2
-            for (int k = 0; k < PER; ++k) copy16(to + k * 2048, from + places[(STEP * k + r0) >> 4], rows >> k & 1);
+            const uint8_t* p[PER];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) p[k] = from + places[(STEP * k + r0) >> 4];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) copy16(to + k * 2048, p[k], rows >> k & 1);
         };
         // Two tiles are on their way while one goes to f16; the tiles of the block's items follow one another.
         bool more = true;
