@@ -16,17 +16,21 @@ using namespace mcu;
 // two operands' shared-memory reads: 2 x 128 columns of S, over which P is written in place, 128 of O, 128 of Q.  O starts
 // from zero for every 128 tokens and is added in registers in f32 (rounded to nearest), times the step of the row's reference and
 // the unit of the tile's value scales: no accumulator is ever rescaled, and the tensor core's truncating sums stay short.
-//   warps 0-15   softmax: warp w has the rows 32 (w & 3) .. and quarter w / 4 of the tokens and of the output's columns
-//   warps 16-19  loaders: e4m3 from the pages by cp.async, two tiles ahead, then to f16 tiles (128-byte swizzle)
-//   warp 20      issues the products: S of tile j + 1 before O of tile j, so that softmax runs under them
-//   warp 21      plans: puts the block's items into a ring, so that the others find theirs without global loads
-// What bounds it is the softmax's instructions, about 13 for two logits, not the products (2 x 1024 cycles a tile): four warps a
-// scheduler hide its latencies (two took 1.36 ms for the prompts below, unrolled for all columns 2.2 ms: the loops of all roles have to
-// fit the SM's instruction cache together).
-constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 768;
-constexpr int kTileLaunch = 80, kSoftRegs = 88, kLoadRegs = 80, kIssueRegs = 48;
-static_assert(4 * kSoftRegs + kLoadRegs + kIssueRegs == 6 * kTileLaunch, "register split must match the launch");
-constexpr int kSoftWarps = 16, kSoftThreads = 32 * kSoftWarps;
+//   warps 0-15   softmax: warp w has the rows 32 (w & 3) .. and quarter w / 4 of the tokens
+//   warps 16-19  sums: O of each tile, in turn, to the rows' f32 sums in registers; the output at the end
+//   warps 20-23  loaders: e4m3 from the pages by cp.async, two tiles ahead, then to f16 tiles (128-byte swizzle)
+//   warp 24      issues the products: S of tile j + 1 before O of tile j
+//   warp 25      plans: puts the block's items into a ring, so that the others find theirs without global loads
+//   warp 26      guides: each tile's places in the pages and its scales, up to four tiles ahead
+// What bounds it is the softmax: about 14 instructions for two logits (390 cycles for 32 x 32 of them with four warps a
+// scheduler, alone), more than the products' 2 x 1024 cycles a tile.  The loops of all roles have to fit the SM's instruction cache
+// together: unrolled for 128 columns they took three times as long.
+constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 896;
+constexpr int kSoftWarps = 16, kSumWarp = 16, kLoadWarp = 20, kIssueWarp = 24, kPlanWarp = 25, kGuideWarp = 26;
+constexpr int kTileLaunch = 72, kSoftRegs = 56, kSumRegs = 168, kLoadRegs = 64, kIssueRegs = 48;
+static_assert(4 * kSoftRegs + kSumRegs + kLoadRegs + kIssueRegs == 7 * kTileLaunch, "register split must match the launch");
+constexpr int kSoftThreads = 32 * kSoftWarps;
+constexpr uint32_t kGiveUp = 25000;   // sleeps of a wait, and the flag that ends all waits
 constexpr int kItems = 4;             // items in the planner's ring
 
 // What the roles need of an item, as the planner leaves it; rows = 0: no more.
@@ -45,16 +49,18 @@ struct TileCfg {
     static constexpr int K = 0, V = 2 * TILE;
     static constexpr int RAW = 4 * TILE;                     // [2] of keys, then values, as loaded: each thread's own pieces
     static constexpr int RAW_TILE = TILE / 2;
-    static constexpr int RAW_SCALES = RAW + 4 * RAW_TILE;    // [2][2][128]
-    static constexpr int SCALES = RAW_SCALES + 2 * 2 * kTileTokens * 4;  // 4 x {keys' scales, values' ratios, valid tokens, unit}
+    static constexpr int SCALES = RAW + 4 * RAW_TILE;        // 4 x {keys' scales, values' ratios, valid tokens, unit}
     static constexpr int SLOT = 2 * kTileTokens * 4 + 32;
-    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][4][128]
-    static constexpr int SUMS = MAXIMA + 2 * 4 * 128 * 4;    // [4][128]
-    static constexpr int TOPS = SUMS + 4 * 128 * 4;          // [2][4] of the loaders
-    static constexpr int PLACES = TOPS + 32;                 // [8] of the loaders
-    static constexpr int ITEMS = PLACES + 64;
+    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][4][128]: of a tile's logits, by quarter
+    static constexpr int SUMS = MAXIMA + 2 * 4 * 128 * 4;    // [4][128]: queries' maxima, by quarter
+    static constexpr int REFS = SUMS + 4 * 128 * 4;          // [4][128] of (maximum, unit): what a tile's O is relative to
+    static constexpr int FACTORS = REFS + 4 * 128 * 8;       // [4][128]: rf of an item's rows
+    static constexpr int STATS = FACTORS + 4 * 128 * 4;      // [4][128]: an item's sums, by quarter
+    static constexpr int PLACES = STATS + 4 * 128 * 4;   // 4 x {8 groups' offsets in the pages, valid tokens}
+    static constexpr int PLACE = 8 * 8 + 16;
+    static constexpr int ITEMS = PLACES + 4 * PLACE;
     static constexpr int BARS = ITEMS + kItems * 64;
-    static constexpr int SMEM = BARS + 256 + 1024;
+    static constexpr int SMEM = BARS + 512 + 1024;
     static constexpr uint32_t S_COL = 0, O_COL = 256, Q_COL = 384;
     static_assert(Share<kTileRows, DP, kTileThreads>::SMEM <= RAW, "the search for work takes the tiles' room");
     static_assert(SMEM <= 227 * 1024, "must fit shared memory");
@@ -65,14 +71,32 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// The whole warp waits: looks once together, then one lane polls.  (The __syncwarp holds the other lanes back; a shuffle
-// whose result is not used does not.)
+// The whole warp waits, asleep on the barrier for up to 20 us at a time and half a second in all, or until a wait was given up
+// elsewhere.  A loop of few instructions: it stands at some twenty places.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
-    if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
-    uint32_t ok = 1;
-    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, ab, code);
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .u32 n, f;\n\t"
+        "mov.u32 n, 0;\n\t"
+        "WAIT_%=:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "@p bra DONE_%=;\n\t"
+        "ld.volatile.shared.u32 f, [%3];\n\t"
+        "add.u32 n, n, 1;\n\t"
+        "add.u32 f, f, n;\n\t"
+        "setp.lt.u32 p, f, %5;\n\t"
+        "@p bra WAIT_%=;\n\t"
+        "DONE_%=:\n\t}\n"
+        : "=&r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32((const void*)ab.flag)), "r"(20000u), "r"(kGiveUp)
+        : "memory");
     __syncwarp();
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    if (!ok && (threadIdx.x & 31) == 0 && !*ab.flag) {
+        *ab.flag = (int)kGiveUp;
+        atomicCAS(ab.status, 0, code);
+    }
+    return __all_sync(0xffffffffu, ok);
 }
 __device__ __forceinline__ void bar_named(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // A barrier that also says whether any of its threads came with true.
@@ -198,7 +222,12 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     uint64_t* drain = q_full + 1;
     uint64_t* i_full = drain + 1;  // kItems each
     uint64_t* i_free = i_full + kItems;
-    uint32_t* tmem_slot = (uint32_t*)(i_free + kItems);
+    uint64_t* fin_full = i_free + kItems;
+    uint64_t* fin_free = fin_full + 1;
+    uint64_t* sc_free = fin_free + 1;  // four each
+    uint64_t* place_full = sc_free + 4;
+    uint64_t* place_free = place_full + 4;
+    uint32_t* tmem_slot = (uint32_t*)(place_free + 4);
     volatile int* gave_up = (volatile int*)(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const Abort ab{gave_up, a.status};
@@ -211,19 +240,26 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], kSoftThreads);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&sc_full[i], 128);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&sc_full[i], 32);
+            mbar_init(&sc_free[i], kSoftWarps);  // a lane of each warp that has read them
+            mbar_init(&place_full[i], 32);
+            mbar_init(&place_free[i], 4);
+        }
         for (int i = 0; i < kItems; ++i) {
             mbar_init(&i_full[i], 1);
-            mbar_init(&i_free[i], kSoftWarps + 5);  // a lane of each softmax and loader warp and of the issuer
+            mbar_init(&i_free[i], kSoftWarps + 6);  // a lane of each softmax and sums warp, of the issuer and the guide
         }
-        mbar_init(o_full, 1);
-        mbar_init(o_free, kSoftThreads);
+        mbar_init(o_full, 2);  // the products' completion, and the issuer's arrival, which hands on what it has seen of P
+        mbar_init(o_free, 128);
+        mbar_init(fin_full, kSoftThreads);
+        mbar_init(fin_free, 128);
         mbar_init(q_full, kSoftThreads);
         mbar_init(drain, 1);
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 20) {
+    if (warp == kIssueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -259,51 +295,26 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     if (!work) {
         // nothing to do but to free TMEM
     } else if (warp < kSoftWarps) {  // ---- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-        constexpr int QD = DP / 4;  // this thread's columns of the output and values of a query
-        const int quarter = warp >> 2, row = 32 * (warp & 3) + lane, group = 1 + (warp & 3);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+        constexpr int QD = DP / 4;  // this thread's values of a query
+        const int quarter = warp >> 2, row = 32 * (warp & 3) + lane, four = 1 + (warp & 3);  // barrier of a row's four warps
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        float* maxima = (float*)(smem + C::MAXIMA);  // the four warps of a row meet here
-        float* sums = (float*)(smem + C::SUMS);
-        uint32_t t = 0;  // tiles done
-        // The item at hand: its rows' maximum and sum, output, the factor that takes S to log2 units.
-        TileItem it = {};
-        uint64_t o[QD / 2];
-        float m = -INFINITY, l = 0.0f, rf = 0.0f, fade = 1.0f, unit = 0.0f;
-        // O of the last tile joins the sums: waits for it, and hands the columns back
-        auto add_tile = [&](uint32_t x) {
-            if (__any_sync(0xffffffffu, fade != 1.0f)) {
-                const uint64_t f = pair_of(fade, fade);
-#pragma unroll
-                for (int k = 0; k < QD / 2; ++k) o[k] = mul2(o[k], f);
-            }
-            const uint64_t u = pair_of(unit, unit);
-            warp_wait(o_full, x & 1, ab, 31);
-            tc_fence_after();
-            uint32_t v[QD];
-            if constexpr (QD == 32) {
-                tmem_ld32(tmem + lanes + C::O_COL + QD * quarter, v);
-            } else {
-                tmem_ld16(tmem + lanes + C::O_COL + QD * quarter, v);
-            }
-            tc_fence_before();
-            mbar_arrive(o_free);
-#pragma unroll
-            for (int k = 0; k < QD / 2; ++k) o[k] = fma2(pair_of(v[2 * k], v[2 * k + 1]), u, o[k]);
-        };
+        float* const maxima = (float*)(smem + C::MAXIMA) + row;
+        uint32_t t = 0;  // tiles before the item's
 #pragma unroll 1
         for (uint32_t i = 0;; ++i) {
-            const TileItem next = item(i, group, 128);
-            float next_rf = 0.0f;
-            if (next.rows && next.n) {
-                // the next item's queries, as two f16 in TMEM (the products that read the last item's are done: their S was
-                // waited for), before the last product of the item at hand is waited for
-                const int r = next.first_row + row;
-                const bool live = row < next.rows;
-                const float* p = a.q + (int64_t)(next.row0 + (live ? r / a.group : 0)) * a.q_s1 +
-                                 (int64_t)(next.head * a.group + (live ? r % a.group : 0)) * a.dim + QD * quarter;
-                float x[QD];
+            const TileItem it = item(i, four, 128);
+            if (!it.rows) break;
+            const int r = it.first_row + row;
+            const bool live = row < it.rows;
+            float rf = 0.0f;
+            if (it.n) {
+                // the queries, as two f16 in TMEM, once the products that read the last item's are done
+                const float* p = a.q + (int64_t)(it.row0 + (live ? r / a.group : 0)) * a.q_s1 +
+                                 (int64_t)(it.head * a.group + (live ? r % a.group : 0)) * a.dim + QD * quarter;
+                float* sums = (float*)(smem + C::SUMS) + row;
                 uint32_t top = 0;
+                float x[QD];
                 if (a.q_vec) {
 #pragma unroll
                     for (int k = 0; k < QD / 4; ++k) {
@@ -316,92 +327,45 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 }
 #pragma unroll
                 for (int k = 0; k < QD; ++k) top = max(top, abs_bits(x[k]));
-                sums[quarter * 128 + row] = __uint_as_float(top);
-                bar_named(group, 128);
+                sums[quarter * 128] = __uint_as_float(top);
+                bar_named(four, 128);
 #pragma unroll
-                for (int k = 1; k < 4; ++k) top = max(top, __float_as_uint(sums[(quarter ^ k) * 128 + row]));
-                bar_named(group, 128);
+                for (int k = 1; k < 4; ++k) top = max(top, __float_as_uint(sums[(quarter ^ k) * 128]));
+                bar_named(four, 128);
                 const float up = query_unit(top);
-                uint32_t h[QD / 2], lo[QD / 2];
-#pragma unroll
-                for (int k = 0; k < QD / 2; ++k) split2(x[2 * k] * up, x[2 * k + 1] * up, h[k], lo[k]);
+                if (t) {
+                    warp_wait(&s_full[(t - 1) & 1], (t - 1) >> 1 & 1, ab, 43);
+                    tc_fence_after();
+                }
                 const uint32_t at = tmem + lanes + C::Q_COL + QD / 2 * quarter;
-                if constexpr (QD == 32) {
-                    tmem_st16(at, h);
-                    tmem_st16(at + DP / 2, lo);
-                } else {
-                    tmem_st8(at, h);
-                    tmem_st8(at + DP / 2, lo);
+#pragma unroll
+                for (int c = 0; c < QD / 16; ++c) {
+                    uint32_t h[8], lo[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) split2(x[16 * c + 2 * k] * up, x[16 * c + 2 * k + 1] * up, h[k], lo[k]);
+                    tmem_st8(at + 8 * c, h);
+                    tmem_st8(at + DP / 2 + 8 * c, lo);
                 }
                 tmem_st_done();
+                rf = fmaxf(a.scale * kLog2e / up, 0x1p-126f);  // (above zero, so that -inf times it is -inf)
+                if (quarter == 0) ((float*)(smem + C::FACTORS))[(i & 3) * 128 + row] = rf;
                 tc_fence_before();
                 mbar_arrive(q_full);
-                next_rf = fmaxf(a.scale * kLog2e / up, 0x1p-126f);  // (above zero, so that -inf times it is -inf)
             }
-            if (it.rows) {  // the item at hand is complete but for its last tile's output
-                if (it.n) add_tile(t - 1);
-                sums[quarter * 128 + row] = l;
-                bar_named(group, 128);
-                l = (sums[row] + sums[128 + row]) + (sums[256 + row] + sums[384 + row]);
-                bar_named(group, 128);
-                if (row < it.rows) {
-                    const int r = it.first_row + row;
-                    const float k = l == 0.0f ? 0.0f : 0x1p16f / l;  // (units are kept 2^-16 of theirs: no sum of theirs overflows)
-                    const float top = top_of(m, rf);
-                    float* dst;
-                    bool vec = true;
-                    if (it.whole) {
-                        const int head = it.head * a.group + r % a.group;
-                        const int64_t token = it.row0 + r / a.group;
-                        dst = a.out + token * a.out_s1 + (int64_t)head * a.dim, vec = a.out_vec;
-                        if (a.lse && quarter == 0) a.lse[token * a.heads * a.group + head] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
-                    } else {
-                        float* p = part_slot(a, kTileRows, DP, blockIdx.x, it.begins);
-                        dst = p + 8 + 2 * kTileRows + row * DP;
-                        if (quarter == 0) {
-                            p[8 + 2 * row] = top, p[9 + 2 * row] = l;
-                            if (row == 0 && it.begins) {
-                                int* w = (int*)p;
-                                w[1] = it.head, w[2] = it.rows, w[3] = it.first_row, w[4] = it.row0, w[5] = it.last_block, w[0] = 1;
-                            }
-                        }
-                    }
-                    dst += QD * quarter;
-                    const uint64_t kk = pair_of(k, k);
-#pragma unroll
-                    for (int c = 0; c < QD / 4; ++c) {
-                        float4 v;
-                        unpair(mul2(o[2 * c], kk), v.x, v.y);
-                        unpair(mul2(o[2 * c + 1], kk), v.z, v.w);
-                        if (QD * quarter + 4 * c >= a.dim) continue;
-                        if (vec) {
-                            *(float4*)(dst + 4 * c) = v;
-                        } else {
-                            dst[4 * c] = v.x, dst[4 * c + 1] = v.y, dst[4 * c + 2] = v.z, dst[4 * c + 3] = v.w;
-                        }
-                    }
-                }
-            }
-            if (!next.rows) break;
-            it = next, rf = next_rf;
-            const int last = row < it.rows ? it.pos + (it.first_row + row) / a.group : -1;
-            const int first = a.window && last >= a.window ? last - a.window + 1 : 0;
+            const int last = live ? it.pos + r / a.group : -1, first = a.window && last >= a.window ? last - a.window + 1 : 0;
             const uint64_t rf2 = pair_of(rf, rf), top2 = pair_of(kTop, kTop);
-#pragma unroll
-            for (int k = 0; k < QD / 2; ++k) o[k] = 0;
-            m = -INFINITY, l = 0.0f, fade = 1.0f, unit = 0.0f;
+            float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
             for (int j = 0; j < it.n; ++j, ++t) {
                 const uint8_t* slot = smem + C::SCALES + (t & 3) * C::SLOT;
                 const ulonglong2* ks = (const ulonglong2*)(slot + 32 * quarter * 4);
                 const ulonglong2* vs = (const ulonglong2*)(slot + (kTileTokens + 32 * quarter) * 4);
-                warp_wait(&sc_full[t & 3], t >> 2 & 1, ab, 32);
+                const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 32 * quarter;
                 const int j0 = it.first + kTileTokens * j;
+                warp_wait(&sc_full[t & 3], t >> 2 & 1, ab, 32);
                 const uint4 ok = *(const uint4*)(slot + 2 * kTileTokens * 4);
-                const float next_unit = *(const float*)(slot + 2 * kTileTokens * 4 + 16);
                 warp_wait(&s_full[t & 1], t >> 1 & 1, ab, 33);
                 tc_fence_after();
-                const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 32 * quarter;
                 uint32_t v[32];
                 tmem_ld32(sc, v);
                 uint64_t s[16];
@@ -433,16 +397,15 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                     unpair(s[k + 1], p, q);
                     y = max3(y, p, q);
                 }
-                float* mine = maxima + (t & 1) * 512 + row;
+                float* mine = maxima + (t & 1) * 512;
                 mine[quarter * 128] = fmaxf(x, y);
-                bar_named(group, 128);
-                x = fmaxf(fmaxf(mine[0], mine[128]), fmaxf(mine[256], mine[384]));
-                float step = 1.0f;
+                bar_named(four, 128);
+                x = fmaxf(max3(mine[0], mine[128], mine[256]), mine[384]);
                 if (x > m) {
-                    step = m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
+                    l *= m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
                     m = x;
-                    l *= step;
                 }
+                if (quarter == 0) ((float2*)(smem + C::REFS))[(t & 3) * 128 + row] = make_float2(m, *(const float*)(slot + 2 * kTileTokens * 4 + 16));
                 const float ref = m == -INFINITY ? 0.0f : -m;
                 const uint64_t ref2 = pair_of(ref, ref);
                 uint64_t sum = 0;
@@ -465,23 +428,101 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 tmem_st_done();
                 tc_fence_before();
                 mbar_arrive(&p_full[t & 1]);
-                if (j) add_tile(t - 1);
-                fade = step, unit = next_unit;
+                if (lane == 0) mbar_arrive(&sc_free[t & 3]);
+            }
+            // the rows' sums, once the last item's have been read
+            warp_wait(fin_free, (i & 1) ^ 1, ab, 44);
+            ((float*)(smem + C::STATS))[quarter * 128 + row] = l;
+            mbar_arrive(fin_full);
+        }
+    } else if (warp < kLoadWarp) {  // ---- sums
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
+        const int row = 32 * (warp & 3) + lane;
+        const uint32_t oc = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + C::O_COL;
+        uint32_t t = 0;
+#pragma unroll 1
+        for (uint32_t i = 0;; ++i) {
+            const TileItem it = item(i, 0, 0);
+            if (!it.rows) break;
+            uint64_t o[DP / 2];
+#pragma unroll
+            for (int k = 0; k < DP / 2; ++k) o[k] = 0;
+            float ref = -INFINITY, rf = 0.0f;
+#pragma unroll 1
+            for (int j = 0; j < it.n; ++j, ++t) {
+                warp_wait(o_full, t & 1, ab, 31);
+                tc_fence_after();
+                rf = ((const float*)(smem + C::FACTORS))[(i & 3) * 128 + row];
+                const float2 mu = ((const float2*)(smem + C::REFS))[(t & 3) * 128 + row];
+                const float fade = ref == mu.x ? 1.0f : ref == -INFINITY ? 0.0f : exp2_f((ref - mu.x) * rf);
+                ref = mu.x;
+                if (__any_sync(0xffffffffu, fade != 1.0f)) {
+                    const uint64_t f = pair_of(fade, fade);
+#pragma unroll
+                    for (int k = 0; k < DP / 2; ++k) o[k] = mul2(o[k], f);
+                }
+                const uint64_t g = pair_of(mu.y, mu.y);
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) {
+                    uint32_t v[16];
+                    tmem_ld16(oc + 16 * c, v);
+                    if (c == DP / 16 - 1) {
+                        tc_fence_before();
+                        mbar_arrive(o_free);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) o[8 * c + k] = fma2(pair_of(v[2 * k], v[2 * k + 1]), g, o[8 * c + k]);
+                }
+            }
+            warp_wait(fin_full, i & 1, ab, 45);
+            const float* stats = (const float*)(smem + C::STATS) + row;
+            const float l = (stats[0] + stats[128]) + (stats[256] + stats[384]);
+            mbar_arrive(fin_free);
+            if (row < it.rows) {
+                const int r = it.first_row + row;
+                const float k = l == 0.0f ? 0.0f : 0x1p16f / l;  // (units are kept 2^-16 of theirs: no sum of theirs overflows)
+                const float top = top_of(ref, rf);
+                float* dst;
+                bool vec = true;
+                if (it.whole) {
+                    const int head = it.head * a.group + r % a.group;
+                    const int64_t token = it.row0 + r / a.group;
+                    dst = a.out + token * a.out_s1 + (int64_t)head * a.dim, vec = a.out_vec;
+                    if (a.lse) a.lse[token * a.heads * a.group + head] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
+                } else {
+                    float* p = part_slot(a, kTileRows, DP, blockIdx.x, it.begins);
+                    dst = p + 8 + 2 * kTileRows + row * DP;
+                    p[8 + 2 * row] = top, p[9 + 2 * row] = l;
+                    if (row == 0 && it.begins) {
+                        int* w = (int*)p;
+                        w[1] = it.head, w[2] = it.rows, w[3] = it.first_row, w[4] = it.row0, w[5] = it.last_block, w[0] = 1;
+                    }
+                }
+                const uint64_t kk = pair_of(k, k);
+#pragma unroll
+                for (int c = 0; c < DP / 4; ++c) {
+                    float4 v;
+                    unpair(mul2(o[2 * c], kk), v.x, v.y);
+                    unpair(mul2(o[2 * c + 1], kk), v.z, v.w);
+                    if (4 * c >= a.dim) continue;
+                    if (vec) {
+                        *(float4*)(dst + 4 * c) = v;
+                    } else {
+                        dst[4 * c] = v.x, dst[4 * c + 1] = v.y, dst[4 * c + 2] = v.z, dst[4 * c + 3] = v.w;
+                    }
+                }
             }
         }
-    } else if (warp < kSoftWarps + 4) {  // ---- loaders
+    } else if (warp < kIssueWarp) {  // ---- loaders
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         constexpr int CH = DP / 16, PER = kTileTokens * CH / 128;  // pieces of 16 bytes of a row, and of a thread
         constexpr int STEP = 128 / CH;                             // rows between a thread's pieces
         // Eight lanes that store 16 bytes each have four pieces of two neighbouring rows, whose places in the swizzle differ by one:
         // no two have the same banks.
-        const int tid = threadIdx.x - kSoftThreads, lw = warp - kSoftWarps;
+        const int tid = threadIdx.x - 32 * kLoadWarp, lw = warp - kLoadWarp;
         const int ch = CH == 8 ? (lane & 3) | (lane >> 1 & 4) : lane & 3;
         const int r0 = CH == 8 ? 4 * lw + (lane >> 2 & 1) + (lane >> 3 & 2) : 8 * lw + (lane >> 2);
-        uint32_t* tops = (uint32_t*)(smem + C::TOPS);
-        int64_t* places = (int64_t*)(smem + C::PLACES);
         const uint32_t raw = smem_u32(smem + C::RAW) + tid * 16;
-        const uint32_t raw_scales = smem_u32(smem + C::RAW_SCALES) + tid * 4;
         const uint32_t piece = (uint32_t)(ch >> 2) * (kTileTokens * 128) + r0 * 128;
         uint8_t* at0 = smem + piece + ((2 * (ch & 3)) ^ (r0 & 7)) * 16;
         uint8_t* at1 = smem + piece + ((2 * (ch & 3) + 1) ^ (r0 & 7)) * 16;
@@ -504,17 +545,9 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
-        TileItem it = {};
-        int j = -1;             // the tile of the item that is being loaded
-        int page = -1;          // lane g & 7: the page of group g (16 tokens) of the tile after
-        uint32_t rows = 0;      // of the thread's pieces, those that exist
-        uint32_t ins = 0;       // whether the thread's token exists, of the last tiles (bit 0: the last one loaded)
         const int64_t own = (int64_t)(r0 & 15) * a.dim + (16 * ch < a.dim ? 16 * ch : 0);
-        auto look = [&](int x) {
-            const int at = it.first + kTileTokens * x + 16 * (lane & 7);
-            page = x < it.n && at < it.high ? a.table[(int64_t)it.seq * a.table_s1 + (at >> a.page_log)] : -1;
-        };
-        auto fetch = [&](const uint8_t* from, int st, int which) {
+        uint32_t rows = 0;  // of the thread's pieces, those that exist
+        auto fetch = [&](const uint8_t* from, const int64_t* places, int st, int which) {
             from += own;
             const uint32_t to = raw + (2 * which + st) * C::RAW_TILE;
             const uint8_t* p[PER];
@@ -523,90 +556,48 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < PER; ++k) copy16(to + k * 2048, p[k], rows >> k & 1);
         };
-        // Two tiles are on their way while one goes to f16; the tiles of the block's items follow one another.
-        bool more = true;
-        uint32_t items = 0, left = 0;  // left: tiles on their way
+        // Two tiles are on their way while one goes to f16, keys and values in turn; the tiles of the block's items follow one another
+        // as the guide has them.
+        uint32_t left = 0;  // tiles on their way
+        bool more = true, have = false;
 #pragma unroll 1
-        for (uint32_t t = 0, x = 0; more || left; ++x) {  // x: the tile to load
-            const bool have = left == 2 || !more;  // tile t is to be put
+        for (uint32_t t = 0, x = 0, which = 0; more || left; which ^= 1) {  // t: the tile to put, x: to load
+            uint64_t* full = k_full + 4 * which;  // (k_full, k_empty, v_full, v_empty)
+            if (which == 0) have = left == 2 || !more;
             if (have) {
-                warp_wait(&k_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 34);
-                put((int)(t & 1), 0);
-                mbar_arrive(&k_full[t & 1]);
-                // scales: the unit is the least power of two above the tile's largest
-                const float* rs = (const float*)(smem + C::RAW_SCALES) + (t & 1) * 2 * kTileTokens + tid;
-                const bool in = ins >> (left - 1) & 1;
-                float ks = in ? rs[0] : 0.0f, vs = in ? rs[kTileTokens] : 0.0f;
-                if (!(vs < kLargestScale) || !(fabsf(ks) < INFINITY)) ks = __uint_as_float(0x7FFFFFFFu), vs = 0.0f;  // who sees it is lost
-                uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(vs));
-                const uint32_t bits = __ballot_sync(0xffffffffu, in);
-                if (lane == 0) tops[(t & 1) * 4 + lw] = top;
-                bar_named(5, 128);
-                const uint4 all = *(const uint4*)(tops + (t & 1) * 4);
-                const float unit = unit_above(fmaxf(__uint_as_float(max(max(all.x, all.y), max(all.z, all.w))), kLeastUnit));
-                float* slot = (float*)(smem + C::SCALES + (t & 3) * C::SLOT);
-                slot[tid] = ks;
-                slot[kTileTokens + tid] = vs * (1.0f / unit);
-                if (lane == 0) slot[2 * kTileTokens + lw] = __uint_as_float(bits);
-                if (tid == 0) slot[2 * kTileTokens + 4] = unit * 0x1p-16f;
-                mbar_arrive(&sc_full[t & 3]);
+                warp_wait(full + 2 + (t & 1), (t >> 1 & 1) ^ 1, ab, 34);
+                put((int)(t & 1), (int)which);
+                mbar_arrive(full + (t & 1));
+                if (which) ++t, --left;
             }
-            // the next tile
-            if (more) {
-                ++j;
-                if (j >= it.n) {
-                    do {
-                        it = item(items++, 5, 128);
-                    } while (it.rows && !it.n);
-                    more = it.rows != 0;
-                    j = 0;
-                    look(0);
-                }
-            }
-            const bool load = more;
-            if (load) {
-                const int tok = it.first + kTileTokens * j;
-                const bool exists = (uint32_t)page < (uint32_t)a.pages;
-                const int at = tok + 16 * (lane & 7);
-                const int64_t slot0 = exists ? ((((int64_t)page * a.heads) + it.head) << a.page_log) + (at & ((1 << a.page_log) - 1)) : (int64_t)0;
-                bar_named(5, 128);  // (the last tile's places have been read)
-                if (lw == 0 && lane < 8) places[lane] = slot0 * a.dim;
-                const uint32_t groups = __ballot_sync(0xffffffffu, exists) & 0xffu;
-                const int64_t s = __shfl_sync(0xffffffffu, slot0, tid >> 4) + (tid & 15);
-                const bool in = (groups >> (tid >> 4) & 1) && tok + tid >= it.low && tok + tid < it.high;
-                ins = ins << 1 | in;
-                const uint32_t to = raw_scales + (x & 1) * (2 * kTileTokens * 4);
-                copy4(to, a.ks + s);
-                copy4(to + kTileTokens * 4, a.vs + s);
-                rows = 16 * ch < a.dim ? 0xffu : 0u;
-                if (groups != 0xffu || tok < it.low || tok + kTileTokens > it.high) {
+            const int64_t* places = (const int64_t*)(smem + C::PLACES + (x & 3) * C::PLACE);
+            if (which == 0 && more) {
+                const bool found = warp_wait(&place_full[x & 3], x >> 2 & 1, ab, 46) && places[0] >= 0;
+                more = __all_sync(0xffffffffu, found);
+                const uint4 ok = *(const uint4*)(places + 8);
+                rows = 0xffu;
+                if ((ok.x & ok.y & ok.z & ok.w) != 0xffffffffu) {
+                    rows = 0;
 #pragma unroll
-                    for (int k = 0; k < PER; ++k) {
-                        const int r = STEP * k + r0;
-                        if (!(groups >> (r >> 4) & 1) || tok + r < it.low || tok + r >= it.high) rows &= ~(1u << k);
-                    }
+                    for (int k = 0; k < PER; ++k) rows |= (((const uint32_t*)(places + 8))[(STEP * k + r0) >> 5] >> ((STEP * k + r0) & 31) & 1) << k;
                 }
-                look(j + 1);
-                bar_named(5, 128);
-                fetch(a.k, (int)(x & 1), 0);
+                if (16 * ch >= a.dim) rows = 0;
             }
+            if (more) fetch(which ? a.v : a.k, places, (int)(x & 1), (int)which);
             asm volatile("cp.async.commit_group;" ::: "memory");
-            if (have) {
-                warp_wait(&v_empty[t & 1], (t >> 1 & 1) ^ 1, ab, 35);
-                put((int)(t & 1), 1);
-                mbar_arrive(&v_full[t & 1]);
-                ++t, --left;
+            if (which) {
+                if (more) {
+                    ++left;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&place_free[x & 3]);
+                }
+                ++x;
             }
-            if (load) {
-                fetch(a.v, (int)(x & 1), 1);
-                ++left;
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        if (warp == 20) {  // ---- issuer
+        if (warp == kIssueWarp) {  // ---- issuer
             const int steps = a.dim / 16;
             const uint32_t is = idesc_f16(kTileTokens, 0), io = idesc_f16(a.dim, 1);
             const uint64_t k0 = tile_desc(smem_u32(smem + C::K), 16), v0 = tile_desc(smem_u32(smem + C::V), kTileTokens * 128);
@@ -618,7 +609,9 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 if (ok && elect_one()) {
                     const uint32_t d = tmem + C::S_COL + 128 * (x & 1);
                     const uint64_t b = k0 + (uint64_t)((x & 1) * (C::TILE >> 4));
+#pragma unroll 1
                     for (int h = 0; h < 2; ++h)
+#pragma unroll 1
                         for (int s = 0; s < steps; ++s)
                             umma_ts(d, tmem + C::Q_COL + h * (DP / 2) + 8 * s, b + (s >> 2) * ((kTileTokens * 128) >> 4) + (s & 3) * 2, is, h + s);
                     umma_commit(&s_full[x & 1]);
@@ -642,11 +635,14 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                     if (ok && elect_one()) {
                         const uint32_t p = tmem + C::S_COL + 128 * (t & 1);
                         const uint64_t b = v0 + (uint64_t)((t & 1) * (C::TILE >> 4));
+#pragma unroll 1
                         for (int h = 0; h < 2; ++h)
+#pragma unroll 1
                             for (int s = 0; s < 8; ++s)
                                 umma_ts(tmem + C::O_COL, p + 32 * (s >> 1) + 8 * (s & 1) + 16 * h, b + s * (2048 >> 4), io, h + s);
                         umma_commit(&v_empty[t & 1]);
                         umma_commit(o_full);
+                        mbar_arrive(o_full);
                     }
                     __syncwarp();
                 }
@@ -657,7 +653,64 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             if (lane == 0)
                 for (uint32_t i = 0; i < kWaitLimit && !mbar_test(drain, 0); ++i) __nanosleep(64);
             __syncwarp();
-        } else if (warp == 21) {  // ---- planner
+        } else if (warp == kGuideWarp) {  // ---- guide: lane l has the tokens 4 l .. 4 l + 3 of a tile, of group l / 4
+            float4 ks = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vs = ks;
+            uint32_t in = 0;  // which of the lane's four tokens exist, of the tile whose scales are on their way
+            bool pending = false;
+            uint32_t x = 0;   // the tile
+            // the scales of tile x - 1: the unit is the least power of two above the tile's largest
+            auto finish = [&]() {
+                const uint32_t y = x - 1;
+                warp_wait(&sc_free[y & 3], (y >> 2 & 1) ^ 1, ab, 47);
+                float k[4] = {ks.x, ks.y, ks.z, ks.w}, v[4] = {vs.x, vs.y, vs.z, vs.w};
+                uint32_t top = 0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (!(in >> q & 1)) k[q] = v[q] = 0.0f;
+                    if (!(v[q] < kLargestScale) || !(fabsf(k[q]) < INFINITY)) k[q] = __uint_as_float(0x7FFFFFFFu), v[q] = 0.0f;  // who sees it is lost
+                    top = max(top, abs_bits(v[q]));
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                const float unit = unit_above(fmaxf(__uint_as_float(top), kLeastUnit)), per = 1.0f / unit;
+                uint8_t* slot = smem + C::SCALES + (y & 3) * C::SLOT;
+                ((float4*)slot)[lane] = make_float4(k[0], k[1], k[2], k[3]);
+                ((float4*)(slot + kTileTokens * 4))[lane] = make_float4(v[0] * per, v[1] * per, v[2] * per, v[3] * per);
+                uint32_t bits = in << 4 * (lane & 7);
+                bits = __reduce_or_sync(0xffu << (lane & 24), bits);
+                if ((lane & 7) == 0) ((uint32_t*)(slot + 2 * kTileTokens * 4))[lane >> 3] = bits;
+                if (lane == 0) ((float*)(slot + 2 * kTileTokens * 4))[4] = unit * 0x1p-16f;
+                mbar_arrive(&sc_full[y & 3]);
+            };
+#pragma unroll 1
+            for (uint32_t i = 0;; ++i) {
+                const TileItem it = item(i, 0, 0);
+                const int32_t* table = a.table + (int64_t)it.seq * a.table_s1;
+                int tok = it.first + 4 * lane, page = it.rows && it.n && (tok & ~15) < it.high ? table[tok >> a.page_log] : -1;
+#pragma unroll 1
+                for (int j = 0; j < (it.rows ? it.n : 1); ++j, ++x) {
+                    const bool exists = (uint32_t)page < (uint32_t)a.pages;
+                    const int64_t s = exists ? ((((int64_t)page * a.heads) + it.head) << a.page_log) + (tok & ((1 << a.page_log) - 1)) : (int64_t)(4 * (lane & 3));
+                    uint32_t now = 0;
+                    if (exists)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) now |= (uint32_t)(tok + q >= it.low && tok + q < it.high) << q;
+                    if (j + 1 < it.n) page = ((tok + kTileTokens) & ~15) < it.high ? table[(tok + kTileTokens) >> a.page_log] : -1;
+                    if (!warp_wait(&place_free[x & 3], (x >> 2 & 1) ^ 1, ab, 48)) break;
+                    int64_t* places = (int64_t*)(smem + C::PLACES + (x & 3) * C::PLACE);
+                    if ((lane & 3) == 0) places[lane >> 2] = it.rows ? s * a.dim : (int64_t)-1;  // (below zero: no more tiles)
+                    const uint32_t bits = __reduce_or_sync(0xffu << (lane & 24), now << 4 * (lane & 7));
+                    if ((lane & 7) == 0) ((uint32_t*)(places + 8))[lane >> 3] = bits;
+                    mbar_arrive(&place_full[x & 3]);
+                    if (pending) finish();
+                    pending = it.rows != 0;
+                    if (!pending) break;
+                    ks = *(const float4*)(a.ks + s), vs = *(const float4*)(a.vs + s);
+                    in = now;
+                    tok += kTileTokens;
+                }
+                if (!it.rows || *gave_up) break;
+            }
+        } else if (warp == kPlanWarp) {  // ---- planner
             for (uint32_t i = 0;; ++i) {
                 TileItem p = {};
                 const bool more = sh.more();
@@ -686,7 +739,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 20) {
+    if (warp == kIssueWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
     }
