@@ -14,7 +14,7 @@ namespace {
 // l + LANES v of four values each, v < V.  All of a norm's and a rotation's exchange is then shuffles within the group.
 // Groups of 16 lanes hold heads of up to 64 values, two to a warp.
 constexpr int kHeadThreads = 256, kHeadWarps = 8;
-constexpr int kMaxPairs = 128;
+constexpr int kMaxPairs = 128;  // of a token
 
 template <int LANES>
 __device__ __forceinline__ float group_sum(float v) {
@@ -65,11 +65,18 @@ struct Turn {
     float mag;
 };
 
-// This lane's factors of one token's turn, from the token's cosines and sines: y = x c + partner s.
+// A warp serves one token at a time.  It forms the token's cosines and sines in shared memory of its own (cs, then sn), and each
+// lane keeps the factors of its values: y = x c + partner s.  All lanes take part.
 template <int LANES, int V>
-__device__ __forceinline__ void turn_factors(float (&c)[4 * V], float (&s)[4 * V], const float* cs, const float* sn, const Turn& t, int l,
-                                             bool back) {
-    const float sign = back ? -1.0f : 1.0f;
+__device__ __forceinline__ void turn_factors(float (&c)[4 * V], float (&s)[4 * V], float* cs, const Turn& t, int64_t row, int l, bool back) {
+    float* sn = cs + kMaxPairs;
+    const int lane = threadIdx.x & 31, pos = t.pos[row];
+    __syncwarp();  // (the last token's have been read)
+    for (int i = lane; i < t.rot / 2; i += 32) {
+        const float2 v = turn_of(pos, t.freq[i], t.mag);
+        cs[i] = v.x, sn[i] = back ? -v.y : v.y;
+    }
+    __syncwarp();
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int d = 4 * (l + LANES * v);
@@ -77,11 +84,11 @@ __device__ __forceinline__ void turn_factors(float (&c)[4 * V], float (&s)[4 * V
         if (t.pairs) {
             const float2 a = *(const float2*)(cs + d / 2), b = *(const float2*)(sn + d / 2);
             c[4 * v] = c[4 * v + 1] = a.x, c[4 * v + 2] = c[4 * v + 3] = a.y;
-            s[4 * v] = -sign * b.x, s[4 * v + 1] = sign * b.x, s[4 * v + 2] = -sign * b.y, s[4 * v + 3] = sign * b.y;
+            s[4 * v] = -b.x, s[4 * v + 1] = b.x, s[4 * v + 2] = -b.y, s[4 * v + 3] = b.y;
         } else {
             const int half = t.rot / 2, p = d < half ? d : d - half;
             const float4 a = *(const float4*)(cs + p), b = *(const float4*)(sn + p);
-            const float g = d < half ? -sign : sign;
+            const float g = d < half ? -1.0f : 1.0f;
             c[4 * v] = a.x, c[4 * v + 1] = a.y, c[4 * v + 2] = a.z, c[4 * v + 3] = a.w;
             s[4 * v] = g * b.x, s[4 * v + 1] = g * b.y, s[4 * v + 2] = g * b.z, s[4 * v + 3] = g * b.w;
         }
@@ -118,12 +125,32 @@ __device__ __forceinline__ void turn(float (&x)[4 * V], const float (&c)[4 * V],
         }
 }
 
+template <int LANES, int V, bool VEC>
+__device__ __forceinline__ void load_row(float (&x)[4 * V], const float* p, int l, int dim) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int d = 4 * (l + LANES * v);
+        float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p && d < dim) t = load4<VEC>(p + d);
+        x[4 * v] = t.x, x[4 * v + 1] = t.y, x[4 * v + 2] = t.z, x[4 * v + 3] = t.w;
+    }
+}
+template <int LANES, int V, bool VEC>
+__device__ __forceinline__ void store_row(float* p, const float (&x)[4 * V], int l, int dim) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int d = 4 * (l + LANES * v);
+        if (d < dim) store4<VEC>(p + d, make_float4(x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]));
+    }
+}
+
 // ------------------------------------------------------------ forward and cache write
 //
-// One block serves one token (blockIdx.x) and up to 8 warps x U head rows of each group: first the loads of all of them,
-// then the token's cosines and sines, once for the block, under the loads' latency, then the rows.  Query rows go out in
-// f32, key and value rows as e4m3 with their scale.
-// What bounds it: HBM, one read and one write of each value.
+// A warp takes a token and up to `rows_a_warp` of its head rows, U a group at a time.  Query rows go out in f32, key and value
+// rows as e4m3 with their scale.
+// What bounds it: instructions and HBM, one read and one write of each value.  The token's angles cost about two head rows' work, so
+// that a warp serves 16 of them where there are enough warps; blocks that share a token's angles took longer (8191 x 32 x 128: 66 us
+// with a token a block, of whose threads a quarter formed the angles; 82 with four tokens; 105 persistent).
 struct HeadArgs {
     const float *q, *k, *v, *q_w, *k_w;
     float *q_out, *rstd;
@@ -131,184 +158,130 @@ struct HeadArgs {
     float *ks, *vs;
     const int32_t* slot;
     Turn turn;
-    float eps;
+    float eps, inv_dim;
     int dim, q_heads, heads, page_log, slots;  // heads: of keys and of values, 0 without a cache
-    int64_t q_s1, k_s1, v_s1, out_s1;
+    int rows_a_warp, shares;                   // head rows of a warp, and the warps that share a token
+    int64_t rows, q_s1, k_s1, v_s1, out_s1;
 };
+constexpr int kForwardWarps = 4;
 
 template <int LANES, int V, int U, bool VEC>
-__global__ void __launch_bounds__(kHeadThreads) heads_forward(HeadArgs a) {
-    __shared__ __align__(16) float cs[kMaxPairs], sn[kMaxPairs];
-    constexpr int GROUPS = kHeadWarps * 32 / LANES;
-    const int l = threadIdx.x & (LANES - 1), group = threadIdx.x / LANES;
-    const int64_t row = blockIdx.x;
-    const int jobs = a.q_heads + 2 * a.heads;
+__global__ void __launch_bounds__(32 * kForwardWarps) heads_forward(HeadArgs a) {
+    __shared__ __align__(16) float turns[kForwardWarps][2 * kMaxPairs];
+    constexpr int GROUPS = 32 / LANES;
+    const int l = threadIdx.x & (LANES - 1), group = (threadIdx.x & 31) / LANES, warp = threadIdx.x >> 5;
+    const int64_t item = (int64_t)blockIdx.x * kForwardWarps + warp, row = item / a.shares;
     pdl_begin();
-    float x[U][4 * V];
-    int job[U];
+    if (row >= a.rows) return;
+    const int jobs = a.q_heads + 2 * a.heads, j0 = (int)(item - row * a.shares) * a.rows_a_warp, j1 = min(j0 + a.rows_a_warp, jobs);
+    const float *q = a.q + row * a.q_s1, *k = a.k + row * a.k_s1, *v = a.v + row * a.v_s1;
+    auto from = [&](int j) -> const float* {
+        if (j >= j1) return nullptr;
+        const int key = j - a.q_heads, value = key - a.heads;
+        return key < 0 ? q + (int64_t)j * a.dim : value < 0 ? k + (int64_t)key * a.dim : v + (int64_t)value * a.dim;
+    };
+    float x[U][4 * V], c[4 * V] = {}, s[4 * V] = {};
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        int j = ((int)blockIdx.y * U + u) * GROUPS + group;
-        const float* p = nullptr;
-        if (j < a.q_heads) {
-            p = a.q + row * a.q_s1 + (int64_t)j * a.dim;
-        } else if (j < a.q_heads + a.heads) {
-            p = a.k + row * a.k_s1 + (int64_t)(j - a.q_heads) * a.dim;
-        } else if (j < jobs) {
-            p = a.v + row * a.v_s1 + (int64_t)(j - a.q_heads - a.heads) * a.dim;
-        }
-        job[u] = p ? j : -1;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int d = 4 * (l + LANES * v);
-            float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (p && d < a.dim) t = load4<VEC>(p + d);
-            x[u][4 * v] = t.x, x[u][4 * v + 1] = t.y, x[u][4 * v + 2] = t.z, x[u][4 * v + 3] = t.w;
-        }
-    }
+    for (int u = 0; u < U; ++u) load_row<LANES, V, VEC>(x[u], from(j0 + u * GROUPS + group), l, a.dim);
     const int slot = a.heads ? a.slot[row] : -1;
-    if (a.turn.rot) {
-        const int pos = a.turn.pos[row];
-        for (int i = threadIdx.x; i < a.turn.rot / 2; i += kHeadThreads) {
-            const float2 t = turn_of(pos, a.turn.freq[i], a.turn.mag);
-            cs[i] = t.x, sn[i] = t.y;
-        }
-        __syncthreads();
-    }
-    float c[4 * V] = {}, s[4 * V] = {};
-    turn_factors<LANES, V>(c, s, cs, sn, a.turn, l, false);
+    if (a.turn.rot) turn_factors<LANES, V>(c, s, turns[warp], a.turn, row, l, false);
+    const bool norm = a.q_w || a.k_w;
+#pragma unroll 1
+    for (int jb = j0; jb < j1; jb += U * GROUPS) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int j = job[u];
-        const bool query = j >= 0 && j < a.q_heads, value = j >= a.q_heads + a.heads;
-        const float* w = query ? a.q_w : value ? nullptr : a.k_w;
-        if (a.q_w || a.k_w) {
-            float ss = 0.0f;
+        for (int u = 0; u < U; ++u) {
+            const int j = jb + u * GROUPS + group;
+            const bool live = j < j1, query = live && j < a.q_heads, value = j >= a.q_heads + a.heads;
+            float(&y)[4 * V] = x[u];
+            if (norm) {
+                const float* w = query ? a.q_w : !live || value ? nullptr : a.k_w;
+                float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4 * V; ++i) ss = fmaf(x[u][i], x[u][i], ss);
-            const float r = inv_sqrt(group_sum<LANES>(ss) / (float)a.dim + a.eps);
-            if (w) {
+                for (int i = 0; i < 4 * V; ++i) ss = fmaf(y[i], y[i], ss);
+                const float r = inv_sqrt(fmaf(group_sum<LANES>(ss), a.inv_dim, a.eps));
+                if (w) {
+                    float f[4 * V];
+                    load_row<LANES, V, VEC>(f, w, l, a.dim);
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const int d = 4 * (l + LANES * v);
-                    if (d < a.dim) {
-                        const float4 t = load4<VEC>(w + d);
-                        x[u][4 * v] = x[u][4 * v] * r * t.x, x[u][4 * v + 1] = x[u][4 * v + 1] * r * t.y;
-                        x[u][4 * v + 2] = x[u][4 * v + 2] * r * t.z, x[u][4 * v + 3] = x[u][4 * v + 3] * r * t.w;
-                    }
+                    for (int i = 0; i < 4 * V; ++i) y[i] = y[i] * r * f[i];
                 }
                 if (query && a.rstd && l == 0) a.rstd[row * a.q_heads + j] = r;
             }
-        }
-        if (a.turn.rot) {
-            float y[4 * V];
+            if (a.turn.rot) {
+                float z[4 * V];
 #pragma unroll
-            for (int i = 0; i < 4 * V; ++i) y[i] = x[u][i];
-            turn<LANES, V>(y, c, s, a.turn, l);
+                for (int i = 0; i < 4 * V; ++i) z[i] = y[i];
+                turn<LANES, V>(z, c, s, a.turn, l);
 #pragma unroll
-            for (int i = 0; i < 4 * V; ++i) x[u][i] = value ? x[u][i] : y[i];
-        }
-        if (query) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int d = 4 * (l + LANES * v);
-                if (d < a.dim)
-                    store4<VEC>(a.q_out + row * a.out_s1 + (int64_t)j * a.dim + d,
-                                make_float4(x[u][4 * v], x[u][4 * v + 1], x[u][4 * v + 2], x[u][4 * v + 3]));
+                for (int i = 0; i < 4 * V; ++i) y[i] = value ? y[i] : z[i];
             }
-        }
-        if (V == 1 && a.heads) {  // (a cache's heads have at most 128 values)
-            uint32_t top = 0;
+            if (query) store_row<LANES, V, VEC>(a.q_out + row * a.out_s1 + (int64_t)j * a.dim, y, l, a.dim);
+            if (V == 1 && a.heads) {  // (a cache's heads have at most 128 values)
+                uint32_t top = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = max(top, abs_bits(x[u][i]));
-            top = group_max<LANES>(top);
-            if (j >= a.q_heads && (uint32_t)slot < (uint32_t)a.slots) {
-                const int h = j - a.q_heads - (value ? a.heads : 0);
-                const int64_t at = ((((int64_t)(slot >> a.page_log) * a.heads) + h) << a.page_log) + (slot & ((1 << a.page_log) - 1));
-                const E4m3Group g = e4m3_group(top);
-                const bool bad = top >= 0x7F800000u;
-                if (4 * l < a.dim)
-                    *(uint32_t*)((value ? a.vq : a.kq) + at * a.dim + 4 * l) =
-                        bad ? 0u : e4m3_quotients(g, x[u][0], x[u][1], x[u][2], x[u][3]);
-                if (l == 0) (value ? a.vs : a.ks)[at] = bad ? __uint_as_float(0x7FFFFFFFu) : g.scale;
+                for (int i = 0; i < 4; ++i) top = max(top, abs_bits(y[i]));
+                top = group_max<LANES>(top);
+                if (live && !query && (uint32_t)slot < (uint32_t)a.slots) {
+                    const int h = j - a.q_heads - (value ? a.heads : 0);
+                    const int64_t at = ((((int64_t)(slot >> a.page_log) * a.heads) + h) << a.page_log) + (slot & ((1 << a.page_log) - 1));
+                    const E4m3Group g = e4m3_group(top);
+                    const bool bad = top >= 0x7F800000u;
+                    if (4 * l < a.dim) *(uint32_t*)((value ? a.vq : a.kq) + at * a.dim + 4 * l) = bad ? 0u : e4m3_quotients(g, y[0], y[1], y[2], y[3]);
+                    if (l == 0) (value ? a.vs : a.ks)[at] = bad ? __uint_as_float(0x7FFFFFFFu) : g.scale;
+                }
             }
+            load_row<LANES, V, VEC>(x[u], from(j + U * GROUPS), l, a.dim);  // the group's next but U rows, meanwhile
         }
     }
 }
 
 // ------------------------------------------------------------ backward
 //
-// A block takes `tokens` tokens at a time and its groups their head rows; a lane keeps its columns, so that the weight's
-// gradient is summed in registers over all of a block's rows, then over its groups in order, then over blocks by
-// weight_sum.
+// Warps as in the forward pass, but they stay: a lane keeps its columns, so that the weight's gradient is summed in registers
+// over all of a warp's rows, then over the block's groups in order, then over blocks by heads_weight_sum.
 struct HeadBackArgs {
     const float *dy, *x, *w, *rstd;
     float *dx, *part;
     Turn turn;
     int64_t rows, dy_s1, x_s1, dx_s1;
-    int dim, heads, tokens;
+    float inv_dim;
+    int dim, heads, rows_a_warp, shares;
 };
-constexpr int kBackTokens = 4, kBackRows = 2;
+constexpr int kBackRows = 2;
 
 template <int LANES, int V, bool VEC>
-__global__ void __launch_bounds__(kHeadThreads) heads_backward(HeadBackArgs a) {
-    __shared__ __align__(16) float cs[kBackTokens][kMaxPairs], sn[kBackTokens][kMaxPairs];
-    constexpr int GROUPS = kHeadWarps * 32 / LANES;
-    __shared__ __align__(16) float sums[GROUPS][4 * V * LANES];
-    const int l = threadIdx.x & (LANES - 1), group = threadIdx.x / LANES;
-    const int pairs = a.turn.rot / 2;
+__global__ void __launch_bounds__(kHeadThreads, V == 1 ? 4 : 2) heads_backward(HeadBackArgs a) {
+    __shared__ __align__(16) float turns[kHeadWarps][2 * kMaxPairs];
+    constexpr int GROUPS = 32 / LANES, ALL = kHeadWarps * GROUPS;
+    __shared__ __align__(16) float sums[ALL][4 * V * LANES];
+    const int l = threadIdx.x & (LANES - 1), group = (threadIdx.x & 31) / LANES, warp = threadIdx.x >> 5;
     pdl_begin();
     float w[4 * V], acc[4 * V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int d = 4 * (l + LANES * v);
-        float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (a.w && d < a.dim) t = load4<VEC>(a.w + d);
-        w[4 * v] = t.x, w[4 * v + 1] = t.y, w[4 * v + 2] = t.z, w[4 * v + 3] = t.w;
-    }
+    load_row<LANES, V, VEC>(w, a.w, l, a.dim);
 #pragma unroll
     for (int i = 0; i < 4 * V; ++i) acc[i] = 0.0f;
-    for (int64_t first = (int64_t)blockIdx.x * a.tokens; first < a.rows; first += (int64_t)gridDim.x * a.tokens) {
-        const int n = (int)min((int64_t)a.tokens, a.rows - first);
-        if (pairs) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < n * pairs; i += kHeadThreads) {
-                const int tok = i / pairs, p = i - tok * pairs;
-                const float2 t = turn_of(a.turn.pos[first + tok], a.turn.freq[p], a.turn.mag);
-                cs[tok][p] = t.x, sn[tok][p] = t.y;
-            }
-            __syncthreads();
-        }
-        const int jobs = n * a.heads;
-        for (int j0 = 0; j0 < jobs; j0 += GROUPS * kBackRows) {
-            float u[kBackRows][4 * V], x[kBackRows][4 * V], rstd[kBackRows];
-            int tok[kBackRows], head[kBackRows];
+    const int64_t items = a.rows * a.shares, all = (int64_t)gridDim.x * kHeadWarps;
+#pragma unroll 1
+    for (int64_t item = (int64_t)blockIdx.x * kHeadWarps + warp; item < items; item += all) {
+        const int64_t row = item / a.shares;
+        const int j0 = (int)(item - row * a.shares) * a.rows_a_warp, j1 = min(j0 + a.rows_a_warp, a.heads);
+        const float *dy = a.dy + row * a.dy_s1, *xr = a.x + row * a.x_s1;
+        float u[kBackRows][4 * V], x[kBackRows][4 * V], rstd[kBackRows], c[4 * V] = {}, s[4 * V] = {};
+        auto load = [&](int k, int j) {
+            const bool live = j < j1;
+            rstd[k] = a.w && live ? a.rstd[row * a.heads + j] : 0.0f;
+            load_row<LANES, V, VEC>(u[k], live ? dy + (int64_t)j * a.dim : nullptr, l, a.dim);
+            load_row<LANES, V, VEC>(x[k], live && a.w ? xr + (int64_t)j * a.dim : nullptr, l, a.dim);
+        };
+#pragma unroll
+        for (int k = 0; k < kBackRows; ++k) load(k, j0 + k * GROUPS + group);
+        if (a.turn.rot) turn_factors<LANES, V>(c, s, turns[warp], a.turn, row, l, true);
+#pragma unroll 1
+        for (int jb = j0; jb < j1; jb += kBackRows * GROUPS) {
 #pragma unroll
             for (int k = 0; k < kBackRows; ++k) {
-                const int j = j0 + k * GROUPS + group;
-                tok[k] = j < jobs ? j / a.heads : -1;
-                head[k] = j - max(tok[k], 0) * a.heads;
-                const int64_t row = first + max(tok[k], 0);
-                rstd[k] = a.w && tok[k] >= 0 ? a.rstd[row * a.heads + head[k]] : 0.0f;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const int d = 4 * (l + LANES * v);
-                    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f), z = t;
-                    if (tok[k] >= 0 && d < a.dim) {
-                        t = load4<VEC>(a.dy + row * a.dy_s1 + (int64_t)head[k] * a.dim + d);
-                        if (a.w) z = load4<VEC>(a.x + row * a.x_s1 + (int64_t)head[k] * a.dim + d);
-                    }
-                    u[k][4 * v] = t.x, u[k][4 * v + 1] = t.y, u[k][4 * v + 2] = t.z, u[k][4 * v + 3] = t.w;
-                    x[k][4 * v] = z.x, x[k][4 * v + 1] = z.y, x[k][4 * v + 2] = z.z, x[k][4 * v + 3] = z.w;
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < kBackRows; ++k) {
-                if (pairs) {
-                    float c[4 * V] = {}, s[4 * V] = {};
-                    turn_factors<LANES, V>(c, s, cs[max(tok[k], 0)], sn[max(tok[k], 0)], a.turn, l, true);
-                    turn<LANES, V>(u[k], c, s, a.turn, l);
-                }
+                const int j = jb + k * GROUPS + group;
+                if (a.turn.rot) turn<LANES, V>(u[k], c, s, a.turn, l);
                 if (a.w) {
                     float dot = 0.0f;
 #pragma unroll
@@ -317,31 +290,24 @@ __global__ void __launch_bounds__(kHeadThreads) heads_backward(HeadBackArgs a) {
                         u[k][i] *= w[i];
                         dot = fmaf(u[k][i], x[k][i], dot);
                     }
-                    const float m = group_sum<LANES>(dot) / (float)a.dim * (rstd[k] * rstd[k]);
+                    const float m = group_sum<LANES>(dot) * a.inv_dim * (rstd[k] * rstd[k]);
 #pragma unroll
                     for (int i = 0; i < 4 * V; ++i) u[k][i] = rstd[k] * fmaf(-x[k][i], m, u[k][i]);
                 }
-                if (tok[k] >= 0) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const int d = 4 * (l + LANES * v);
-                        if (d < a.dim)
-                            store4<VEC>(a.dx + (first + tok[k]) * a.dx_s1 + (int64_t)head[k] * a.dim + d,
-                                        make_float4(u[k][4 * v], u[k][4 * v + 1], u[k][4 * v + 2], u[k][4 * v + 3]));
-                    }
-                }
+                if (j < j1) store_row<LANES, V, VEC>(a.dx + row * a.dx_s1 + (int64_t)j * a.dim, u[k], l, a.dim);
+                load(k, j + kBackRows * GROUPS);
             }
         }
     }
     if (a.part) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            *(float4*)&sums[group][4 * (l + LANES * v)] = make_float4(acc[4 * v], acc[4 * v + 1], acc[4 * v + 2], acc[4 * v + 3]);
+            *(float4*)&sums[warp * GROUPS + group][4 * (l + LANES * v)] = make_float4(acc[4 * v], acc[4 * v + 1], acc[4 * v + 2], acc[4 * v + 3]);
         __syncthreads();
         for (int d = threadIdx.x; d < a.dim; d += kHeadThreads) {
             float t = 0.0f;
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) t += sums[g][d];
+            for (int g = 0; g < ALL; ++g) t += sums[g][d];
             a.part[(int64_t)blockIdx.x * a.dim + d] = t;
         }
     }
@@ -375,7 +341,7 @@ struct ReadArgs {
     int64_t rows, k_s1, v_s1;
     int dim, heads, page_log, slots;
 };
-constexpr int kReadRows = 4;
+constexpr int kReadRows = 8;
 
 __device__ __forceinline__ float4 e4m3_values(uint32_t b) {
     uint32_t lo, hi;
@@ -431,30 +397,41 @@ int log2_of(int v) {
 }
 Turn turn_args(const mag_cuda_rotation* r) { return Turn{r->pos, r->inv_freq, r->rot, r->interleaved != 0, r->magnitude}; }
 
+// Head rows of a warp: 16 of them share the token's angles where that leaves two warps a scheduler's slot, fewer for few tokens,
+// down to one step of a warp (least).
+int rows_a_warp(int64_t rows, int jobs, int least) {
+    int n = 16;
+    while (n > least && rows * ((jobs + n - 1) / n) < (int64_t)kSms * 64) n /= 2;
+    return n;
+}
+
 template <int LANES, int V, bool VEC>
-int run_forward(const HeadArgs& a, int64_t rows, cudaStream_t st) {
-    constexpr int groups = kHeadWarps * 32 / LANES;
-    const int jobs = a.q_heads + 2 * a.heads, few = (jobs + groups - 1) / groups, many = (jobs + 4 * groups - 1) / (4 * groups);
-    // few tokens: a head row a group, so that more SMs share a token
-    if (rows * many < kSms) return (int)launch_dep(heads_forward<LANES, V, 1, VEC>, dim3((unsigned)rows, (unsigned)few), dim3(kHeadThreads), 0, st, a);
-    return (int)launch_dep(heads_forward<LANES, V, 4, VEC>, dim3((unsigned)rows, (unsigned)many), dim3(kHeadThreads), 0, st, a);
+int run_forward(HeadArgs& a, int64_t rows, cudaStream_t st) {
+    const int jobs = a.q_heads + 2 * a.heads;
+    a.rows = rows, a.inv_dim = 1.0f / (float)a.dim;
+    a.rows_a_warp = rows_a_warp(rows, jobs, 32 / LANES), a.shares = (jobs + a.rows_a_warp - 1) / a.rows_a_warp;
+    const dim3 grid((unsigned)((rows * a.shares + kForwardWarps - 1) / kForwardWarps)), block(32 * kForwardWarps);
+    if (a.rows_a_warp < 4) return (int)launch_dep(heads_forward<LANES, V, 1, VEC>, grid, block, 0, st, a);
+    return (int)launch_dep(heads_forward<LANES, V, V == 1 ? 4 : 2, VEC>, grid, block, 0, st, a);
 }
 template <bool VEC>
-int forward(const HeadArgs& a, int64_t rows, cudaStream_t st) {
+int forward(HeadArgs& a, int64_t rows, cudaStream_t st) {
     if (a.dim <= 64) return run_forward<16, 1, VEC>(a, rows, st);
     if (a.dim <= 128) return run_forward<32, 1, VEC>(a, rows, st);
     return run_forward<32, 2, VEC>(a, rows, st);
 }
 
-constexpr int kBackBlocks = 3 * kSms;
-int back_tokens(int64_t rows) { return rows <= kBackBlocks ? 1 : kBackTokens; }
-int back_blocks(int64_t rows) {
-    const int64_t n = (rows + back_tokens(rows) - 1) / back_tokens(rows);
+constexpr int kBackBlocks = 4 * kSms;
+int back_share(int64_t rows, int64_t heads, int64_t dim) { return rows_a_warp(rows, (int)heads, dim <= 64 ? 4 : 2); }
+int back_blocks(int64_t rows, int64_t heads, int64_t dim) {
+    const int share = back_share(rows, heads, dim);
+    const int64_t n = (rows * ((heads + share - 1) / share) + kHeadWarps - 1) / kHeadWarps;
     return (int)(n < kBackBlocks ? n : kBackBlocks);
 }
 template <bool VEC>
-int backward(const HeadBackArgs& a, cudaStream_t st) {
-    const dim3 grid((unsigned)back_blocks(a.rows)), block(kHeadThreads);
+int backward(HeadBackArgs& a, cudaStream_t st) {
+    a.rows_a_warp = back_share(a.rows, a.heads, a.dim), a.shares = (a.heads + a.rows_a_warp - 1) / a.rows_a_warp;
+    const dim3 grid((unsigned)back_blocks(a.rows, a.heads, a.dim)), block(kHeadThreads);
     if (a.dim <= 64) return (int)launch_dep(heads_backward<16, 1, VEC>, grid, block, 0, st, a);
     if (a.dim <= 128) return (int)launch_dep(heads_backward<32, 1, VEC>, grid, block, 0, st, a);
     return (int)launch_dep(heads_backward<32, 2, VEC>, grid, block, 0, st, a);
@@ -498,22 +475,21 @@ extern "C" int mcu_launch_kv_write(const mag_cuda_kv_cache* cache, const int32_t
 }
 
 extern "C" size_t mcu_rotate_heads_backward_scratch_bytes(int64_t rows, int64_t heads, int64_t head_dim) {
-    (void)heads;
-    return (size_t)back_blocks(rows) * (size_t)head_dim * 4;
+    return (size_t)back_blocks(rows, heads, head_dim) * (size_t)head_dim * 4;
 }
 
 extern "C" int mcu_launch_rotate_heads_backward(float* dx, float* dw, const float* dy, const float* x, const float* w, const float* rstd,
                                                 const mag_cuda_rotation* rot, int64_t rows, int64_t heads, int64_t head_dim,
                                                 int64_t dx_s1, int64_t dy_s1, int64_t x_s1, void* scratch, cudaStream_t st,
                                                 int* launches) {
-    const HeadBackArgs a{dy, x, w, rstd, dx, dw ? (float*)scratch : nullptr, turn_args(rot), rows, dy_s1, x_s1, dx_s1,
-                         (int)head_dim, (int)heads, back_tokens(rows)};
+    HeadBackArgs a{dy, x, w, rstd, dx, dw ? (float*)scratch : nullptr, turn_args(rot), rows, dy_s1, x_s1, dx_s1,
+                   1.0f / (float)head_dim, (int)head_dim, (int)heads, 0, 0};
     *launches = 1;
     const bool vec = aligned16(dx) && aligned16(dy) && aligned16(x) && aligned16(w) && !((dx_s1 | dy_s1) & 3) && (!x || !(x_s1 & 3));
     int rc = vec ? backward<true>(a, st) : backward<false>(a, st);
     if (!rc && dw) {
         rc = (int)launch_dep(heads_weight_sum, dim3((unsigned)((head_dim + 31) / 32)), dim3(1024), 0, st, dw, (const float*)scratch,
-                             back_blocks(rows), (int)head_dim);
+                             back_blocks(rows, heads, head_dim), (int)head_dim);
         ++*launches;
     }
     return rc;
