@@ -165,73 +165,84 @@ struct HeadArgs {
 };
 constexpr int kForwardWarps = 4;
 
-template <int LANES, int V, int U, bool VEC>
-__global__ void __launch_bounds__(32 * kForwardWarps) heads_forward(HeadArgs a) {
-    __shared__ __align__(16) float turns[kForwardWarps][2 * kMaxPairs];
+// What becomes of a run of `rows` head rows of one kind from `from` on, GROUPS at a time, U on their way.
+enum Kind { QUERY, KEY, VALUE };
+template <int LANES, int V, int U, bool VEC, int KIND>
+__device__ __forceinline__ void head_run(const HeadArgs& a, const float* from, int rows, int64_t row, int first, const float* w, const float (&c)[4 * V],
+                                         const float (&s)[4 * V], int64_t place) {
     constexpr int GROUPS = 32 / LANES;
-    const int l = threadIdx.x & (LANES - 1), group = (threadIdx.x & 31) / LANES, warp = threadIdx.x >> 5;
-    const int64_t item = (int64_t)blockIdx.x * kForwardWarps + warp, row = item / a.shares;
-    pdl_begin();
-    if (row >= a.rows) return;
-    const int jobs = a.q_heads + 2 * a.heads, j0 = (int)(item - row * a.shares) * a.rows_a_warp, j1 = min(j0 + a.rows_a_warp, jobs);
-    const float *q = a.q + row * a.q_s1, *k = a.k + row * a.k_s1, *v = a.v + row * a.v_s1;
-    auto from = [&](int j) -> const float* {
-        if (j >= j1) return nullptr;
-        const int key = j - a.q_heads, value = key - a.heads;
-        return key < 0 ? q + (int64_t)j * a.dim : value < 0 ? k + (int64_t)key * a.dim : v + (int64_t)value * a.dim;
-    };
-    float x[U][4 * V], c[4 * V] = {}, s[4 * V] = {};
+    const int l = threadIdx.x & (LANES - 1), group = (threadIdx.x & 31) / LANES, step = GROUPS * a.dim;
+    from += group * a.dim;
+    float x[U][4 * V], f[4 * V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_row<LANES, V, VEC>(x[u], from(j0 + u * GROUPS + group), l, a.dim);
-    const int slot = a.heads ? a.slot[row] : -1;
-    if (a.turn.rot) turn_factors<LANES, V>(c, s, turns[warp], a.turn, row, l, false);
-    const bool norm = a.q_w || a.k_w;
+    for (int u = 0; u < U; ++u) load_row<LANES, V, VEC>(x[u], u * GROUPS + group < rows ? from + u * step : nullptr, l, a.dim);
+    if (KIND != VALUE && w) load_row<LANES, V, VEC>(f, w, l, a.dim);
+    float* to = KIND == QUERY ? a.q_out + row * a.out_s1 + (int64_t)(first + group) * a.dim : nullptr;
+    // (a head's rows of a page lie page_size rows apart)
+    uint8_t* bytes = KIND == QUERY ? nullptr : (KIND == KEY ? a.kq : a.vq) + (place + ((int64_t)(first + group) << a.page_log)) * a.dim + 4 * l;
+    float* scale = KIND == QUERY ? nullptr : (KIND == KEY ? a.ks : a.vs) + place + ((int64_t)(first + group) << a.page_log);
 #pragma unroll 1
-    for (int jb = j0; jb < j1; jb += U * GROUPS) {
+    for (int j = group; j < rows + group; j += U * GROUPS) {
+        from += U * step;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = jb + u * GROUPS + group;
-            const bool live = j < j1, query = live && j < a.q_heads, value = j >= a.q_heads + a.heads;
+            const bool live = j + u * GROUPS < rows;
             float(&y)[4 * V] = x[u];
-            if (norm) {
-                const float* w = query ? a.q_w : !live || value ? nullptr : a.k_w;
+            if (KIND != VALUE && w) {
                 float ss = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4 * V; ++i) ss = fmaf(y[i], y[i], ss);
                 const float r = inv_sqrt(fmaf(group_sum<LANES>(ss), a.inv_dim, a.eps));
-                if (w) {
-                    float f[4 * V];
-                    load_row<LANES, V, VEC>(f, w, l, a.dim);
 #pragma unroll
-                    for (int i = 0; i < 4 * V; ++i) y[i] = y[i] * r * f[i];
-                }
-                if (query && a.rstd && l == 0) a.rstd[row * a.q_heads + j] = r;
+                for (int i = 0; i < 4 * V; ++i) y[i] = y[i] * r * f[i];
+                if (KIND == QUERY && a.rstd && l == 0 && live) a.rstd[row * a.q_heads + first + j + u * GROUPS] = r;
             }
-            if (a.turn.rot) {
-                float z[4 * V];
-#pragma unroll
-                for (int i = 0; i < 4 * V; ++i) z[i] = y[i];
-                turn<LANES, V>(z, c, s, a.turn, l);
-#pragma unroll
-                for (int i = 0; i < 4 * V; ++i) y[i] = value ? y[i] : z[i];
-            }
-            if (query) store_row<LANES, V, VEC>(a.q_out + row * a.out_s1 + (int64_t)j * a.dim, y, l, a.dim);
-            if (V == 1 && a.heads) {  // (a cache's heads have at most 128 values)
+            if (KIND != VALUE && a.turn.rot) turn<LANES, V>(y, c, s, a.turn, l);
+            if (KIND == QUERY) {
+                if (live) store_row<LANES, V, VEC>(to + u * step, y, l, a.dim);
+            } else if (V == 1) {  // (a cache's heads have at most 128 values)
                 uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = max(top, abs_bits(y[i]));
                 top = group_max<LANES>(top);
-                if (live && !query && (uint32_t)slot < (uint32_t)a.slots) {
-                    const int h = j - a.q_heads - (value ? a.heads : 0);
-                    const int64_t at = ((((int64_t)(slot >> a.page_log) * a.heads) + h) << a.page_log) + (slot & ((1 << a.page_log) - 1));
+                if (live && place >= 0) {
                     const E4m3Group g = e4m3_group(top);
                     const bool bad = top >= 0x7F800000u;
-                    if (4 * l < a.dim) *(uint32_t*)((value ? a.vq : a.kq) + at * a.dim + 4 * l) = bad ? 0u : e4m3_quotients(g, y[0], y[1], y[2], y[3]);
-                    if (l == 0) (value ? a.vs : a.ks)[at] = bad ? __uint_as_float(0x7FFFFFFFu) : g.scale;
+                    const int64_t up = (int64_t)(u * GROUPS) << a.page_log;
+                    if (4 * l < a.dim) *(uint32_t*)(bytes + up * a.dim) = bad ? 0u : e4m3_quotients(g, y[0], y[1], y[2], y[3]);
+                    if (l == 0) scale[up] = bad ? __uint_as_float(0x7FFFFFFFu) : g.scale;
                 }
             }
-            load_row<LANES, V, VEC>(x[u], from(j + U * GROUPS), l, a.dim);  // the group's next but U rows, meanwhile
+            load_row<LANES, V, VEC>(x[u], j + (u + U) * GROUPS < rows ? from + u * step : nullptr, l, a.dim);  // meanwhile
         }
+        if (KIND == QUERY) {
+            to += U * step;
+        } else {
+            const int64_t up = (int64_t)(U * GROUPS) << a.page_log;
+            bytes += up * a.dim, scale += up;
+        }
+    }
+}
+
+template <int LANES, int V, int U, bool VEC, bool CACHE>
+__global__ void __launch_bounds__(32 * kForwardWarps) heads_forward(HeadArgs a) {
+    __shared__ __align__(16) float turns[kForwardWarps][2 * kMaxPairs];
+    const int l = threadIdx.x & (LANES - 1), warp = threadIdx.x >> 5;
+    const int64_t item = (int64_t)blockIdx.x * kForwardWarps + warp, row = item / a.shares;
+    pdl_begin();
+    if (row >= a.rows) return;
+    const int j0 = (int)(item - row * a.shares) * a.rows_a_warp, j1 = min(j0 + a.rows_a_warp, a.q_heads + 2 * a.heads);
+    float c[4 * V] = {}, s[4 * V] = {};
+    if (a.turn.rot && j0 < a.q_heads + a.heads) turn_factors<LANES, V>(c, s, turns[warp], a.turn, row, l, false);
+    if (j0 < a.q_heads)
+        head_run<LANES, V, U, VEC, QUERY>(a, a.q + row * a.q_s1 + (int64_t)j0 * a.dim, min(j1, a.q_heads) - j0, row, j0, a.q_w, c, s, 0);
+    if constexpr (CACHE) {
+        const int slot = a.slot[row];
+        const int64_t place =
+            (uint32_t)slot < (uint32_t)a.slots ? (((int64_t)(slot >> a.page_log) * a.heads) << a.page_log) + (slot & ((1 << a.page_log) - 1)) : (int64_t)-1;
+        const int k0 = max(j0 - a.q_heads, 0), k1 = min(j1 - a.q_heads, a.heads), v0 = max(j0 - a.q_heads - a.heads, 0), v1 = j1 - a.q_heads - a.heads;
+        if (k0 < k1) head_run<LANES, V, U, VEC, KEY>(a, a.k + row * a.k_s1 + (int64_t)k0 * a.dim, k1 - k0, row, k0, a.k_w, c, s, place);
+        if (v0 < v1) head_run<LANES, V, U, VEC, VALUE>(a, a.v + row * a.v_s1 + (int64_t)v0 * a.dim, v1 - v0, row, v0, nullptr, c, s, place);
     }
 }
 
@@ -331,17 +342,17 @@ __global__ void __launch_bounds__(1024) heads_weight_sum(float* dw, const float*
 
 // ------------------------------------------------------------ cache read
 //
-// The rows' head rows of keys, then of values, in one order; a group takes every GROUPS-th of a run of kReadRows * GROUPS,
-// all of its loads first.  Bound by HBM: 1 byte in and 4 out a value.
+// A warp takes the keys or the values of a slot: its heads' rows lie page_size rows apart, so that one address serves them all;
+// a lane holds four values, its group every GROUPS-th head, U on their way.  Bound by HBM: 1 byte in and 4 out a value (with an
+// address for every row it was bound by instructions, 137 us for 65000 x 8 x 128).
 struct ReadArgs {
     const uint8_t *kq, *vq;
     const float *ks, *vs;
     float *k, *v;
     const int32_t* slot;
     int64_t rows, k_s1, v_s1;
-    int dim, heads, page_log, slots;
+    int dim, heads, page_log, slots, shares, rows_a_warp;
 };
-constexpr int kReadRows = 8;
 
 __device__ __forceinline__ float4 e4m3_values(uint32_t b) {
     uint32_t lo, hi;
@@ -355,35 +366,38 @@ __device__ __forceinline__ float4 e4m3_values(uint32_t b) {
 
 template <int LANES, bool VEC>
 __global__ void __launch_bounds__(kHeadThreads) cache_read(ReadArgs a) {
-    constexpr int GROUPS = kHeadWarps * 32 / LANES;
-    const int l = threadIdx.x & (LANES - 1), group = threadIdx.x / LANES;
-    const int jobs = a.heads * ((a.k != nullptr) + (a.v != nullptr));
-    const int64_t first = (int64_t)blockIdx.x * (GROUPS * kReadRows), row0 = first / jobs;
-    const int rem = (int)(first - row0 * jobs);
+    constexpr int GROUPS = 32 / LANES, U = 4;
+    const int l = threadIdx.x & (LANES - 1), group = (threadIdx.x & 31) / LANES;
+    const int both = (a.k != nullptr) + (a.v != nullptr);
+    const int64_t item = (int64_t)blockIdx.x * kHeadWarps + (threadIdx.x >> 5), row = item / (both * a.shares);
     pdl_begin();
-    uint32_t b[kReadRows];
-    float s[kReadRows];
-    float* to[kReadRows];
+    if (row >= a.rows) return;
+    const int part = (int)(item - row * (both * a.shares)), share = part >> (both - 1);
+    const bool value = both == 2 ? part & 1 : a.v != nullptr;
+    const int j0 = share * a.rows_a_warp + group, j1 = min(share * a.rows_a_warp + a.rows_a_warp, a.heads), slot = a.slot[row];
+    const bool there = (uint32_t)slot < (uint32_t)a.slots;
+    const int64_t place = there ? (((int64_t)(slot >> a.page_log) * a.heads + j0) << a.page_log) + (slot & ((1 << a.page_log) - 1)) : 0;
+    const uint8_t* bytes = (value ? a.vq : a.kq) + place * a.dim + 4 * l;
+    const float* scale = (value ? a.vs : a.ks) + place;
+    float* to = (value ? a.v + row * a.v_s1 : a.k + row * a.k_s1) + (int64_t)j0 * a.dim + 4 * l;
+    const int64_t up = (int64_t)GROUPS << a.page_log, up_bytes = up * a.dim;
+    if (4 * l >= a.dim) return;
+#pragma unroll 1
+    for (int j = j0; j < j1; j += U * GROUPS) {
+        uint32_t b[U];
+        float s[U];
 #pragma unroll
-    for (int u = 0; u < kReadRows; ++u) {
-        const int t = rem + u * GROUPS + group, up = t / jobs, j = t - up * jobs;
-        const int64_t row = row0 + up;
-        b[u] = 0, s[u] = 0.0f, to[u] = nullptr;
-        if (row < a.rows && 4 * l < a.dim) {
-            const bool value = !a.k || j >= a.heads;
-            const int h = j - (a.k && value ? a.heads : 0), slot = a.slot[row];
-            to[u] = (value ? a.v + row * a.v_s1 : a.k + row * a.k_s1) + (int64_t)h * a.dim + 4 * l;
-            if ((uint32_t)slot < (uint32_t)a.slots) {
-                const int64_t at = ((((int64_t)(slot >> a.page_log) * a.heads) + h) << a.page_log) + (slot & ((1 << a.page_log) - 1));
-                b[u] = *(const uint32_t*)((value ? a.vq : a.kq) + at * a.dim + 4 * l);
-                s[u] = (value ? a.vs : a.ks)[at];
-            }
+        for (int u = 0; u < U; ++u) {
+            const bool live = there && j + u * GROUPS < j1;
+            b[u] = live ? __ldg((const uint32_t*)(bytes + u * up_bytes)) : 0u;
+            s[u] = live ? __ldg(scale + u * up) : 0.0f;
         }
-    }
 #pragma unroll
-    for (int u = 0; u < kReadRows; ++u) {
-        const float4 v = e4m3_values(b[u]);
-        if (to[u]) store4<VEC>(to[u], make_float4(v.x * s[u], v.y * s[u], v.z * s[u], v.w * s[u]));
+        for (int u = 0; u < U; ++u) {
+            const float4 v = e4m3_values(b[u]);
+            if (j + u * GROUPS < j1) store4<VEC>(to + u * GROUPS * a.dim, make_float4(v.x * s[u], v.y * s[u], v.z * s[u], v.w * s[u]));
+        }
+        bytes += U * up_bytes, scale += U * up, to += U * GROUPS * a.dim;
     }
 }
 
@@ -411,8 +425,14 @@ int run_forward(HeadArgs& a, int64_t rows, cudaStream_t st) {
     a.rows = rows, a.inv_dim = 1.0f / (float)a.dim;
     a.rows_a_warp = rows_a_warp(rows, jobs, 32 / LANES), a.shares = (jobs + a.rows_a_warp - 1) / a.rows_a_warp;
     const dim3 grid((unsigned)((rows * a.shares + kForwardWarps - 1) / kForwardWarps)), block(32 * kForwardWarps);
-    if (a.rows_a_warp < 4) return (int)launch_dep(heads_forward<LANES, V, 1, VEC>, grid, block, 0, st, a);
-    return (int)launch_dep(heads_forward<LANES, V, V == 1 ? 4 : 2, VEC>, grid, block, 0, st, a);
+    constexpr int U = V == 1 ? 4 : 2;
+    if constexpr (V == 1) {
+        if (a.heads)
+            return (int)(a.rows_a_warp < 4 ? launch_dep(heads_forward<LANES, V, 1, VEC, true>, grid, block, 0, st, a)
+                                           : launch_dep(heads_forward<LANES, V, U, VEC, true>, grid, block, 0, st, a));
+    }
+    return (int)(a.rows_a_warp < 4 ? launch_dep(heads_forward<LANES, V, 1, VEC, false>, grid, block, 0, st, a)
+                                   : launch_dep(heads_forward<LANES, V, U, VEC, false>, grid, block, 0, st, a));
 }
 template <bool VEC>
 int forward(HeadArgs& a, int64_t rows, cudaStream_t st) {
@@ -438,9 +458,10 @@ int backward(HeadBackArgs& a, cudaStream_t st) {
 }
 
 template <bool VEC>
-int read(const ReadArgs& a, cudaStream_t st) {
-    const int64_t all = a.rows * a.heads * ((a.k != nullptr) + (a.v != nullptr)), per = kReadRows * (a.dim <= 64 ? 16 : 8);
-    const dim3 grid((unsigned)((all + per - 1) / per)), block(kHeadThreads);
+int read(ReadArgs& a, cudaStream_t st) {
+    const int both = (a.k != nullptr) + (a.v != nullptr);
+    a.rows_a_warp = rows_a_warp(a.rows * both, a.heads, a.dim <= 64 ? 2 : 1), a.shares = (a.heads + a.rows_a_warp - 1) / a.rows_a_warp;
+    const dim3 grid((unsigned)((a.rows * both * a.shares + kHeadWarps - 1) / kHeadWarps)), block(kHeadThreads);
     if (a.dim <= 64) return (int)launch_dep(cache_read<16, VEC>, grid, block, 0, st, a);
     return (int)launch_dep(cache_read<32, VEC>, grid, block, 0, st, a);
 }
@@ -497,8 +518,8 @@ extern "C" int mcu_launch_rotate_heads_backward(float* dx, float* dw, const floa
 
 extern "C" int mcu_launch_kv_read(const mag_cuda_kv_cache* cache, float* k, float* v, const int32_t* slot, int64_t rows, int64_t k_s1,
                                   int64_t v_s1, cudaStream_t st, int* launches) {
-    const ReadArgs a{cache->k, cache->v, cache->k_scale, cache->v_scale, k, v, slot, rows, k_s1, v_s1, cache->head_dim, cache->heads,
-                     log2_of(cache->page_size), cache->pages * cache->page_size};
+    ReadArgs a{cache->k, cache->v, cache->k_scale, cache->v_scale, k, v, slot, rows, k_s1, v_s1, cache->head_dim, cache->heads,
+               log2_of(cache->page_size), cache->pages * cache->page_size, 0, 0};
     *launches = 1;
     const bool vec = aligned16(k) && aligned16(v) && (!k || !(k_s1 & 3)) && (!v || !(v_s1 & 3));
     return vec ? read<true>(a, st) : read<false>(a, st);
