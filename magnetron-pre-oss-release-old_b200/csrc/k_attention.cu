@@ -21,33 +21,36 @@ namespace {
 // operand, so that the split costs no instruction and a thread finds both halves' results in its own registers.
 // The order of a product's inner index is free, so it is chosen such that a thread's operands are 16 consecutive bytes
 // of a row of keys (inner index: the head's values) and of four rows of values (columns: the head's values).
-constexpr int kFewWarps = 8, kFewStages = 4;
 constexpr int kGroup = 16;               // tokens of a warp's step; pages hold a multiple
 constexpr int kFlush = 16;               // groups between two flushes: the tensor core's sums lose up to a step each
 
-template <int DP>
+template <int DP, bool STACK>
 struct FewCfg {
+    static constexpr int WARPS = STACK ? 12 : 8, STAGES = STACK ? 3 : 4;
     static constexpr int STAGE = 2 * kGroup * DP + 2 * kGroup * 4;  // keys, values, their scales
-    static constexpr int RING = kFewStages * STAGE;
+    static constexpr int RING = STAGES * STAGE;
 };
 template <int DP, bool STACK>
 struct FewSmem {
     static constexpr int VALS = (STACK ? DP / 4 : DP / 2);  // outputs a thread holds
-    static constexpr int SUMS = FewCfg<DP>::RING * kFewWarps;
-    static constexpr int STATS = SUMS + kFewWarps * 32 * VALS * 4;  // [warp][16] of (m, l), then [warp] of the values' unit
-    static constexpr int BYTES = STATS + kFewWarps * 16 * 8 + kFewWarps * 4;
-    static_assert(Share<16, DP, 32 * kFewWarps>::SMEM <= SUMS, "the search for work takes the rings' room");
+    static constexpr int WARPS = FewCfg<DP, STACK>::WARPS;
+    static constexpr int SUMS = FewCfg<DP, STACK>::RING * WARPS;
+    static constexpr int STATS = SUMS + WARPS * 32 * VALS * 4;  // [warp][16] of (m, l), then [warp] of the values' unit
+    static constexpr int BYTES = STATS + WARPS * 16 * 8 + WARPS * 4;
+    static_assert(BYTES <= 227 * 1024, "must fit shared memory");
+    static_assert(Share<16, DP, 32 * WARPS>::SMEM <= SUMS, "the search for work takes the rings' room");
 };
 
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 template <int DP, bool STACK>
-__global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
-    using C = FewCfg<DP>;
+__global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_few(AttnArgs a) {
+    using C = FewCfg<DP, STACK>;
+    constexpr int kFewWarps = C::WARPS, kFewStages = C::STAGES;
     using S = FewSmem<DP, STACK>;
     extern __shared__ __align__(128) uint8_t smem[];
     constexpr int KI = DP / 64;      // 16-byte pieces of a key a thread holds
@@ -132,14 +135,14 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < S::VALS / 4; ++e) sums[e * 32 + lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
-        const int g0 = it.from * 8 + warp, g1 = min(it.to * 8, (it.high - it.base + kGroup - 1) / kGroup), steps = g0 < g1 ? (g1 - g0 + 7) / 8 : 0;
+        const int g0 = it.from * 8 + warp, g1 = min(it.to * 8, (it.high - it.base + kGroup - 1) / kGroup), steps = g0 < g1 ? (g1 - g0 + kFewWarps - 1) / kFewWarps : 0;
         const int32_t* table = a.table + (int64_t)it.seq * a.table_s1;
         int page = steps > 0 ? table[(it.base + kGroup * g0) >> a.page_log] : -1;
         uint32_t there = 0;  // bit s: the group in stage s has a page
-        int issued = 0;
+        int issued = 0, to = 0;  // groups issued, and the next one's stage
         auto issue = [&]() {
             if (issued < steps) {
-                const int j0 = it.base + kGroup * (g0 + 8 * issued), st = issued & (kFewStages - 1);
+                const int j0 = it.base + kGroup * (g0 + kFewWarps * issued), st = to;
                 const bool ok = (uint32_t)page < (uint32_t)a.pages;
                 there = (there & ~(1u << st)) | ((uint32_t)ok << st);
                 if (ok) {
@@ -158,10 +161,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
                     }
                     if (lane < 8) copy16(dst + 2 * kGroup * DP + 16 * lane, (lane < 4 ? a.ks : a.vs) + at + 4 * (lane & 3), true);
                 }
-                if (issued + 1 < steps) page = table[(j0 + 8 * kGroup) >> a.page_log];
+                if (issued + 1 < steps) page = table[(j0 + kFewWarps * kGroup) >> a.page_log];
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
-            ++issued;
+            ++issued, to = to == kFewStages - 1 ? 0 : to + 1;
         };
         auto flush = [&]() {
 #pragma unroll
@@ -183,14 +186,15 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
         };
 #pragma unroll
         for (int s = 0; s < kFewStages - 1; ++s) issue();
-        for (int i = 0; i < steps; ++i) {
+        for (int i = 0, st = kFewStages - 1; i < steps; ++i) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
             __syncwarp();
-            const int st = i & (kFewStages - 1), j0 = it.base + kGroup * (g0 + 8 * i);
+            const int j0 = it.base + kGroup * (g0 + kFewWarps * i);
+            st = st == kFewStages - 1 ? 0 : st + 1;
             const bool has = there >> st & 1;
             issue();
             if (!has) continue;  // (the same for the whole warp)
-            const uint32_t at = ring + st * C::STAGE;
+            const uint8_t* at = smem + warp * C::RING + st * C::STAGE;
             // ---- logits of 16 tokens: tiles of 8, the inner index in the order of the thread's bytes
             float s[2][4];
 #pragma unroll
@@ -198,7 +202,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
                 s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
 #pragma unroll
                 for (int p = 0; p < KI; ++p) {
-                    const uint4 w = lds128(at + (8 * t + g) * DP + 16 * key_chunk<DP>(4 * p + c, 8 * t + g));
+                    const uint4 w = *(const uint4*)(at + (8 * t + g) * DP + 16 * key_chunk<DP>(4 * p + c, 8 * t + g));
                     const uint32_t b[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -210,8 +214,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
             }
             float ks[4], vs[4];
             {
-                const float2 k0 = lds64(at + 2 * kGroup * DP + 8 * c), k1 = lds64(at + 2 * kGroup * DP + 32 + 8 * c);
-                const float2 v0 = lds64(at + 2 * kGroup * DP + 64 + 8 * c), v1 = lds64(at + 2 * kGroup * DP + 96 + 8 * c);
+                const float2* f = (const float2*)(at + 2 * kGroup * DP) + c;
+                const float2 k0 = f[0], k1 = f[4], v0 = f[8], v1 = f[12];
                 ks[0] = k0.x, ks[1] = k0.y, ks[2] = k1.x, ks[3] = k1.y, vs[0] = v0.x, vs[1] = v0.y, vs[2] = v1.x, vs[3] = v1.y;
             }
             const bool edge = j0 < all_first || j0 + kGroup - 1 > all_last;
@@ -302,13 +306,13 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) attention_few(AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int row = 8 * (k >> 1) + 2 * c + (k & 1);
-                const uint32_t va = at + kGroup * DP + row * DP;
+                const uint8_t* va = at + kGroup * DP + row * DP;
                 if (DP == 128) {
-                    const uint4 w = lds128(va + 16 * value_chunk<DP>(g, row));
+                    const uint4 w = *(const uint4*)(va + 16 * value_chunk<DP>(g, row));
                     b[k][0] = w.x, b[k][1] = w.y, b[k][VB / 4 - 2] = w.z, b[k][VB / 4 - 1] = w.w;
                 } else {
-                    const float2 w = lds64(va + 16 * value_chunk<DP>(g >> 1, row) + 8 * (g & 1));
-                    b[k][0] = __float_as_uint(w.x), b[k][1] = __float_as_uint(w.y);
+                    const uint2 w = *(const uint2*)(va + 16 * value_chunk<DP>(g >> 1, row) + 8 * (g & 1));
+                    b[k][0] = w.x, b[k][1] = w.y;
                 }
             }
 #pragma unroll
@@ -371,7 +375,7 @@ int run_few(const AttnArgs& a, cudaStream_t st) {
     constexpr int bytes = FewSmem<DP, STACK>::BYTES;
     const cudaError_t e = allow_smem(attention_few<DP, STACK>, bytes, done);
     if (e != cudaSuccess) return (int)e;
-    const int rc = (int)launch_dep(attention_few<DP, STACK>, dim3((unsigned)a.blocks), dim3(32 * kFewWarps), bytes, st, a);
+    const int rc = (int)launch_dep(attention_few<DP, STACK>, dim3((unsigned)a.blocks), dim3(32 * FewCfg<DP, STACK>::WARPS), bytes, st, a);
     if (rc) return rc;
     return (int)launch_dep(attention_join<16, DP>, dim3((unsigned)a.blocks, 4), dim3(128), 0, st, a);
 }
