@@ -47,7 +47,8 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int DP, bool STACK>
+// EXACT: the head has DP values, so that a group's rows lie at constant distances.
+template <int DP, bool STACK, bool EXACT>
 __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_few(AttnArgs a) {
     using C = FewCfg<DP, STACK>;
     constexpr int kFewWarps = C::WARPS, kFewStages = C::STAGES;
@@ -67,13 +68,96 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_fe
 
     Share<16, DP, 32 * kFewWarps> sh;
     if (!sh.find(a, (int64_t*)smem)) return;
-    if (a.dim != DP) {  // columns past the head's stay zero: no copy writes them
+    if (!EXACT) {  // columns past the head's stay zero: no copy writes them
         for (int i = lane; i < C::RING / 16; i += 32) *(uint4*)(smem + warp * C::RING + 16 * i) = make_uint4(0, 0, 0, 0);
         __syncwarp();
     }
     while (sh.more()) {
         const Item it = sh.item(a);
         const int rows = it.rows;
+        // ---- what each row sees, and what all rows do
+        int first[NR], last[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int row = g + 8 * r;
+            last[r] = row < rows ? it.pos + row / a.group : -1;
+            first[r] = a.window && last[r] >= a.window ? last[r] - a.window + 1 : 0;
+        }
+        const int all_last = it.pos, all_first = it.top_first;  // tokens within are seen by every row
+
+        float o[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        float m[NR], l[NR], fade[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f, fade[r] = 1.0f;
+        float unit = kLeastUnit, per_unit = 1.0f / kLeastUnit;
+#pragma unroll
+        for (int e = 0; e < S::VALS / 4; ++e) sums[e * 32 + lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+        const int g0 = it.from * 8 + warp, g1 = min(it.to * 8, (it.high - it.base + kGroup - 1) / kGroup);
+        const int steps = g0 < g1 ? (g1 - g0 + kFewWarps - 1) / kFewWarps : 0;
+        const int32_t* table = a.table + (int64_t)it.seq * a.table_s1;
+        int page = steps > 0 ? table[(it.base + kGroup * g0) >> a.page_log] : -1;
+        uint32_t there = 0;               // bit s: the group in stage s has a page
+        int issued = 0, to = 0;           // groups issued, and the next one's stage
+        int next = it.base + kGroup * g0;  // its first token
+        auto issue = [&]() {
+            if (issued < steps) {
+                const bool ok = (uint32_t)page < (uint32_t)a.pages;
+                there = (there & ~(1u << to)) | ((uint32_t)ok << to);
+                if (ok) {
+                    const int64_t at = ((((int64_t)page * a.heads) + it.head) << a.page_log) + (next & ((1 << a.page_log) - 1));
+                    constexpr int PR = 512 / DP;  // rows of one copy of the warp
+                    const int r0 = lane / (DP / 16), ch = lane % (DP / 16), dim = EXACT ? DP : a.dim;
+                    const int64_t from = (at + r0) * dim + 16 * ch;
+                    const uint8_t *pk = a.k + from, *pv = a.v + from;
+                    const uint32_t dst = ring + to * C::STAGE + r0 * DP;
+                    // (row r0 + PR i has r0's place among the swizzled pieces, but for values of 128 that of two)
+                    const uint32_t kd = dst + 16 * key_chunk<DP>(ch, r0), vd = dst + kGroup * DP + 16 * value_chunk<DP>(ch, r0);
+                    if (EXACT && next >= it.low && next + kGroup <= it.high) {
+#pragma unroll
+                        for (int i = 0; i < kGroup / PR; ++i) {
+                            copy16(kd + i * PR * DP, pk + i * PR * DP);
+                            copy16((vd ^ value_turn<DP>(i)) + i * PR * DP, pv + i * PR * DP);
+                        }
+                    } else if (EXACT || 16 * ch < dim) {
+#pragma unroll
+                        for (int i = 0; i < kGroup / PR; ++i) {
+                            const int j = next + r0 + PR * i;
+                            const bool in = j >= it.low && j < it.high;
+                            copy16(kd + i * PR * DP, pk + i * PR * dim, in);
+                            copy16((vd ^ value_turn<DP>(i)) + i * PR * DP, pv + i * PR * dim, in);
+                        }
+                    }
+                    if (lane < 8) copy16(ring + to * C::STAGE + 2 * kGroup * DP + 16 * lane, (lane < 4 ? a.ks : a.vs) + at + 4 * (lane & 3));
+                }
+                next += kFewWarps * kGroup;
+                if (issued + 1 < steps) page = table[next >> a.page_log];
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ++issued, to = to == kFewStages - 1 ? 0 : to + 1;
+        };
+        auto flush = [&]() {
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int e = 0; e < DP / 16; ++e) {  // half of the columns, four tiles
+                    float4 t = sums[(r * (DP / 16) + e) * 32 + lane];
+                    const int half = e / (DP / 32), j = 4 * (e % (DP / 32));
+                    float v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = STACK ? o[j + k][half] + o[j + k][2 + half] : o[j + k][2 * r + half];
+                    t.x = fmaf(t.x, fade[r], v[0]), t.y = fmaf(t.y, fade[r], v[1]), t.z = fmaf(t.z, fade[r], v[2]), t.w = fmaf(t.w, fade[r], v[3]);
+                    sums[(r * (DP / 16) + e) * 32 + lane] = t;
+                }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) fade[r] = 1.0f;
+        };
+#pragma unroll
+        for (int s = 0; s < kFewStages - 1; ++s) issue();
         // ---- queries: operand fragments and each row's factor to log2 units
         uint32_t qf[QF][4 * KI][4];
         float rf[NR];
@@ -115,82 +199,14 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_fe
                     }
                 }
         }
-        // ---- what each row sees, and what all rows do
-        int first[NR], last[NR];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const int row = g + 8 * r;
-            last[r] = row < rows ? it.pos + row / a.group : -1;
-            first[r] = a.window && last[r] >= a.window ? last[r] - a.window + 1 : 0;
-        }
-        const int all_last = it.pos, all_first = it.top_first;  // tokens within are seen by every row
-
-        float o[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        float m[NR], l[NR], fade[NR];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f, fade[r] = 1.0f;
-        float unit = kLeastUnit, per_unit = 1.0f / kLeastUnit;
-#pragma unroll
-        for (int e = 0; e < S::VALS / 4; ++e) sums[e * 32 + lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-
-        const int g0 = it.from * 8 + warp, g1 = min(it.to * 8, (it.high - it.base + kGroup - 1) / kGroup), steps = g0 < g1 ? (g1 - g0 + kFewWarps - 1) / kFewWarps : 0;
-        const int32_t* table = a.table + (int64_t)it.seq * a.table_s1;
-        int page = steps > 0 ? table[(it.base + kGroup * g0) >> a.page_log] : -1;
-        uint32_t there = 0;  // bit s: the group in stage s has a page
-        int issued = 0, to = 0;  // groups issued, and the next one's stage
-        auto issue = [&]() {
-            if (issued < steps) {
-                const int j0 = it.base + kGroup * (g0 + kFewWarps * issued), st = to;
-                const bool ok = (uint32_t)page < (uint32_t)a.pages;
-                there = (there & ~(1u << st)) | ((uint32_t)ok << st);
-                if (ok) {
-                    const int64_t at = ((((int64_t)page * a.heads) + it.head) << a.page_log) + (j0 & ((1 << a.page_log) - 1));
-                    const uint32_t dst = ring + st * C::STAGE;
-                    constexpr int PR = 512 / DP;  // rows of one copy of the warp
-                    const int r0 = lane / (DP / 16), ch = lane % (DP / 16);
-#pragma unroll
-                    for (int i = 0; i < kGroup / PR; ++i) {
-                        const int row = r0 + PR * i, j = j0 + row;
-                        const bool in = j >= it.low && j < it.high;
-                        if (16 * ch < a.dim) {
-                            copy16(dst + row * DP + 16 * key_chunk<DP>(ch, row), a.k + (at + row) * a.dim + 16 * ch, in);
-                            copy16(dst + kGroup * DP + row * DP + 16 * value_chunk<DP>(ch, row), a.v + (at + row) * a.dim + 16 * ch, in);
-                        }
-                    }
-                    if (lane < 8) copy16(dst + 2 * kGroup * DP + 16 * lane, (lane < 4 ? a.ks : a.vs) + at + 4 * (lane & 3), true);
-                }
-                if (issued + 1 < steps) page = table[(j0 + kFewWarps * kGroup) >> a.page_log];
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            ++issued, to = to == kFewStages - 1 ? 0 : to + 1;
-        };
-        auto flush = [&]() {
-#pragma unroll
-            for (int r = 0; r < NR; ++r)
-#pragma unroll
-                for (int e = 0; e < DP / 16; ++e) {  // half of the columns, four tiles
-                    float4 t = sums[(r * (DP / 16) + e) * 32 + lane];
-                    const int half = e / (DP / 32), j = 4 * (e % (DP / 32));
-                    float v[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = STACK ? o[j + k][half] + o[j + k][2 + half] : o[j + k][2 * r + half];
-                    t.x = fmaf(t.x, fade[r], v[0]), t.y = fmaf(t.y, fade[r], v[1]), t.z = fmaf(t.z, fade[r], v[2]), t.w = fmaf(t.w, fade[r], v[3]);
-                    sums[(r * (DP / 16) + e) * 32 + lane] = t;
-                }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-#pragma unroll
-            for (int r = 0; r < NR; ++r) fade[r] = 1.0f;
-        };
-#pragma unroll
-        for (int s = 0; s < kFewStages - 1; ++s) issue();
+        int first_token = it.base + kGroup * g0;
+        const int key0 = g * DP + 16 * key_chunk<DP>(c, g), value0 = kGroup * DP + 2 * c * DP + 16 * value_chunk<DP>(DP == 128 ? g : g >> 1, 2 * c) + (DP == 128 ? 0 : 8 * (g & 1));
         for (int i = 0, st = kFewStages - 1; i < steps; ++i) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
             __syncwarp();
-            const int j0 = it.base + kGroup * (g0 + kFewWarps * i);
             st = st == kFewStages - 1 ? 0 : st + 1;
+            const int j0 = first_token;
+            first_token += kFewWarps * kGroup;
             const bool has = there >> st & 1;
             issue();
             if (!has) continue;  // (the same for the whole warp)
@@ -202,7 +218,7 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_fe
                 s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
 #pragma unroll
                 for (int p = 0; p < KI; ++p) {
-                    const uint4 w = *(const uint4*)(at + (8 * t + g) * DP + 16 * key_chunk<DP>(4 * p + c, 8 * t + g));
+                    const uint4 w = *(const uint4*)(at + 8 * t * DP + (key0 ^ 64 * p));  // (piece 4 p + c of row 8 t + g)
                     const uint32_t b[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -305,13 +321,12 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_fe
             uint32_t b[4][VB / 4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int row = 8 * (k >> 1) + 2 * c + (k & 1);
-                const uint8_t* va = at + kGroup * DP + row * DP;
+                const uint8_t* va = at + value0 + (8 * (k >> 1) + (k & 1)) * DP;  // row 8 (k / 2) + 2 c + k % 2
                 if (DP == 128) {
-                    const uint4 w = *(const uint4*)(va + 16 * value_chunk<DP>(g, row));
+                    const uint4 w = *(const uint4*)va;
                     b[k][0] = w.x, b[k][1] = w.y, b[k][VB / 4 - 2] = w.z, b[k][VB / 4 - 1] = w.w;
                 } else {
-                    const uint2 w = *(const uint2*)(va + 16 * value_chunk<DP>(g >> 1, row) + 8 * (g & 1));
+                    const uint2 w = *(const uint2*)va;
                     b[k][0] = w.x, b[k][1] = w.y;
                 }
             }
@@ -369,15 +384,21 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_fe
     }
 }
 
-template <int DP, bool STACK>
+template <int DP, bool STACK, bool EXACT>
 int run_few(const AttnArgs& a, cudaStream_t st) {
     static bool done[64];
     constexpr int bytes = FewSmem<DP, STACK>::BYTES;
-    const cudaError_t e = allow_smem(attention_few<DP, STACK>, bytes, done);
+    const cudaError_t e = allow_smem(attention_few<DP, STACK, EXACT>, bytes, done);
     if (e != cudaSuccess) return (int)e;
-    const int rc = (int)launch_dep(attention_few<DP, STACK>, dim3((unsigned)a.blocks), dim3(32 * FewCfg<DP, STACK>::WARPS), bytes, st, a);
+    const int rc = (int)launch_dep(attention_few<DP, STACK, EXACT>, dim3((unsigned)a.blocks), dim3(32 * FewCfg<DP, STACK>::WARPS), bytes, st, a);
     if (rc) return rc;
     return (int)launch_dep(attention_join<16, DP>, dim3((unsigned)a.blocks, 4), dim3(128), 0, st, a);
+}
+
+template <int DP>
+int few(const AttnArgs& a, cudaStream_t st) {
+    if (a.most <= 8) return a.dim == DP ? run_few<DP, true, true>(a, st) : run_few<DP, true, false>(a, st);
+    return a.dim == DP ? run_few<DP, false, true>(a, st) : run_few<DP, false, false>(a, st);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -430,8 +451,7 @@ extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, int* 
     }
     if (!rc && f.few) {
         a.least = 1, a.most = f.few;
-        const bool stack = f.few <= 8;
-        rc = wide ? stack ? run_few<128, true>(a, st) : run_few<128, false>(a, st) : stack ? run_few<64, true>(a, st) : run_few<64, false>(a, st);
+        rc = wide ? few<128>(a, st) : few<64>(a, st);
         *launches += 2;
     }
     return rc;

@@ -46,8 +46,8 @@ __device__ __forceinline__ float2 lds64(uint32_t a) {
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ float4 load4(const float* p, int vec) {
     if (vec) return *(const float4*)p;
@@ -106,6 +106,11 @@ template <int DP>
 __device__ __forceinline__ int value_chunk(int ch, int row) {
     return DP == 128 ? ch ^ (row & 6) : ch ^ (row >> 1 & 3);
 }
+// What the place of a piece of values changes by, in bytes, from row r0 to row r0 + i 512 / DP (r0 below 512 / DP).
+template <int DP>
+__device__ __forceinline__ constexpr uint32_t value_turn(int i) {
+    return DP == 128 ? 16 * (4 * i & 6) : 0;
+}
 
 // One item: up to MAX rows (new token, query head of the group) of a sequence and kv head, and this block's part of the
 // tokens that they see.  Row r of the item is row first_row + r of the sequence's rows, of token (first_row + r) / group.
@@ -154,104 +159,92 @@ __device__ __forceinline__ float* part_slot(const AttnArgs& a, int max, int dp, 
     return a.parts + (2 * block + which) * part_floats(max, dp);
 }
 
+// a / b for a below 2^53, b above 0: the f64 quotient is off by one at most.  (The compiler's 64-bit division is a long way round.)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    int64_t q = (int64_t)((double)a / (double)b);
+    const int64_t r = a - q * b;
+    return r < 0 ? q - 1 : r >= b ? q + 1 : q;
+}
+
 // A block's share of all units, in the order sequence, kv head, tile, tokens: equal shares, so that ragged lengths load
 // the GPU evenly whatever the lengths are, which only the device knows.  An item that a share's end cuts is joined from its
-// parts afterwards.  THREADS threads of the block call every member together.
+// parts afterwards.  THREADS threads of the block look for its first item together; each of them, or some, then goes on alone.
 template <int MAX, int DP, int THREADS>
 struct Share {
-    static constexpr int SEQS = 1024;  // sequences looked at together
-    static constexpr int SMEM = SEQS * 8 + 32 * 8 + 32;
-    int64_t total, at, left, blocks, tile;
-    int seq, head, off;
+    static constexpr bool BY_WARP = MAX > 16;  // a sequence has many tiles: the lanes of a warp share them
+    static constexpr int WARPS = THREADS / 32, SMEM = 32 * 8 + 32;
+    int64_t total, at, left, tile;
+    int blocks, seq, head, off;
 
-    // Units of one kv head of sequence s.  MAX = 16: one tile, each thread another sequence; else a warp's lanes share the tiles.
-    __device__ static int64_t seq_units(const AttnArgs& a, int s, bool by_warp) {
-        const Seq q(a, s);
+    // Units of one kv head of a sequence.
+    __device__ static int64_t seq_units(const AttnArgs& a, const Seq& q) {
         const int64_t n = tiles_of<MAX>(a, q);
         int64_t u = 0;
         int lo, hi;
-        for (int64_t t = by_warp ? threadIdx.x & 31 : 0; t < n; t += by_warp ? 32 : 1) u += span_of<MAX>(a, q, t, lo, hi);
-        if (by_warp)
+        if (!BY_WARP) return n ? span_of<MAX>(a, q, 0, lo, hi) : 0;
+        for (int64_t t = threadIdx.x & 31; t < n; t += 32) u += span_of<MAX>(a, q, t, lo, hi);
 #pragma unroll
-            for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+        for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
         return u;
     }
-    // Fills sh[0 .. SEQS) with the units of sequences from `first`; returns this thread's sum of its run of them, its
-    // exclusive prefix and the sum of all.
-    __device__ void chunk(const AttnArgs& a, int first, int64_t* sh, int64_t& mine, int64_t& before, int64_t& all) const {
-        constexpr int RUN = (SEQS + THREADS - 1) / THREADS;
-        int64_t* warps = sh + SEQS;
-        const int n = min(SEQS, a.seqs - first), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        __syncthreads();
-        if (MAX <= 16) {
-            for (int i = threadIdx.x; i < n; i += THREADS) sh[i] = seq_units(a, first + i, false) * a.heads;
-        } else {
-            for (int i = warp; i < n; i += THREADS / 32) {
-                const int64_t u = seq_units(a, first + i, true);
-                if (lane == 0) sh[i] = u * a.heads;
-            }
-        }
-        __syncthreads();
-        mine = 0;
-#pragma unroll
-        for (int i = 0; i < RUN; ++i)
-            if (threadIdx.x * RUN + i < n) mine += sh[threadIdx.x * RUN + i];
-        int64_t inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += t;
-        }
-        if (lane == 31) warps[warp] = inc;
-        __syncthreads();
-        before = inc - mine, all = 0;
-#pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) {
-            if (w < warp) before += warps[w];
-            all += warps[w];
-        }
-    }
+    // The first unit of block b.
+    __device__ int64_t begin_of(int b) const { return quotient(total * b, blocks); }
     // Finds the block's first item; false when the block has no work.  sh: SMEM bytes of shared memory.
     __device__ bool find(const AttnArgs& a, int64_t* sh) {
-        constexpr int RUN = (SEQS + THREADS - 1) / THREADS;
-        int64_t* found = sh + SEQS + 32;
-        int64_t mine = 0, before = 0, all = 0;
+        int64_t* found = sh + 32;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         if (threadIdx.x == 0) *(int*)slot(a, 0) = *(int*)slot(a, 1) = 0;
-        total = 0;
-        for (int s = 0; s < a.seqs; s += SEQS) {
-            chunk(a, s, sh, mine, before, all);
-            total += all;
-        }
-        blocks = min((int64_t)gridDim.x, total);  // each has a unit at least, so that an item's parts lie in consecutive blocks
-        if (blockIdx.x >= blocks) return false;
-        at = total * blockIdx.x / blocks;
-        left = total * (blockIdx.x + 1) / blocks - at;
-        int64_t run = 0;
-        for (int s = 0; s < a.seqs; s += SEQS) {
-            if (a.seqs > SEQS) chunk(a, s, sh, mine, before, all);
-            if (at >= run + before && at < run + before + mine) {
-                int64_t x = at - run - before;
-                int i = threadIdx.x * RUN;
-                for (; x >= sh[i]; ++i) x -= sh[i];
-                found[0] = s + i, found[1] = x, found[2] = sh[i] / a.heads;
+        // each thread (or warp) has a run of sequences
+        const int workers = BY_WARP ? WARPS : THREADS, me = BY_WARP ? warp : threadIdx.x;
+        const int run = (a.seqs + workers - 1) / workers, s0 = min(me * run, a.seqs), s1 = min(s0 + run, a.seqs);
+        int64_t mine = 0;
+#pragma unroll 1
+        for (int s = s0; s < s1; ++s) mine += seq_units(a, Seq(a, s)) * a.heads;
+        int64_t inc = mine;
+        if (!BY_WARP) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += t;
             }
-            run += all;
-            if (at < run) break;
+        }
+        if (lane == 31) sh[warp] = inc;
+        __syncthreads();
+        int64_t before = 0;
+        total = lane < WARPS ? sh[lane] : 0;
+        before = lane < warp ? total : 0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o), before += __shfl_xor_sync(0xffffffffu, before, o);
+        before += inc - mine;
+        blocks = (int)min((int64_t)gridDim.x, total);  // each has a unit at least, so that an item's parts lie in consecutive blocks
+        if ((int)blockIdx.x >= blocks) return false;
+        at = begin_of(blockIdx.x);
+        left = begin_of(blockIdx.x + 1) - at;
+        if (at >= before && at < before + mine) {
+            int64_t x = at - before, u = 0;
+            int s = s0;
+#pragma unroll 1
+            for (; s < s1; ++s) {
+                u = seq_units(a, Seq(a, s));
+                if (x < u * a.heads) break;
+                x -= u * a.heads;
+            }
+            if (!BY_WARP || lane == 0) found[0] = s, found[1] = x, found[2] = u;
         }
         __syncthreads();
         seq = (int)found[0];
         const int64_t x = found[1], per = found[2];
-        head = (int)(x / per);
+        head = (int)quotient(x, per);
         int64_t rest = x - head * per;
         tile = 0;
-        if (MAX > 16) {  // (each warp for itself)
+        if (BY_WARP) {  // (each warp for itself)
             const Seq q(a, seq);
             const int64_t n = tiles_of<MAX>(a, q);
-            const int lane = threadIdx.x & 31;
+#pragma unroll 1
             for (;; tile += 32) {
                 int lo, hi;
                 const int64_t u = tile + lane < n ? span_of<MAX>(a, q, tile + lane, lo, hi) : 0;
-                int64_t inc = u;
+                inc = u;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
@@ -303,8 +296,11 @@ struct Share {
     }
     // The block that holds the last unit of the item that begins at unit `at`.
     __device__ int last_block(const Item& it) const {
-        const int64_t end = at - it.from + it.units;
-        return (int)((end * blocks + total - 1) / total) - 1;
+        const int64_t x = at - it.from + it.units - 1;
+        int b = (int)quotient((x + 1) * blocks, total);
+        while (begin_of(b) > x) --b;
+        while (begin_of(b + 1) <= x) ++b;
+        return b;
     }
     __device__ static float* slot(const AttnArgs& a, int which) { return part_slot(a, MAX, DP, blockIdx.x, which); }
 };
