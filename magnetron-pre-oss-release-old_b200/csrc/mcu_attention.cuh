@@ -126,6 +126,7 @@ struct Item {
 // Tokens that the rows [first_row, first_row + rows) of a sequence see together.
 struct Seq {
     int row0, n, take, length;  // take: rows of q that are taken (at most max_new)
+    __device__ Seq() {}
     __device__ Seq(const AttnArgs& a, int s) {
         row0 = min(max(a.start[s], 0), a.rows);
         const int end = min(max(a.start[s + 1], row0), a.rows);
@@ -159,8 +160,10 @@ __device__ __forceinline__ float* part_slot(const AttnArgs& a, int max, int dp, 
     return a.parts + (2 * block + which) * part_floats(max, dp);
 }
 
-// a / b for a below 2^53, b above 0: the f64 quotient is off by one at most.  (The compiler's 64-bit division is a long way round.)
+// a / b for a from 0 to 2^53, b above 0: in 32 bits where both fit, else the f64 quotient, which is off by one at most.  (The
+// compiler's 64-bit division is a long way round.)
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
     int64_t q = (int64_t)((double)a / (double)b);
     const int64_t r = a - q * b;
     return r < 0 ? q - 1 : r >= b ? q + 1 : q;
@@ -172,9 +175,10 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 template <int MAX, int DP, int THREADS>
 struct Share {
     static constexpr bool BY_WARP = MAX > 16;  // a sequence has many tiles: the lanes of a warp share them
-    static constexpr int WARPS = THREADS / 32, SMEM = 32 * 8 + 32;
+    static constexpr int WARPS = THREADS / 32, SMEM = 32 * 8 + 48;
     int64_t total, at, left, tile;
     int blocks, seq, head, off;
+    Seq here;  // the sequence at hand
 
     // Units of one kv head of a sequence.
     __device__ static int64_t seq_units(const AttnArgs& a, const Seq& q) {
@@ -223,27 +227,33 @@ struct Share {
         if (at >= before && at < before + mine) {
             int64_t x = at - before, u = 0;
             int s = s0;
+            Seq q;
 #pragma unroll 1
             for (; s < s1; ++s) {
-                u = seq_units(a, Seq(a, s));
+                q = Seq(a, s);
+                u = seq_units(a, q);
                 if (x < u * a.heads) break;
                 x -= u * a.heads;
             }
-            if (!BY_WARP || lane == 0) found[0] = s, found[1] = x, found[2] = u;
+            if (!BY_WARP || lane == 0) {
+                found[0] = s, found[1] = x, found[2] = u;
+                *(int4*)(found + 4) = make_int4(q.row0, q.n, q.take, q.length);
+            }
         }
         __syncthreads();
         seq = (int)found[0];
+        const int4 h = *(const int4*)(found + 4);
+        here.row0 = h.x, here.n = h.y, here.take = h.z, here.length = h.w;
         const int64_t x = found[1], per = found[2];
         head = (int)quotient(x, per);
         int64_t rest = x - head * per;
         tile = 0;
         if (BY_WARP) {  // (each warp for itself)
-            const Seq q(a, seq);
-            const int64_t n = tiles_of<MAX>(a, q);
+            const int64_t n = tiles_of<MAX>(a, here);
 #pragma unroll 1
             for (;; tile += 32) {
                 int lo, hi;
-                const int64_t u = tile + lane < n ? span_of<MAX>(a, q, tile + lane, lo, hi) : 0;
+                const int64_t u = tile + lane < n ? span_of<MAX>(a, here, tile + lane, lo, hi) : 0;
                 inc = u;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -267,7 +277,7 @@ struct Share {
     }
     __device__ bool more() const { return left > 0; }
     __device__ Item item(const AttnArgs& a) const {
-        const Seq q(a, seq);
+        const Seq& q = here;
         Item it;
         it.seq = seq, it.head = head, it.row0 = q.row0;
         it.first_row = (int)(tile * MAX);
@@ -285,13 +295,15 @@ struct Share {
         if (left <= 0) return;
         if (MAX > 16) {
             ++tile;
-            if (tile < tiles_of<MAX>(a, Seq(a, seq))) return;
+            if (tile < tiles_of<MAX>(a, here)) return;
         }
         tile = 0;
         if (++head < a.heads) return;
         head = 0;
-        while (++seq < a.seqs)
-            if (Seq(a, seq).take) return;
+        while (++seq < a.seqs) {
+            here = Seq(a, seq);
+            if (here.take) return;
+        }
         left = 0;  // (not reached: the shares add up to all units)
     }
     // The block that holds the last unit of the item that begins at unit `at`.

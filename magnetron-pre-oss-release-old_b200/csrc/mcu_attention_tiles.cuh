@@ -16,21 +16,21 @@ using namespace mcu;
 // two operands' shared-memory reads: 2 x 128 columns of S, over which P is written in place, 128 of O, 128 of Q.  O starts
 // from zero for every 128 tokens and is added in registers in f32 (rounded to nearest), times the step of the row's reference and
 // the unit of the tile's value scales: no accumulator is ever rescaled, and the tensor core's truncating sums stay short.
-//   warps 0-15   softmax: warp w has the rows 32 (w & 3) .. and quarter w / 4 of the tokens
-//   warps 16-19  sums: O of each tile, in turn, to the rows' f32 sums in registers; the output at the end
-//   warps 20-23  loaders: e4m3 from the pages by cp.async, two tiles ahead, then to f16 tiles (128-byte swizzle)
-//   warp 24      issues the products: S of tile j + 1 before O of tile j
-//   warp 25      plans: puts the block's items into a ring, so that the others find theirs without global loads
-//   warp 26      guides: each tile's places in the pages and its scales, up to four tiles ahead
+//   warps 0-7    softmax: warp w has the rows 32 (w & 3) .. and half w / 4 of the tokens
+//   warps 8-11   sums: O of each tile, in turn, to the rows' f32 sums in registers; the output at the end
+//   warps 12-15  loaders: e4m3 from the pages by cp.async, two tiles ahead, then to f16 tiles (128-byte swizzle)
+//   warp 16      issues the products: S of tile j + 1 before O of tile j
+//   warp 17      plans: puts the block's items into a ring, so that the others find theirs without global loads
+//   warp 18      guides: each tile's places in the pages and its scales, up to four tiles ahead
 // What bounds it is the softmax: about 14 instructions for two logits (390 cycles for 32 x 32 of them with four warps a
 // scheduler, alone), more than the products' 2 x 1024 cycles a tile.  The loops of all roles have to fit the SM's instruction cache
 // together: unrolled for 128 columns they took three times as long.
-constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 896;
-constexpr int kSoftWarps = 16, kSumWarp = 16, kLoadWarp = 20, kIssueWarp = 24, kPlanWarp = 25, kGuideWarp = 26;
-constexpr int kTileLaunch = 72, kSoftRegs = 56, kSumRegs = 168, kLoadRegs = 64, kIssueRegs = 48;
-static_assert(4 * kSoftRegs + kSumRegs + kLoadRegs + kIssueRegs == 7 * kTileLaunch, "register split must match the launch");
+constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 640;
+constexpr int kSoftWarps = 8, kLoadWarp = 12, kIssueWarp = 16, kPlanWarp = 17, kGuideWarp = 18;  // (sums from kSoftWarps on)
+constexpr int kTileLaunch = 96, kSoftRegs = 104, kSumRegs = 168, kLoadRegs = 56, kIssueRegs = 48;
+static_assert(kSoftRegs >= kTileLaunch && kSumRegs >= kTileLaunch && kLoadRegs <= kTileLaunch && kIssueRegs <= kTileLaunch, "inc or dec as the code has it");
+static_assert(2 * kSoftRegs + kSumRegs + kLoadRegs + kIssueRegs == 5 * kTileLaunch, "register split must match the launch");
 constexpr int kSoftThreads = 32 * kSoftWarps;
-constexpr uint32_t kGiveUp = 25000;   // sleeps of a wait, and the flag that ends all waits
 constexpr int kItems = 4;             // items in the planner's ring
 
 // What the roles need of an item, as the planner leaves it; rows = 0: no more.
@@ -51,12 +51,12 @@ struct TileCfg {
     static constexpr int RAW_TILE = TILE / 2;
     static constexpr int SCALES = RAW + 4 * RAW_TILE;        // 4 x {keys' scales, values' ratios, valid tokens, unit}
     static constexpr int SLOT = 2 * kTileTokens * 4 + 32;
-    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][4][128]: of a tile's logits, by quarter
-    static constexpr int SUMS = MAXIMA + 2 * 4 * 128 * 4;    // [4][128]: queries' maxima, by quarter
-    static constexpr int REFS = SUMS + 4 * 128 * 4;          // [4][128] of (maximum, unit): what a tile's O is relative to
+    static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][2][128]: of a tile's logits, by half
+    static constexpr int SUMS = MAXIMA + 2 * 2 * 128 * 4;    // [2][128]: queries' maxima, by half
+    static constexpr int REFS = SUMS + 2 * 128 * 4;          // [4][128] of (maximum, unit): what a tile's O is relative to
     static constexpr int FACTORS = REFS + 4 * 128 * 8;       // [4][128]: rf of an item's rows
-    static constexpr int STATS = FACTORS + 4 * 128 * 4;      // [4][128]: an item's sums, by quarter
-    static constexpr int PLACES = STATS + 4 * 128 * 4;   // 4 x {8 groups' offsets in the pages, valid tokens}
+    static constexpr int STATS = FACTORS + 4 * 128 * 4;      // [2][128]: an item's sums, by half
+    static constexpr int PLACES = STATS + 2 * 128 * 4;   // 4 x {8 groups' offsets in the pages, valid tokens}
     static constexpr int PLACE = 8 * 8 + 16;
     static constexpr int ITEMS = PLACES + 4 * PLACE;
     static constexpr int BARS = ITEMS + kItems * 64;
@@ -71,29 +71,21 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// The whole warp waits, asleep on the barrier for up to 20 us at a time and half a second in all, or until a wait was given up
-// elsewhere.  A loop of few instructions: it stands at some twenty places.
+// The whole warp waits, for up to half a second or until a wait was given up elsewhere.  A loop of few instructions: it stands at
+// some twenty places.  NAP: how many ns to sleep between two looks, for roles that run ahead (their looks would take issue slots from
+// the warps that compute).
+template <int NAP = 0>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .u32 n, f;\n\t"
-        "mov.u32 n, 0;\n\t"
-        "WAIT_%=:\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t"
-        "@p bra DONE_%=;\n\t"
-        "ld.volatile.shared.u32 f, [%3];\n\t"
-        "add.u32 n, n, 1;\n\t"
-        "add.u32 f, f, n;\n\t"
-        "setp.lt.u32 p, f, %5;\n\t"
-        "@p bra WAIT_%=;\n\t"
-        "DONE_%=:\n\t}\n"
-        : "=&r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32((const void*)ab.flag)), "r"(20000u), "r"(kGiveUp)
-        : "memory");
+    constexpr uint32_t kLooks = NAP ? 500000000u / (NAP + 50) : 1u << 23;
+    uint32_t ok, n = 0;
+    while (true) {
+        ok = mbar_test(bar, parity);
+        if (ok || ++n == kLooks || ((NAP || (n & 63) == 0) && *ab.flag)) break;
+        if (NAP) __nanosleep(NAP);
+    }
     __syncwarp();
     if (!ok && (threadIdx.x & 31) == 0 && !*ab.flag) {
-        *ab.flag = (int)kGiveUp;
+        *ab.flag = 1;
         atomicCAS(ab.status, 0, code);
     }
     return __all_sync(0xffffffffu, ok);
@@ -295,15 +287,15 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     if (!work) {
         // nothing to do but to free TMEM
     } else if (warp < kSoftWarps) {  // ---- softmax
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-        constexpr int QD = DP / 4;  // this thread's values of a query
-        const int quarter = warp >> 2, row = 32 * (warp & 3) + lane, four = 1 + (warp & 3);  // barrier of a row's four warps
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+        constexpr int QD = DP / 2;  // this thread's values of a query
+        const int half = warp >> 2, row = 32 * (warp & 3) + lane, pair = 1 + (warp & 3);  // barrier of a row's two warps
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         float* const maxima = (float*)(smem + C::MAXIMA) + row;
         uint32_t t = 0;  // tiles before the item's
 #pragma unroll 1
         for (uint32_t i = 0;; ++i) {
-            const TileItem it = item(i, four, 128);
+            const TileItem it = item(i, pair, 64);
             if (!it.rows) break;
             const int r = it.first_row + row;
             const bool live = row < it.rows;
@@ -311,33 +303,32 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             if (it.n) {
                 // the queries, as two f16 in TMEM, once the products that read the last item's are done
                 const float* p = a.q + (int64_t)(it.row0 + (live ? r / a.group : 0)) * a.q_s1 +
-                                 (int64_t)(it.head * a.group + (live ? r % a.group : 0)) * a.dim + QD * quarter;
+                                 (int64_t)(it.head * a.group + (live ? r % a.group : 0)) * a.dim + QD * half;
                 float* sums = (float*)(smem + C::SUMS) + row;
                 uint32_t top = 0;
                 float x[QD];
                 if (a.q_vec) {
 #pragma unroll
                     for (int k = 0; k < QD / 4; ++k) {
-                        const float4 v = live && QD * quarter + 4 * k < a.dim ? *(const float4*)(p + 4 * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        const float4 v = live && QD * half + 4 * k < a.dim ? *(const float4*)(p + 4 * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
                     }
                 } else {
 #pragma unroll
-                    for (int k = 0; k < QD; ++k) x[k] = live && QD * quarter + k < a.dim ? p[k] : 0.0f;
+                    for (int k = 0; k < QD; ++k) x[k] = live && QD * half + k < a.dim ? p[k] : 0.0f;
                 }
 #pragma unroll
                 for (int k = 0; k < QD; ++k) top = max(top, abs_bits(x[k]));
-                sums[quarter * 128] = __uint_as_float(top);
-                bar_named(four, 128);
-#pragma unroll
-                for (int k = 1; k < 4; ++k) top = max(top, __float_as_uint(sums[(quarter ^ k) * 128]));
-                bar_named(four, 128);
+                sums[half * 128] = __uint_as_float(top);
+                bar_named(pair, 64);
+                top = max(top, __float_as_uint(sums[(half ^ 1) * 128]));
+                bar_named(pair, 64);
                 const float up = query_unit(top);
                 if (t) {
                     warp_wait(&s_full[(t - 1) & 1], (t - 1) >> 1 & 1, ab, 43);
                     tc_fence_after();
                 }
-                const uint32_t at = tmem + lanes + C::Q_COL + QD / 2 * quarter;
+                const uint32_t at = tmem + lanes + C::Q_COL + QD / 2 * half;
 #pragma unroll
                 for (int c = 0; c < QD / 16; ++c) {
                     uint32_t h[8], lo[8];
@@ -348,7 +339,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 }
                 tmem_st_done();
                 rf = fmaxf(a.scale * kLog2e / up, 0x1p-126f);  // (above zero, so that -inf times it is -inf)
-                if (quarter == 0) ((float*)(smem + C::FACTORS))[(i & 3) * 128 + row] = rf;
+                if (half == 0) ((float*)(smem + C::FACTORS))[(i & 3) * 128 + row] = rf;
                 tc_fence_before();
                 mbar_arrive(q_full);
             }
@@ -358,71 +349,80 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
 #pragma unroll 1
             for (int j = 0; j < it.n; ++j, ++t) {
                 const uint8_t* slot = smem + C::SCALES + (t & 3) * C::SLOT;
-                const ulonglong2* ks = (const ulonglong2*)(slot + 32 * quarter * 4);
-                const ulonglong2* vs = (const ulonglong2*)(slot + (kTileTokens + 32 * quarter) * 4);
-                const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 32 * quarter;
+                const ulonglong2* ks = (const ulonglong2*)(slot + 64 * half * 4);
+                const ulonglong2* vs = (const ulonglong2*)(slot + (kTileTokens + 64 * half) * 4);
+                const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 64 * half;
                 const int j0 = it.first + kTileTokens * j;
                 warp_wait(&sc_full[t & 3], t >> 2 & 1, ab, 32);
                 const uint4 ok = *(const uint4*)(slot + 2 * kTileTokens * 4);
                 warp_wait(&s_full[t & 1], t >> 1 & 1, ab, 33);
                 tc_fence_after();
-                uint32_t v[32];
-                tmem_ld32(sc, v);
-                uint64_t s[16];
+                uint64_t s[32];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const ulonglong2 kk = ks[k];
-                    s[2 * k] = mul2(pair_of(v[4 * k], v[4 * k + 1]), kk.x);
-                    s[2 * k + 1] = mul2(pair_of(v[4 * k + 2], v[4 * k + 3]), kk.y);
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(sc + 32 * c, v);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const ulonglong2 kk = ks[8 * c + k];
+                        s[16 * c + 2 * k] = mul2(pair_of(v[4 * k], v[4 * k + 1]), kk.x);
+                        s[16 * c + 2 * k + 1] = mul2(pair_of(v[4 * k + 2], v[4 * k + 3]), kk.y);
+                    }
                 }
                 // not all tokens seen by all rows
                 if (j0 < it.all_first || j0 + kTileTokens - 1 > it.all_last || (ok.x & ok.y & ok.z & ok.w) != 0xffffffffu) {
-                    const int lo = max(first - j0 - 32 * quarter, 0), hi = min(last - j0 - 32 * quarter, 31);  // those of this quarter
-                    const uint32_t bits = quarter & 2 ? (quarter & 1 ? ok.w : ok.z) : (quarter & 1 ? ok.y : ok.x);
-                    const uint32_t seen = lo > hi ? 0u : bits & (0xffffffffu << lo) & (0xffffffffu >> (31 - hi));
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        float x, y;
-                        unpair(s[k], x, y);
-                        s[k] = pair_of(seen >> (2 * k) & 1 ? x : -INFINITY, seen >> (2 * k + 1) & 1 ? y : -INFINITY);
+                    for (int c = 0; c < 2; ++c) {
+                        const int at = j0 + 64 * half + 32 * c, lo = max(first - at, 0), hi = min(last - at, 31);
+                        const uint32_t bits = half ? (c ? ok.w : ok.z) : (c ? ok.y : ok.x);
+                        const uint32_t seen = lo > hi ? 0u : bits & (0xffffffffu << lo) & (0xffffffffu >> (31 - hi));
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            float x, y;
+                            unpair(s[16 * c + k], x, y);
+                            s[16 * c + k] = pair_of(seen >> (2 * k) & 1 ? x : -INFINITY, seen >> (2 * k + 1) & 1 ? y : -INFINITY);
+                        }
                     }
                 }
                 // the rows' maxima
                 float x = -INFINITY, y = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < 16; k += 2) {
+                for (int k = 0; k < 32; k += 2) {
                     float p, q;
                     unpair(s[k], p, q);
                     x = max3(x, p, q);
                     unpair(s[k + 1], p, q);
                     y = max3(y, p, q);
                 }
-                float* mine = maxima + (t & 1) * 512;
-                mine[quarter * 128] = fmaxf(x, y);
-                bar_named(four, 128);
-                x = fmaxf(max3(mine[0], mine[128], mine[256]), mine[384]);
+                float* mine = maxima + (t & 1) * 256;
+                mine[half * 128] = fmaxf(x, y);
+                bar_named(pair, 64);
+                x = fmaxf(mine[0], mine[128]);
                 if (x > m) {
                     l *= m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
                     m = x;
                 }
-                if (quarter == 0) ((float2*)(smem + C::REFS))[(t & 3) * 128 + row] = make_float2(m, *(const float*)(slot + 2 * kTileTokens * 4 + 16));
+                if (half == 0) ((float2*)(smem + C::REFS))[(t & 3) * 128 + row] = make_float2(m, *(const float*)(slot + 2 * kTileTokens * 4 + 16));
                 const float ref = m == -INFINITY ? 0.0f : -m;
                 const uint64_t ref2 = pair_of(ref, ref);
                 uint64_t sum = 0;
-                uint32_t h[16], lo[16];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const ulonglong2 vv = vs[k];
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t h[16], lo[16];
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        unpair(fma2(add2(s[2 * k + q], ref2), rf2, top2), x, y);
-                        const uint64_t p = pair_of(exp2_f(x), exp2_f(y));
-                        sum = add2(sum, p);
-                        split_pair(mul2(p, q ? vv.y : vv.x), h[2 * k + q], lo[2 * k + q]);
+                    for (int k = 0; k < 8; ++k) {
+                        const ulonglong2 vv = vs[8 * c + k];
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            unpair(fma2(add2(s[16 * c + 2 * k + q], ref2), rf2, top2), x, y);
+                            const uint64_t p = pair_of(exp2_f(x), exp2_f(y));
+                            sum = add2(sum, p);
+                            split_pair(mul2(p, q ? vv.y : vv.x), h[2 * k + q], lo[2 * k + q]);
+                        }
                     }
+                    tmem_st16(sc + 32 * c, h);
+                    tmem_st16(sc + 32 * c + 16, lo);
                 }
-                tmem_st16(sc, h);
-                tmem_st16(sc + 16, lo);
                 unpair(sum, x, y);
                 l += x + y;
                 tmem_st_done();
@@ -431,8 +431,8 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 if (lane == 0) mbar_arrive(&sc_free[t & 3]);
             }
             // the rows' sums, once the last item's have been read
-            warp_wait(fin_free, (i & 1) ^ 1, ab, 44);
-            ((float*)(smem + C::STATS))[quarter * 128 + row] = l;
+            warp_wait<50>(fin_free, (i & 1) ^ 1, ab, 44);
+            ((float*)(smem + C::STATS))[half * 128 + row] = l;
             mbar_arrive(fin_full);
         }
     } else if (warp < kLoadWarp) {  // ---- sums
@@ -450,7 +450,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             float ref = -INFINITY, rf = 0.0f;
 #pragma unroll 1
             for (int j = 0; j < it.n; ++j, ++t) {
-                warp_wait(o_full, t & 1, ab, 31);
+                warp_wait<100>(o_full, t & 1, ab, 31);
                 tc_fence_after();
                 rf = ((const float*)(smem + C::FACTORS))[(i & 3) * 128 + row];
                 const float2 mu = ((const float2*)(smem + C::REFS))[(t & 3) * 128 + row];
@@ -474,9 +474,9 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                     for (int k = 0; k < 8; ++k) o[8 * c + k] = fma2(pair_of(v[2 * k], v[2 * k + 1]), g, o[8 * c + k]);
                 }
             }
-            warp_wait(fin_full, i & 1, ab, 45);
+            warp_wait<100>(fin_full, i & 1, ab, 45);
             const float* stats = (const float*)(smem + C::STATS) + row;
-            const float l = (stats[0] + stats[128]) + (stats[256] + stats[384]);
+            const float l = stats[0] + stats[128];
             mbar_arrive(fin_free);
             if (row < it.rows) {
                 const int r = it.first_row + row;
@@ -565,14 +565,14 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             uint64_t* full = k_full + 4 * which;  // (k_full, k_empty, v_full, v_empty)
             if (which == 0) have = left == 2 || !more;
             if (have) {
-                warp_wait(full + 2 + (t & 1), (t >> 1 & 1) ^ 1, ab, 34);
+                warp_wait<200>(full + 2 + (t & 1), (t >> 1 & 1) ^ 1, ab, 34);
                 put((int)(t & 1), (int)which);
                 mbar_arrive(full + (t & 1));
                 if (which) ++t, --left;
             }
             const int64_t* places = (const int64_t*)(smem + C::PLACES + (x & 3) * C::PLACE);
             if (which == 0 && more) {
-                const bool found = warp_wait(&place_full[x & 3], x >> 2 & 1, ab, 46) && places[0] >= 0;
+                const bool found = warp_wait<200>(&place_full[x & 3], x >> 2 & 1, ab, 46) && places[0] >= 0;
                 more = __all_sync(0xffffffffu, found);
                 const uint4 ok = *(const uint4*)(places + 8);
                 rows = 0xffu;
@@ -661,7 +661,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             // the scales of tile x - 1: the unit is the least power of two above the tile's largest
             auto finish = [&]() {
                 const uint32_t y = x - 1;
-                warp_wait(&sc_free[y & 3], (y >> 2 & 1) ^ 1, ab, 47);
+                warp_wait<300>(&sc_free[y & 3], (y >> 2 & 1) ^ 1, ab, 47);
                 float k[4] = {ks.x, ks.y, ks.z, ks.w}, v[4] = {vs.x, vs.y, vs.z, vs.w};
                 uint32_t top = 0;
 #pragma unroll
@@ -695,7 +695,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q) now |= (uint32_t)(tok + q >= it.low && tok + q < it.high) << q;
                     if (j + 1 < it.n) page = ((tok + kTileTokens) & ~15) < it.high ? table[(tok + kTileTokens) >> a.page_log] : -1;
-                    if (!warp_wait(&place_free[x & 3], (x >> 2 & 1) ^ 1, ab, 48)) break;
+                    if (!warp_wait<300>(&place_free[x & 3], (x >> 2 & 1) ^ 1, ab, 48)) break;
                     int64_t* places = (int64_t*)(smem + C::PLACES + (x & 3) * C::PLACE);
                     if ((lane & 3) == 0) places[lane >> 2] = it.rows ? s * a.dim : (int64_t)-1;  // (below zero: no more tiles)
                     const uint32_t bits = __reduce_or_sync(0xffu << (lane & 24), now << 4 * (lane & 7));
@@ -723,7 +723,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                     p.whole = it.from == 0 && it.to == it.units, p.begins = it.from == 0, p.last_block = sh.last_block(it);
                     sh.advance(a, it);
                 }
-                const bool ok = warp_wait(&i_free[i & (kItems - 1)], (i / kItems & 1) ^ 1, ab, 42);
+                const bool ok = warp_wait<1000>(&i_free[i & (kItems - 1)], (i / kItems & 1) ^ 1, ab, 42);
                 if (lane == 0) {
                     const int* w = (const int*)&p;
 #pragma unroll
