@@ -143,14 +143,20 @@ template <int MAX>
 __device__ __forceinline__ int64_t tiles_of(const AttnArgs& a, const Seq& q) {
     return ((int64_t)q.take * a.group + MAX - 1) / MAX;
 }
-// Tokens and units of tile t of a sequence: at least one unit, so that rows that see nothing are written.
+// Tokens and units of tile t of a sequence: at least one unit, so that rows that see nothing are written.  Tiles of many rows
+// count kItemUnits more, for what an item costs besides its tokens (its queries, its output, the way from one to the next).
+constexpr int kItemUnits = 4;
+template <int MAX>
+__host__ __device__ constexpr int extra_units() {
+    return MAX > 16 ? kItemUnits : 0;
+}
 template <int MAX>
 __device__ __forceinline__ int span_of(const AttnArgs& a, const Seq& q, int64_t t, int& low, int& high) {
     const int tok0 = (int)(t * MAX / a.group), tok1 = (int)(min(t * MAX + MAX, (int64_t)q.take * a.group) - 1) / a.group;
     const int p0 = q.length - q.n + tok0, p1 = q.length - q.n + tok1;
     low = first_seen(a, p0), high = p1 + 1;
     if (high <= low) low = high = 0;
-    return max(1, (high - (low & ~15) + kUnitTokens - 1) / kUnitTokens);
+    return max(1, (high - (low & ~15) + kUnitTokens - 1) / kUnitTokens + extra_units<MAX>());
 }
 
 // A slot of a block's part of an item: 8 ints (1 if it begins an item that ends elsewhere, the item's head, rows, first row,

@@ -717,7 +717,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 if (more) {
                     const Item it = sh.item(a);
                     p.rows = it.rows, p.row0 = it.row0, p.first_row = it.first_row;
-                    p.n = max(0, min(it.to, (it.high - it.base + kTileTokens - 1) / kTileTokens) - it.from);
+                    p.n = max(0, min(it.to, (it.high - it.base + kTileTokens - 1) / kTileTokens) - it.from);  // (the units behind the tokens hold none)
                     p.pos = it.pos, p.all_first = it.top_first, p.all_last = it.pos + it.first_row / a.group, p.head = it.head;
                     p.low = it.low, p.high = it.high, p.first = it.base + kTileTokens * it.from, p.seq = it.seq;
                     p.whole = it.from == 0 && it.to == it.units, p.begins = it.from == 0, p.last_block = sh.last_block(it);
