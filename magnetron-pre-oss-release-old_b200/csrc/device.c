@@ -117,7 +117,7 @@ typedef struct mcu_device {
     int stage_next;
     void* scratch;
     size_t scratch_bytes;
-    int* d_status;
+    int* d_status; /* MCU_STATUS_WORDS of them */
     mcu_graph* graphs;
     void* graph_scratch; /* scratch of the graph being captured */
     int profiling;
@@ -613,8 +613,8 @@ mag_compute_device_t* mag_init_device_cuda(mag_ctx_t* ctx) {
         MCU_CHECK(cudaEventCreateWithFlags(&d->stage_ev[i], cudaEventDisableTiming));
         MCU_CHECK(cudaEventRecord(d->stage_ev[i], d->stream));
     }
-    MCU_CHECK(cudaMalloc((void**)&d->d_status, sizeof(int)));
-    MCU_CHECK(cudaMemset(d->d_status, 0, sizeof(int)));
+    MCU_CHECK(cudaMalloc((void**)&d->d_status, MCU_STATUS_WORDS * sizeof(int)));
+    MCU_CHECK(cudaMemset(d->d_status, 0, MCU_STATUS_WORDS * sizeof(int)));
     snprintf(dvc->name, sizeof(dvc->name), "%.96s (sm_%d%d, %d SMs)", prop.name, prop.major, prop.minor,
              prop.multiProcessorCount);
     dvc->impl = d;

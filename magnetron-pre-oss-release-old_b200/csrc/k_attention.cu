@@ -14,7 +14,7 @@ namespace {
 // work: each is read once, by one warp, for all rows.  A block works through its share of all (sequence, kv head) items'
 // units of 128 tokens; a warp takes every eighth group of 16 tokens, four groups in flight by cp.async in a ring of its
 // own, and keeps its own running maximum, sum and output.  The block's warps are joined in shared memory when an item
-// ends, blocks that share an item by attention_join.
+// ends; of the blocks that share an item the last one joins their parts.
 //
 // Products run on mma.sync m16n8k16 (f16, f32 sums): e4m3 bytes become f16 in registers, exactly.  Queries and
 // probabilities are split in two f16, high and low.  Up to 8 rows (STACK) the halves are rows 0-7 and 8-15 of one
@@ -35,8 +35,8 @@ struct FewSmem {
     static constexpr int VALS = (STACK ? DP / 4 : DP / 2);  // outputs a thread holds
     static constexpr int WARPS = FewCfg<DP, STACK>::WARPS;
     static constexpr int SUMS = FewCfg<DP, STACK>::RING * WARPS;
-    static constexpr int STATS = SUMS + WARPS * 32 * VALS * 4;  // [warp][16] of (m, l), then [warp] of the values' unit
-    static constexpr int BYTES = STATS + WARPS * 16 * 8 + WARPS * 4;
+    static constexpr int STATS = SUMS + WARPS * 32 * VALS * 4;  // [warp][16] of (m, l), then [warp] of the values' unit, 16 ints
+    static constexpr int BYTES = STATS + WARPS * 16 * 8 + WARPS * 4 + 64;
     static_assert(BYTES <= 227 * 1024, "must fit shared memory");
     static_assert(Share<16, DP, 32 * WARPS>::SMEM <= SUMS, "the search for work takes the rings' room");
 };
@@ -64,9 +64,11 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_fe
     float4* sums = (float4*)(smem + S::SUMS) + warp * 8 * S::VALS;  // [VALS / 4][32]
     float2* stats = (float2*)(smem + S::STATS);
     float* units = (float*)(stats + kFewWarps * 16);
+    int* cut = (int*)(units + kFewWarps);  // what an item that ends, or begins, elsewhere is: 8 ints each
         pdl_begin();
 
     Share<16, DP, 32 * kFewWarps> sh;
+    if (threadIdx.x < 16) cut[threadIdx.x] = 0;
     if (!sh.find(a, (int64_t*)smem)) return;
     if (!EXACT) {  // columns past the head's stay zero: no copy writes them
         for (int i = lane; i < C::RING / 16; i += 32) *(uint4*)(smem + warp * C::RING + 16 * i) = make_uint4(0, 0, 0, 0);
@@ -354,6 +356,11 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_fe
             if (c == 0) stats[warp * 16 + g + 8 * r] = make_float2(top_of(m[r], rf[r]), l[r]);
         }
         if (lane == 0) units[warp] = unit;
+        const bool whole = it.from == 0 && it.to == it.units;
+        if (!whole && warp == kFewWarps - 1 && lane == 0) {
+            int* c = cut + 8 * (it.from == 0);
+            c[0] = sh.first_block(it), c[1] = sh.last_block(it) - c[0] + 1, c[2] = rows, c[3] = it.row0, c[4] = it.head * a.group;
+        }
         __syncthreads();
         for (int x = threadIdx.x; x < 8 * S::VALS; x += 32 * kFewWarps) {
             const int e = x >> 5, ln = x & 31, r = e / (DP / 16), row = (ln >> 2) + 8 * r;
@@ -382,6 +389,21 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_fe
         __syncthreads();
         sh.advance(a, it);
     }
+    // ---- items that other blocks have parts of, one at either end of the block's share at most: the last of an item's blocks
+    // joins its parts.  The item's counter returns to zero with it.
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        int* c = cut + 8 * threadIdx.x;
+        c[5] = c[1] && atomicInc(a.joins + c[0], (uint32_t)(c[1] - 1)) == (uint32_t)(c[1] - 1);
+    }
+    __syncthreads();
+    for (int w = 0; w < 2; ++w) {
+        const int* c = cut + 8 * w;
+        if (!c[5]) continue;
+        __threadfence();
+        for (int r = warp; r < c[2]; r += kFewWarps) join_row<16, DP>(a, c[0], c[1], r, c[3] + r / a.group, c[4] + r % a.group);
+    }
 }
 
 template <int DP, bool STACK, bool EXACT>
@@ -390,9 +412,7 @@ int run_few(const AttnArgs& a, cudaStream_t st) {
     constexpr int bytes = FewSmem<DP, STACK>::BYTES;
     const cudaError_t e = allow_smem(attention_few<DP, STACK, EXACT>, bytes, done);
     if (e != cudaSuccess) return (int)e;
-    const int rc = (int)launch_dep(attention_few<DP, STACK, EXACT>, dim3((unsigned)a.blocks), dim3(32 * FewCfg<DP, STACK>::WARPS), bytes, st, a);
-    if (rc) return rc;
-    return (int)launch_dep(attention_join<16, DP>, dim3((unsigned)a.blocks, 4), dim3(128), 0, st, a);
+    return (int)launch_dep(attention_few<DP, STACK, EXACT>, dim3((unsigned)a.blocks), dim3(32 * FewCfg<DP, STACK>::WARPS), bytes, st, a);
 }
 
 template <int DP>
@@ -403,6 +423,7 @@ int few(const AttnArgs& a, cudaStream_t st) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int kSms = 148;
+static_assert(MCU_JOIN_WORD + kSms <= MCU_STATUS_WORDS, "a counter for each block");
 constexpr int kFewRows = 16;
 int padded(const mcu_attention* a) { return a->cache.head_dim <= 64 ? 64 : 128; }
 
@@ -433,7 +454,7 @@ extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, int* 
     AttnArgs a = {};
     a.out = c->out, a.lse = c->lse, a.q = c->q, a.k = c->cache.k, a.v = c->cache.v, a.ks = c->cache.k_scale, a.vs = c->cache.v_scale;
     a.table = c->table, a.start = c->start, a.length = c->length, a.table_s1 = c->table_s1, a.q_s1 = c->q_s1, a.out_s1 = c->out_s1;
-    a.parts = (float*)scratch, a.status = status, a.seqs = (int)c->seqs, a.rows = (int)c->rows, a.max_new = (int)c->max_new;
+    a.parts = (float*)scratch, a.status = status, a.joins = (uint32_t*)status + MCU_JOIN_WORD, a.seqs = (int)c->seqs, a.rows = (int)c->rows, a.max_new = (int)c->max_new;
     a.heads = c->cache.heads, a.group = group, a.dim = c->cache.head_dim, a.pages = c->cache.pages;
     while ((1 << a.page_log) < c->cache.page_size) ++a.page_log;
     a.window = c->window >= ((int64_t)1 << 31) - 1 ? 0 : (int)c->window;
@@ -452,7 +473,7 @@ extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, int* 
     if (!rc && f.few) {
         a.least = 1, a.most = f.few;
         rc = wide ? few<128>(a, st) : few<64>(a, st);
-        *launches += 2;
+        *launches += 1;
     }
     return rc;
 }

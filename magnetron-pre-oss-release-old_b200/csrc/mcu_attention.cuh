@@ -25,6 +25,7 @@ struct AttnArgs {
     int64_t table_s1, q_s1, out_s1;
     float* parts;  // two slots a block, of part_floats() floats
     int* status;
+    uint32_t* joins;  // attention_few's counters, one a block: parts of the item that the block begins
     int seqs, rows, max_new, heads, group, dim, pages, page_log, window;
     int longest;             // tokens that a sequence's table has room for
     int least, most;         // the rows of a kv head (new tokens x group) of the sequences that this launch takes
@@ -159,8 +160,8 @@ __device__ __forceinline__ int span_of(const AttnArgs& a, const Seq& q, int64_t 
     return max(1, (high - (low & ~15) + kUnitTokens - 1) / kUnitTokens + extra_units<MAX>());
 }
 
-// A slot of a block's part of an item: 8 ints (1 if it begins an item that ends elsewhere, the item's head, rows, first row,
-// row0, last block), then maximum and sum of each row, then its rows of output.
+// A slot of a block's part of an item: 8 ints (for tiles of many rows: 1 if it begins an item that ends elsewhere, the item's
+// head, rows, first row, row0, last block), then maximum and sum of each row, then its rows of output.
 __host__ __device__ constexpr int64_t part_floats(int max, int dp) { return 8 + 2 * max + (int64_t)max * dp; }
 __device__ __forceinline__ float* part_slot(const AttnArgs& a, int max, int dp, int64_t block, int which) {
     return a.parts + (2 * block + which) * part_floats(max, dp);
@@ -191,7 +192,7 @@ struct Share {
         const int64_t n = tiles_of<MAX>(a, q);
         int64_t u = 0;
         int lo, hi;
-        if (!BY_WARP) return n ? span_of<MAX>(a, q, 0, lo, hi) : 0;
+        if constexpr (!BY_WARP) return n ? span_of<MAX>(a, q, 0, lo, hi) : 0;
         for (int64_t t = threadIdx.x & 31; t < n; t += 32) u += span_of<MAX>(a, q, t, lo, hi);
 #pragma unroll
         for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
@@ -203,7 +204,7 @@ struct Share {
     __device__ bool find(const AttnArgs& a, int64_t* sh) {
         int64_t* found = sh + 32;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        if (threadIdx.x == 0) *(int*)slot(a, 0) = *(int*)slot(a, 1) = 0;
+        if (MAX > 16 && threadIdx.x == 0) *(int*)slot(a, 1) = 0;
         // each thread (or warp) has a run of sequences
         const int workers = BY_WARP ? WARPS : THREADS, me = BY_WARP ? warp : threadIdx.x;
         const int run = (a.seqs + workers - 1) / workers, s0 = min(me * run, a.seqs), s1 = min(s0 + run, a.seqs);
@@ -312,9 +313,10 @@ struct Share {
         }
         left = 0;  // (not reached: the shares add up to all units)
     }
-    // The block that holds the last unit of the item that begins at unit `at`.
-    __device__ int last_block(const Item& it) const {
-        const int64_t x = at - it.from + it.units - 1;
+    // The blocks that hold the first and the last unit of the item at hand.
+    __device__ int first_block(const Item& it) const { return it.from ? block_of(at - it.from) : (int)blockIdx.x; }
+    __device__ int last_block(const Item& it) const { return block_of(at - it.from + it.units - 1); }
+    __device__ int block_of(int64_t x) const {
         int b = (int)quotient((x + 1) * blocks, total);
         while (begin_of(b) > x) --b;
         while (begin_of(b + 1) <= x) ++b;
@@ -337,7 +339,7 @@ __device__ __forceinline__ void put_out(const AttnArgs& a, const Share<MAX, DP, 
     float* p = sh.slot(a, it.from == 0);
     if (d == 0) {
         p[8 + 2 * row] = top, p[9 + 2 * row] = total;
-        if (row == 0 && it.from == 0) {
+        if (MAX > 16 && row == 0 && it.from == 0) {
             int* m = (int*)p;
             m[1] = it.head, m[2] = it.rows, m[3] = it.first_row, m[4] = it.row0, m[5] = sh.last_block(it), m[0] = 1;
         }
@@ -345,36 +347,39 @@ __device__ __forceinline__ void put_out(const AttnArgs& a, const Share<MAX, DP, 
     *(float4*)(p + 8 + 2 * MAX + row * DP + d) = v;
 }
 
-// Items whose units several blocks had: blockIdx.x is the block that began it, a warp takes a row.  The parts' weights are
-// their sums times 2^(top - the highest top); parts are added in the blocks' order.
+// Row `row` of an item whose units the blocks [first, first + parts) had; a warp.  The parts' weights are their sums times
+// 2^(top - the highest top); parts are added in the blocks' order.
 template <int MAX, int DP>
-__global__ void __launch_bounds__(128) attention_join(AttnArgs a) {
-    pdl_begin();
-    const int* m = (const int*)part_slot(a, MAX, DP, blockIdx.x, 1);
-    if (!m[0]) return;
-    const int row = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (row >= m[2]) return;
-    const int parts = m[5] - (int)blockIdx.x + 1, r = m[3] + row, head = m[1] * a.group + r % a.group;
-    const int64_t to = m[4] + r / a.group;
-    float top = kNone, total = 0.0f;
-    for (int p = lane; p < parts; p += 32) top = fmaxf(top, part_slot(a, MAX, DP, blockIdx.x + p, p == 0)[8 + 2 * row]);
+__device__ __forceinline__ void join_row(const AttnArgs& a, int first, int parts, int row, int64_t to, int head) {
+    const int lane = threadIdx.x & 31;
+    auto stats = [&](int p) {
+        return p < parts ? __ldcg((const float2*)(part_slot(a, MAX, DP, first + p, p == 0) + 8 + 2 * row)) : make_float2(kNone, 0.0f);
+    };
+    auto values = [&](int p) {
+        return p < parts && 4 * lane < DP ? __ldcg((const float4*)(part_slot(a, MAX, DP, first + p, p == 0) + 8 + 2 * MAX + row * DP + 4 * lane))
+                                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    };
+    const float2 mine = stats(lane);
+    float4 t[4];  // the next parts' values, under way
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = values(k);
+    float top = mine.x, total = 0.0f;
+    for (int p = lane + 32; p < parts; p += 32) top = fmaxf(top, stats(p).x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int p0 = 0; p0 < parts; p0 += 32) {
-        float w = 0.0f;
-        if (p0 + lane < parts) {
-            const float* p = part_slot(a, MAX, DP, blockIdx.x + p0 + lane, p0 + lane == 0) + 8 + 2 * row;
-            w = p[1] * exp2_f(p[0] - top);
-        }
+        const float2 s = p0 ? stats(p0 + lane) : mine;
+        const float w = p0 + lane < parts ? s.y * exp2_f(s.x - top) : 0.0f;
         const int n = min(32, parts - p0);
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-            const float k = __shfl_sync(0xffffffffu, w, i);
-            total += k;
-            if (4 * lane < DP) {
-                const float4 t = *(const float4*)(part_slot(a, MAX, DP, blockIdx.x + p0 + i, p0 + i == 0) + 8 + 2 * MAX + row * DP + 4 * lane);
-                v.x = fmaf(k, t.x, v.x), v.y = fmaf(k, t.y, v.y), v.z = fmaf(k, t.z, v.z), v.w = fmaf(k, t.w, v.w);
+#pragma unroll 1
+        for (int i = 0; i < n; i += 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float f = __shfl_sync(0xffffffffu, w, i + k);  // (zero past the parts)
+                total += f;
+                v.x = fmaf(f, t[k].x, v.x), v.y = fmaf(f, t[k].y, v.y), v.z = fmaf(f, t[k].z, v.z), v.w = fmaf(f, t[k].w, v.w);
+                t[k] = values(p0 + i + 4 + k);
             }
         }
     }

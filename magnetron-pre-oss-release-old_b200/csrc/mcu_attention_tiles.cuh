@@ -196,6 +196,19 @@ __device__ __forceinline__ void split_pair(uint64_t w, uint32_t& high, uint32_t&
         : "l"(w));
 }
 
+// Items whose units several blocks had: blockIdx.x is the block that began it, a warp takes a row.  A kernel of its own: a
+// block whose wait was given up would not be counted.
+template <int DP>
+__global__ void __launch_bounds__(128) attention_join(AttnArgs a) {
+    pdl_begin();
+    const int* m = (const int*)part_slot(a, kTileRows, DP, blockIdx.x, 1);
+    if (!m[0]) return;
+    const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
+    if (row >= m[2]) return;
+    const int r = m[3] + row;
+    join_row<kTileRows, DP>(a, blockIdx.x, m[5] - (int)blockIdx.x + 1, row, m[4] + r / a.group, m[1] * a.group + r % a.group);
+}
+
 template <int DP>
 __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     using C = TileCfg<DP>;
@@ -752,7 +765,7 @@ int run_tiles(const AttnArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return (int)e;
     const int rc = (int)launch_dep(attention_tiles<DP>, dim3((unsigned)a.blocks), dim3(kTileThreads), TileCfg<DP>::SMEM, st, a);
     if (rc) return rc;
-    return (int)launch_dep(attention_join<kTileRows, DP>, dim3((unsigned)a.blocks, kTileRows / 4), dim3(128), 0, st, a);
+    return (int)launch_dep(attention_join<DP>, dim3((unsigned)a.blocks, kTileRows / 4), dim3(128), 0, st, a);
 }
 
 }  // namespace
