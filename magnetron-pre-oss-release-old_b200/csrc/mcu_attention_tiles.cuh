@@ -71,16 +71,18 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// The whole warp waits, for up to half a second or until a wait was given up elsewhere.  A loop of few instructions: it stands at
-// some twenty places.  NAP: how many ns to sleep between two looks, for roles that run ahead (their looks would take issue slots from
-// the warps that compute).
+// The whole warp waits, for about half a second or until a wait was given up elsewhere.  A loop of few instructions: it stands at
+// some twenty places.  A look that finds nothing holds the warp for some 4 us (measured; it ends as soon as there is something), so
+// the limit is 2^17 looks; were they to return at once it would be 3 ms, still a hundred times what a tile takes.  The planner, which
+// waits for whole items and whose wait is never the first to be given up, has more.  NAP: how many ns to sleep between two looks, for
+// roles that run ahead.
 template <int NAP = 0>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
-    constexpr uint32_t kLooks = NAP ? 500000000u / (NAP + 50) : 1u << 23;
+    constexpr uint32_t kLooks = NAP < 1000 ? 1u << 17 : 1u << 24;
     uint32_t ok, n = 0;
     while (true) {
         ok = mbar_test(bar, parity);
-        if (ok || ++n == kLooks || ((NAP || (n & 63) == 0) && *ab.flag)) break;
+        if (ok || ++n == kLooks || *ab.flag) break;
         if (NAP) __nanosleep(NAP);
     }
     __syncwarp();
@@ -293,7 +295,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&i_free[i & (kItems - 1)]);
         const bool over = *gave_up != 0;
-        if (threads ? bar_any(id, threads, over) : __any_sync(0xffffffffu, over)) it.rows = 0;
+        if (threads ? bar_any(id, threads, over) : __any_sync(0xffffffffu, over)) it.rows = it.n = 0;  // (what was read may be torn)
         return it;
     };
 
