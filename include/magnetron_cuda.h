@@ -342,7 +342,7 @@ MAG_CUDA_EXPORT int mag_cuda_token_logprobs_backward_f32(mag_compute_device_t* d
  * stride of x_s1 values (at least heads * head_dim), so that queries, keys and values may be parts of one
  * row of a fused projection.  Calls check, order, capture and count as those of the section above; what lies on
  * the device (positions, slots, tables, lengths) is checked by the kernels, which skip what is out of range.
- * Sums are formed in f32 in a fixed order, without atomics. */
+ * Sums are formed in f32 in a fixed order, so that the same call gives the same bits. */
 
 /* The position's rotation of the first rot values of a head (rot a multiple of 8, at most head_dim; the rest
  * pass): pair p < rot / 2 turns by the angle pos[row] * inv_freq[p],
@@ -410,7 +410,10 @@ MAG_CUDA_EXPORT int mag_cuda_kv_read(mag_compute_device_t* dvc, const mag_cuda_k
  * a sequence past its first max_new (an upper bound of n that the caller knows on the host); lengths are taken as at most
  * table_s1 * page_size and at least 0.
  * Products are formed on the tensor cores from f16 halves of the queries and the probabilities (22 bits each; the cache's
- * values are exact), sums and statistics in f32.  scale: finite, not negative. */
+ * values are exact), sums and statistics in f32.  scale: finite, not negative.
+ * The cache's scales are NaN or as mag_cuda_kv_write forms them: not negative and below 2^126.  A value's NaN scale makes out
+ * NaN and may make lse NaN.  Logits are formed in f32 from queries brought to 2^13 .. 2^14, so that keys have to stay below about 2^98
+ * in magnitude; above it a logit may overflow, and the rows that see it are NaN. */
 MAG_CUDA_EXPORT int mag_cuda_attention_paged_f32(mag_compute_device_t* dvc, float* out, float* lse, const float* q,
                                                  const mag_cuda_kv_cache* cache, const int32_t* table,
                                                  const int32_t* start, const int32_t* length, int64_t seqs,

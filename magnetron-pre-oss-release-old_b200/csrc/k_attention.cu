@@ -12,8 +12,8 @@ namespace {
 //
 // The rows of one kv head (new tokens x query heads of the group) are at most 16 here, so the cache's bytes bound the
 // work: each is read once, by one warp, for all rows.  A block works through its share of all (sequence, kv head) items'
-// units of 128 tokens; a warp takes every eighth group of 16 tokens, four groups in flight by cp.async in a ring of its
-// own, and keeps its own running maximum, sum and output.  The block's warps are joined in shared memory when an item
+// units of 128 tokens; its warps take groups of 16 tokens in turn, two or three on their way by cp.async in a ring of the warp's
+// own, and each keeps its own running maximum, sum and output.  The block's warps are joined in shared memory when an item
 // ends; of the blocks that share an item the last one joins their parts.
 //
 // Products run on mma.sync m16n8k16 (f16, f32 sums): e4m3 bytes become f16 in registers, exactly.  Queries and
@@ -21,6 +21,11 @@ namespace {
 // operand, so that the split costs no instruction and a thread finds both halves' results in its own registers.
 // The order of a product's inner index is free, so it is chosen such that a thread's operands are 16 consecutive bytes
 // of a row of keys (inner index: the head's values) and of four rows of values (columns: the head's values).
+//
+// Measured (32 query heads on 8 of 128): 64 sequences of up to 16000 tokens 255 us, 5.5 TB/s of the cache (8 warps of four stages
+// 306; with a second launch that joins the parts 264); four of up to 2000 tokens 17 us, which is latency: about 1.6 us to find the
+// share, 1.3 to the first copies, 2.5 for the groups, 0.8 to join the warps, and four of fences, counter and the parts' join, at
+// the pace of code that runs once.
 constexpr int kGroup = 16;               // tokens of a warp's step; pages hold a multiple
 constexpr int kFlush = 16;               // groups between two flushes: the tensor core's sums lose up to a step each
 

@@ -24,7 +24,11 @@ using namespace mcu;
 //   warp 18      guides: each tile's places in the pages and its scales, up to four tiles ahead
 // What bounds it is the softmax: about 14 instructions for two logits (390 cycles for 32 x 32 of them with four warps a
 // scheduler, alone), more than the products' 2 x 1024 cycles a tile.  The loops of all roles have to fit the SM's instruction cache
-// together: unrolled for 128 columns they took three times as long.
+// together: unrolled for 128 columns they took three times as long.  Eight softmax warps hold half a row's logits each in registers
+// (chunks of 300 over 20000 tokens 214 us; sixteen that read them twice from TMEM 245; two groups of eight in turn on tiles of their
+// own more than either).  Writing the next item's queries under the last tile's softmax made the loops longer than it hid (prompts
+// 1205 us), and fetching them to L2 ahead moved nothing (1059).
+// Measured: four prompts of up to 4100 tokens, 32 query heads on 8 of 128: 1.00 ms, 0.35 PFLOP/s (both halves' products 0.7); three chunks of up to 300 over 20000 tokens, 20 heads on 4 of 96: 208 us.
 constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 640;
 constexpr int kSoftWarps = 8, kLoadWarp = 12, kIssueWarp = 16, kPlanWarp = 17, kGuideWarp = 18;  // (sums from kSoftWarps on)
 constexpr int kTileLaunch = 96, kSoftRegs = 104, kSumRegs = 168, kLoadRegs = 56, kIssueRegs = 48;
