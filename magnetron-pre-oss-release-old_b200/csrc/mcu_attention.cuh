@@ -168,15 +168,21 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
     return r < 0 ? q - 1 : r >= b ? q + 1 : q;
 }
 
+// A share's end moves to the beginning or end of its item where that is no further than so many units, the item's middle and half
+// a share: a block that begins an item pays for it what some units of tokens cost (four sequences of up to 2000 tokens 18.2 -> 13.6
+// us, eight of 64 values a head 16.7 -> 13.4; up to 3 units 15.4 and 14.1, and without the bound of half a share one sequence of 500
+// tokens took 11.5 us, 10.8 with it).  Few rows; with many, an item's own units (kItemUnits) stand for that.
+constexpr int kSnapUnits = 2;
+
 // A block's share of all units, in the order sequence, kv head, tile, tokens: equal shares, so that ragged lengths load
 // the GPU evenly whatever the lengths are, which only the device knows.  An item that a share's end cuts is joined from its
 // parts afterwards.  THREADS threads of the block look for its first item together; each of them, or some, then goes on alone.
 template <int MAX, int DP, int THREADS>
 struct Share {
     static constexpr bool BY_WARP = MAX > 16;  // a sequence has many tiles: the lanes of a warp share them
-    static constexpr int WARPS = THREADS / 32, SMEM = 32 * 8 + 48;
+    static constexpr int WARPS = THREADS / 32, SMEM = 32 * 8 + 48 + 16;
     int64_t total, at, left, tile;
-    int blocks, seq, head, off;
+    int blocks, seq, head, off, reach;
     Seq here;  // the sequence at hand
 
     // Units of one kv head of a sequence.
@@ -190,7 +196,7 @@ struct Share {
         for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
         return u;
     }
-    // The first unit of block b.
+    // The first unit of block b, before it is moved to an item's beginning or end.
     __device__ int64_t begin_of(int b) const { return quotient(total * b, blocks); }
     // Finds the block's first item; false when the block has no work.  sh: SMEM bytes of shared memory.
     __device__ bool find(const AttnArgs& a, int64_t* sh) {
@@ -222,7 +228,22 @@ struct Share {
         blocks = (int)min((int64_t)gridDim.x, total);  // each has a unit at least, so that an item's parts lie in consecutive blocks
         if ((int)blockIdx.x >= blocks) return false;
         at = begin_of(blockIdx.x);
+        reach = BY_WARP ? 0 : (int)min((int64_t)kSnapUnits, quotient(total, blocks) / 2);
         left = begin_of(blockIdx.x + 1) - at;
+        if (!BY_WARP) {
+            const int64_t end = at + left;
+            if (end >= before && end < before + mine) {
+                int64_t x = end - before, u = 0;
+#pragma unroll 1
+                for (int s = s0; s < s1; ++s) {
+                    u = seq_units(a, Seq(a, s)) * a.heads;
+                    if (x < u) break;
+                    x -= u;
+                }
+                found[6] = moved(x, (int)quotient(u, a.heads)) - x;
+            }
+            if (end == total && threadIdx.x == 0) found[6] = 0;
+        }
         if (at >= before && at < before + mine) {
             int64_t x = at - before, u = 0;
             int s = s0;
@@ -247,6 +268,12 @@ struct Share {
         head = (int)quotient(x, per);
         int64_t rest = x - head * per;
         tile = 0;
+        if (!BY_WARP) {
+            const int64_t to = moved(x, (int)per) - x;
+            at += to, left += found[6] - to, rest += to;
+            if (left <= 0) return false;
+            if (rest == per) rest = 0, next_head(a);
+        }
         if (BY_WARP) {  // (each warp for itself)
             const int64_t n = tiles_of<MAX>(a, here);
 #pragma unroll 1
@@ -274,6 +301,21 @@ struct Share {
         __syncthreads();
         return true;
     }
+    // Where unit x of a sequence, `units` to a head, is moved to.
+    __device__ int64_t moved(int64_t x, int units) const {
+        const int64_t first = quotient(x, units) * units;
+        const int r = (int)(x - first), t = min(reach, units / 2);
+        return r <= t ? first : units - r <= t ? first + units : x;
+    }
+    __device__ void next_head(const AttnArgs& a) {
+        if (++head < a.heads) return;
+        head = 0;
+        while (++seq < a.seqs) {
+            here = Seq(a, seq);
+            if (here.take) return;
+        }
+        left = 0;  // (not reached: the shares add up to all units)
+    }
     __device__ bool more() const { return left > 0; }
     __device__ Item item(const AttnArgs& a) const {
         const Seq& q = here;
@@ -297,17 +339,17 @@ struct Share {
             if (tile < tiles_of<MAX>(a, here)) return;
         }
         tile = 0;
-        if (++head < a.heads) return;
-        head = 0;
-        while (++seq < a.seqs) {
-            here = Seq(a, seq);
-            if (here.take) return;
-        }
-        left = 0;  // (not reached: the shares add up to all units)
+        next_head(a);
     }
     // The blocks that hold the first and the last unit of the item at hand.
-    __device__ int first_block(const Item& it) const { return it.from ? block_of(at - it.from) : (int)blockIdx.x; }
-    __device__ int last_block(const Item& it) const { return block_of(at - it.from + it.units - 1); }
+    __device__ int first_block(const Item& it) const {
+        return it.from ? block_of(at - it.from + min(reach, it.units / 2)) : (int)blockIdx.x;
+    }
+    __device__ int last_block(const Item& it) const {
+        const int t = min(reach, it.units / 2);
+        return block_of(at - it.from + max(it.units - 1 - t, t));
+    }
+    // The last block whose share, before it is moved, begins at or before unit x.
     __device__ int block_of(int64_t x) const {
         int b = (int)quotient((x + 1) * blocks, total);
         while (begin_of(b) > x) --b;

@@ -428,6 +428,14 @@ def test_many_sequences_of_chunks():
     Batch([(1 + i % 19, 20 + (37 * i) % 90) for i in range(600)], 2, 1, 16, 16).check()
 
 
+@pytest.mark.parametrize("count,longest,q_heads,heads", [(1, 500, 4, 2), (3, 300, 8, 8), (7, 700, 2, 1), (40, 300, 16, 4), (150, 260, 3, 3), (400, 130, 4, 1),
+                                                         (2, 9000, 40, 4), (5, 2100, 36, 4)])
+def test_shares_that_end_anywhere(count, longest, q_heads, heads):
+    """Sequences of all lengths, so that the blocks' shares end at items' beginnings, near them and within."""
+    g = rng(count, longest)
+    Batch([(1, int(n)) for n in g.integers(1, longest, count)], q_heads, heads, 64, 16).check()
+
+
 def test_strides_and_rows_outside():
     """Padded rows, rows before the first and behind the last sequence: left as they were."""
     for seqs in ([(1, 40), (1, 9)], [(30, 50), (1, 20)]):
