@@ -22,27 +22,28 @@ namespace {
 // The order of a product's inner index is free, so it is chosen such that a thread's operands are 16 consecutive bytes
 // of a row of keys (inner index: the head's values) and of four rows of values (columns: the head's values).
 //
-// Measured (32 query heads on 8 of 128): 64 sequences of up to 16000 tokens 255 us, 5.5 TB/s of the cache (8 warps of four stages
-// 306; with a second launch that joins the parts 264); four of up to 2000 tokens 17 us, which is latency: about 1.6 us to find the
-// share, 1.3 to the first copies, 2.5 for the groups, 0.8 to join the warps, and four of fences, counter and the parts' join, at
-// the pace of code that runs once.
+// Measured (32 query heads on 8 of 128): 64 sequences of up to 16000 tokens 237 us, 6.0 TB/s of the cache; four of up to 2000
+// tokens 14 us, which is latency: about 1.6 us to find the share, 1.3 to the first copies, 2.5 for the groups, 0.8 to join the warps,
+// and three to four of fences, counter and the parts' join, at the pace of code that runs once.  (With one block of twelve warps an SM
+// the former took 306 us with eight warps of four stages, 264 with a second launch that joins the parts, 255 without.)
+constexpr int kSms = 148;
 constexpr int kGroup = 16;               // tokens of a warp's step; pages hold a multiple
 constexpr int kFlush = 16;               // groups between two flushes: the tensor core's sums lose up to a step each
 
-template <int DP, bool STACK>
+template <int DP, bool STACK, int BLOCKS>
 struct FewCfg {
-    static constexpr int WARPS = STACK ? 12 : 8, STAGES = STACK ? 3 : 4;
+    static constexpr int WARPS = (STACK ? 12 : 8) / BLOCKS, STAGES = STACK ? 3 : 4;
     static constexpr int STAGE = 2 * kGroup * DP + 2 * kGroup * 4;  // keys, values, their scales
     static constexpr int RING = STAGES * STAGE;
 };
-template <int DP, bool STACK>
+template <int DP, bool STACK, int BLOCKS>
 struct FewSmem {
     static constexpr int VALS = (STACK ? DP / 4 : DP / 2);  // outputs a thread holds
-    static constexpr int WARPS = FewCfg<DP, STACK>::WARPS;
-    static constexpr int SUMS = FewCfg<DP, STACK>::RING * WARPS;
+    static constexpr int WARPS = FewCfg<DP, STACK, BLOCKS>::WARPS;
+    static constexpr int SUMS = FewCfg<DP, STACK, BLOCKS>::RING * WARPS;
     static constexpr int STATS = SUMS + WARPS * 32 * VALS * 4;  // [warp][16] of (m, l), then [warp] of the values' unit, 16 ints
     static constexpr int BYTES = STATS + WARPS * 16 * 8 + WARPS * 4 + 64;
-    static_assert(BYTES <= 227 * 1024, "must fit shared memory");
+    static_assert(BLOCKS * (BYTES + 1024) <= 228 * 1024, "must fit shared memory");
     static_assert(Share<16, DP, 32 * WARPS>::SMEM <= SUMS, "the search for work takes the rings' room");
 };
 
@@ -53,11 +54,11 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
 }
 
 // EXACT: the head has DP values, so that a group's rows lie at constant distances.
-template <int DP, bool STACK, bool EXACT>
-__global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_few(AttnArgs a) {
-    using C = FewCfg<DP, STACK>;
+template <int DP, bool STACK, bool EXACT, int BLOCKS>
+__global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS) attention_few(AttnArgs a) {
+    using C = FewCfg<DP, STACK, BLOCKS>;
     constexpr int kFewWarps = C::WARPS, kFewStages = C::STAGES;
-    using S = FewSmem<DP, STACK>;
+    using S = FewSmem<DP, STACK, BLOCKS>;
     extern __shared__ __align__(128) uint8_t smem[];
     constexpr int KI = DP / 64;      // 16-byte pieces of a key a thread holds
     constexpr int NT = DP / 8;       // column tiles of the output
@@ -411,24 +412,33 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK>::WARPS, 1) attention_fe
     }
 }
 
-template <int DP, bool STACK, bool EXACT>
+template <int DP, bool STACK, bool EXACT, int BLOCKS>
 int run_few(const AttnArgs& a, cudaStream_t st) {
     static bool done[64];
-    constexpr int bytes = FewSmem<DP, STACK>::BYTES;
-    const cudaError_t e = allow_smem(attention_few<DP, STACK, EXACT>, bytes, done);
+    constexpr int bytes = FewSmem<DP, STACK, BLOCKS>::BYTES;
+    const cudaError_t e = allow_smem(attention_few<DP, STACK, EXACT, BLOCKS>, bytes, done);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_dep(attention_few<DP, STACK, EXACT>, dim3((unsigned)a.blocks), dim3(32 * FewCfg<DP, STACK>::WARPS), bytes, st, a);
+    return (int)launch_dep(attention_few<DP, STACK, EXACT, BLOCKS>, dim3(kSms * BLOCKS), dim3(32 * FewCfg<DP, STACK, BLOCKS>::WARPS), bytes, st, a);
 }
 
+// An SM's warps are one block, or several where there are many items: one block's beginnings and ends of items then lie under the others'
+// copies.  64 sequences of up to 500 tokens 37 us with one block, 27 with two, 25 with three; 256 of up to 1000 160, 115, 101; 64 of up to
+// 16000 255, 248, 237 (16 rows: 407, 384 with two); 16 of up to 4000 34, 32, 31.  Fewer items are cut in more parts then: four
+// sequences of up to 2000 13.8, 19.5, 15.7 us, one of 20000 26.8, 25.3, 28.1.
+constexpr int kManyItems = 96, kMostBlocks = 3;
+template <int DP, bool EXACT>
+int few(const AttnArgs& a, cudaStream_t st) {
+    const bool many = (int64_t)a.seqs * a.heads >= kManyItems;
+    if (a.most <= 8) return many ? run_few<DP, true, EXACT, kMostBlocks>(a, st) : run_few<DP, true, EXACT, 1>(a, st);
+    return many ? run_few<DP, false, EXACT, 2>(a, st) : run_few<DP, false, EXACT, 1>(a, st);
+}
 template <int DP>
 int few(const AttnArgs& a, cudaStream_t st) {
-    if (a.most <= 8) return a.dim == DP ? run_few<DP, true, true>(a, st) : run_few<DP, true, false>(a, st);
-    return a.dim == DP ? run_few<DP, false, true>(a, st) : run_few<DP, false, false>(a, st);
+    return a.dim == DP ? few<DP, true>(a, st) : few<DP, false>(a, st);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-constexpr int kSms = 148;
-static_assert(MCU_JOIN_WORD + kSms <= MCU_STATUS_WORDS, "a counter for each block");
+static_assert(MCU_JOIN_WORD + kMostBlocks * kSms <= MCU_STATUS_WORDS, "a counter for each block");
 constexpr int kFewRows = 16;
 int padded(const mcu_attention* a) { return a->cache.head_dim <= 64 ? 64 : 128; }
 
@@ -450,7 +460,7 @@ Forms forms_of(const mcu_attention* a) {
 
 extern "C" size_t mcu_attention_scratch_bytes(const mcu_attention* a) {
     const Forms f = forms_of(a);
-    return (size_t)(2 * kSms * ((f.few ? part_floats(kFewRows, padded(a)) : 0) + (f.tiles ? part_floats(kTileRows, padded(a)) : 0))) * 4;
+    return (size_t)(2 * kSms * ((f.few ? kMostBlocks * part_floats(kFewRows, padded(a)) : 0) + (f.tiles ? part_floats(kTileRows, padded(a)) : 0))) * 4;
 }
 
 extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, int* status, cudaStream_t st, int* launches) {

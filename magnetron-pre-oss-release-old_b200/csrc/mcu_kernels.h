@@ -186,7 +186,7 @@ typedef struct mcu_attention {
 size_t mcu_attention_scratch_bytes(const mcu_attention* a);
 /* The words at `status`: the first is that of the bounded waits; from MCU_JOIN_WORD on a counter for each block of
    attention_few, zero between its launches, which the device's stream puts in order. */
-enum { MCU_JOIN_WORD = 64, MCU_STATUS_WORDS = MCU_JOIN_WORD + 192 };
+enum { MCU_JOIN_WORD = 64, MCU_STATUS_WORDS = MCU_JOIN_WORD + 640 };
 int mcu_launch_attention(const mcu_attention* a, void* scratch, int* status, cudaStream_t st, int* launches);
 
 #ifdef __cplusplus
