@@ -22,7 +22,8 @@ namespace {
 // The order of a product's inner index is free, so it is chosen such that a thread's operands are 16 consecutive bytes
 // of a row of keys (inner index: the head's values) and of four rows of values (columns: the head's values).
 //
-// Measured (32 query heads on 8 of 128): 64 sequences of up to 16000 tokens 237 us, 6.0 TB/s of the cache; four of up to 2000
+// Measured (32 query heads on 8 of 128): 64 sequences of up to 16000 tokens 236 us, 6.0 TB/s of the cache
+// (274 in runs of a second, when the power limit lowers the clock); four of up to 2000
 // tokens 14 us, which is latency: about 1.6 us to find the share, 1.3 to the first copies, 2.5 for the groups, 0.8 to join the warps,
 // and three to four of fences, counter and the parts' join, at the pace of code that runs once.  (With one block of twelve warps an SM
 // the former took 306 us with eight warps of four stages, 264 with a second launch that joins the parts, 255 without.)
