@@ -87,6 +87,10 @@ __device__ __forceinline__ float query_unit(uint32_t top) {
 // The least power of two above v (v finite, positive, below 2^126).
 __device__ __forceinline__ float unit_above(float v) { return __uint_as_float((__float_as_uint(v) & 0x7F800000u) + 0x00800000u); }
 
+// The least power of two not below v (v positive and normal, at most 2^126), and 1 / v of such a power.
+__device__ __forceinline__ float unit_from(float v) { return __uint_as_float((__float_as_uint(v) + 0x007FFFFFu) & 0x7F800000u); }
+__device__ __forceinline__ float one_by(float v) { return __uint_as_float(0x7F000000u - __float_as_uint(v)); }
+
 // Where a piece of 16 bytes of a staged row of keys or values lies within its row, so that the lanes that read
 // together find other banks.
 template <int DP>
@@ -401,10 +405,12 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, int first, int parts
     for (int p = lane + 32; p < parts; p += 32) top = fmaxf(top, stats(p).x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // a power of two that keeps the weights' sum, at most 2^kTop a token, at 1 or below: no sum of values overflows
+    const float less = one_by(unit_from((float)a.longest)) * 0x1p-15f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int p0 = 0; p0 < parts; p0 += 32) {
         const float2 s = p0 ? stats(p0 + lane) : mine;
-        const float w = p0 + lane < parts ? s.y * exp2_f(s.x - top) : 0.0f;
+        const float w = p0 + lane < parts ? s.y * less * exp2_f(s.x - top) : 0.0f;
         const int n = min(32, parts - p0);
 #pragma unroll 1
         for (int i = 0; i < n; i += 4) {
@@ -419,6 +425,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, int first, int parts
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (4 * lane < a.dim) store_row(a, to, head, 4 * lane, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    total /= less;
     if (lane == 0 && a.lse) a.lse[to * a.heads * a.group + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 

@@ -35,6 +35,7 @@ constexpr int kTileLaunch = 96, kSoftRegs = 104, kSumRegs = 168, kLoadRegs = 56,
 static_assert(kSoftRegs >= kTileLaunch && kSumRegs >= kTileLaunch && kLoadRegs <= kTileLaunch && kIssueRegs <= kTileLaunch, "inc or dec as the code has it");
 static_assert(2 * kSoftRegs + kSumRegs + kLoadRegs + kIssueRegs == 5 * kTileLaunch, "register split must match the launch");
 constexpr int kSoftThreads = 32 * kSoftWarps;
+constexpr float kLeastBase = 0x1p-78f;  // unit of a row's sums
 constexpr int kItems = 4;             // items in the planner's ring
 
 // What the roles need of an item, as the planner leaves it; rows = 0: no more.
@@ -467,20 +468,24 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < DP / 2; ++k) o[k] = 0;
             float ref = -INFINITY, rf = 0.0f;
+            // o is in units of `base`, a power of two that grows with the tiles' units and fades with the older weights, so that no sum
+            // overflows; per = 1 / base.  (Not below kLeastBase, so that base / l is normal.)
+            float base = kLeastBase, per = 1.0f / kLeastBase;
 #pragma unroll 1
             for (int j = 0; j < it.n; ++j, ++t) {
                 warp_wait<100>(o_full, t & 1, ab, 31);
                 tc_fence_after();
                 rf = ((const float*)(smem + C::FACTORS))[(i & 3) * 128 + row];
                 const float2 mu = ((const float2*)(smem + C::REFS))[(t & 3) * 128 + row];
-                const float fade = ref == mu.x ? 1.0f : ref == -INFINITY ? 0.0f : exp2_f((ref - mu.x) * rf);
-                ref = mu.x;
-                if (__any_sync(0xffffffffu, fade != 1.0f)) {
-                    const uint64_t f = pair_of(fade, fade);
+                if (__any_sync(0xffffffffu, mu.x > ref || mu.y > base)) {
+                    const float fade = ref == mu.x ? 1.0f : exp2_f((ref - mu.x) * rf), held = base * fade;  // (from -inf: 0)
+                    ref = mu.x;
+                    base = unit_from(fmaxf(fmaxf(held, mu.y), kLeastBase)), per = one_by(base);
+                    const uint64_t f = pair_of(held * per, held * per);
 #pragma unroll
                     for (int k = 0; k < DP / 2; ++k) o[k] = mul2(o[k], f);
                 }
-                const uint64_t g = pair_of(mu.y, mu.y);
+                const uint64_t g = pair_of(mu.y * per, mu.y * per);
 #pragma unroll
                 for (int c = 0; c < DP / 16; ++c) {
                     uint32_t v[16];
@@ -499,7 +504,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             mbar_arrive(fin_free);
             if (row < it.rows) {
                 const int r = it.first_row + row;
-                const float k = l == 0.0f ? 0.0f : 0x1p16f / l;  // (units are kept 2^-16 of theirs: no sum of theirs overflows)
+                const float k = l == 0.0f ? 0.0f : base / l;
                 const float top = top_of(ref, rf);
                 float* dst;
                 bool vec = true;
@@ -697,7 +702,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 uint32_t bits = in << 4 * (lane & 7);
                 bits = __reduce_or_sync(0xffu << (lane & 24), bits);
                 if ((lane & 7) == 0) ((uint32_t*)(slot + 2 * kTileTokens * 4))[lane >> 3] = bits;
-                if (lane == 0) ((float*)(slot + 2 * kTileTokens * 4))[4] = unit * 0x1p-16f;
+                if (lane == 0) ((float*)(slot + 2 * kTileTokens * 4))[4] = unit;
                 mbar_arrive(&sc_full[y & 3]);
             };
 #pragma unroll 1
