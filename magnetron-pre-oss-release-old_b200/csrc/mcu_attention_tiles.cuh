@@ -76,8 +76,9 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// The whole warp waits, for about half a second or until a wait was given up elsewhere.  A loop of few instructions: it stands at
-// some twenty places.  A look that finds nothing holds the warp for some 4 us (measured; it ends as soon as there is something), so
+// The whole warp waits, for about half a second or until a wait was given up elsewhere; the flag then holds the code of a wait that
+// was, which goes to the status word when the block ends.  A loop of few instructions: it stands at some twenty places, whose size
+// shows in instruction fetches (with the status word written here prompts took 1015 us, 936 so).  A look that finds nothing holds the warp for some 4 us (measured; it ends as soon as there is something), so
 // the limit is 2^17 looks; were they to return at once it would be 3 ms, still a hundred times what a tile takes.  The planner, which
 // waits for whole items and whose wait is never the first to be given up, has more.  NAP: how many ns to sleep between two looks, for
 // roles that run ahead.
@@ -85,15 +86,9 @@ template <int NAP = 0>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
     constexpr uint32_t kLooks = NAP < 1000 ? 1u << 17 : 1u << 24;
     uint32_t ok, n = 0;
-    while (true) {
-        ok = mbar_test(bar, parity);
-        if (ok || ++n == kLooks || *ab.flag) break;
+    while (!(ok = mbar_test(bar, parity)) && !*ab.flag) {
+        if (++n == kLooks) *ab.flag = code;
         if (NAP) __nanosleep(NAP);
-    }
-    __syncwarp();
-    if (!ok && (threadIdx.x & 31) == 0 && !*ab.flag) {
-        *ab.flag = 1;
-        atomicCAS(ab.status, 0, code);
     }
     return __all_sync(0xffffffffu, ok);
 }
@@ -216,7 +211,8 @@ __global__ void __launch_bounds__(128) attention_join(AttnArgs a) {
     join_row<kTileRows, DP>(a, blockIdx.x, m[5] - (int)blockIdx.x + 1, row, m[4] + r / a.group, m[1] * a.group + r % a.group);
 }
 
-template <int DP>
+// VEC: queries and outputs are 16-byte aligned.
+template <int DP, bool VEC>
 __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     using C = TileCfg<DP>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -327,7 +323,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 float* sums = (float*)(smem + C::SUMS) + row;
                 uint32_t top = 0;
                 float x[QD];
-                if (a.q_vec) {
+                if (VEC) {
 #pragma unroll
                     for (int k = 0; k < QD / 4; ++k) {
                         const float4 v = live && QD * half + 4 * k < a.dim ? *(const float4*)(p + 4 * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -507,15 +503,15 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 const float k = l == 0.0f ? 0.0f : base / l;
                 const float top = top_of(ref, rf);
                 float* dst;
-                bool vec = true;
+                bool vec = VEC;
                 if (it.whole) {
                     const int head = it.head * a.group + r % a.group;
                     const int64_t token = it.row0 + r / a.group;
-                    dst = a.out + token * a.out_s1 + (int64_t)head * a.dim, vec = a.out_vec;
+                    dst = a.out + token * a.out_s1 + (int64_t)head * a.dim;
                     if (a.lse) a.lse[token * a.heads * a.group + head] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
                 } else {
                     float* p = part_slot(a, kTileRows, DP, blockIdx.x, it.begins);
-                    dst = p + 8 + 2 * kTileRows + row * DP;
+                    dst = p + 8 + 2 * kTileRows + row * DP, vec = true;
                     p[8 + 2 * row] = top, p[9 + 2 * row] = l;
                     if (row == 0 && it.begins) {
                         int* w = (int*)p;
@@ -744,7 +740,8 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                     p.n = max(0, min(it.to, (it.high - it.base + kTileTokens - 1) / kTileTokens) - it.from);  // (the units behind the tokens hold none)
                     p.pos = it.pos, p.all_first = it.top_first, p.all_last = it.pos + it.first_row / a.group, p.head = it.head;
                     p.low = it.low, p.high = it.high, p.first = it.base + kTileTokens * it.from, p.seq = it.seq;
-                    p.whole = it.from == 0 && it.to == it.units, p.begins = it.from == 0, p.last_block = sh.last_block(it);
+                    p.whole = it.from == 0 && it.to == it.units, p.begins = it.from == 0;
+                    if (p.begins && !p.whole) p.last_block = sh.last_block(it);
                     sh.advance(a, it);
                 }
                 const bool ok = warp_wait<1000>(&i_free[i & (kItems - 1)], (i / kItems & 1) ^ 1, ab, 42);
@@ -763,20 +760,25 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *gave_up) atomicCAS(a.status, 0, *gave_up);
     if (warp == kIssueWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
     }
 }
 
-template <int DP>
+template <int DP, bool VEC>
 int run_tiles(const AttnArgs& a, cudaStream_t st) {
     static bool done[64];
-    const cudaError_t e = allow_smem(attention_tiles<DP>, TileCfg<DP>::SMEM, done);
+    const cudaError_t e = allow_smem(attention_tiles<DP, VEC>, TileCfg<DP>::SMEM, done);
     if (e != cudaSuccess) return (int)e;
-    const int rc = (int)launch_dep(attention_tiles<DP>, dim3((unsigned)a.blocks), dim3(kTileThreads), TileCfg<DP>::SMEM, st, a);
+    const int rc = (int)launch_dep(attention_tiles<DP, VEC>, dim3((unsigned)a.blocks), dim3(kTileThreads), TileCfg<DP>::SMEM, st, a);
     if (rc) return rc;
     return (int)launch_dep(attention_join<DP>, dim3((unsigned)a.blocks, kTileRows / 4), dim3(128), 0, st, a);
+}
+template <int DP>
+int run_tiles(const AttnArgs& a, cudaStream_t st) {
+    return a.q_vec && a.out_vec ? run_tiles<DP, true>(a, st) : run_tiles<DP, false>(a, st);
 }
 
 }  // namespace
