@@ -409,8 +409,10 @@ MAG_CUDA_EXPORT int mag_cuda_kv_read(mag_compute_device_t* dvc, const mag_cuda_k
  * reaches the rows that see it and no other.  Rows outside start[0] .. start[seqs] keep what out and lse hold, and so do rows of
  * a sequence past its first max_new (an upper bound of n that the caller knows on the host); lengths are taken as at most
  * table_s1 * page_size and at least 0.
- * Products are formed on the tensor cores from f16 halves of the queries and the probabilities (22 bits each; the cache's
- * values are exact), sums and statistics in f32.  scale: finite, not negative.
+ * Products are formed on the tensor cores from f16 halves of the queries and the weights (22 bits each; the cache's
+ * values are exact), sums and statistics in f32.  A weight, a probability times its value's scale, is held to 2^-40 of the largest
+ * that the row sees (of kv heads with more than 16 rows in a sequence: to 2^-32), however far the scales lie apart; tokens that a
+ * row does not see change nothing but the rounding of its sums.  scale: finite, not negative.
  * The cache's scales are NaN or as mag_cuda_kv_write forms them: not negative and below 2^126.  A value's NaN scale makes out
  * NaN and may make lse NaN.  Logits are formed in f32 from queries brought to 2^13 .. 2^14, so that keys have to stay below about 2^98
  * in magnitude; above it a logit may overflow, and the rows that see it are NaN. */

@@ -29,6 +29,7 @@ namespace {
 // the former took 306 us with eight warps of four stages, 264 with a second launch that joins the parts, 255 without.)
 constexpr int kSms = 148;
 constexpr int kGroup = 16;               // tokens of a warp's step; pages hold a multiple
+constexpr float kLowest = -3.402823466e38f;  // the maximum of no logits
 constexpr int kFlush = 16;               // groups between two flushes: the tensor core's sums lose up to a step each
 
 template <int DP, bool STACK, int BLOCKS>
@@ -42,8 +43,8 @@ struct FewSmem {
     static constexpr int VALS = (STACK ? DP / 4 : DP / 2);  // outputs a thread holds
     static constexpr int WARPS = FewCfg<DP, STACK, BLOCKS>::WARPS;
     static constexpr int SUMS = FewCfg<DP, STACK, BLOCKS>::RING * WARPS;
-    static constexpr int STATS = SUMS + WARPS * 32 * VALS * 4;  // [warp][16] of (m, l), then [warp] of the values' unit, 16 ints
-    static constexpr int BYTES = STATS + WARPS * 16 * 8 + WARPS * 4 + 64;
+    static constexpr int STATS = SUMS + WARPS * 32 * VALS * 4;  // [warp][16] of (m, l), then [warp][16] of the outputs' unit, 16 ints
+    static constexpr int BYTES = STATS + WARPS * 16 * 12 + 64;
     static_assert(BLOCKS * (BYTES + 1024) <= 228 * 1024, "must fit shared memory");
     static_assert(Share<16, DP, 32 * WARPS>::SMEM <= SUMS, "the search for work takes the rings' room");
 };
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
     float4* sums = (float4*)(smem + S::SUMS) + warp * 8 * S::VALS;  // [VALS / 4][32]
     float2* stats = (float2*)(smem + S::STATS);
     float* units = (float*)(stats + kFewWarps * 16);
-    int* cut = (int*)(units + kFewWarps);  // what an item that ends, or begins, elsewhere is: 8 ints each
+    int* cut = (int*)(units + kFewWarps * 16);  // what an item that ends, or begins, elsewhere is: 8 ints each
         pdl_begin();
 
     Share<16, DP, 32 * kFewWarps> sh;
@@ -97,10 +98,9 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
         float o[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        float m[NR], l[NR], fade[NR];
+        float m[NR], l[NR], fade[NR], per[NR];  // per: 1 / the unit of the row's weights
 #pragma unroll
-        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f, fade[r] = 1.0f;
-        float unit = kLeastUnit, per_unit = 1.0f / kLeastUnit;
+        for (int r = 0; r < NR; ++r) m[r] = kLowest, l[r] = 0.0f, fade[r] = 1.0f, per[r] = 1.0f / kLeastUnit;
 #pragma unroll
         for (int e = 0; e < S::VALS / 4; ++e) sums[e * 32 + lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float up = query_unit(top);
-            rf[r] = a.scale * kLog2e / up;
+            rf[r] = fmaxf(a.scale * kLog2e / up, 0x1p-126f);  // (above zero, so that -inf times it is -inf)
 #pragma unroll
             for (int i = 0; i < KI; ++i)
 #pragma unroll
@@ -258,7 +258,6 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int j = j0 + 8 * (k >> 1) + 2 * c + (k & 1);
-                    if (j < it.low || j >= it.high) vs[k] = 0.0f;
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
                         seen[r][k] = j >= first[r] && j <= last[r];
@@ -266,24 +265,25 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
                     }
                 }
             }
-            // ---- the running maxima and the values' unit, where one of them grows
+            // ---- probabilities and weights (probability times the value's scale, in the row's unit); the running maxima and the
+            // units, where one of them grows
+            float p[NR][4], w[NR][4];
+            auto weigh = [&]() {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float e = exp2_f(fmaf(t[r][k] - m[r], rf[r], kTop));
+                        p[r][k] = e;  // (zero for -inf)
+                        w[r][k] = seen[r][k] ? e * per[r] * vs[k] : 0.0f;  // (in this order: neither product overflows)
+                    }
+            };
+            weigh();
             bool grows = false;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                grows |= vs[k] > unit;
-#pragma unroll
-                for (int r = 0; r < NR; ++r) grows |= t[r][k] > m[r];
-            }
+            for (int r = 0; r < NR; ++r)
+                grows |= fmaxf(fmaxf(t[r][0], t[r][1]), fmaxf(t[r][2], t[r][3])) > m[r] || fmaxf(fmaxf(w[r][0], w[r][1]), fmaxf(w[r][2], w[r][3])) > 0x1p15f;
             if (__any_sync(0xffffffffu, grows)) {
-                float v = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-                float shrink = 1.0f;
-                if (v > unit && v < kLargestScale) {
-                    const float next = unit_above(v);
-                    shrink = unit / next;
-                    unit = next, per_unit = 1.0f / next;
-                }
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
                     float x = fmaxf(fmaxf(t[r][0], t[r][1]), fmaxf(t[r][2], t[r][3]));
@@ -291,11 +291,20 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
                     float f = 1.0f;
                     if (x > m[r]) {
-                        f = m[r] == -INFINITY ? 0.0f : exp2_f((m[r] - x) * rf[r]);
+                        f = exp2_f((m[r] - x) * rf[r]);
                         m[r] = x;
                         l[r] *= f;
                     }
-                    f *= shrink;
+                    float big = 0.0f;  // the largest weight, as it is
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (seen[r][k]) big = fmaxf(big, exp2_f((t[r][k] - m[r]) * rf[r]) * vs[k]);
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                    const float held = one_by(per[r]) * f;  // what the older weights' unit has become
+                    const float unit = fmaxf(unit_from(fmaxf(held, kLeastUnit)), big > kLeastUnit && big < kLargestScale ? unit_above(big) : 0.0f);
+                    per[r] = one_by(unit);
+                    f = held * per[r];
                     fade[r] *= f;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
@@ -303,22 +312,17 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
                         if (STACK) o[j][2] *= f, o[j][3] *= f;
                     }
                 }
+                weigh();
             }
-            // ---- probabilities, times their values' scales in the unit, as operand fragments
+            // ---- as operand fragments
             uint32_t pf[QF][4];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                float w[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float p = exp2_f(fmaf(t[r][k] - m[r], rf[r], kTop));
-                    if (!seen[r][k]) p = 0.0f;
-                    l[r] += p;
-                    w[k] = seen[r][k] ? p * (vs[k] * per_unit) : 0.0f;
-                }
+                for (int k = 0; k < 4; ++k) l[r] += p[r][k];
                 uint32_t h0, l0, h1, l1;
-                split2(w[0], w[1], h0, l0);
-                split2(w[2], w[3], h1, l1);
+                split2(w[r][0], w[r][1], h0, l0);
+                split2(w[r][2], w[r][3], h1, l1);
                 if (STACK) {
                     pf[0][0] = h0, pf[0][1] = l0, pf[0][2] = h1, pf[0][3] = l1;
                 } else {
@@ -360,9 +364,8 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
         for (int r = 0; r < NR; ++r) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (c == 0) stats[warp * 16 + g + 8 * r] = make_float2(top_of(m[r], rf[r]), l[r]);
+            if (c == 0) stats[warp * 16 + g + 8 * r] = make_float2(m[r] == kLowest ? kNone : top_of(m[r], rf[r]), l[r]), units[warp * 16 + g + 8 * r] = one_by(per[r]);
         }
-        if (lane == 0) units[warp] = unit;
         const bool whole = it.from == 0 && it.to == it.units;
         if (!whole && warp == kFewWarps - 1 && lane == 0) {
             int* c = cut + 8 * (it.from == 0);
@@ -388,8 +391,8 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
 #pragma unroll
             for (int w = 0; w < kFewWarps; ++w) {
                 const float4 t = ((float4*)(smem + S::SUMS))[w * 8 * S::VALS + x];
-                const float k = f[w] * inv * units[w];
-                v.x = fmaf(t.x, k, v.x), v.y = fmaf(t.y, k, v.y), v.z = fmaf(t.z, k, v.z), v.w = fmaf(t.w, k, v.w);
+                const float k = f[w] * inv, unit = units[w * 16 + row];  // (their product may be less than f32 holds)
+                v.x = fmaf(t.x * k, unit, v.x), v.y = fmaf(t.y * k, unit, v.y), v.z = fmaf(t.z * k, unit, v.z), v.w = fmaf(t.w * k, unit, v.w);
             }
             put_out(a, sh, it, row, d, v, top, total);
         }

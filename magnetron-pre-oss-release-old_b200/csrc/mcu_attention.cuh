@@ -12,7 +12,10 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 constexpr float kNone = -3.0e38f;               // the maximum of no logits: finite, so that differences of it stay numbers
 constexpr float kTop = 15.0f;                   // probabilities are formed as 2^kTop p: their f16 halves keep 22 bits down to 2^-18
-constexpr float kLeastUnit = 0x1p-120f;         // unit of the values' scales before any was seen (the least scale is 2^-109)
+// Weights p s (probability times the value's scale) are formed in units of a power of two above the largest of a row's, so that
+// their f16 halves hold them to 2^-40 of that: of what the row itself sees, whatever else lies beside it, and however small the
+// probabilities are.
+constexpr float kLeastUnit = 0x1p-110f;         // a row's unit before any weight was seen (the least scale is 2^-109)
 constexpr float kLargestScale = 0x1p126f;       // a scale that is no number or not finite does not set the unit
 constexpr int kUnitTokens = 128;                // tokens of a unit of work
 

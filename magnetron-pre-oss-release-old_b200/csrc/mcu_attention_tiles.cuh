@@ -14,14 +14,15 @@ using namespace mcu;
 //   S = Qh K^T + Ql K^T,   O = Ph V + Pl V,
 // Q and P as two f16 (22 bits), K and V exact in f16.  Both left operands lie in TMEM, where a product's rate does not hang on
 // two operands' shared-memory reads: 2 x 128 columns of S, over which P is written in place, 128 of O, 128 of Q.  O starts
-// from zero for every 128 tokens and is added in registers in f32 (rounded to nearest), times the step of the row's reference and
-// the unit of the tile's value scales: no accumulator is ever rescaled, and the tensor core's truncating sums stay short.
+// from zero for every 128 tokens and is added in registers in f32 (rounded to nearest), times the step from the tile's highest logit
+// to the row's and the unit of the tile's value scales: no accumulator is ever rescaled, and the tensor core's truncating sums stay short.
 //   warps 0-7    softmax: warp w has the rows 32 (w & 3) .. and half w / 4 of the tokens
 //   warps 8-11   sums: O of each tile, in turn, to the rows' f32 sums in registers; the output at the end
 //   warps 12-15  loaders: e4m3 from the pages by cp.async, two tiles ahead, then to f16 tiles (128-byte swizzle)
 //   warp 16      issues the products: S of tile j + 1 before O of tile j
 //   warp 17      plans: puts the block's items into a ring, so that the others find theirs without global loads
-//   warp 18      guides: each tile's places in the pages and its scales, up to four tiles ahead
+//   warp 18      guides: each tile's places in the pages and its scales, up to four tiles ahead; tokens of very different scales of
+//                values go into tiles of their own
 // What bounds it is the softmax: about 14 instructions for two logits (390 cycles for 32 x 32 of them with four warps a
 // scheduler, alone), more than the products' 2 x 1024 cycles a tile.  The loops of all roles have to fit the SM's instruction cache
 // together: unrolled for 128 columns they took three times as long.  Eight softmax warps hold half a row's logits each in registers
@@ -36,6 +37,9 @@ static_assert(kSoftRegs >= kTileLaunch && kSumRegs >= kTileLaunch && kLoadRegs <
 static_assert(2 * kSoftRegs + kSumRegs + kLoadRegs + kIssueRegs == 5 * kTileLaunch, "register split must match the launch");
 constexpr int kSoftThreads = 32 * kSoftWarps;
 constexpr float kLeastBase = 0x1p-78f;  // unit of a row's sums
+// Scales that may share a unit.  A row's largest weight of a tile is at least 2^15 kNear then, and each weight is off by 2^-25 at most (half
+// of f16's least step): 128 of them by 2^-33 / kNear of the largest, half an f32 step of it.
+constexpr float kNear = 0x1p-8f;
 constexpr int kItems = 4;             // items in the planner's ring
 
 // What the roles need of an item, as the planner leaves it; rows = 0: no more.
@@ -54,11 +58,11 @@ struct TileCfg {
     static constexpr int K = 0, V = 2 * TILE;
     static constexpr int RAW = 4 * TILE;                     // [2] of keys, then values, as loaded: each thread's own pieces
     static constexpr int RAW_TILE = TILE / 2;
-    static constexpr int SCALES = RAW + 4 * RAW_TILE;        // 4 x {keys' scales, values' ratios, valid tokens, unit}
+    static constexpr int SCALES = RAW + 4 * RAW_TILE;        // 4 x {keys' scales, values' ratios, valid tokens, {unit, item's last, first token}}
     static constexpr int SLOT = 2 * kTileTokens * 4 + 32;
     static constexpr int MAXIMA = SCALES + 4 * SLOT;         // [2][2][128]: of a tile's logits, by half
     static constexpr int SUMS = MAXIMA + 2 * 2 * 128 * 4;    // [2][128]: queries' maxima, by half
-    static constexpr int REFS = SUMS + 2 * 128 * 4;          // [4][128] of (maximum, unit): what a tile's O is relative to
+    static constexpr int REFS = SUMS + 2 * 128 * 4;          // [4][128] of (the row's maximum, unit): what a tile's O is relative to; the unit below zero: the item's last
     static constexpr int FACTORS = REFS + 4 * 128 * 8;       // [4][128]: rf of an item's rows
     static constexpr int STATS = FACTORS + 4 * 128 * 4;      // [2][128]: an item's sums, by half
     static constexpr int PLACES = STATS + 2 * 128 * 4;   // 4 x {8 groups' offsets in the pages, valid tokens}
@@ -198,6 +202,9 @@ __device__ __forceinline__ void split_pair(uint64_t w, uint32_t& high, uint32_t&
         : "l"(w));
 }
 
+// 2^((x - top) rf): the weight beside a maximum of top of what is relative to x (x at most top; both may be -inf).
+__device__ __forceinline__ float lift_of(float x, float top, float rf) { return x == top ? 1.0f : exp2_f((x - top) * rf); }
+
 // Items whose units several blocks had: blockIdx.x is the block that began it, a warp takes a row.  A kernel of its own: a
 // block whose wait was given up would not be counted.
 template <int DP>
@@ -250,7 +257,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&sc_full[i], 32);
-            mbar_init(&sc_free[i], kSoftWarps);  // a lane of each warp that has read them
+            mbar_init(&sc_free[i], kSoftWarps + 1);  // a lane of each warp that has read them, the issuer's too
             mbar_init(&place_full[i], 32);
             mbar_init(&place_free[i], 4);
         }
@@ -359,19 +366,19 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 tc_fence_before();
                 mbar_arrive(q_full);
             }
-            const int last = live ? it.pos + r / a.group : -1, first = a.window && last >= a.window ? last - a.window + 1 : 0;
+            const int newest = live ? it.pos + r / a.group : -1, oldest = a.window && newest >= a.window ? newest - a.window + 1 : 0;
             const uint64_t rf2 = pair_of(rf, rf), top2 = pair_of(kTop, kTop);
             float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
-            for (int j = 0; j < it.n; ++j, ++t) {
+            for (bool last = !it.n; !last; ++t) {
                 const uint8_t* slot = smem + C::SCALES + (t & 3) * C::SLOT;
                 const ulonglong2* ks = (const ulonglong2*)(slot + 64 * half * 4);
                 const ulonglong2* vs = (const ulonglong2*)(slot + (kTileTokens + 64 * half) * 4);
                 const uint32_t sc = tmem + lanes + C::S_COL + 128 * (t & 1) + 64 * half;
-                const int j0 = it.first + kTileTokens * j;
-                warp_wait(&sc_full[t & 3], t >> 2 & 1, ab, 32);
+                bool on = warp_wait(&sc_full[t & 3], t >> 2 & 1, ab, 32);
+                const int j0 = *(const int*)(slot + 2 * kTileTokens * 4 + 24);
                 const uint4 ok = *(const uint4*)(slot + 2 * kTileTokens * 4);
-                warp_wait(&s_full[t & 1], t >> 1 & 1, ab, 33);
+                on &= warp_wait(&s_full[t & 1], t >> 1 & 1, ab, 33);
                 tc_fence_after();
                 uint64_t s[32];
 #pragma unroll
@@ -389,7 +396,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 if (j0 < it.all_first || j0 + kTileTokens - 1 > it.all_last || (ok.x & ok.y & ok.z & ok.w) != 0xffffffffu) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const int at = j0 + 64 * half + 32 * c, lo = max(first - at, 0), hi = min(last - at, 31);
+                        const int at = j0 + 64 * half + 32 * c, lo = max(oldest - at, 0), hi = min(newest - at, 31);
                         const uint32_t bits = half ? (c ? ok.w : ok.z) : (c ? ok.y : ok.x);
                         const uint32_t seen = lo > hi ? 0u : bits & (0xffffffffu << lo) & (0xffffffffu >> (31 - hi));
 #pragma unroll
@@ -412,15 +419,18 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 }
                 float* mine = maxima + (t & 1) * 256;
                 mine[half * 128] = fmaxf(x, y);
-                bar_named(pair, 64);
-                x = fmaxf(mine[0], mine[128]);
-                if (x > m) {
-                    l *= m == -INFINITY ? 0.0f : exp2_f((m - x) * rf);
-                    m = x;
+                const float2 common = *(const float2*)(slot + 2 * kTileTokens * 4 + 16);
+                const float unit = common.x;
+                last = bar_any(pair, 64, common.y != 0.0f || !on);  // (both warps' answer is one, whatever was read after a wait was given up)
+                const float top = fmaxf(mine[0], mine[128]);
+                if (top > m) {
+                    l *= m == -INFINITY ? 0.0f : exp2_f((m - top) * rf);
+                    m = top;
                 }
-                if (half == 0) ((float2*)(smem + C::REFS))[(t & 3) * 128 + row] = make_float2(m, *(const float*)(slot + 2 * kTileTokens * 4 + 16));
-                const float ref = m == -INFINITY ? 0.0f : -m;
+                const float ref = top == -INFINITY ? 0.0f : -top;  // (weights are relative to the tile's own maximum)
                 const uint64_t ref2 = pair_of(ref, ref);
+                const float lift = lift_of(top, m, rf);  // (of the tile's weights beside the row's)
+                if (half == 0) ((float2*)(smem + C::REFS))[(t & 3) * 128 + row] = make_float2(m, copysignf(unit * lift, last ? -1.0f : 1.0f));
                 uint64_t sum = 0;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -440,7 +450,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                     tmem_st16(sc + 32 * c + 16, lo);
                 }
                 unpair(sum, x, y);
-                l += x + y;
+                l = fmaf(x + y, lift, l);
                 tmem_st_done();
                 tc_fence_before();
                 mbar_arrive(&p_full[t & 1]);
@@ -468,11 +478,13 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
             // overflows; per = 1 / base.  (Not below kLeastBase, so that base / l is normal.)
             float base = kLeastBase, per = 1.0f / kLeastBase;
 #pragma unroll 1
-            for (int j = 0; j < it.n; ++j, ++t) {
-                warp_wait<100>(o_full, t & 1, ab, 31);
+            for (bool last = !it.n; !last; ++t) {
+                const bool on = warp_wait<100>(o_full, t & 1, ab, 31);
                 tc_fence_after();
                 rf = ((const float*)(smem + C::FACTORS))[(i & 3) * 128 + row];
-                const float2 mu = ((const float2*)(smem + C::REFS))[(t & 3) * 128 + row];
+                float2 mu = ((const float2*)(smem + C::REFS))[(t & 3) * 128 + row];
+                last = __any_sync(0xffffffffu, signbit(mu.y) || !on);
+                mu.y = fabsf(mu.y);
                 if (__any_sync(0xffffffffu, mu.x > ref || mu.y > base)) {
                     const float fade = ref == mu.x ? 1.0f : exp2_f((ref - mu.x) * rf), held = base * fade;  // (from -inf: 0)
                     ref = mu.x;
@@ -646,8 +658,12 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 ok = warp_wait(q_full, queries++ & 1, ab, 37);
                 tc_fence_after();
                 logits(t);
-                for (int j = 0; ok && j < it.n; ++j, ++t) {
-                    if (j + 1 < it.n) logits(t + 1);
+                for (bool last = false; ok && !last; ++t) {
+                    ok = warp_wait(&sc_full[t & 3], t >> 2 & 1, ab, 49);
+                    last = *(const float*)(smem + C::SCALES + (t & 3) * C::SLOT + 2 * kTileTokens * 4 + 20) != 0.0f;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_free[t & 3]);
+                    if (ok && !last) logits(t + 1);
                     ok = ok && warp_wait(&v_full[t & 1], t >> 1 & 1, ab, 38);
                     ok = ok && warp_wait(&p_full[t & 1], t >> 1 & 1, ab, 39);
                     ok = ok && (t == 0 || warp_wait(o_free, (t - 1) & 1, ab, 40));
@@ -674,58 +690,69 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                 for (uint32_t i = 0; i < kWaitLimit && !mbar_test(drain, 0); ++i) __nanosleep(64);
             __syncwarp();
         } else if (warp == kGuideWarp) {  // ---- guide: lane l has the tokens 4 l .. 4 l + 3 of a tile, of group l / 4
-            float4 ks = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vs = ks;
-            uint32_t in = 0;  // which of the lane's four tokens exist, of the tile whose scales are on their way
-            bool pending = false;
-            uint32_t x = 0;   // the tile
-            // the scales of tile x - 1: the unit is the least power of two above the tile's largest
-            auto finish = [&]() {
-                const uint32_t y = x - 1;
-                warp_wait<300>(&sc_free[y & 3], (y >> 2 & 1) ^ 1, ab, 47);
-                float k[4] = {ks.x, ks.y, ks.z, ks.w}, v[4] = {vs.x, vs.y, vs.z, vs.w};
-                uint32_t top = 0;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if (!(in >> q & 1)) k[q] = v[q] = 0.0f;
-                    if (!(v[q] < kLargestScale) || !(fabsf(k[q]) < INFINITY)) k[q] = __uint_as_float(0x7FFFFFFFu), v[q] = 0.0f;  // who sees it is lost
-                    top = max(top, abs_bits(v[q]));
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-                const float unit = unit_above(fmaxf(__uint_as_float(top), kLeastUnit)), per = 1.0f / unit;
-                uint8_t* slot = smem + C::SCALES + (y & 3) * C::SLOT;
-                ((float4*)slot)[lane] = make_float4(k[0], k[1], k[2], k[3]);
-                ((float4*)(slot + kTileTokens * 4))[lane] = make_float4(v[0] * per, v[1] * per, v[2] * per, v[3] * per);
-                uint32_t bits = in << 4 * (lane & 7);
-                bits = __reduce_or_sync(0xffu << (lane & 24), bits);
-                if ((lane & 7) == 0) ((uint32_t*)(slot + 2 * kTileTokens * 4))[lane >> 3] = bits;
-                if (lane == 0) ((float*)(slot + 2 * kTileTokens * 4))[4] = unit;
-                mbar_arrive(&sc_full[y & 3]);
-            };
+            // Tokens whose scales lie within 2^kNear share a unit, the least power of two above the largest, so that the weights' f16 halves
+            // keep f32's bits beside the largest that a row sees.  Where a tile's differ by more it is taken in several rounds, of tokens
+            // of like scales, largest first: tiles of the same places, of which other tokens are there.
+            uint32_t x = 0;  // the tile
 #pragma unroll 1
             for (uint32_t i = 0;; ++i) {
                 const TileItem it = item(i, 0, 0);
                 const int32_t* table = a.table + (int64_t)it.seq * a.table_s1;
                 int tok = it.first + 4 * lane, page = it.rows && it.n && (tok & ~15) < it.high ? table[tok >> a.page_log] : -1;
+                bool on = it.rows != 0;
 #pragma unroll 1
-                for (int j = 0; j < (it.rows ? it.n : 1); ++j, ++x) {
+                for (int j = 0; j < (it.rows ? it.n : 1); ++j) {
                     const bool exists = (uint32_t)page < (uint32_t)a.pages;
                     const int64_t s = exists ? ((((int64_t)page * a.heads) + it.head) << a.page_log) + (tok & ((1 << a.page_log) - 1)) : (int64_t)(4 * (lane & 3));
-                    uint32_t now = 0;
+                    uint32_t in = 0;  // which of the lane's four tokens exist
                     if (exists)
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) now |= (uint32_t)(tok + q >= it.low && tok + q < it.high) << q;
+                        for (int q = 0; q < 4; ++q) in |= (uint32_t)(tok + q >= it.low && tok + q < it.high) << q;
+                    const float4 ks = *(const float4*)(a.ks + s), vs = *(const float4*)(a.vs + s);
                     if (j + 1 < it.n) page = ((tok + kTileTokens) & ~15) < it.high ? table[(tok + kTileTokens) >> a.page_log] : -1;
-                    if (!warp_wait<300>(&place_free[x & 3], (x >> 2 & 1) ^ 1, ab, 48)) break;
-                    int64_t* places = (int64_t*)(smem + C::PLACES + (x & 3) * C::PLACE);
-                    if ((lane & 3) == 0) places[lane >> 2] = it.rows ? s * a.dim : (int64_t)-1;  // (below zero: no more tiles)
-                    const uint32_t bits = __reduce_or_sync(0xffu << (lane & 24), now << 4 * (lane & 7));
-                    if ((lane & 7) == 0) ((uint32_t*)(places + 8))[lane >> 3] = bits;
-                    mbar_arrive(&place_full[x & 3]);
-                    if (pending) finish();
-                    pending = it.rows != 0;
-                    if (!pending) break;
-                    ks = *(const float4*)(a.ks + s), vs = *(const float4*)(a.vs + s);
-                    in = now;
+                    const uint32_t all = __reduce_or_sync(0xffu << (lane & 24), in << 4 * (lane & 7));
+                    float k[4] = {ks.x, ks.y, ks.z, ks.w}, v[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (!(in >> q & 1)) k[q] = v[q] = 0.0f;
+                        if (!(v[q] < kLargestScale) || !(fabsf(k[q]) < INFINITY)) k[q] = __uint_as_float(0x7FFFFFFFu), v[q] = 0.0f;  // who sees it is lost
+                    }
+                    bool more;  // another round
+                    do {
+                        on = warp_wait<300>(&place_free[x & 3], (x >> 2 & 1) ^ 1, ab, 48) && on;
+                        int64_t* places = (int64_t*)(smem + C::PLACES + (x & 3) * C::PLACE);
+                        if ((lane & 3) == 0) places[lane >> 2] = it.rows ? s * a.dim : (int64_t)-1;  // (below zero: no more tiles)
+                        if ((lane & 7) == 0) ((uint32_t*)(places + 8))[lane >> 3] = all;
+                        mbar_arrive(&place_full[x & 3]);
+                        if (!on) break;
+                        uint32_t top = 0, take = 0;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            if (in >> q & 1) top = max(top, abs_bits(v[q]));
+                        top = __reduce_max_sync(0xffffffffu, top);
+                        const float unit = unit_above(fmaxf(__uint_as_float(top), kLeastUnit)), per = one_by(unit);
+                        float w[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const bool like = in >> q & 1 && v[q] >= __uint_as_float(top) * kNear;
+                            take |= (uint32_t)like << q;
+                            w[q] = like ? v[q] * per : 0.0f;
+                        }
+                        in &= ~take;
+                        more = __any_sync(0xffffffffu, in != 0);
+                        warp_wait<300>(&sc_free[x & 3], (x >> 2 & 1) ^ 1, ab, 47);
+                        uint8_t* slot = smem + C::SCALES + (x & 3) * C::SLOT;
+                        ((float4*)slot)[lane] = make_float4(k[0], k[1], k[2], k[3]);
+                        ((float4*)(slot + kTileTokens * 4))[lane] = make_float4(w[0], w[1], w[2], w[3]);
+                        const uint32_t bits = __reduce_or_sync(0xffu << (lane & 24), take << 4 * (lane & 7));
+                        if ((lane & 7) == 0) ((uint32_t*)(slot + 2 * kTileTokens * 4))[lane >> 3] = bits;
+                        if (lane == 0)
+                            *(float4*)(slot + 2 * kTileTokens * 4 + 16) =
+                                make_float4(unit, j + 1 == it.n && !more ? 1.0f : 0.0f, __int_as_float(it.first + kTileTokens * j), 0.0f);
+                        mbar_arrive(&sc_full[x & 3]);
+                        ++x;
+                    } while (more);
+                    if (!on) break;
                     tok += kTileTokens;
                 }
                 if (!it.rows || *gave_up) break;
