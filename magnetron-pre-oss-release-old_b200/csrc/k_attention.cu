@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
         }
         int first_token = it.base + kGroup * g0;
         const int key0 = g * DP + 16 * key_chunk<DP>(c, g), value0 = kGroup * DP + 2 * c * DP + 16 * value_chunk<DP>(DP == 128 ? g : g >> 1, 2 * c) + (DP == 128 ? 0 : 8 * (g & 1));
-        for (int i = 0, st = kFewStages - 1; i < steps; ++i) {
+        for (int i = 0, st = kFewStages - 1, summed = 0; i < steps; ++i) {  // summed: groups since the last flush
             asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
             __syncwarp();
             st = st == kFewStages - 1 ? 0 : st + 1;
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
                         for (int f = 0; f < QF; ++f) mma16(o[4 * w + 2 * h + k], pf[f], b0, b1);
                     }
                 }
-            if ((i & (kFlush - 1)) == kFlush - 1) flush();
+            if (++summed == kFlush) flush(), summed = 0;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         flush();

@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 
 from attention_ref import U
-from test_gpu_lm_attention import Batch
+from gpu_util import device
+from test_gpu_lm_attention import Batch, blank, get, ints, up
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +184,28 @@ def test_scales_over_many_powers_of_two(new, length, group, low, high, window):
     g = np.random.default_rng([0x5C, new, length, group, 200 + low])
     set_scales(b, np.float32(2.0) ** g.integers(low, high, scales(b).shape).astype(np.float32) * np.float32(1.3))
     close(b)
+
+
+def test_sums_stay_short_where_pages_are_missing():
+    """A single token over 8.5 million, of which every block's warps miss each sixteenth group of 16 tokens (twelve warps take groups
+    in turn, blocks have equal shares in units of 128 tokens): the sums between two flushes are no longer for it.  All logits are
+    zero and the values 448 and 13 of a unit in turn, so that the mean is half their sum and no sum is exact."""
+    d, page, dim, blocks, warps = device(), 16, 16, 148, 12
+    units = blocks * 450
+    pages = units * 128 // page
+    c = d.kv_cache(pages, 1, dim, page)
+    value = np.float32(0.7123457)
+    c.v.write(np.tile(np.repeat(np.uint8([TOP, 0x55]), dim), c.v.numel * 4 // (2 * dim)).view(np.float32))
+    c.v_scale.write(np.full(c.v_scale.numel, value, np.float32))
+    c.k_scale.write(np.ones(c.k_scale.numel, np.float32))
+    table = np.arange(pages)
+    begin = (units * np.arange(blocks + 1) // blocks) * 8  # of each block, in groups
+    at = table - begin[np.searchsorted(begin, table, side="right") - 1]
+    table[at // warps % 16 == 15] = -1
+    out, lse = blank(1, dim), blank(1, 1)
+    d.attention_paged(c, 1, 1, out, up(np.ones(dim)), ints(table), ints([0, 1]), ints([pages * page]), 1, pages, max_new=1, scale=1.0, lse=lse)
+    want, count = (448.0 + 13.0) / 2 * float(value), int((table >= 0).sum()) * page
+    # 16 tensor instructions between flushes, each losing up to a step (2 U) of the sum; 300 / 16 flushes, 12 warps and 148 parts with a
+    # rounding each; the weights' halves (4 U), and some ten roundings more
+    assert np.all(np.abs(get(out, dim) - want) <= (16 * 2 + 19 + 12 + 148 + 4 + 10) * U * want)
+    assert abs(get(lse, 1)[0] - np.log(count)) <= (300 * 4 + 12 + 148 + 10) * U + 4 * U * np.log(count)
