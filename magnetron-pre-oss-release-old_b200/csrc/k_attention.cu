@@ -55,6 +55,22 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Four values of an item's row from column d on, normed by the sum `total` of 2^(logit - top): to out, with the row's lse, where
+// the block has the whole item, else to the block's slot.
+template <int DP, int THREADS>
+__device__ __forceinline__ void put_out(const AttnArgs& a, const Share<16, DP, THREADS>& sh, const Item& it, int row, int d, float4 v, float top,
+                                        float total) {
+    if (it.from == 0 && it.to == it.units) {
+        const int r = it.first_row + row, token = r / a.group, head = it.head * a.group + r % a.group;
+        store_row(a, it.row0 + token, head, d, v);
+        if (d == 0 && a.lse) a.lse[(int64_t)(it.row0 + token) * a.heads * a.group + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+        return;
+    }
+    float* p = sh.slot(a, it.from == 0);
+    if (d == 0) p[8 + 2 * row] = top, p[9 + 2 * row] = total;
+    *(float4*)(p + 8 + 2 * 16 + row * DP + d) = v;
+}
+
 // EXACT: the head has DP values, so that a group's rows lie at constant distances.
 template <int DP, bool STACK, bool EXACT, int BLOCKS>
 __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS) attention_few(AttnArgs a) {

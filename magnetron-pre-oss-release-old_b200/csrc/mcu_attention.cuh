@@ -159,7 +159,7 @@ __device__ __forceinline__ int span_of(const AttnArgs& a, const Seq& q, int64_t 
     return max(1, (high - (low & ~15) + kUnitTokens - 1) / kUnitTokens + extra_units<MAX>());
 }
 
-// A slot of a block's part of an item: 8 ints (for tiles of many rows: 1 if it begins an item that ends elsewhere, the item's
+// A slot of a block's part of an item: 8 ints (attention_tiles alone uses them: 1 if it begins an item that ends elsewhere, the item's
 // head, rows, first row, row0, last block), then maximum and sum of each row, then its rows of output.
 __host__ __device__ constexpr int64_t part_floats(int max, int dp) { return 8 + 2 * max + (int64_t)max * dp; }
 __device__ __forceinline__ float* part_slot(const AttnArgs& a, int max, int dp, int64_t block, int which) {
@@ -365,28 +365,6 @@ struct Share {
     }
     __device__ static float* slot(const AttnArgs& a, int which) { return part_slot(a, MAX, DP, blockIdx.x, which); }
 };
-
-// Four values of an item's row from column d on, normed by the sum `total` of 2^(logit - top): to out, with the row's lse, where
-// the block has the whole item, else to the block's slot.
-template <int MAX, int DP, int THREADS>
-__device__ __forceinline__ void put_out(const AttnArgs& a, const Share<MAX, DP, THREADS>& sh, const Item& it, int row, int d, float4 v,
-                                        float top, float total) {
-    if (it.from == 0 && it.to == it.units) {
-        const int r = it.first_row + row, token = r / a.group, head = it.head * a.group + r % a.group;
-        store_row(a, it.row0 + token, head, d, v);
-        if (d == 0 && a.lse) a.lse[(int64_t)(it.row0 + token) * a.heads * a.group + head] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
-        return;
-    }
-    float* p = sh.slot(a, it.from == 0);
-    if (d == 0) {
-        p[8 + 2 * row] = top, p[9 + 2 * row] = total;
-        if (MAX > 16 && row == 0 && it.from == 0) {
-            int* m = (int*)p;
-            m[1] = it.head, m[2] = it.rows, m[3] = it.first_row, m[4] = it.row0, m[5] = sh.last_block(it), m[0] = 1;
-        }
-    }
-    *(float4*)(p + 8 + 2 * MAX + row * DP + d) = v;
-}
 
 // Row `row` of an item whose units the blocks [first, first + parts) had; a warp.  The parts' weights are their sums times
 // 2^(top - the highest top); parts are added in the blocks' order.
