@@ -348,7 +348,8 @@ MAG_CUDA_EXPORT int mag_cuda_token_logprobs_backward_f32(mag_compute_device_t* d
  * pass): pair p < rot / 2 turns by the angle pos[row] * inv_freq[p],
  *   (a, b) -> magnitude (a cos - b sin, b cos + a sin),
  * the pair being values (p, p + rot / 2), or with interleaved != 0 values (2 p, 2 p + 1).  Angles are formed and
- * reduced in f64: positions of any int32 value keep their turn's fraction.  Scaled rotations (linear, by
+ * reduced in f64, each product rounded there (by 2^-53 of the angle at most: 2^-23 for a frequency of 1 at the last int32 positions): positions
+ * of any int32 value keep their turn's fraction to about that.  Scaled rotations (linear, by
  * wavelength, with a magnitude) lie in the table and the magnitude. */
 typedef struct mag_cuda_rotation {
     const int32_t* pos;    /* [rows], device */
