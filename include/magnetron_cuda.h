@@ -342,7 +342,8 @@ MAG_CUDA_EXPORT int mag_cuda_token_logprobs_backward_f32(mag_compute_device_t* d
  * stride of x_s1 values (at least heads * head_dim), so that queries, keys and values may be parts of one
  * row of a fused projection.  Calls check, order, capture and count as those of the section above; what lies on
  * the device (positions, slots, tables, lengths) is checked by the kernels, which skip what is out of range.
- * Sums are formed in f32 in a fixed order, so that the same call gives the same bits. */
+ * Sums are formed in f32 in a fixed order, so that the same call gives the same bits.  Captured graphs share neither scratch nor
+ * counters with one another or with eager calls: their replays may run beside them, where the caller orders the tensors' uses. */
 
 /* The position's rotation of the first rot values of a head (rot a multiple of 8, at most head_dim; the rest
  * pass): pair p < rot / 2 turns by the angle pos[row] * inv_freq[p],

@@ -117,7 +117,10 @@ typedef struct mcu_device {
     int stage_next;
     void* scratch;
     size_t scratch_bytes;
-    int* d_status; /* MCU_STATUS_WORDS of them */
+    int* d_status;
+    uint32_t* counters;          /* sets of MCU_COUNTERS: of eager calls, then of captured graphs */
+    int counter_sets;            /* handed to captured graphs */
+    unsigned long long counter_capture; /* the capture that has the last of them */
     mcu_graph* graphs;
     void* graph_scratch; /* scratch of the graph being captured */
     int profiling;
@@ -613,8 +616,11 @@ mag_compute_device_t* mag_init_device_cuda(mag_ctx_t* ctx) {
         MCU_CHECK(cudaEventCreateWithFlags(&d->stage_ev[i], cudaEventDisableTiming));
         MCU_CHECK(cudaEventRecord(d->stage_ev[i], d->stream));
     }
-    MCU_CHECK(cudaMalloc((void**)&d->d_status, MCU_STATUS_WORDS * sizeof(int)));
-    MCU_CHECK(cudaMemset(d->d_status, 0, MCU_STATUS_WORDS * sizeof(int)));
+    MCU_CHECK(cudaMalloc((void**)&d->d_status, sizeof(int)));
+    MCU_CHECK(cudaMemset(d->d_status, 0, sizeof(int)));
+    const size_t counters = (size_t)(1 + MCU_COUNTER_SETS) * MCU_COUNTERS * sizeof(uint32_t);
+    MCU_CHECK(cudaMalloc((void**)&d->counters, counters));
+    MCU_CHECK(cudaMemset(d->counters, 0, counters));
     snprintf(dvc->name, sizeof(dvc->name), "%.96s (sm_%d%d, %d SMs)", prop.name, prop.major, prop.minor,
              prop.multiProcessorCount);
     dvc->impl = d;
@@ -663,6 +669,7 @@ void mag_destroy_device_cuda(mag_compute_device_t* dvc) {
     }
     cudaStreamSynchronize(d->stream);
     cudaFree(d->d_status);
+    cudaFree(d->counters);
     cudaStreamSynchronize(d->copy_stream);
     for (size_t i = 0; i < d->tab_cap; ++i)
         if (d->tab[i].io_ev) cudaEventDestroy(d->tab[i].io_ev);
@@ -714,7 +721,7 @@ int mcu_call_begin(mcu_call* c, mag_compute_device_t* dvc, const mcu_buf* bufs, 
     if (c->prev_device != d->ordinal && (e = cudaSetDevice(d->ordinal)) != cudaSuccess) return (int)e;
     enum cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     int rc = (int)cudaStreamIsCapturing(d->stream, &cap);
-    const int captured = cap != cudaStreamCaptureStatusNone;
+    const int captured = c->captured = cap != cudaStreamCaptureStatusNone;
     if (!rc && captured) {
         for (int i = 0; i < n; ++i) {
             mcu_block* b = bufs[i].p ? tab_find_containing(d, (uintptr_t)bufs[i].p) : NULL;
@@ -756,6 +763,20 @@ int mcu_call_begin(mcu_call* c, mag_compute_device_t* dvc, const mcu_buf* bufs, 
     for (int i = 0; i < n; ++i)
         if (bufs[i].p && bufs[i].out) ext_out(d, (void*)bufs[i].p, bufs[i].bytes);
     return 0;
+}
+
+uint32_t* mcu_call_counters(mcu_call* c) {
+    mcu_device* d = dev_of(c->dvc);
+    if (!c->captured) return d->counters;
+    enum cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(d->stream, &cap, &id, NULL, NULL, NULL) != cudaSuccess) return NULL;
+    if (!d->counter_sets || id != d->counter_capture) { /* (a graph's calls follow one another) */
+        if (d->counter_sets == MCU_COUNTER_SETS) return NULL;
+        d->counter_sets++;
+        d->counter_capture = id;
+    }
+    return d->counters + (size_t)d->counter_sets * MCU_COUNTERS;
 }
 
 int mcu_call_end(mcu_call* c, int rc, int kernels) {

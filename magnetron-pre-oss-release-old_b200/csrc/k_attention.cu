@@ -3,6 +3,7 @@
 #include <cstdint>
 #include "mcu_attention.cuh"
 #include "mcu_attention_tiles.cuh"
+#include "mcu_device.h"
 
 using namespace mcu;
 
@@ -458,7 +459,7 @@ int few(const AttnArgs& a, cudaStream_t st) {
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-static_assert(MCU_JOIN_WORD + kMostBlocks * kSms <= MCU_STATUS_WORDS, "a counter for each block");
+static_assert(kMostBlocks * kSms <= MCU_COUNTERS, "a counter for each block");
 constexpr int kFewRows = 16;
 int padded(const mcu_attention* a) { return a->cache.head_dim <= 64 ? 64 : 128; }
 
@@ -476,20 +477,24 @@ Forms forms_of(const mcu_attention* a) {
     return Forms{group <= 8 ? 8 : group <= kFewRows ? kFewRows : 0, true};
 }
 
+// Scratch: the parts of tiles, then those of few rows, then counters for a call that got none.
+int64_t few_floats(const mcu_attention* a, const Forms& f) { return f.few ? 2 * kSms * kMostBlocks * part_floats(kFewRows, padded(a)) : 0; }
+int64_t tile_floats(const mcu_attention* a, const Forms& f) { return f.tiles ? 2 * kSms * part_floats(kTileRows, padded(a)) : 0; }
+
 }  // namespace
 
 extern "C" size_t mcu_attention_scratch_bytes(const mcu_attention* a) {
     const Forms f = forms_of(a);
-    return (size_t)(2 * kSms * ((f.few ? kMostBlocks * part_floats(kFewRows, padded(a)) : 0) + (f.tiles ? part_floats(kTileRows, padded(a)) : 0))) * 4;
+    return (size_t)(tile_floats(a, f) + few_floats(a, f) + (f.few ? kMostBlocks * kSms : 0)) * 4;
 }
 
-extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, int* status, cudaStream_t st, int* launches) {
+extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, uint32_t* joins, int* status, cudaStream_t st, int* launches) {
     const int group = (int)(c->q_heads / c->cache.heads);
     const Forms f = forms_of(c);
     AttnArgs a = {};
     a.out = c->out, a.lse = c->lse, a.q = c->q, a.k = c->cache.k, a.v = c->cache.v, a.ks = c->cache.k_scale, a.vs = c->cache.v_scale;
     a.table = c->table, a.start = c->start, a.length = c->length, a.table_s1 = c->table_s1, a.q_s1 = c->q_s1, a.out_s1 = c->out_s1;
-    a.parts = (float*)scratch, a.status = status, a.joins = (uint32_t*)status + MCU_JOIN_WORD, a.seqs = (int)c->seqs, a.rows = (int)c->rows, a.max_new = (int)c->max_new;
+    a.parts = (float*)scratch, a.status = status, a.joins = joins, a.seqs = (int)c->seqs, a.rows = (int)c->rows, a.max_new = (int)c->max_new;
     a.heads = c->cache.heads, a.group = group, a.dim = c->cache.head_dim, a.pages = c->cache.pages;
     while ((1 << a.page_log) < c->cache.page_size) ++a.page_log;
     a.window = c->window >= ((int64_t)1 << 31) - 1 ? 0 : (int)c->window;
@@ -503,10 +508,14 @@ extern "C" int mcu_launch_attention(const mcu_attention* c, void* scratch, int* 
         a.least = f.few + 1, a.most = 0x7fffffff;
         rc = wide ? run_tiles<128>(a, st) : run_tiles<64>(a, st);
         *launches += 2;
-        a.parts += 2 * kSms * part_floats(kTileRows, padded(c));
+        a.parts += tile_floats(c, f);
     }
     if (!rc && f.few) {
         a.least = 1, a.most = f.few;
+        if (!joins) {
+            a.joins = (uint32_t*)(a.parts + few_floats(c, f));
+            if ((rc = (int)cudaMemsetAsync(a.joins, 0, kMostBlocks * kSms * 4, st))) return rc;
+        }
         rc = wide ? few<128>(a, st) : few<64>(a, st);
         *launches += 1;
     }

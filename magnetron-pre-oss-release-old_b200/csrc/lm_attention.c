@@ -143,6 +143,6 @@ int mag_cuda_attention_paged_f32(mag_compute_device_t* dvc, float* out, float* l
     mcu_call c;
     int n = 0, rc = mcu_call_begin(&c, dvc, bufs, 10, mcu_attention_scratch_bytes(&a));
     if (rc) return rc;
-    rc = mcu_launch_attention(&a, c.scratch, c.status, c.stream, &n);
+    rc = mcu_launch_attention(&a, c.scratch, mcu_call_counters(&c), c.status, c.stream, &n);
     return mcu_call_end(&c, rc, n);
 }

@@ -6,6 +6,7 @@
 
 #include <cuda_runtime_api.h>
 #include <stddef.h>
+#include <stdint.h>
 
 #ifdef __cplusplus
 extern "C" {
@@ -36,7 +37,13 @@ typedef struct mcu_call {
     void* scratch;
     int prev_device;
     int own_scratch;
+    int captured;
 } mcu_call;
+/* MCU_COUNTERS words of device memory that are zero between the launches of kernels that count on them.  Eager calls, which the
+ * stream puts in order, share a set; each captured graph has one of its own, so that replays may run beside others.  Null
+ * once MCU_COUNTER_SETS graphs have had theirs: the call then needs words of its own. */
+enum { MCU_COUNTERS = 512, MCU_COUNTER_SETS = 512 };
+uint32_t* mcu_call_counters(mcu_call* c);
 int mcu_call_begin(mcu_call* c, mag_compute_device_t* dvc, const mcu_buf* bufs, int n, size_t scratch_bytes);
 int mcu_call_end(mcu_call* c, int rc, int kernels);
 

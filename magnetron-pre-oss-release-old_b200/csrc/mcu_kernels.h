@@ -184,10 +184,8 @@ typedef struct mcu_attention {
     int64_t window, q_s1, out_s1;
 } mcu_attention;
 size_t mcu_attention_scratch_bytes(const mcu_attention* a);
-/* The words at `status`: the first is that of the bounded waits; from MCU_JOIN_WORD on a counter for each block of
-   attention_few, zero between its launches, which the device's stream puts in order. */
-enum { MCU_JOIN_WORD = 64, MCU_STATUS_WORDS = MCU_JOIN_WORD + 640 };
-int mcu_launch_attention(const mcu_attention* a, void* scratch, int* status, cudaStream_t st, int* launches);
+/* joins: MCU_COUNTERS words, zero, which the call leaves zero; null: words of the scratch, cleared on the stream first (3 us). */
+int mcu_launch_attention(const mcu_attention* a, void* scratch, uint32_t* joins, int* status, cudaStream_t st, int* launches);
 
 #ifdef __cplusplus
 }
