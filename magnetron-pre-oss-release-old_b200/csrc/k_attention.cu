@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float up = query_unit(top);
-            rf[r] = fmaxf(a.scale * kLog2e / up, 0x1p-126f);  // (above zero, so that -inf times it is -inf)
+            rf[r] = logit_unit(a.scale, up);
 #pragma unroll
             for (int i = 0; i < KI; ++i)
 #pragma unroll

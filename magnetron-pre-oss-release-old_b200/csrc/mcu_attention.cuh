@@ -82,10 +82,10 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& high, uint32_
         : "f"(a), "f"(b));
 }
 // The power of two that takes a query row of largest magnitude `top` (its bits) to 2^13 .. 2^14, where both halves of a
-// value have their bits; 1 for a row of zeros or with a NaN or infinity.
+// value have their bits, or as near to it as 2^126 does (rows of zeros and of the smallest values); 1 for a row with a NaN or infinity.
 __device__ __forceinline__ float query_unit(uint32_t top) {
     const int e = (int)(top >> 23);
-    return e == 0 || e == 255 ? 1.0f : __uint_as_float((uint32_t)min(254, 127 + 127 + 13 - e) << 23);
+    return e == 255 ? 1.0f : __uint_as_float((uint32_t)min(253, 127 + 127 + 13 - e) << 23);
 }
 // The least power of two above v (v finite, positive, below 2^126).
 __device__ __forceinline__ float unit_above(float v) { return __uint_as_float((__float_as_uint(v) & 0x7F800000u) + 0x00800000u); }
@@ -93,6 +93,9 @@ __device__ __forceinline__ float unit_above(float v) { return __uint_as_float((_
 // The least power of two not below v (v positive and normal, at most 2^126), and 1 / v of such a power.
 __device__ __forceinline__ float unit_from(float v) { return __uint_as_float((__float_as_uint(v) + 0x007FFFFFu) & 0x7F800000u); }
 __device__ __forceinline__ float one_by(float v) { return __uint_as_float(0x7F000000u - __float_as_uint(v)); }
+
+// What takes a logit of queries times `up` to powers of two: finite, and above zero, so that -inf times it is -inf.
+__device__ __forceinline__ float logit_unit(float scale, float up) { return fminf(fmaxf(scale * one_by(up) * kLog2e, 0x1p-126f), 3.402823466e38f); }
 
 // Where a piece of 16 bytes of a staged row of keys or values lies within its row, so that the lanes that read
 // together find other banks.

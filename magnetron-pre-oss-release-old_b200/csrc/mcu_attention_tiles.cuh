@@ -361,7 +361,7 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
                     tmem_st8(at + DP / 2 + 8 * c, lo);
                 }
                 tmem_st_done();
-                rf = fmaxf(a.scale * kLog2e / up, 0x1p-126f);  // (above zero, so that -inf times it is -inf)
+                rf = logit_unit(a.scale, up);
                 if (half == 0) ((float*)(smem + C::FACTORS))[(i & 3) * 128 + row] = rf;
                 tc_fence_before();
                 mbar_arrive(q_full);

@@ -209,3 +209,19 @@ def test_sums_stay_short_where_pages_are_missing():
     # rounding each; the weights' halves (4 U), and some ten roundings more
     assert np.all(np.abs(get(out, dim) - want) <= (16 * 2 + 19 + 12 + 148 + 4 + 10) * U * want)
     assert abs(get(lse, 1)[0] - np.log(count)) <= (300 * 4 + 12 + 148 + 10) * U + 4 * U * np.log(count)
+
+
+@pytest.mark.parametrize("new", [1, 33])
+def test_scales_near_the_end_and_queries_near_zero(new):
+    """Every finite scale: the largest with queries of zero (equal weights) and with queries below the least normal value (logits of
+    ordinary size)."""
+    b = Batch([(new, 70)], 4, 1, 64, 16)
+    q = b.q.copy()
+    b.q[:] = 0.0
+    for scale in (3.4e38, 1e38, 1e-45):
+        b.scale = float(np.float32(scale))
+        close(b)
+    b.q[:] = q * np.float32(2.0) ** -126
+    b.q[:, 1] = q[:, 1] * np.float32(2.0) ** -132  # (few bits are left of them)
+    b.scale = float(np.float32(2.0 ** 125))
+    close(b)
