@@ -1,10 +1,10 @@
-"""Captured attention calls whose replays run beside one another: they share no scratch and no counters."""
+"""Attention and cache calls after and beside one another: captured ones share no scratch and no counters, and a read sees the write before it."""
 import numpy as np
 import pytest
 
 import mag_b200 as MB
 from gpu_util import device
-from test_gpu_lm_attention import Batch
+from test_gpu_lm_attention import Batch, blank, ints, up
 from test_gpu_lm_graphs import capture
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +85,27 @@ def test_more_graphs_than_the_device_keeps_counters_for():
         del graphs
     finally:
         T.device = old
+
+
+@pytest.mark.parametrize("rows,heads,dim", [(1, 1, 16), (40, 8, 128), (3000, 4, 64)])
+def test_reads_follow_writes_at_once(rows, heads, dim):
+    """Slots written again and again and read after each write, without a wait by the host: every read gives what was last written."""
+    d, n = device(), heads * dim
+    c = d.kv_cache(rows // 16 + 1, heads, dim, 16)
+    g = np.random.default_rng([0x52, rows])
+    slot = ints(g.permutation(rows))
+    sides = [up(g.normal(0, 1, (rows, n))) for _ in range(3)]
+    outs = [blank(rows, n) for _ in range(12)]
+    for i in range(0, 12, 2):
+        d.kv_write(c, rows, slot, sides[i % 3], sides[(i + 1) % 3])
+        d.kv_read(c, rows, slot, k=outs[i], v=outs[i + 1])
+    first = []
+    for side in sides:  # each alone
+        d.kv_write(c, rows, slot, side, side)
+        one, two = blank(rows, n), blank(rows, n)
+        d.sync()
+        d.kv_read(c, rows, slot, k=one, v=two)
+        first.append(one.read())
+        assert np.array_equal(first[-1], two.read())
+    for i, o in enumerate(outs):
+        assert np.array_equal(o.read(), first[i % 3]), i
