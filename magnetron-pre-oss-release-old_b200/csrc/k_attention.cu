@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
     float2* stats = (float2*)(smem + S::STATS);
     float* units = (float*)(stats + kFewWarps * 16);
     int* cut = (int*)(units + kFewWarps * 16);  // what an item that ends, or begins, elsewhere is: 8 ints each
-        pdl_begin();
+    pdl_begin();
 
     Share<16, DP, 32 * kFewWarps> sh;
     if (threadIdx.x < 16) cut[threadIdx.x] = 0;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(32 * FewCfg<DP, STACK, BLOCKS>::WARPS, BLOCKS)
                 const int d = 64 * i + 16 * c;
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
-                    const float4 t = live && d < a.dim ? load4(p + d + 4 * v, a.q_vec) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    const float4 t = live && d < a.dim ? four_of(p + d + 4 * v, a.q_vec) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     x[i][4 * v] = t.x, x[i][4 * v + 1] = t.y, x[i][4 * v + 2] = t.z, x[i][4 * v + 3] = t.w;
                 }
 #pragma unroll

@@ -43,7 +43,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ float4 load4(const float* p, int vec) {
+__device__ __forceinline__ float4 four_of(const float* p, int vec) {
     if (vec) return *(const float4*)p;
     return make_float4(p[0], p[1], p[2], p[3]);
 }
@@ -200,10 +200,13 @@ struct Share {
         const int64_t n = tiles_of<MAX>(a, q);
         int64_t u = 0;
         int lo, hi;
-        if constexpr (!BY_WARP) return n ? span_of<MAX>(a, q, 0, lo, hi) : 0;
-        for (int64_t t = threadIdx.x & 31; t < n; t += 32) u += span_of<MAX>(a, q, t, lo, hi);
+        if constexpr (!BY_WARP) {
+            u = n ? span_of<MAX>(a, q, 0, lo, hi) : 0;
+        } else {
+            for (int64_t t = threadIdx.x & 31; t < n; t += 32) u += span_of<MAX>(a, q, t, lo, hi);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+            for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+        }
         return u;
     }
     // The first unit of block b, before it is moved to an item's beginning or end.
