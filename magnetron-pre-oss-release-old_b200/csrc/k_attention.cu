@@ -14,20 +14,23 @@ namespace {
 // The rows of one kv head (new tokens x query heads of the group) are at most 16 here, so the cache's bytes bound the
 // work: each is read once, by one warp, for all rows.  A block works through its share of all (sequence, kv head) items'
 // units of 128 tokens; its warps take groups of 16 tokens in turn, two or three on their way by cp.async in a ring of the warp's
-// own, and each keeps its own running maximum, sum and output.  The block's warps are joined in shared memory when an item
-// ends; of the blocks that share an item the last one joins their parts.
+// own, and each keeps its own running maximum, sum and output, and for each row the unit of its weights (the largest probability times
+// scale so far).  The block's warps are joined in shared memory when an item ends; of the blocks that share an item the last one joins
+// their parts.
 //
 // Products run on mma.sync m16n8k16 (f16, f32 sums): e4m3 bytes become f16 in registers, exactly.  Queries and
-// probabilities are split in two f16, high and low.  Up to 8 rows (STACK) the halves are rows 0-7 and 8-15 of one
+// weights are split in two f16, high and low.  Up to 8 rows (STACK) the halves are rows 0-7 and 8-15 of one
 // operand, so that the split costs no instruction and a thread finds both halves' results in its own registers.
 // The order of a product's inner index is free, so it is chosen such that a thread's operands are 16 consecutive bytes
 // of a row of keys (inner index: the head's values) and of four rows of values (columns: the head's values).
 //
-// Measured (32 query heads on 8 of 128): 64 sequences of up to 16000 tokens 236 us, 6.0 TB/s of the cache
-// (274 in runs of a second, when the power limit lowers the clock); four of up to 2000
-// tokens 14 us, which is latency: about 1.6 us to find the share, 1.3 to the first copies, 2.5 for the groups, 0.8 to join the warps,
-// and three to four of fences, counter and the parts' join, at the pace of code that runs once.  (With one block of twelve warps an SM
-// the former took 306 us with eight warps of four stages, 264 with a second launch that joins the parts, 255 without.)
+// Measured (32 query heads on 8 of 128): 64 sequences of up to 16000 tokens 271 us in runs of a second, 5.2 TB/s of the cache, when
+// the power limit lowers the clock (234 in runs of some milliseconds); four of up to 2000
+// tokens 13 us, which is latency: about 1.6 us to find the share, 1.3 to the first copies, 2.5 for the groups, 0.8 to join the warps,
+// and three to four of fences, counter and the parts' join, at the pace of code that runs once.  (Short runs of one block of twelve
+// warps an SM: the former took 306 us with eight warps of four stages, 264 with a second launch that joins the parts, 255 without.)  Up
+// to 16 rows: 404 us with 128 query heads; with one unit of scales for a warp instead of one for a row 384, but rows lost bits beside
+// others' large values.
 constexpr int kSms = 148;
 constexpr int kGroup = 16;               // tokens of a warp's step; pages hold a multiple
 constexpr float kLowest = -3.402823466e38f;  // the maximum of no logits
@@ -443,9 +446,11 @@ int run_few(const AttnArgs& a, cudaStream_t st) {
 }
 
 // An SM's warps are one block, or several where there are many items: one block's beginnings and ends of items then lie under the others'
-// copies.  64 sequences of up to 500 tokens 37 us with one block, 27 with two, 25 with three; 256 of up to 1000 160, 115, 101; 64 of up to
-// 16000 255, 248, 237 (16 rows: 407, 384 with two); 16 of up to 4000 34, 32, 31.  Fewer items are cut in more parts then: four
-// sequences of up to 2000 13.8, 19.5, 15.7 us, one of 20000 26.8, 25.3, 28.1.
+// copies.  256 sequences of up to 1000 tokens, 8 heads, 151 us with one block, 98 with three; 64 of up to 16000 254 and 233, in runs
+// of a second 283 and 270 (16 rows: 425 and 403 with two).  Fewer items are cut in more parts then.  One block and three at 64, 80, 96,
+// 112 and 128 items: of up to 4000 tokens 23.3 24.4, 24.1 24.7, 27.4 26.2, 28.9 28.8, 33.1 30.4 us; of up to 16000 44.6 46.5, 53.1 53.8,
+// 60.7 60.2, 70.4 68.8, 74.1 71.6; of up to 300 10.8 12.2, then 15.5 12.2 from 80 items on.  Two blocks for 16 rows lose a little at 96
+// (41.5 45.8, 97.7 100.2) and gain from 128 on (51.0 50.5, 121.2 119.2).
 constexpr int kManyItems = 96, kMostBlocks = 3;
 template <int DP, bool EXACT>
 int few(const AttnArgs& a, cudaStream_t st) {

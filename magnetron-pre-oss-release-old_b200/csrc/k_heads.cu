@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(1024) heads_weight_sum(float* dw, const float*
 // A warp takes the keys or the values of a slot: its heads' rows lie page_size rows apart, so that one address serves them all;
 // a lane holds four values, its group every GROUPS-th head, U on their way.  (Plain loads: the call before it may still write the cache when
 // this kernel begins, so that its bytes are not read-only for it.)  Bound by HBM: 1 byte in and 4 out a value (with an
-// address for every row it was bound by instructions, 137 us for 65000 x 8 x 128; 107 so, 6.2 TB/s).
+// address for every row it was bound by instructions, 137 us for 65000 x 8 x 128; 104 so, 6.4 TB/s).
 struct ReadArgs {
     const uint8_t *kq, *vq;
     const float *ks, *vs;

@@ -146,8 +146,8 @@ __device__ __forceinline__ int64_t tiles_of(const AttnArgs& a, const Seq& q) {
 }
 // Tokens and units of tile t of a sequence: at least one unit, so that rows that see nothing are written.  Tiles of many rows
 // count kItemUnits more, for what an item costs besides its tokens (its queries, its output, the way from one to the next): four
-// prompts of up to 4100 tokens took 1148, 1086, 1040, 1052 and 1079 us with 1, 2, 4, 6 and 8 more (1215 with none), 200 of 100
-// tokens 344 to 347 with each.
+// prompts of up to 4100 tokens took 1090, 967, 895, 913 and 945 us with 0, 2, 4, 6 and 8 more, with a window of 1000 723, 657, 638,
+// 642 and 640, three chunks of up to 300 over 20000 204, 198, 196, 199 and 201; 100 prompts of up to 100 tokens 166 to 167 with each.
 constexpr int kItemUnits = 4;
 template <int MAX>
 __host__ __device__ constexpr int extra_units() {

@@ -12,7 +12,7 @@ using namespace mcu;
 //
 // A block takes tiles of 128 rows of a kv head through their tokens, 128 at a time, on tcgen05.mma kind::f16:
 //   S = Qh K^T + Ql K^T,   O = Ph V + Pl V,
-// Q and P as two f16 (22 bits), K and V exact in f16.  Both left operands lie in TMEM, where a product's rate does not hang on
+// Q and P (probability times the value's scale) as two f16 (22 bits), K and V exact in f16.  Both left operands lie in TMEM, where a product's rate does not hang on
 // two operands' shared-memory reads: 2 x 128 columns of S, over which P is written in place, 128 of O, 128 of Q.  O starts
 // from zero for every 128 tokens and is added in registers in f32 (rounded to nearest), times the step from the tile's highest logit
 // to the row's and the unit of the tile's value scales: no accumulator is ever rescaled, and the tensor core's truncating sums stay short.
@@ -26,10 +26,12 @@ using namespace mcu;
 // What bounds it is the softmax: about 14 instructions for two logits (390 cycles for 32 x 32 of them with four warps a
 // scheduler, alone), more than the products' 2 x 1024 cycles a tile.  The loops of all roles have to fit the SM's instruction cache
 // together: unrolled for 128 columns they took three times as long.  Eight softmax warps hold half a row's logits each in registers
-// (chunks of 300 over 20000 tokens 214 us; sixteen that read them twice from TMEM 245; two groups of eight in turn on tiles of their
-// own more than either).  Writing the next item's queries under the last tile's softmax made the loops longer than it hid (prompts
+// (when that was tried, chunks of 300 over 20000 tokens took 214 us; sixteen that read them twice from TMEM 245; two groups of eight in
+// turn on tiles of their own more than either).  A unit for each row, found from its weights before they are split, was tried for tiles of
+// wide scales: a branch of 220 instructions that no call took made chunks 228 us and prompts 1104, so that such tiles go round instead.  Writing the next item's queries under the last tile's softmax made the loops longer than it hid (prompts
 // 1205 us), and fetching them to L2 ahead moved nothing (1059).
-// Measured: four prompts of up to 4100 tokens, 32 query heads on 8 of 128: 1.00 ms, 0.35 PFLOP/s (both halves' products 0.7); three chunks of up to 300 over 20000 tokens, 20 heads on 4 of 96: 208 us.
+// Measured: four prompts of up to 4100 tokens, 32 query heads on 8 of 128: 0.95 ms (0.90 in runs of some milliseconds, before the clock
+// falls), 0.37 PFLOP/s (both halves' products 0.75); three chunks of up to 300 over 20000 tokens, 20 heads on 4 of 96: 200 us (196).
 constexpr int kTileRows = 128, kTileTokens = 128, kTileThreads = 640;
 constexpr int kSoftWarps = 8, kLoadWarp = 12, kIssueWarp = 16, kPlanWarp = 17, kGuideWarp = 18;  // (sums from kSoftWarps on)
 constexpr int kTileLaunch = 96, kSoftRegs = 104, kSumRegs = 168, kLoadRegs = 56, kIssueRegs = 48;
@@ -692,7 +694,8 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
         } else if (warp == kGuideWarp) {  // ---- guide: lane l has the tokens 4 l .. 4 l + 3 of a tile, of group l / 4
             // Tokens whose scales lie within 2^kNear share a unit, the least power of two above the largest, so that the weights' f16 halves
             // keep f32's bits beside the largest that a row sees.  Where a tile's differ by more it is taken in several rounds, of tokens
-            // of like scales, largest first: tiles of the same places, of which other tokens are there.
+            // of like scales, largest first: tiles of the same places, of which other tokens are there.  (Scales of e^(s n), n normal, for s of
+            // 0.3, 1, 2, 4 and 8: prompts 0.90, 1.25, 2.0, 3.4 and 5.9 ms; with one token of 2^-109 in every page 1.7.)
             uint32_t x = 0;  // the tile
 #pragma unroll 1
             for (uint32_t i = 0;; ++i) {
