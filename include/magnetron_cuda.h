@@ -417,7 +417,7 @@ MAG_CUDA_EXPORT int mag_cuda_kv_read(mag_compute_device_t* dvc, const mag_cuda_k
  * row does not see change nothing but the rounding of its sums.  scale: finite, not negative.
  * The cache's scales are NaN or as mag_cuda_kv_write forms them: not negative and below 2^126.  A value's NaN scale makes out
  * NaN and may make lse NaN.  Logits are formed in f32 from queries brought to 2^13 .. 2^14, so that keys have to stay below about 2^98
- * in magnitude; above it a logit may overflow, and the rows that see it are NaN. */
+ * in magnitude; above it a logit may overflow: the rows that see it are NaN, or take it as one of no weight where it is negative. */
 MAG_CUDA_EXPORT int mag_cuda_attention_paged_f32(mag_compute_device_t* dvc, float* out, float* lse, const float* q,
                                                  const mag_cuda_kv_cache* cache, const int32_t* table,
                                                  const int32_t* start, const int32_t* length, int64_t seqs,

@@ -718,7 +718,8 @@ __global__ void __maxnreg__(kTileLaunch) attention_tiles(AttnArgs a) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         if (!(in >> q & 1)) k[q] = v[q] = 0.0f;
-                        if (!(v[q] < kLargestScale) || !(fabsf(k[q]) < INFINITY)) k[q] = __uint_as_float(0x7FFFFFFFu), v[q] = 0.0f;  // who sees it is lost
+                        // (who sees a scale that is none is lost; none below zero is left, so that a round takes one token at least, the largest)
+                        if (!(v[q] >= 0.0f && v[q] < kLargestScale) || !(fabsf(k[q]) < INFINITY)) k[q] = __uint_as_float(0x7FFFFFFFu), v[q] = 0.0f;
                     }
                     bool more;  // another round
                     do {

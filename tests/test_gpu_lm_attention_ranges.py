@@ -225,3 +225,32 @@ def test_scales_near_the_end_and_queries_near_zero(new):
     b.q[:, 1] = q[:, 1] * np.float32(2.0) ** -132  # (few bits are left of them)
     b.scale = float(np.float32(2.0 ** 125))
     close(b)
+
+
+@pytest.mark.parametrize("new,length,group", FORMS)
+def test_scales_that_are_none_stay_with_their_rows(new, length, group):
+    """Scales below zero, infinite or NaN (the first two no call of the library writes): every call ends, and the rows that do not see them
+    are right.  The token before the last has one, so that all rows but the last two of the sequence hold to the bounds; of a sequence
+    beside it all do."""
+    for bad in (-1.0, -2.0 ** 100, np.inf, np.nan, -0.0):
+        b = Batch([(new, length), (new, 50 + new)], group, 1, 64, 16)
+        s, v = scales(b), b.v.copy()
+        at = slots(b, 0)[length - 2]
+        s[at] = bad
+        b.cache.v_scale.write(np.ascontiguousarray(s.reshape(b.pages, b.page, -1).transpose(0, 2, 1)))
+        o, l = b.run()
+        keep = np.ones(b.rows, bool)
+        keep[max(0, new - 2):new] = False
+        s[at], b.v = 1.0, v
+        b.cache.v_scale.write(np.ascontiguousarray(s.reshape(b.pages, b.page, -1).transpose(0, 2, 1)))
+        want = [b.want(i) for i in range(2)]
+        out, lse, tol, ltol = (np.concatenate([w[k] for w in want]) for k in range(4))
+        assert np.all(np.abs(o - out)[keep] <= tol[keep]) and np.all(np.abs(l - lse)[keep] <= ltol[keep])
+
+
+@pytest.mark.parametrize("dim", [16, 64, 96, 128])
+@pytest.mark.parametrize("seqs", [[(40, 40), (150, 333)], [(30, 9001)], [(1, 300), (90, 700), (3, 40)]])
+def test_rows_that_are_not_aligned(dim, seqs):
+    """Queries and outputs at strides that are no multiple of 16 bytes."""
+    Batch(seqs, 10, 2, dim, 32, extra=3).check()
+    Batch(seqs, 10, 2, dim, 32, extra=4).check()
